@@ -162,6 +162,77 @@ int kk3_status(kk3_ctx* ctx);
 int kk3_step_noalloc(const kk3_config* cfg, const void* const* table, int table_size, void* stream,
                      int* error_word);
 
+/* --- the paged latent cache of the MLA layers ------------------------------------------------------
+ *
+ * Operators on one layer's cache for what happens around the decode step (no counterpart in the reference, whose
+ * caches are contiguous and advance one token at a time): prompts and drafted tokens are appended and attended many
+ * at a time, the attention weight of cached positions is accumulated, and full sequences are cut down to the
+ * positions that carry it. A contiguous step cache [B, capacity, 512] is a paged one whose table counts up
+ * (capacity / page_size pages a sequence), so these operators prepare the caches that kk3_step_append continues. The
+ * model's MLA has no rotary part: an entry does not depend on its slot, and a cut-down cache stays valid.
+ *
+ * A sequence's position p is slot p % page_size of page table[b][p / page_size]. cu_new [batch + 1] gives the packed
+ * rows of each sequence's new tokens: cu_new[b] .. cu_new[b + 1], ascending from 0; rows at or behind cu_new[batch]
+ * belong to no one and their outputs are left as they are. `lengths` are int64 as kk3_step_append's. All pointers are
+ * device pointers on the current device, entries 16-byte aligned, strides in elements and multiples of 8. Calls
+ * enqueue kernels on `stream` and return; nothing is allocated or read back, so they can be captured. A table entry
+ * outside the pool or a length outside [0, columns * page_size] is clamped (the position reads as zeros and is not
+ * written) and sets *error_word (optional, zeroed by the caller) to a nonzero device code. What pages hold at or
+ * behind a sequence's length is never used. Limits: batch <= 4096, heads <= 128, page_size <= 65536,
+ * columns * page_size <= 2^27. */
+typedef struct kk3_cache {
+    const void* kv;              /* bf16 [num_pages, page_size, 512] */
+    const void* pe;              /* bf16 [num_pages, page_size, 64] */
+    int64_t kv_page_stride, kv_row_stride, pe_page_stride, pe_row_stride;
+    const int32_t* table;        /* [batch, columns] page numbers */
+    int64_t table_stride;
+    int32_t num_pages, page_size, columns, batch;
+} kk3_cache;
+
+/* Append: for each new token i of sequence b, position lengths[b] + i gets the entry of its projection row
+ * raw[t] (bf16 [tokens, 576], the step's `ka` product): latent = x / sqrt(mean(x^2) + eps) * norm_weight over the
+ * first 512 values (FP32, one rounding), rope part as it is. new_lengths[b] = lengths[b] + new tokens (another buffer
+ * than lengths). A token that does not fit behind the last column is not written. */
+int kk3_cache_append(const kk3_cache* cache, const void* raw, int64_t raw_stride, const void* norm_weight, float eps,
+                     const int64_t* lengths, const int32_t* cu_new, int tokens, int64_t* new_lengths, int* error_word,
+                     void* stream);
+
+/* Attention of the new tokens over their sequence's cache in the latent space. `lengths` includes the new tokens
+ * (already appended): token i of n sees the first lengths[b] - n + i + 1 positions. Per token and head
+ *   s_p = scale * (q_latent . c_p + q_pe . r_p),  out = sum_p softmax(s)_p c_p  (bf16 [tokens, heads, 512]),
+ *   lse = log sum_p exp(s_p)  (f32 [tokens, heads]).
+ * A token that sees nothing gets out = 0 and lse = -infinity. Queries: bf16, last dim contiguous, strides per token
+ * and head. Sums and softmax statistics are FP32, probabilities are rounded to bf16 for the second product. The
+ * positions that a sequence holds must be finite for its tokens' results to be. workspace: 16-byte aligned,
+ * kk3_cache_attend_workspace bytes (0: bad arguments or no device), used until the call's kernels end: calls that may
+ * overlap need one each. Results do not depend on the order in which CTAs run. */
+int64_t kk3_cache_attend_workspace(int batch, int tokens, int heads);
+int kk3_cache_attend(const kk3_cache* cache, const void* q_latent, int64_t ql_token, int64_t ql_head, const void* q_pe,
+                     int64_t qp_token, int64_t qp_head, const int64_t* lengths, const int32_t* cu_new, int tokens,
+                     int heads, float scale, void* out, float* lse, void* workspace, int64_t workspace_bytes,
+                     int* error_word, void* stream);
+
+/* Accumulated attention weight: new_mass[b][p] = mass[b][p] + sum over the sequence's new tokens that see p and over
+ * heads of exp(s_p - lse), with kk3_cache_attend's lse (rows with lse = -infinity add nothing). mass (optional, NULL:
+ * zeros) and new_mass are f32 [batch, columns * page_size], mass with its own row stride; they may be the same buffer.
+ * Positions at or behind the length keep their mass. FP32 sums in a fixed order. */
+int64_t kk3_cache_mass_workspace(int batch, int tokens, int heads);
+int kk3_cache_mass(const kk3_cache* cache, const void* q_latent, int64_t ql_token, int64_t ql_head, const void* q_pe,
+                   int64_t qp_token, int64_t qp_head, const float* lse, const int64_t* lengths, const int32_t* cu_new,
+                   int tokens, int heads, float scale, const float* mass, int64_t mass_stride, float* new_mass,
+                   void* workspace, int64_t workspace_bytes, int* error_word, void* stream);
+
+/* Eviction: each sequence keeps min(lengths[b], budget) positions: its first `sinks`, its last `recent`
+ * (sinks + recent <= budget), and of the others those of the largest mass (f32 [batch, columns * page_size] with a
+ * row stride; equal ones: the lowest position; a NaN counts as the largest). The kept entries move, in ascending
+ * order, to positions 0, 1, ... of dst_table's pages (int32 [batch, dst_columns], pages that no listed sequence
+ * uses: shared pages stay as they are), or in place (dst_table = NULL). new_lengths, new_mass [batch,
+ * columns * page_size] (the kept positions' mass, zeros behind) and kept [batch, budget] (their old positions, -1
+ * behind) are other buffers than the inputs. */
+int kk3_cache_evict(const kk3_cache* cache, const int64_t* lengths, const float* mass, int64_t mass_stride, int budget,
+                    int sinks, int recent, const int32_t* dst_table, int64_t dst_stride, int dst_columns,
+                    int64_t* new_lengths, float* new_mass, int32_t* kept, int* error_word, void* stream);
+
 /* Human-readable text for a return code. */
 const char* kk3_error_string(int code);
 

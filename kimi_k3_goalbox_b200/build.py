@@ -25,7 +25,8 @@ CHECK = PKG / "_lib" / "kk3_tc_check"   # checker of the tensor-core expert engi
 # the oracle's C restatement of the MXFP4 decode (test infrastructure: the checker and the timed CPU baseline)
 ORACLE_SRC = ROOT / "oracle" / "mxfp4.c"
 ORACLE_LIB = ROOT / "oracle" / "libkk3_oracle_mxfp4.so"
-UNITS = ["kk3_host.cu", "kk3_kernel_nt1.cu", "kk3_kernel_nt2.cu", "kk3_kernel_nt4.cu", "kk3_kernel_nt8.cu"]
+UNITS = ["kk3_host.cu", "kk3_kernel_nt1.cu", "kk3_kernel_nt2.cu", "kk3_kernel_nt4.cu", "kk3_kernel_nt8.cu",
+         "kk3_cache.cu", "kk3_cache_tc.cu"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 FLAGS = ["-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC", "-Xptxas", "-v", f"-I{ROOT / 'include'}"]
 
@@ -38,7 +39,7 @@ def nvcc() -> str:
 
 
 def _deps() -> list[Path]:
-    return sorted(CSRC.glob("*.cuh")) + [ROOT / "include" / "kk3.h"]
+    return sorted([*CSRC.glob("*.cuh"), *CSRC.glob("*.h")]) + [ROOT / "include" / "kk3.h"]
 
 
 def _stale(obj: Path, src: Path) -> bool:

@@ -1,0 +1,749 @@
+// kk3_cache.cu - kernels and C entry points of the paged latent cache (include/kk3.h, kk3_cache_*): append, attention
+// of new tokens at warp level, the join of split attention tiles, eviction.
+#include <cuda_runtime.h>
+
+#include "kk3_cache.cuh"
+#include "kk3_cache_host.h"
+
+namespace kk3 {
+
+KK3_DEV void cp_async16_zfill(void* smem, const void* src, bool live) {
+  const unsigned dst = (unsigned)__cvta_generic_to_shared(smem);
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(live ? 16 : 0) : "memory");
+}
+KK3_DEV void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+KK3_DEV void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+KK3_DEV void ldsm4(unsigned (&r)[4], const void* p) {
+  const unsigned a = (unsigned)__cvta_generic_to_shared(p);
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a) : "memory");
+}
+KK3_DEV void ldsm4t(unsigned (&r)[4], const void* p) {
+  const unsigned a = (unsigned)__cvta_generic_to_shared(p);
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a) : "memory");
+}
+
+// ---------------------------------------------------------------------------------------------
+// append: latent = x[:512] / rms(x[:512]) * weight (FP32, rounded to BF16 once), rope = x[512:], into the page of the
+// token's position. One warp per token, bound by its 2304 bytes of traffic; 16-byte accesses throughout (lane l owns
+// the latent values 8 l .. 8 l + 7 and 256 + 8 l ..; eight lanes copy the rope part).
+
+struct AppendArgs {
+  CachePages c;
+  const bf16* raw;
+  long long raw_row;
+  const bf16* weight;
+  const long long* lengths;
+  long long* new_lengths;
+  const int* cu_new;
+  int tokens;
+  float eps;
+};
+
+constexpr int kAppendWarps = 4;
+
+__global__ void __launch_bounds__(kAppendWarps * 32) kk3_cache_append_kernel(const AppendArgs a) {
+  const int lane = threadIdx.x & 31;
+  const int tok = blockIdx.x * kAppendWarps + (threadIdx.x >> 5);
+  const int B = a.c.batch;
+  const long long cap = (long long)a.c.columns * a.c.page_size;
+  if (blockIdx.x == 0) {
+    for (int b = threadIdx.x; b < B; b += blockDim.x) {
+      const int q0 = min(max(a.cu_new[b], 0), a.tokens), q1 = min(max(a.cu_new[b + 1], q0), a.tokens);
+      const long long l = a.lengths[b], sum = (l < 0 ? 0 : l) + (q1 - q0);
+      if (l < 0 || sum > cap) cache_error(a.c);
+      a.new_lengths[b] = sum > cap ? cap : sum;
+    }
+  }
+  if (tok >= a.tokens) return;
+  int lo = 0, hi = B;   // the sequence of this token: cu_new[lo] <= tok < cu_new[lo + 1]
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (a.cu_new[mid] <= tok) lo = mid; else hi = mid;
+  }
+  const int first = a.cu_new[lo];
+  if (tok < first || tok >= a.cu_new[lo + 1] || first < 0) return;   // behind the last sequence: no one's token
+  const long long pos = max(a.lengths[lo], 0ll) + (tok - first);
+  if (pos >= cap) return;
+  int slot;
+  const int page = page_at(a.c, lo, (int)pos, &slot);
+  if (page < 0) return;
+  const bf16* x = a.raw + (long long)tok * a.raw_row;
+  uint4 v[2], w[2];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    v[h] = *reinterpret_cast<const uint4*>(x + h * 256 + lane * 8);
+    w[h] = *reinterpret_cast<const uint4*>(a.weight + h * 256 + lane * 8);
+  }
+  uint4 rope = {};
+  if (lane < 8) rope = *reinterpret_cast<const uint4*>(x + kLat + lane * 8);
+  float sum = 0.0f;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const __nv_bfloat162* p = reinterpret_cast<const __nv_bfloat162*>(&v[h]);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 f = __bfloat1622float2(p[i]);
+      sum = fmaf(f.x, f.x, fmaf(f.y, f.y, sum));
+    }
+  }
+  const float r = rsqrtf(warp_sum(sum) * (1.0f / kLat) + a.eps);
+  bf16* kv = a.c.kv + (long long)page * a.c.kv_page + (long long)slot * a.c.kv_row;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    __nv_bfloat162* p = reinterpret_cast<__nv_bfloat162*>(&v[h]);
+    const __nv_bfloat162* q = reinterpret_cast<const __nv_bfloat162*>(&w[h]);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 f = __bfloat1622float2(p[i]), g = __bfloat1622float2(q[i]);
+      p[i] = __floats2bfloat162_rn(f.x * r * g.x, f.y * r * g.y);
+    }
+    *reinterpret_cast<uint4*>(kv + h * 256 + lane * 8) = v[h];
+  }
+  if (lane < 8)
+    *reinterpret_cast<uint4*>(a.c.pe + (long long)page * a.c.pe_page + (long long)slot * a.c.pe_row + lane * 8) = rope;
+}
+
+// ---------------------------------------------------------------------------------------------
+// Attention at warp level: a tile is 16 (token, head) rows, a unit 32 cached positions.
+//
+//   s = scale (q . e_p), running maximum m and sum l per row, O = O 2^(m - m') + sum_p 2^(s - m') c_p
+//
+// Each cached entry is read once per tile and serves both products from shared memory, so few rows per sequence
+// leave the call bound by the cache's bytes: 1088 multiply-adds a row and position at the warp-level rate of
+// m16n8k16 take less time than 1152 bytes from HBM up to 32 rows. 8 warps; the query's fragments stay in registers
+// (each warp holds one half of the 576 dims: 18 k-steps), five 36.5 KB stages of positions arrive by cp.async two
+// units and more ahead, warp w owns the output dims 64 w .. 64 w + 63.
+// Probabilities are rounded to BF16 for the second product, the type that the instruction takes with BF16 latents; the
+// running sum adds them unrounded, since lse is an FP32 result.
+
+constexpr int kWaRows = 16;
+constexpr int kWaUnit = 32;
+constexpr int kWaStages = 5;
+constexpr int kWaPitch = kEntry + 8;      // 1168-byte rows: consecutive rows fall on different banks (ldmatrix)
+constexpr int kWaPPitch = kWaUnit + 8;
+constexpr int kWaThreads = 256;
+constexpr int kWaMinUnits = 4;
+struct WaSmem {
+  bf16 ring[kWaStages][kWaUnit][kWaPitch];
+  bf16 q[kWaRows][kWaPitch];
+  float s[2][kWaRows][kWaUnit + 4];
+  bf16 p[kWaRows][kWaPPitch];
+  float alpha[kWaRows];
+  float m[kWaRows], l[kWaRows];
+  long long red[kWaThreads / 32 + 4];
+};
+
+KK3_DEV void wa_load(const AttendArgs& a, WaSmem& sm, const Seq& s, int b, int unit, int sees, int stage) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  // lanes 0..3 look up the warp's four positions
+  long long kv = -1, pe = -1;
+  if (lane < 4) {
+    const int pos = unit * kWaUnit + warp * 4 + lane;
+    if (pos < sees) {
+      int slot;
+      const int page = page_at(a.c, b, pos, &slot);
+      if (page >= 0) {
+        kv = (long long)page * a.c.kv_page + (long long)slot * a.c.kv_row;
+        pe = (long long)page * a.c.pe_page + (long long)slot * a.c.pe_row;
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int row = i >> 1, chunk = (i & 1) * 32 + lane;
+    const long long o = __shfl_sync(0xffffffffu, kv, row);
+    cp_async16_zfill(&sm.ring[stage][warp * 4 + row][chunk * 8], o >= 0 ? a.c.kv + o + chunk * 8 : a.c.kv, o >= 0);
+  }
+  const long long o = __shfl_sync(0xffffffffu, pe, lane >> 3);
+  cp_async16_zfill(&sm.ring[stage][warp * 4 + (lane >> 3)][kLat + (lane & 7) * 8],
+                   o >= 0 ? a.c.pe + o + (lane & 7) * 8 : a.c.pe, o >= 0);
+}
+
+__global__ void __launch_bounds__(kWaThreads, 1) kk3_cache_attend_warp_kernel(const AttendArgs a) {
+  extern __shared__ __align__(128) unsigned char smem_raw[];
+  WaSmem& sm = *reinterpret_cast<WaSmem*>(smem_raw);
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int worker = blockIdx.x;
+  static_assert(sizeof(sm.ring) >= (kMaxSeqs + 1) * sizeof(int), "the sequences' tile prefix lies in the ring");
+  const AttendSplit split{kWaRows, a.heads, kWaUnit};
+  const Share sh = plan_share<kWaThreads>(a, split, worker, kWaMinUnits, reinterpret_cast<int*>(&sm.ring[0][0][0]),
+                                          sm.red);
+  if (tid == 0) a.meta[worker * 4 + 2] = 0;
+  if (worker >= sh.workers) return;
+  int b = sh.b, t = sh.t;
+  long long at = sh.at;
+  while (at < sh.end) {
+    Seq s = a.seq(b);
+    for (; t >= split.tiles(s); t = 0) s = a.seq(++b);
+    const int units = split.units(s, t);
+    const int u0 = (int)max(0ll, sh.begin - at), u1 = (int)min((long long)units, sh.end - at);
+    const bool whole = u0 == 0 && u1 == units;
+    const int row0 = t * kWaRows, rows = min(kWaRows, s.n * a.heads - row0);
+    const int sees_max = s.len - s.n + min(s.n - 1, (row0 + rows - 1) / a.heads) + 1;
+    __syncthreads();   // the previous tile's readers are done with q, p and the ring
+    // query rows, zeros below the last
+    for (int i = tid; i < kWaRows * (kEntry / 8); i += kWaThreads) {
+      const int r = i / (kEntry / 8), ch = i % (kEntry / 8);
+      const int g = row0 + min(r, rows - 1), tok = s.q0 + g / a.heads, head = g % a.heads;
+      const bf16* src = ch < kLat / 8 ? a.q_lat + tok * a.ql_tok + head * a.ql_head + ch * 8
+                                      : a.q_pe + tok * a.qp_tok + head * a.qp_head + (ch - kLat / 8) * 8;
+      cp_async16_zfill(&sm.q[r][ch * 8], src, r < rows);
+    }
+    cp_async_commit();
+#pragma unroll
+    for (int i = 0; i < kWaStages - 1; ++i) {
+      if (u0 + i < u1) wa_load(a, sm, s, b, u0 + i, sees_max, i);
+      cp_async_commit();
+    }
+    cp_async_wait<kWaStages - 1>();
+    __syncthreads();
+    // this warp's query fragments: k-steps 18 (warp / 4) .. + 17
+    const int ntile = warp & 3, khalf = warp >> 2;
+    unsigned qf[18][4];
+#pragma unroll
+    for (int k = 0; k < 18; ++k)
+      ldsm4(qf[k], &sm.q[lane & 15][(khalf * 18 + k) * 16 + (lane >> 4) * 8]);
+    float acc[8][4] = {};
+    // softmax rows of this warp: 2 warp and 2 warp + 1, one position a lane
+    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
+    int sees[2];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const int r = warp * 2 + j;
+      sees[j] = r < rows ? s.len - s.n + (row0 + r) / a.heads + 1 : 0;
+    }
+    for (int u = u0; u < u1; ++u) {
+      const int stage = (u - u0) % kWaStages;
+      cp_async_wait<kWaStages - 2>();
+      __syncthreads();   // unit u is in; every warp is done with unit u - 1
+      if (u + kWaStages - 1 < u1) wa_load(a, sm, s, b, u + kWaStages - 1, sees_max, (u - u0 + kWaStages - 1) % kWaStages);
+      cp_async_commit();
+      {
+        float c0[4] = {}, c1[4] = {};
+#pragma unroll
+        for (int k = 0; k < 18; k += 2) {
+          unsigned bf[4];
+          ldsm4(bf, &sm.ring[stage][ntile * 8 + (lane & 7)][(khalf * 18 + k) * 16 + (lane >> 3) * 8]);
+          mma_bf16(c0, qf[k][0], qf[k][1], qf[k][2], qf[k][3], bf[0], bf[1]);
+          mma_bf16(c1, qf[k + 1][0], qf[k + 1][1], qf[k + 1][2], qf[k + 1][3], bf[2], bf[3]);
+        }
+        const int r = lane >> 2, col = ntile * 8 + (lane & 3) * 2;
+        *reinterpret_cast<float2*>(&sm.s[khalf][r][col]) = make_float2(c0[0] + c1[0], c0[1] + c1[1]);
+        *reinterpret_cast<float2*>(&sm.s[khalf][r + 8][col]) = make_float2(c0[2] + c1[2], c0[3] + c1[3]);
+      }
+      __syncthreads();
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int r = warp * 2 + j;
+        float v = (sm.s[0][r][lane] + sm.s[1][r][lane]) * a.scale_log2;
+        if (u * kWaUnit + lane >= sees[j]) v = -INFINITY;
+        const float top = fmaxf(m[j], warp_max(v));
+        const float ref = top == -INFINITY ? 0.0f : top;
+        const float al = exp2f(m[j] - ref);
+        const float p = exp2f(v - ref);
+        l[j] = l[j] * al + p;
+        m[j] = top;
+        sm.p[r][lane] = f2bf(p);
+        if (lane == 0) sm.alpha[r] = al;
+      }
+      __syncthreads();
+      {
+        const float a0 = sm.alpha[lane >> 2], a1 = sm.alpha[(lane >> 2) + 8];
+#pragma unroll
+        for (int n = 0; n < 8; ++n) {
+          acc[n][0] *= a0;
+          acc[n][1] *= a0;
+          acc[n][2] *= a1;
+          acc[n][3] *= a1;
+        }
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          unsigned pf[4];
+          ldsm4(pf, &sm.p[lane & 15][k * 16 + (lane >> 4) * 8]);
+#pragma unroll
+          for (int n = 0; n < 8; n += 2) {
+            unsigned bf[4];
+            ldsm4t(bf, &sm.ring[stage][k * 16 + (lane & 15)][warp * 64 + n * 8 + (lane >> 4) * 8]);
+            mma_bf16(acc[n], pf[0], pf[1], pf[2], pf[3], bf[0], bf[1]);
+            mma_bf16(acc[n + 1], pf[0], pf[1], pf[2], pf[3], bf[2], bf[3]);
+          }
+        }
+      }
+    }
+    cp_async_wait<0>();
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      l[j] = warp_sum(l[j]);
+      if (lane == 0) {
+        sm.m[warp * 2 + j] = m[j];
+        sm.l[warp * 2 + j] = l[j];
+      }
+    }
+    __syncthreads();
+    const int r = lane >> 2;
+    if (whole) {
+      const long long g = (long long)s.q0 * a.heads + row0;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int rr = r + 8 * h;
+        if (rr < rows) {
+          const float lr = sm.l[rr], inv = lr > 0.0f || lr != lr ? 1.0f / lr : 0.0f;
+          bf16* o = a.out + (g + rr) * kLat + warp * 64 + (lane & 3) * 2;
+#pragma unroll
+          for (int n = 0; n < 8; ++n)
+            *reinterpret_cast<__nv_bfloat162*>(o + n * 8) = __floats2bfloat162_rn(acc[n][h * 2] * inv, acc[n][h * 2 + 1] * inv);
+        }
+      }
+      if (tid < rows) a.lse[g + tid] = (sm.m[tid] + log2f(sm.l[tid])) * 0.69314718055994531f;
+    } else {
+      // running sums for the join: slot 1 for the tile this worker begins and leaves, slot 0 for one it comes into
+      float* part = a.part + ((long long)worker * 2 + (u0 == 0 ? 1 : 0)) * kWaRows * kPartRow;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int rr = r + 8 * h;
+        if (rr < rows) {
+          float* o = part + rr * kPartRow + warp * 64 + (lane & 3) * 2;
+#pragma unroll
+          for (int n = 0; n < 8; ++n) *reinterpret_cast<float2*>(o + n * 8) = make_float2(acc[n][h * 2], acc[n][h * 2 + 1]);
+        }
+      }
+      if (tid < rows) {
+        part[tid * kPartRow + kLat] = sm.m[tid];
+        part[tid * kPartRow + kLat + 1] = sm.l[tid];
+      }
+      if (u0 == 0 && tid == 0) {   // the workers of this tile: up to the one that holds its last unit
+        int last = worker;
+        while (sh.total * (last + 1) / sh.workers < at + units) ++last;
+        a.meta[worker * 4] = b;
+        a.meta[worker * 4 + 1] = t;
+        a.meta[worker * 4 + 2] = last - worker + 1;
+      }
+    }
+    at += units;
+    ++t;
+  }
+}
+
+// ---------------------------------------------------------------------------------------------
+// Join of a split tile: out = sum_w 2^(m_w - m) O_w / sum_w 2^(m_w - m) l_w over the tile's workers in order. One CTA
+// per (worker that begins a split tile, row); four groups of 128 threads (4 dims each) take a quarter of the workers'
+// sums each, so that the loads of many short pieces are in flight together.
+__global__ void __launch_bounds__(512) kk3_cache_join_kernel(const AttendArgs a, int tile_rows) {
+  const int worker = blockIdx.x, row = blockIdx.y;
+  const int n = a.meta[worker * 4 + 2];
+  if (n == 0) return;
+  const int b = a.meta[worker * 4], t = a.meta[worker * 4 + 1];
+  const Seq s = a.seq(b);
+  if ((long long)t * tile_rows + row >= (long long)s.n * a.heads) return;
+  __shared__ float4 sums[3][128];
+  const int grp = threadIdx.x >> 7, i = threadIdx.x & 127;
+  const auto part = [&](int w) {
+    return a.part + (((long long)(worker + w) * 2 + (w == 0 ? 1 : 0)) * tile_rows + row) * kPartRow;
+  };
+  float top = -INFINITY;
+  for (int w = 0; w < n; ++w) top = fmaxf(top, part(w)[kLat]);
+  const float ref = top == -INFINITY ? 0.0f : top;
+  float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  float l = 0.0f;
+  for (int w = 0; w < n; ++w) l += exp2f(part(w)[kLat] - ref) * part(w)[kLat + 1];
+  const int per = (n + 3) / 4;
+#pragma unroll 4
+  for (int w = grp * per; w < min(n, (grp + 1) * per); ++w) {
+    const float* p = part(w);
+    const float4 v = *reinterpret_cast<const float4*>(p + i * 4);
+    const float f = exp2f(p[kLat] - ref);
+    sum.x = fmaf(f, v.x, sum.x);
+    sum.y = fmaf(f, v.y, sum.y);
+    sum.z = fmaf(f, v.z, sum.z);
+    sum.w = fmaf(f, v.w, sum.w);
+  }
+  if (grp > 0) sums[grp - 1][i] = sum;
+  __syncthreads();
+  if (grp > 0) return;
+#pragma unroll
+  for (int k = 0; k < 3; ++k) {
+    sum.x += sums[k][i].x;
+    sum.y += sums[k][i].y;
+    sum.z += sums[k][i].z;
+    sum.w += sums[k][i].w;
+  }
+  const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
+  const long long g = (long long)s.q0 * a.heads + (long long)t * tile_rows + row;
+  __nv_bfloat162* o = reinterpret_cast<__nv_bfloat162*>(a.out + g * kLat + i * 4);
+  o[0] = __floats2bfloat162_rn(sum.x * inv, sum.y * inv);
+  o[1] = __floats2bfloat162_rn(sum.z * inv, sum.w * inv);
+  if (i == 0) a.lse[g] = (ref + log2f(l)) * 0.69314718055994531f;
+}
+
+// ---------------------------------------------------------------------------------------------
+// Eviction, selection: one CTA per sequence. The positions are ordered by (protected, weight, lowest index); the
+// weights' bits are mapped to unsigned keys of the same order, the key of the last kept position is found digit by
+// digit (four histograms of 8 bits), and one pass in ascending position writes the kept ones.
+
+struct EvictArgs {
+  CachePages c;
+  const long long* lengths;
+  const float* mass;
+  long long mass_row;
+  int budget, sinks, recent;
+  const int* dst;          // destination table, or null: in place
+  long long dst_row;
+  int dst_columns;
+  long long* new_lengths;
+  float* new_mass;         // [batch, columns * page_size]
+  int* kept;               // [batch, budget]
+};
+
+constexpr int kEvThreads = 1024;
+
+// unsigned key in the order of the floats; every NaN above +infinity, -0 equal to 0
+KK3_DEV unsigned mass_key(float v) {
+  if (v != v) return 0xffffffffu;
+  const unsigned u = __float_as_uint(v + 0.0f);
+  return u & 0x80000000u ? ~u : u | 0x80000000u;
+}
+
+__global__ void __launch_bounds__(kEvThreads) kk3_cache_select_kernel(const EvictArgs a) {
+  const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  __shared__ int hist[256];
+  __shared__ int tell[2];
+  __shared__ int sums[32], ties[32];
+  const long long cap = (long long)a.c.columns * a.c.page_size;
+  long long len64 = a.lengths[b];
+  if (len64 < 0 || len64 > cap) {
+    if (tid == 0) cache_error(a.c);
+    len64 = len64 < 0 ? 0 : cap;
+  }
+  const int len = (int)len64;
+  const int keep = min(len, a.budget);
+  const float* mass = a.mass + (long long)b * a.mass_row;
+  float* out = a.new_mass + (long long)b * cap;
+  int* kept = a.kept + (long long)b * a.budget;
+  const int sinks = min(a.sinks, len), tail = max(sinks, len - a.recent);   // free positions: [sinks, tail)
+  unsigned border = 0;   // key of the last kept free position
+  int want = keep - (sinks + len - tail);   // free positions to keep; at the end: those of the border's key
+  const bool all = keep == len;
+  if (!all && want > 0) {
+    unsigned prefix = 0, mask = 0;
+    for (int shift = 24; shift >= 0; shift -= 8) {
+      if (tid < 256) hist[tid] = 0;
+      __syncthreads();
+      for (int p = sinks + tid; p < tail; p += kEvThreads) {
+        const unsigned k = mass_key(mass[p]);
+        if ((k & mask) == prefix) atomicAdd(&hist[(k >> shift) & 255], 1);
+      }
+      __syncthreads();
+      if (warp == 0) {   // digits from the top: lane l owns 255 - 8 l .. 248 - 8 l
+        int c[8], mine = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) mine += c[i] = hist[255 - lane * 8 - i];
+        int before = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const int u = __shfl_up_sync(0xffffffffu, before, o);
+          if (lane >= o) before += u;
+        }
+        before -= mine;
+        if (before < want && want <= before + mine) {
+          int i = 0;
+          while (before + c[i] < want) before += c[i++];
+          tell[0] = 255 - lane * 8 - i;
+          tell[1] = want - before;
+        }
+      }
+      __syncthreads();
+      prefix |= (unsigned)tell[0] << shift;
+      mask |= 255u << shift;
+      want = tell[1];
+      __syncthreads();
+    }
+    border = prefix;
+  }
+  // ascending pass: thread t owns a run of positions
+  const int run = (len + kEvThreads - 1) / kEvThreads, p0 = min(len, tid * run), p1 = min(len, p0 + run);
+  const auto state = [&](int p) -> int {   // 0 dropped, 1 kept, 2 kept if among the first `want` of the border's key
+    if (all || p < sinks || p >= tail) return 1;
+    if (want <= 0) return 0;
+    const unsigned k = mass_key(mass[p]);
+    return k > border ? 1 : k == border ? 2 : 0;
+  };
+  int sure = 0, tie = 0;
+  for (int p = p0; p < p1; ++p) {
+    const int v = state(p);
+    sure += v == 1;
+    tie += v == 2;
+  }
+  int x = sure, y = tie;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int u = __shfl_up_sync(0xffffffffu, x, o), v = __shfl_up_sync(0xffffffffu, y, o);
+    if (lane >= o) {
+      x += u;
+      y += v;
+    }
+  }
+  if (lane == 31) {
+    sums[warp] = x;
+    ties[warp] = y;
+  }
+  __syncthreads();
+  x -= sure;
+  y -= tie;
+  for (int w = 0; w < warp; ++w) {
+    x += sums[w];
+    y += ties[w];
+  }
+  // x certain ones and y ties lie before this run; a tie is kept while fewer than `want` came before it
+  int j = x + min(y, max(want, 0));
+  for (int p = p0; p < p1; ++p) {
+    const int v = state(p);
+    if (v == 1 || (v == 2 && y < want)) {
+      kept[j] = p;
+      out[j] = mass[p];
+      ++j;
+    }
+    y += v == 2;
+  }
+  for (int i = keep + tid; i < a.budget; i += kEvThreads) kept[i] = -1;
+  for (long long i = keep + tid; i < cap; i += kEvThreads) out[i] = 0.0f;
+  if (tid == 0) a.new_lengths[b] = keep;
+}
+
+// Eviction, move into pages of their own: one warp per kept entry (1152 bytes), bound by the traffic.
+constexpr int kMoveWarps = 8;
+__global__ void __launch_bounds__(kMoveWarps * 32) kk3_cache_move_kernel(const EvictArgs a) {
+  const int b = blockIdx.y, lane = threadIdx.x & 31;
+  const int j = blockIdx.x * kMoveWarps + (threadIdx.x >> 5);
+  if (j >= a.budget) return;
+  const int from = a.kept[(long long)b * a.budget + j];
+  if (from < 0) return;
+  CachePages d = a.c;
+  d.table = a.dst;
+  d.table_stride = a.dst_row;
+  int slot, to_slot;
+  const int page = page_at(a.c, b, from, &slot), to = page_at(d, b, j, &to_slot);
+  if (page < 0 || to < 0) return;
+  const bf16* kv = a.c.kv + (long long)page * a.c.kv_page + (long long)slot * a.c.kv_row + lane * 8;
+  const bf16* pe = a.c.pe + (long long)page * a.c.pe_page + (long long)slot * a.c.pe_row + lane * 8;
+  const uint4 v0 = ldg_stream16(kv), v1 = ldg_stream16(kv + 256);
+  uint4 v2 = {};
+  if (lane < 8) v2 = ldg_stream16(pe);
+  bf16* okv = a.c.kv + (long long)to * a.c.kv_page + (long long)to_slot * a.c.kv_row + lane * 8;
+  *reinterpret_cast<uint4*>(okv) = v0;
+  *reinterpret_cast<uint4*>(okv + 256) = v1;
+  if (lane < 8)
+    *reinterpret_cast<uint4*>(a.c.pe + (long long)to * a.c.pe_page + (long long)to_slot * a.c.pe_row + lane * 8) = v2;
+}
+
+// Eviction, move in place: entry kept[j] >= j goes to slot j, so batches in ascending j are safe when a batch is read
+// whole before it is written: later batches read slots at or above their own j, which earlier ones did not write.
+// The order holds per (sequence, 64-byte slice of the entry); the 18 slices of a sequence run side by side.
+constexpr int kSlideThreads = 512;
+constexpr int kSlideDeep = 8;    // rows in flight per thread: 1024 rows a batch
+__global__ void __launch_bounds__(kSlideThreads) kk3_cache_slide_kernel(const EvictArgs a) {
+  const int b = blockIdx.y, ch = blockIdx.x * 4 + (threadIdx.x & 3);   // 16-byte piece of the entry: 0 .. 71
+  const int keep = (int)a.new_lengths[b];
+  const int* kept = a.kept + (long long)b * a.budget;
+  constexpr int kRows = kSlideThreads / 4;
+  const auto where = [&](int pos) -> bf16* {
+    int slot;
+    const int page = page_at(a.c, b, pos, &slot);
+    if (page < 0) return nullptr;
+    return ch < kLat / 8 ? a.c.kv + (long long)page * a.c.kv_page + (long long)slot * a.c.kv_row + ch * 8
+                         : a.c.pe + (long long)page * a.c.pe_page + (long long)slot * a.c.pe_row + (ch - kLat / 8) * 8;
+  };
+  for (int j0 = 0; j0 < keep; j0 += kRows * kSlideDeep) {
+    uint4 v[kSlideDeep];
+    bool move[kSlideDeep];
+#pragma unroll
+    for (int i = 0; i < kSlideDeep; ++i) {
+      const int j = j0 + i * kRows + (threadIdx.x >> 2);
+      move[i] = false;
+      if (j < keep) {
+        const int from = kept[j];
+        const bf16* src = from != j ? where(from) : nullptr;
+        if (src) {
+          v[i] = *reinterpret_cast<const uint4*>(src);
+          move[i] = true;
+        }
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kSlideDeep; ++i) {
+      if (move[i]) {
+        bf16* dst = where(j0 + i * kRows + (threadIdx.x >> 2));
+        if (dst) *reinterpret_cast<uint4*>(dst) = v[i];
+      }
+    }
+    __syncthreads();
+  }
+}
+
+}  // namespace kk3
+
+// ---------------------------------------------------------------------------------------------
+// C entry points
+
+using namespace kk3;
+
+namespace kk3 {
+
+
+
+int cache_cuda(cudaError_t e, const char* what) {
+  if (e == cudaSuccess) return KK3_OK;
+  fprintf(stderr, "kk3: %s: %s\n", what, cudaGetErrorString(e));
+  (void)cudaGetLastError();
+  return KK3_ERR_CUDA;
+}
+
+int cache_pages(const kk3_cache* c, CachePages* out, int* error_word) {
+  if (!c || !cache_aligned(c->kv, 16) || !cache_aligned(c->pe, 16) || !cache_aligned(c->table, 4)) return KK3_ERR_ARG;
+  if (c->batch < 1 || c->columns < 1 || c->page_size < 1 || c->num_pages < 1 || c->table_stride < 0) return KK3_ERR_ARG;
+  if (c->kv_row_stride < kLat || c->pe_row_stride < kRope || c->kv_page_stride < 0 || c->pe_page_stride < 0 ||
+      c->kv_row_stride % 8 || c->pe_row_stride % 8 || c->kv_page_stride % 8 || c->pe_page_stride % 8)
+    return KK3_ERR_ARG;
+  if (c->batch > kMaxSeqs || c->page_size > 65536 || (long long)c->columns * c->page_size > (1ll << 27))
+    return KK3_ERR_UNSUPPORTED;
+  out->kv = (bf16*)c->kv;
+  out->pe = (bf16*)c->pe;
+  out->kv_page = c->kv_page_stride;
+  out->kv_row = c->kv_row_stride;
+  out->pe_page = c->pe_page_stride;
+  out->pe_row = c->pe_row_stride;
+  out->table = c->table;
+  out->table_stride = c->table_stride;
+  out->num_pages = c->num_pages;
+  out->page_size = c->page_size;
+  out->columns = c->columns;
+  out->batch = c->batch;
+  out->page_magic = c->page_size > 1 ? (unsigned)((1ull << 32) / (unsigned)c->page_size + 1) : 0;
+  out->error_word = error_word;
+  return KK3_OK;
+}
+
+int cache_sms(int* sms) {
+  int dev = 0;
+  int rc = cache_cuda(cudaGetDevice(&dev), "cudaGetDevice");
+  if (rc) return rc;
+  return cache_cuda(cudaDeviceGetAttribute(sms, cudaDevAttrMultiProcessorCount, dev), "cudaDeviceGetAttribute");
+}
+
+}  // namespace kk3
+
+extern "C" int kk3_cache_append(const kk3_cache* cache, const void* raw, int64_t raw_stride, const void* norm_weight,
+                                float eps, const int64_t* lengths, const int32_t* cu_new, int tokens,
+                                int64_t* new_lengths, int* error_word, void* stream) {
+  AppendArgs a;
+  const int rc = cache_pages(cache, &a.c, error_word);
+  if (rc) return rc;
+  if (tokens < 0 || (tokens > 0 && !cache_aligned(raw, 16)) || raw_stride % 8 || raw_stride < kEntry ||
+      !cache_aligned(norm_weight, 16) || !cache_aligned(lengths, 8) || !cache_aligned(cu_new, 4) || !cache_aligned(new_lengths, 8) ||
+      lengths == new_lengths || !(eps >= 0.0f))
+    return KK3_ERR_ARG;
+  a.raw = (const bf16*)raw;
+  a.raw_row = raw_stride;
+  a.weight = (const bf16*)norm_weight;
+  a.lengths = (const long long*)lengths;
+  a.new_lengths = (long long*)new_lengths;
+  a.cu_new = cu_new;
+  a.tokens = tokens;
+  a.eps = eps;
+  const int grid = tokens > 0 ? (tokens + kAppendWarps - 1) / kAppendWarps : 1;
+  kk3_cache_append_kernel<<<grid, kAppendWarps * 32, 0, (cudaStream_t)stream>>>(a);
+  return cache_cuda(cudaGetLastError(), "kk3_cache_append_kernel");
+}
+
+extern "C" int64_t kk3_cache_attend_workspace(int batch, int tokens, int heads) {
+  if (batch < 1 || tokens < 0 || heads < 1 || heads > kMaxHeads) return 0;
+  int sms = 0;
+  if (cache_sms(&sms)) return 0;
+  return (int64_t)sms * 16 + (int64_t)sms * 2 * kWaRows * kPartRow * 4;
+}
+
+extern "C" int kk3_cache_attend(const kk3_cache* cache, const void* q_latent, int64_t ql_token, int64_t ql_head,
+                                const void* q_pe, int64_t qp_token, int64_t qp_head, const int64_t* lengths,
+                                const int32_t* cu_new, int tokens, int heads, float scale, void* out, float* lse,
+                                void* workspace, int64_t workspace_bytes, int* error_word, void* stream) {
+  AttendArgs a;
+  const int rc = cache_pages(cache, &a.c, error_word);
+  if (rc) return rc;
+  if (tokens < 0 || heads < 1 || !cache_aligned(lengths, 8) || !cache_aligned(cu_new, 4) || !(scale == scale)) return KK3_ERR_ARG;
+  if (heads > kMaxHeads || (int64_t)tokens * heads > INT32_MAX / 2) return KK3_ERR_UNSUPPORTED;
+  if (tokens == 0) return KK3_OK;
+  if (!cache_aligned(q_latent, 16) || !cache_aligned(q_pe, 16) || !cache_aligned(out, 16) || !cache_aligned(lse, 4) || ql_token % 8 ||
+      ql_head % 8 || qp_token % 8 || qp_head % 8 || ql_token < 0 || ql_head < 0 || qp_token < 0 || qp_head < 0)
+    return KK3_ERR_ARG;
+  const int64_t need = kk3_cache_attend_workspace(a.c.batch, tokens, heads);
+  if (need == 0) return KK3_ERR_CUDA;
+  if (!cache_aligned(workspace, 16) || workspace_bytes < need) return KK3_ERR_ARG;
+  int sms = 0;
+  if (cache_sms(&sms)) return KK3_ERR_CUDA;
+  a.q_lat = (const bf16*)q_latent;
+  a.q_pe = (const bf16*)q_pe;
+  a.ql_tok = ql_token;
+  a.ql_head = ql_head;
+  a.qp_tok = qp_token;
+  a.qp_head = qp_head;
+  a.lengths = (const long long*)lengths;
+  a.cu_new = cu_new;
+  a.tokens = tokens;
+  a.heads = heads;
+  a.scale_log2 = scale * 1.4426950408889634f;
+  a.out = (bf16*)out;
+  a.lse = lse;
+  a.workers = sms;
+  a.meta = (int*)workspace;
+  a.part = (float*)((char*)workspace + (size_t)sms * 16);
+  int r = cache_cuda(cudaFuncSetAttribute(kk3_cache_attend_warp_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                          (int)sizeof(WaSmem)), "cudaFuncSetAttribute(kk3_cache_attend_warp_kernel)");
+  if (r) return r;
+  kk3_cache_attend_warp_kernel<<<sms, kWaThreads, sizeof(WaSmem), (cudaStream_t)stream>>>(a);
+  r = cache_cuda(cudaGetLastError(), "kk3_cache_attend_warp_kernel");
+  if (r) return r;
+  kk3_cache_join_kernel<<<dim3(sms, kWaRows), 512, 0, (cudaStream_t)stream>>>(a, kWaRows);
+  return cache_cuda(cudaGetLastError(), "kk3_cache_join_kernel");
+}
+
+extern "C" int kk3_cache_evict(const kk3_cache* cache, const int64_t* lengths, const float* mass, int64_t mass_stride,
+                               int budget, int sinks, int recent, const int32_t* dst_table, int64_t dst_stride,
+                               int dst_columns, int64_t* new_lengths, float* new_mass, int32_t* kept, int* error_word,
+                               void* stream) {
+  EvictArgs a;
+  const int rc = cache_pages(cache, &a.c, error_word);
+  if (rc) return rc;
+  if (!cache_aligned(lengths, 8) || !cache_aligned(mass, 4) || mass_stride < 0 || budget < 1 || sinks < 0 || recent < 0 ||
+      (int64_t)sinks + recent > budget || !cache_aligned(new_lengths, 8) || !cache_aligned(new_mass, 4) || !cache_aligned(kept, 4) ||
+      lengths == new_lengths || mass == new_mass)
+    return KK3_ERR_ARG;
+  const int64_t cap = (int64_t)cache->columns * cache->page_size;
+  if (budget > cap) return KK3_ERR_ARG;
+  if (dst_table && (((uintptr_t)dst_table % 4) || dst_stride < 0 || (int64_t)dst_columns * cache->page_size < budget))
+    return KK3_ERR_ARG;
+  a.lengths = (const long long*)lengths;
+  a.mass = mass;
+  a.mass_row = mass_stride;
+  a.budget = budget;
+  a.sinks = sinks;
+  a.recent = recent;
+  a.dst = dst_table;
+  a.dst_row = dst_stride;
+  a.dst_columns = dst_columns;
+  a.new_lengths = (long long*)new_lengths;
+  a.new_mass = new_mass;
+  a.kept = kept;
+  const cudaStream_t st = (cudaStream_t)stream;
+  kk3_cache_select_kernel<<<a.c.batch, kEvThreads, 0, st>>>(a);
+  int r = cache_cuda(cudaGetLastError(), "kk3_cache_select_kernel");
+  if (r) return r;
+  if (dst_table) {
+    kk3_cache_move_kernel<<<dim3((budget + kMoveWarps - 1) / kMoveWarps, a.c.batch), kMoveWarps * 32, 0, st>>>(a);
+    return cache_cuda(cudaGetLastError(), "kk3_cache_move_kernel");
+  }
+  kk3_cache_slide_kernel<<<dim3(kEntry / 32, a.c.batch), kSlideThreads, 0, st>>>(a);
+  return cache_cuda(cudaGetLastError(), "kk3_cache_slide_kernel");
+}
