@@ -174,7 +174,8 @@ int kk3_step_noalloc(const kk3_config* cfg, const void* const* table, int table_
  * A sequence's position p is slot p % page_size of page table[b][p / page_size]. cu_new [batch + 1] gives the packed
  * rows of each sequence's new tokens: cu_new[b] .. cu_new[b + 1], ascending from 0; rows at or behind cu_new[batch]
  * belong to no one and their outputs are left as they are. `lengths` are int64 as kk3_step_append's. All pointers are
- * device pointers on the current device, entries 16-byte aligned, strides in elements and multiples of 8. Calls
+ * device pointers on the current device, entries 16-byte aligned, strides in elements and multiples of 8, a page's
+ * stride a multiple of its row's. Calls
  * enqueue kernels on `stream` and return; nothing is allocated or read back, so they can be captured. A table entry
  * outside the pool or a length outside [0, columns * page_size] is clamped (the position reads as zeros and is not
  * written) and sets *error_word (optional, zeroed by the caller) to a nonzero device code. What pages hold at or
@@ -201,8 +202,8 @@ int kk3_cache_append(const kk3_cache* cache, const void* raw, int64_t raw_stride
  * (already appended): token i of n sees the first lengths[b] - n + i + 1 positions. Per token and head
  *   s_p = scale * (q_latent . c_p + q_pe . r_p),  out = sum_p softmax(s)_p c_p  (bf16 [tokens, heads, 512]),
  *   lse = log sum_p exp(s_p)  (f32 [tokens, heads]).
- * A token that sees nothing gets out = 0 and lse = -infinity. Queries: bf16, last dim contiguous, strides per token
- * and head. Sums and softmax statistics are FP32, probabilities are rounded to bf16 for the second product. The
+ * A token that sees nothing gets out = 0 and lse = -infinity. Queries: bf16, last dim contiguous, all (token,
+ * head) rows at one pitch: the token stride is heads times the head stride (KK3_ERR_UNSUPPORTED otherwise). Sums and softmax statistics are FP32, probabilities are rounded to bf16 for the second product. The
  * positions that a sequence holds must be finite for its tokens' results to be. workspace: 16-byte aligned,
  * kk3_cache_attend_workspace bytes (0: bad arguments or no device), used until the call's kernels end: calls that may
  * overlap need one each. Results do not depend on the order in which CTAs run. */

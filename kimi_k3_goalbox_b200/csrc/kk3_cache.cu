@@ -333,6 +333,7 @@ __global__ void __launch_bounds__(kWaThreads, 1) kk3_cache_attend_warp_kernel(co
 // sums each, so that the loads of many short pieces are in flight together.
 __global__ void __launch_bounds__(512) kk3_cache_join_kernel(const AttendArgs a, int tile_rows) {
   const int worker = blockIdx.x, row = blockIdx.y;
+  cache_follow();
   const int n = a.meta[worker * 4 + 2];
   if (n == 0) return;
   const int b = a.meta[worker * 4], t = a.meta[worker * 4 + 1];
@@ -518,6 +519,7 @@ __global__ void __launch_bounds__(kMoveWarps * 32) kk3_cache_move_kernel(const E
   const int b = blockIdx.y, lane = threadIdx.x & 31;
   const int j = blockIdx.x * kMoveWarps + (threadIdx.x >> 5);
   if (j >= a.budget) return;
+  cache_follow();
   const int from = a.kept[(long long)b * a.budget + j];
   if (from < 0) return;
   CachePages d = a.c;
@@ -545,6 +547,7 @@ constexpr int kSlideThreads = 512;
 constexpr int kSlideDeep = 8;    // rows in flight per thread: 1024 rows a batch
 __global__ void __launch_bounds__(kSlideThreads) kk3_cache_slide_kernel(const EvictArgs a) {
   const int b = blockIdx.y, ch = blockIdx.x * 4 + (threadIdx.x & 3);   // 16-byte piece of the entry: 0 .. 71
+  cache_follow();
   const int keep = (int)a.new_lengths[b];
   const int* kept = a.kept + (long long)b * a.budget;
   constexpr int kRows = kSlideThreads / 4;
@@ -627,10 +630,14 @@ int cache_pages(const kk3_cache* c, CachePages* out, int* error_word) {
 }
 
 int cache_sms(int* sms) {
+  static std::atomic<int> known[kCacheMaxDevices];
   int dev = 0;
   int rc = cache_cuda(cudaGetDevice(&dev), "cudaGetDevice");
   if (rc) return rc;
-  return cache_cuda(cudaDeviceGetAttribute(sms, cudaDevAttrMultiProcessorCount, dev), "cudaDeviceGetAttribute");
+  if (dev < kCacheMaxDevices && (*sms = known[dev].load(std::memory_order_relaxed)) > 0) return KK3_OK;
+  rc = cache_cuda(cudaDeviceGetAttribute(sms, cudaDevAttrMultiProcessorCount, dev), "cudaDeviceGetAttribute");
+  if (rc == KK3_OK && dev < kCacheMaxDevices) known[dev].store(*sms, std::memory_order_relaxed);
+  return rc;
 }
 
 }  // namespace kk3
@@ -699,14 +706,13 @@ extern "C" int kk3_cache_attend(const kk3_cache* cache, const void* q_latent, in
   a.workers = sms;
   a.meta = (int*)workspace;
   a.part = (float*)((char*)workspace + (size_t)sms * 16);
-  int r = cache_cuda(cudaFuncSetAttribute(kk3_cache_attend_warp_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                          (int)sizeof(WaSmem)), "cudaFuncSetAttribute(kk3_cache_attend_warp_kernel)");
+  static std::atomic<bool> done[kCacheMaxDevices];
+  int r = cache_allow_smem(kk3_cache_attend_warp_kernel, sizeof(WaSmem), done, "cudaFuncSetAttribute(kk3_cache_attend_warp_kernel)");
   if (r) return r;
   kk3_cache_attend_warp_kernel<<<sms, kWaThreads, sizeof(WaSmem), (cudaStream_t)stream>>>(a);
   r = cache_cuda(cudaGetLastError(), "kk3_cache_attend_warp_kernel");
   if (r) return r;
-  kk3_cache_join_kernel<<<dim3(sms, kWaRows), 512, 0, (cudaStream_t)stream>>>(a, kWaRows);
-  return cache_cuda(cudaGetLastError(), "kk3_cache_join_kernel");
+  return cache_launch_after(kk3_cache_join_kernel, dim3(sms, kWaRows), 512, (cudaStream_t)stream, "kk3_cache_join_kernel", a, kWaRows);
 }
 
 extern "C" int kk3_cache_evict(const kk3_cache* cache, const int64_t* lengths, const float* mass, int64_t mass_stride,
@@ -741,9 +747,9 @@ extern "C" int kk3_cache_evict(const kk3_cache* cache, const int64_t* lengths, c
   int r = cache_cuda(cudaGetLastError(), "kk3_cache_select_kernel");
   if (r) return r;
   if (dst_table) {
-    kk3_cache_move_kernel<<<dim3((budget + kMoveWarps - 1) / kMoveWarps, a.c.batch), kMoveWarps * 32, 0, st>>>(a);
-    return cache_cuda(cudaGetLastError(), "kk3_cache_move_kernel");
+    return cache_launch_after(kk3_cache_move_kernel, dim3((budget + kMoveWarps - 1) / kMoveWarps, a.c.batch),
+                              kMoveWarps * 32, st, "kk3_cache_move_kernel", a);
   }
-  kk3_cache_slide_kernel<<<dim3(kEntry / 32, a.c.batch), kSlideThreads, 0, st>>>(a);
-  return cache_cuda(cudaGetLastError(), "kk3_cache_slide_kernel");
+  return cache_launch_after(kk3_cache_slide_kernel, dim3(kEntry / 32, a.c.batch), kSlideThreads, st,
+                            "kk3_cache_slide_kernel", a);
 }

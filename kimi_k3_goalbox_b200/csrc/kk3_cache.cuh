@@ -54,6 +54,9 @@ KK3_DEV int page_at(const CachePages& c, int b, int pos, int* slot) {
   return page;
 }
 
+// Wait for the kernel before this one on the stream (cache_launch_after) and see what it wrote.
+KK3_DEV void cache_follow() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 // A sequence of one call: its rows in the packed token arrays and its cached positions (new ones included).
 struct Seq {
   int q0, n, len;

@@ -4,6 +4,8 @@
 #include <cuda_runtime.h>
 #include <stdio.h>
 
+#include <atomic>
+
 #include "kk3_cache.cuh"
 
 namespace kk3 {
@@ -14,7 +16,37 @@ int cache_cuda(cudaError_t e, const char* what);
 inline bool cache_aligned(const void* p, size_t n) { return p && (uintptr_t)p % n == 0; }
 // checks a kk3_cache and turns it into the kernels' form
 int cache_pages(const kk3_cache* c, CachePages* out, int* error_word);
-// SMs of the current device
+// SMs of the current device, looked up once per device
 int cache_sms(int* sms);
+
+// Allow `kernel` its dynamic shared memory on the current device, once per device (`done`: a zeroed array of
+// kCacheMaxDevices flags that belongs to the kernel; setting an attribute twice does no harm).
+constexpr int kCacheMaxDevices = 64;
+template <class K>
+int cache_allow_smem(K kernel, size_t bytes, std::atomic<bool>* done, const char* what) {
+  int dev = 0;
+  int rc = cache_cuda(cudaGetDevice(&dev), "cudaGetDevice");
+  if (rc) return rc;
+  if (dev < kCacheMaxDevices && done[dev].load(std::memory_order_acquire)) return KK3_OK;
+  rc = cache_cuda(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes), what);
+  if (rc == KK3_OK && dev < kCacheMaxDevices) done[dev].store(true, std::memory_order_release);
+  return rc;
+}
+
+// Launch a kernel that follows another of the same call on the stream: its launch overlaps the end of the one
+// before, and it begins with cache_follow().
+template <class K, class... Args>
+int cache_launch_after(K kernel, dim3 grid, int threads, cudaStream_t st, const char* what, const Args&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.stream = st;
+  cudaLaunchAttribute at = {};
+  at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &at;
+  cfg.numAttrs = 1;
+  return cache_cuda(cudaLaunchKernelEx(&cfg, kernel, args...), what);
+}
 
 }  // namespace kk3

@@ -1,9 +1,16 @@
-// kk3_cache_tc.cu - tensor-core kernels of the paged latent cache (tcgen05, sm_100a): the accumulated attention weight.
+// kk3_cache_tc.cu - tensor-core kernels of the paged latent cache (tcgen05 on CTA pairs, sm_100a): the accumulated
+// attention weight.
 //
-// Operands are gathered row by row through the page table with 16-byte cp.async (any page size; rows behind a
-// sequence's end arrive as zeros, whatever their page holds) straight into the 128-byte swizzled form that the
-// matrix instructions read, in blocks of 64 dims (128 bytes a row).
+// Operands come through the page table by TMA, in blocks of 64 dims in the 128-byte swizzled form that the matrix
+// instructions read: boxes of as many rows as divide a page and a tile, or gathers of four rows where that is below
+// eight (odd page sizes) and where rows behind a sequence's end have to arrive as zeros. A gather costs its issuing
+// warp as much as a box of any size (about 100 clocks), so boxes carry the bulk. Two CTAs of a cluster work as one
+// (cta_group::2): each loads half of the second operand, which halves the shared-memory reads per matrix instruction,
+// the bound of these shapes at 128 bytes a clock.
+#include <cuda.h>
 #include <cuda_runtime.h>
+#include <cudaTypedefs.h>
+#include <string.h>
 
 #include "kk3_cache.cuh"
 #include "kk3_cache_host.h"
@@ -14,14 +21,50 @@ namespace kk3 {
 constexpr int kBlocks = kEntry / 64;                    // 64-dim blocks of an entry
 constexpr unsigned long long kWaitNs = 2000000000ull;   // bound of every wait; a healthy one takes microseconds
 
-KK3_DEV unsigned smem_u32(const void* p) { return (unsigned)__cvta_generic_to_shared(p); }
+// The tensors of a call: cached entries in boxes of `box` rows and row by row, query rows in boxes. Cached rows are
+// numbered page * ratio + slot, query rows token * heads + head.
+struct PairMaps {
+  CUtensorMap kv_box, pe_box, kv_row, pe_row, ql, qp;
+};
+struct PairRows {
+  int kv_ratio, pe_ratio;   // rows from one page to the next
+  int kv_end, pe_end;       // number of the first row behind the pool: reads as zeros
+  int box;                  // rows of a box: divides a page and 64, 8 at least; 0: gathers only
+};
 
+KK3_DEV unsigned smem_u32(const void* p) { return (unsigned)__cvta_generic_to_shared(p); }
+KK3_DEV unsigned cluster_rank() {
+  unsigned r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+// shared::cluster address of `addr` in CTA `rank` of the cluster
+KK3_DEV unsigned in_cta(unsigned addr, unsigned rank) {
+  unsigned r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+  return r;
+}
+KK3_DEV void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+KK3_DEV void arrive_cluster(unsigned addr) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(addr) : "memory");
+}
+KK3_DEV bool pair_test(unsigned bar, unsigned parity) {
+  unsigned ok;
+  asm volatile(
+      "{\n .reg .pred p;\n mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n"
+      " selp.u32 %0, 1, 0, p;\n}"
+      : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+  return ok != 0;
+}
 // Bounded wait; false when it ran out or another role of the CTA gave up (*dead).
-KK3_DEV bool bar_wait(const CachePages& c, unsigned bar, unsigned parity, volatile int* dead) {
-  if (mbar_test(bar, parity)) return true;
+KK3_DEV bool pair_wait(const CachePages& c, unsigned bar, unsigned parity, volatile int* dead) {
+  if (pair_test(bar, parity)) return true;
+  if (*dead) return false;
   const unsigned long long t0 = globaltimer();
   for (unsigned spin = 1;; ++spin) {
-    if (mbar_test(bar, parity)) return true;
+    if (pair_test(bar, parity)) return true;
     if ((spin & 15) == 0) {
       if (*dead) return false;
       if (globaltimer() - t0 > kWaitNs) {
@@ -32,14 +75,40 @@ KK3_DEV bool bar_wait(const CachePages& c, unsigned bar, unsigned parity, volati
     }
   }
 }
-KK3_DEV void cp16(unsigned dst, const void* src, bool live) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(live ? 16 : 0) : "memory");
+// Rows row[0..3] of 64 elements from column x into 512 bytes of this CTA's shared memory; the bytes are counted on
+// `bar`, a barrier of either CTA of the pair.
+KK3_DEV void gather4(unsigned dst, const CUtensorMap* map, int x, const int (&row)[4], unsigned bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes.cta_group::2 [%0], "
+      "[%1, {%2, %3, %4, %5, %6}], [%7];"
+      ::"r"(dst), "l"(map), "r"(x), "r"(row[0]), "r"(row[1]), "r"(row[2]), "r"(row[3]), "r"(bar)
+      : "memory");
 }
-KK3_DEV void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-KK3_DEV void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
-// 16-byte piece `ch` of row `r` in a 128-byte swizzled block (1024-byte aligned)
-KK3_DEV unsigned sw128(int r, int ch) { return (unsigned)(r * 128 + ((ch ^ (r & 7)) << 4)); }
+// A box of the map's rows from `row` on, likewise.
+KK3_DEV void load_box(unsigned dst, const CUtensorMap* map, int x, int row, unsigned bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 [%0], "
+      "[%1, {%2, %3}], [%4];"
+      ::"r"(dst), "l"(map), "r"(x), "r"(row), "r"(bar)
+      : "memory");
+}
+KK3_DEV void pair_mma(unsigned d, unsigned long long a, unsigned long long b, unsigned idesc, unsigned accumulate) {
+  asm volatile(
+      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+      " tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n}"
+      ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+}
+// one arrival on `bar` of both CTAs when the matrix instructions issued so far are done
+KK3_DEV void pair_commit(unsigned bar) {
+  asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
+               ::"r"(bar), "h"((unsigned short)3) : "memory");
+}
+KK3_DEV void pair_alloc(unsigned dst, unsigned ncols) {
+  asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(dst), "r"(ncols) : "memory");
+}
+KK3_DEV void pair_dealloc(unsigned taddr, unsigned ncols) {
+  asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(ncols) : "memory");
+}
 KK3_DEV float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -61,89 +130,142 @@ KK3_DEV void tmem_ld32(unsigned taddr, float (&v)[32]) {
   for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
 }
 
+
+// instruction descriptor: kind::f16, D = F32, A = B = BF16, M rows and N columns over the pair, operands K-major
+KK3_DEV constexpr unsigned pair_idesc(int m, int n) {
+  return (1u << 4) | (1u << 7) | (1u << 10) | ((unsigned)(n >> 3) << 17) | ((unsigned)(m >> 4) << 24);
+}
+
+// row numbers of the cached position `pos` of sequence `b`; at or behind `end`, or without a page: past the pool
+KK3_DEV void entry_row(const CachePages& c, const PairRows& pr, int b, int pos, int end, int* kv, int* pe) {
+  *kv = pr.kv_end;
+  *pe = pr.pe_end;
+  if (pos < end) {
+    int slot;
+    const int page = page_at(c, b, pos, &slot);
+    if (page >= 0) {
+      *kv = page * pr.kv_ratio + slot;
+      *pe = page * pr.pe_ratio + slot;
+    }
+  }
+}
+// A warp's part in loading `count` (64 or 128) cached positions from `pos` on: the row of a lane's box or gather.
+struct EntryRows {
+  int kv[4], pe[4];
+  KK3_DEV void find(const CachePages& c, const PairRows& pr, int b, int pos, int count, int end) {
+    const int lane = threadIdx.x & 31;
+    if (pr.box) {
+      if (lane * pr.box < count) entry_row(c, pr, b, pos + lane * pr.box, end, &kv[0], &pe[0]);
+    } else if (lane * 4 < count) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) entry_row(c, pr, b, pos + lane * 4 + i, end, &kv[i], &pe[i]);
+    }
+  }
+  // 64-dim block `d` of the positions into [count][64] at `dst`
+  KK3_DEV void load(const PairMaps& m, const PairRows& pr, int d, int count, unsigned dst, unsigned bar) const {
+    const int lane = threadIdx.x & 31;
+    if (pr.box) {
+      if (lane * pr.box < count) {
+        if (d < kBlocks - 1) load_box(dst + lane * pr.box * 128, &m.kv_box, d * 64, kv[0], bar);
+        else load_box(dst + lane * pr.box * 128, &m.pe_box, 0, pe[0], bar);
+      }
+    } else if (lane * 4 < count) {
+      if (d < kBlocks - 1) gather4(dst + lane * 512, &m.kv_row, d * 64, kv, bar);
+      else gather4(dst + lane * 512, &m.pe_row, 0, pe, bar);
+    }
+  }
+};
+
 // ---------------------------------------------------------------------------------------------
 // Attention weight of cached positions: w_p = sum over rows of 2^(s_p - lse), s_p = q . e_p.
 //
-// One product, positions x rows, with the positions as the 128 rows of the matrix instruction: a thread then owns a
-// position (its TMEM lane) and adds up its columns in registers, in row order; no reduction crosses threads and
-// no atomic is needed. A tile is 128 positions: its 147 KB stay in shared memory while the sequence's rows pass
-// through a ring in units of NR rows x 576 dims; two accumulators let the sums of one unit run under the products
-// of the next. When the rows fit one unit (single tokens) the tile's blocks are freed block by block instead and
-// the kernel streams the cache: LAG blocks of 16 KB are in flight.
+// One product, positions x rows, with the positions as the 256 rows of the pair's matrix instruction: a thread then
+// owns a position (its TMEM lane) and adds up its columns in registers, in row order; no reduction crosses threads
+// and no atomic is needed. A tile is 256 positions, 147 KB in each CTA, that stay in shared memory while the
+// sequence's rows pass through a ring in units of `rows` x 576 dims, half of them in each CTA; two accumulators let
+// the sums of one unit run under the products of the next. Where the rows fit one unit (single tokens) the tile's
+// blocks are freed one by one instead, and the kernel streams the cache with up to 147 KB in flight in each SM.
 //
-// Bounds, per unit of 128 x 128 x 576: shared memory feeds the instructions 295 KB, 2304 clocks at 128 bytes a
-// clock, against 1152 clocks of tensor time; exponentials take 1024.
+// Bounds of a unit of 256 rows: 2304 clocks of tensor time, as many of shared-memory reads (8 KB per 64-clock
+// instruction), and 2048 of exponentials (16 a clock).
 
-constexpr int kMassPos = 128;
-constexpr int kMassThreads = 288;   // warps 0-3 sums, 4-7 copies, 8 matrix instructions and TMEM
-constexpr int kMassKBlock = kMassPos * 128;
+constexpr int kMassPos = 256;
+constexpr int kMassThreads = 320;   // warps 0-7 sums, 8 copies, 9 matrix instructions and TMEM
+constexpr int kMassKBlock = 128 * 128;
 constexpr int kMassRing = 65536;
-
-template <int NR>
-struct MassLayout {
-  static constexpr int kSlotBytes = NR * 128;
-  static constexpr int kSlots = kMassRing / kSlotBytes < 16 ? kMassRing / kSlotBytes : 16;
-  static constexpr int kLag = kSlots - 1 < kBlocks - 1 ? kSlots - 1 : kBlocks - 1;   // groups in flight behind the newest
-  static constexpr int kCtl = kBlocks * kMassKBlock + kSlots * kSlotBytes;           // byte offset of the control block
-};
+constexpr int kMassSlots = 16;
 struct MassCtl {
-  unsigned long long full[16], empty[16], kempty[kBlocks], dfull[2], dempty[2], done;
+  unsigned long long full[kMassSlots], empty[kMassSlots], kempty[kBlocks], dfull[2], dempty[2], done;
   unsigned tmem;
   int dead;
   long long red[kMassThreads / 32 + 4];
-  float lse[2][128];
-  int sees[2][128];
+  alignas(16) float lse[2][256];   // read four at a time
+  alignas(16) int sees[2][256];
+  float sum[128];
 };
+constexpr int kMassSmem = kBlocks * kMassKBlock + kMassRing + (int)sizeof(MassCtl) + 1024;
+static_assert(kMassSmem <= 232448, "shared memory of a CTA");
 
-template <int NR>
-__global__ void __launch_bounds__(kMassThreads, 1) kk3_cache_mass_kernel(const MassArgs a) {
-  using L = MassLayout<NR>;
+// What the call leaves as it is: positions behind the sequences' ends, and sequences without new tokens. The CTAs are
+// dealt out to the sequences; `threads` threads of each take part.
+KK3_DEV void mass_rest(const MassArgs& a, int tid, int threads) {
+  const long long cap = (long long)a.c.columns * a.c.page_size;
+  const int per = max(1, (int)gridDim.x / a.c.batch), groups = gridDim.x / per;
+  if ((int)blockIdx.x >= groups * per) return;
+  for (int b = blockIdx.x / per; b < a.c.batch; b += groups) {
+    const Seq s = a.seq(b);
+    const float* from = a.mass ? a.mass + b * a.mass_row : nullptr;
+#pragma unroll 4
+    for (long long p = (s.n > 0 ? s.len : 0) + (int)(blockIdx.x % per) * threads + tid; p < cap; p += per * threads)
+      a.out[b * cap + p] = from ? from[p] : 0.0f;
+  }
+}
+
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMassThreads, 1)
+    kk3_cache_mass_kernel(const MassArgs a, const PairRows pr, const __grid_constant__ PairMaps maps, int rows) {
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   unsigned char* base = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
-  MassCtl& ctl = *reinterpret_cast<MassCtl*>(base + L::kCtl);
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, worker = blockIdx.x;
+  MassCtl& ctl = *reinterpret_cast<MassCtl*>(base + kBlocks * kMassKBlock + kMassRing);
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, worker = blockIdx.x >> 1;
+  const unsigned rank = cluster_rank();
   const unsigned kbase = smem_u32(base), qbase = kbase + kBlocks * kMassKBlock;
-  const MassSplit split{kMassPos, NR, a.heads};
+  const int half = rows / 2, slot_bytes = half * 128, slots = min(kMassSlots, kMassRing / slot_bytes);
+  const MassSplit split{kMassPos, rows, a.heads};
   const Share sh = plan_share<kMassThreads>(a, split, worker, 1, reinterpret_cast<int*>(base), ctl.red);
-  if (tid == 0) a.meta[worker * 4 + 2] = 0;
-  // what the call leaves as it is: positions behind the sequences' ends, and sequences without new tokens
-  {
-    const long long cap = (long long)a.c.columns * a.c.page_size;
-    for (int b = worker; b < a.c.batch; b += gridDim.x) {
-      const Seq s = a.seq(b);
-      for (long long p = (s.n > 0 ? s.len : 0) + tid; p < cap; p += kMassThreads)
-        a.out[b * cap + p] = a.mass ? a.mass[b * a.mass_row + p] : 0.0f;
-    }
+  if (tid == 0 && rank == 0) a.meta[worker * 4 + 2] = 0;
+  if (worker >= sh.workers) {   // both CTAs of the pair
+    mass_rest(a, tid, kMassThreads);
+    return;
   }
-  if (worker >= sh.workers || sh.total == 0) return;
   const unsigned full = smem_u32(ctl.full), empty = smem_u32(ctl.empty), kempty = smem_u32(ctl.kempty),
                  dfull = smem_u32(ctl.dfull), dempty = smem_u32(ctl.dempty), done = smem_u32(&ctl.done);
   volatile int* dead = &ctl.dead;
   if (tid == 0) {
-    for (int i = 0; i < L::kSlots; ++i) {
-      mbar_init(full + 8 * i, 4);
+    for (int i = 0; i < kMassSlots; ++i) {
+      mbar_init(full + 8 * i, 1);
       mbar_init(empty + 8 * i, 1);
     }
     for (int i = 0; i < kBlocks; ++i) mbar_init(kempty + 8 * i, 1);
     for (int i = 0; i < 2; ++i) {
       mbar_init(dfull + 8 * i, 1);
-      mbar_init(dempty + 8 * i, 4);
+      mbar_init(dempty + 8 * i, 16);   // eight warps of either CTA
     }
     mbar_init(done, 1);
     ctl.dead = 0;
     fence_mbar_init();
   }
-  if (warp == 8) tmem_alloc(smem_u32(&ctl.tmem), 2 * NR);
+  if (warp == 9) pair_alloc(smem_u32(&ctl.tmem), 512);
   tc_fence_before();
   __syncthreads();
+  cluster_sync();
   tc_fence_after();
   const unsigned tmem = *reinterpret_cast<volatile unsigned*>(&ctl.tmem);
 
   int b = sh.b, t = sh.t;
   long long at = sh.at;
-  if (warp >= 4 && warp < 8) {
+  if (warp == 8) {
     // ---- copies
-    const int pw = warp - 4, sub = lane >> 3, ch = lane & 7;
+    const unsigned lead_full = in_cta(full, 0);
     int job = 0, tile = 0;
     bool ok = true;
     while (ok && at < sh.end) {
@@ -151,76 +273,41 @@ __global__ void __launch_bounds__(kMassThreads, 1) kk3_cache_mass_kernel(const M
       for (; t >= split.tiles(s); t = 0) s = a.seq(++b);
       const int units = split.units(s, t), first = split.first_unit(s, t);
       const int u0 = (int)max(0ll, sh.begin - at), u1 = (int)min((long long)units, sh.end - at);
-      long long koff[8], poff[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int pos = t * kMassPos + pw * 32 + i * 4 + sub;
-        koff[i] = poff[i] = -1;
-        if (pos < s.len) {
-          int slot;
-          const int page = page_at(a.c, b, pos, &slot);
-          if (page >= 0) {
-            koff[i] = (long long)page * a.c.kv_page + (long long)slot * a.c.kv_row + ch * 8;
-            poff[i] = (long long)page * a.c.pe_page + (long long)slot * a.c.pe_row + ch * 8;
-          }
-        }
-      }
+      EntryRows er;
+      er.find(a.c, pr, b, t * kMassPos + (int)rank * 128, 128, s.len);
       for (int u = u0; ok && u < u1; ++u) {
-        long long qoff[NR / 16], roff[NR / 16];
-#pragma unroll
-        for (int i = 0; i < NR / 16; ++i) {
-          const long long g = (long long)(first + u) * NR + pw * (NR / 4) + i * 4 + sub;
-          qoff[i] = roff[i] = -1;
-          if (g < (long long)s.n * a.heads) {
-            const int tok = s.q0 + (int)(g / a.heads), head = (int)(g % a.heads);
-            qoff[i] = tok * a.ql_tok + head * a.ql_head + ch * 8;
-            roff[i] = tok * a.qp_tok + head * a.qp_head + ch * 8;
-          }
-        }
-        for (int d = 0; d < kBlocks; ++d) {
-          const int slot = job % L::kSlots;
-          ok = bar_wait(a.c, empty + 8 * slot, ((job / L::kSlots) & 1) ^ 1, dead);
-          if (ok && u == u0) ok = bar_wait(a.c, kempty + 8 * d, (tile & 1) ^ 1, dead);
+        const int q = s.q0 * a.heads + (first + u) * rows + (int)rank * half;   // rows behind the sequence's: masked
+        for (int d = 0; d < kBlocks; ++d, ++job) {
+          const int slot = job % slots;
+          const unsigned bar = lead_full + 8 * slot;
+          ok = pair_wait(a.c, empty + 8 * slot, ((job / slots) & 1) ^ 1, dead);
+          if (ok && u == u0) ok = pair_wait(a.c, kempty + 8 * d, (tile & 1) ^ 1, dead);
+          ok = __all_sync(0xffffffffu, ok);
           if (!ok) break;
-          if (u == u0) {
-            const unsigned dst = kbase + d * kMassKBlock;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              const long long o = d < kBlocks - 1 ? koff[i] : poff[i];
-              const bf16* src = d < kBlocks - 1 ? a.c.kv + o + d * 64 : a.c.pe + o;
-              cp16(dst + sw128(pw * 32 + i * 4 + sub, ch), o >= 0 ? src : a.c.kv, o >= 0);
-            }
+          if (rank == 0 && lane == 0)
+            mbar_arrive_tx(full + 8 * slot, 2 * (slot_bytes + (u == u0 ? kMassKBlock : 0)));
+          __syncwarp();
+          if (u == u0) er.load(maps, pr, d, 128, kbase + d * kMassKBlock, bar);
+          if (lane == 0) {
+            const unsigned qd = qbase + slot * slot_bytes;
+            if (d < kBlocks - 1) load_box(qd, &maps.ql, d * 64, q, bar);
+            else load_box(qd, &maps.qp, 0, q, bar);
           }
-          const unsigned dst = qbase + slot * L::kSlotBytes;
-#pragma unroll
-          for (int i = 0; i < NR / 16; ++i) {
-            const long long o = d < kBlocks - 1 ? qoff[i] : roff[i];
-            const bf16* src = d < kBlocks - 1 ? a.q_lat + o + d * 64 : a.q_pe + o;
-            cp16(dst + sw128(pw * (NR / 4) + i * 4 + sub, ch), o >= 0 ? src : a.q_lat, o >= 0);
-          }
-          cp_commit();
-          if (job >= L::kLag) {
-            cp_wait<L::kLag>();
-            fence_async_smem();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(full + 8 * ((job - L::kLag) % L::kSlots));
-          }
-          ++job;
         }
       }
       at += units;
       ++t;
       ++tile;
     }
-    cp_wait<0>();
-    fence_async_smem();
+    // the last copies have landed before the CTA can leave: their consumers waited for them, or (after a failed
+    // wait) the slots' barriers are given a bounded time here
+    if (!ok && rank == 0 && lane == 0)
+      for (int j = max(0, job - slots); j < job; ++j) mbar_wait_for(full + 8 * (j % slots), (j / slots) & 1, kWaitNs);
     __syncwarp();
-    if (lane == 0)
-      for (int j = max(0, job - L::kLag); j < job; ++j) mbar_arrive(full + 8 * (j % L::kSlots));
-  } else if (warp == 8) {
-    // ---- matrix instructions (one thread)
-    if (lane == 0) {
-      constexpr unsigned idesc = (1u << 4) | (1u << 7) | (1u << 10) | ((unsigned)(NR >> 3) << 17) | ((128u >> 4) << 24);
+  } else if (warp == 9) {
+    // ---- matrix instructions: one thread of the pair
+    if (lane == 0 && rank == 0) {
+      const unsigned idesc = pair_idesc(256, rows);
       int job = 0, unit = 0;
       bool ok = true;
       while (ok && at < sh.end) {
@@ -230,96 +317,104 @@ __global__ void __launch_bounds__(kMassThreads, 1) kk3_cache_mass_kernel(const M
         const int u0 = (int)max(0ll, sh.begin - at), u1 = (int)min((long long)units, sh.end - at);
         for (int u = u0; ok && u < u1; ++u, ++unit) {
           const int buf = unit & 1;
-          ok = bar_wait(a.c, dempty + 8 * buf, ((unit >> 1) & 1) ^ 1, dead);
+          ok = pair_wait(a.c, dempty + 8 * buf, ((unit >> 1) & 1) ^ 1, dead);
           tc_fence_after();
           for (int d = 0; ok && d < kBlocks; ++d, ++job) {
-            const int slot = job % L::kSlots;
-            ok = bar_wait(a.c, full + 8 * slot, (job / L::kSlots) & 1, dead);
+            const int slot = job % slots;
+            ok = pair_wait(a.c, full + 8 * slot, (job / slots) & 1, dead);
             if (!ok) break;
             tc_fence_after();
-            const unsigned ka = kbase + d * kMassKBlock, qa = qbase + slot * L::kSlotBytes;
+            const unsigned ka = kbase + d * kMassKBlock, qa = qbase + slot * slot_bytes;
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              asm volatile(
-                  "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-                  " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}"
-                  ::"r"(tmem + buf * NR), "l"(sdesc_sw128(ka + k * 32)), "l"(sdesc_sw128(qa + k * 32)), "r"(idesc),
-                    "r"((unsigned)(d | k))
-                  : "memory");
-            }
-            umma_commit(empty + 8 * slot);
-            if (u == u1 - 1) umma_commit(kempty + 8 * d);
+            for (int k = 0; k < 4; ++k)
+              pair_mma(tmem + buf * 256, sdesc_sw128(ka + k * 32), sdesc_sw128(qa + k * 32), idesc, (unsigned)(d | k));
+            pair_commit(empty + 8 * slot);
+            if (u == u1 - 1) pair_commit(kempty + 8 * d);
           }
-          if (ok) umma_commit(dfull + 8 * buf);
+          if (ok) pair_commit(dfull + 8 * buf);
         }
         at += units;
         ++t;
       }
-      umma_commit(done);   // all matrix instructions end before TMEM is given back
+      pair_commit(done);   // all matrix instructions end before TMEM is given back
       mbar_wait_for(done, 0, kWaitNs);
     }
     __syncwarp();
   } else {
-    // ---- sums: thread = position
-    const unsigned tlane = (unsigned)(warp * 32) << 16;
+    // ---- sums: thread = position; warps 0-3 take the first half of the columns, warps 4-7 the second
+    mass_rest(a, tid, 256);
+    const unsigned tlane = (unsigned)((warp & 3) * 32) << 16, lead_dempty = in_cta(dempty, 0);
+    const int group = warp >> 2, row = tid & 127;
     int unit = 0;
     bool ok = true;
-    while (ok && at < sh.end) {
+    while (at < sh.end) {   // after a failed wait the rounds go on without work: the warps meet at barriers
       Seq s = a.seq(b);
       for (; t >= split.tiles(s); t = 0) s = a.seq(++b);
       const int units = split.units(s, t), first = split.first_unit(s, t);
       const int u0 = (int)max(0ll, sh.begin - at), u1 = (int)min((long long)units, sh.end - at);
-      const int pos = t * kMassPos + tid;
-      float sum = 0.0f;
-      for (int u = u0; ok && u < u1; ++u, ++unit) {
+      const int pos = t * kMassPos + (int)rank * 128 + row;
+      const long long all = (long long)s.n * a.heads;
+      // a thread fetches one row's log sum, one unit ahead (rows that do not exist or see nothing: -infinity)
+      const auto fetch = [&](int u) {
+        const long long g = (long long)(first + u) * rows + tid;
+        return tid < rows && u < u1 && g < all ? a.lse[(long long)s.q0 * a.heads + g] : -INFINITY;
+      };
+      float next = fetch(u0), sum = 0.0f;
+      for (int u = u0; u < u1; ++u, ++unit) {
         const int buf = unit & 1;
-        // this unit's rows: negative log sums (rows that do not exist or see nothing: the products vanish)
-        const long long g0 = (long long)(first + u) * NR, all = (long long)s.n * a.heads;
-        if (tid < NR) {
-          const long long g = g0 + tid;
-          const float l = g < all ? a.lse[(long long)s.q0 * a.heads + g] : -INFINITY;
-          ctl.lse[buf][tid] = l == -INFINITY ? -INFINITY : -l * 1.4426950408889634f;
-          ctl.sees[buf][tid] = g < all ? s.len - s.n + (int)(g / a.heads) + 1 : 0;
+        const long long g0 = (long long)(first + u) * rows;
+        if (tid < rows) {
+          ctl.lse[buf][tid] = next == -INFINITY ? -INFINITY : -next * 1.4426950408889634f;
+          ctl.sees[buf][tid] = g0 + tid < all ? s.len - s.n + (int)((g0 + tid) / a.heads) + 1 : 0;
         }
-        asm volatile("bar.sync 1, 128;" ::: "memory");
-        const bool causal = s.len - s.n + (int)(g0 / a.heads) + 1 < min(s.len, (t + 1) * kMassPos);
-        ok = bar_wait(a.c, dfull + 8 * buf, (unit >> 1) & 1, dead);
+        next = fetch(u + 1);
+        asm volatile("bar.sync 1, 256;" ::: "memory");
+        // rows that see not all of the tile, or are another sequence's or no one's: select
+        const bool causal = g0 + rows > all || s.len - s.n + (int)(g0 / a.heads) + 1 < min(s.len, (t + 1) * kMassPos);
+        ok = pair_wait(a.c, dfull + 8 * buf, (unit >> 1) & 1, dead) && ok;
+        ok = __all_sync(0xffffffffu, ok);
         tc_fence_after();
         if (ok) {
 #pragma unroll 1
-          for (int c = 0; c < NR; c += 32) {
+          for (int c = group * 32; c < rows; c += 64) {
             float v[32];
-            tmem_ld32(tmem + tlane + buf * NR + c, v);
+            tmem_ld32(tmem + tlane + buf * 256 + c, v);
             tmem_ld_wait();
-            float part = 0.0f;
+            float part[4] = {};
 #pragma unroll
             for (int i = 0; i < 32; i += 4) {
               const float4 l = *reinterpret_cast<const float4*>(&ctl.lse[buf][c + i]);
-              const float w0 = ex2(fmaf(v[i], a.scale_log2, l.x)), w1 = ex2(fmaf(v[i + 1], a.scale_log2, l.y));
-              const float w2 = ex2(fmaf(v[i + 2], a.scale_log2, l.z)), w3 = ex2(fmaf(v[i + 3], a.scale_log2, l.w));
+              float w[4] = {ex2(fmaf(v[i], a.scale_log2, l.x)), ex2(fmaf(v[i + 1], a.scale_log2, l.y)),
+                            ex2(fmaf(v[i + 2], a.scale_log2, l.z)), ex2(fmaf(v[i + 3], a.scale_log2, l.w))};
               if (causal) {
                 const int4 n = *reinterpret_cast<const int4*>(&ctl.sees[buf][c + i]);
-                part += (pos < n.x ? w0 : 0.0f) + (pos < n.y ? w1 : 0.0f) + (pos < n.z ? w2 : 0.0f) + (pos < n.w ? w3 : 0.0f);
-              } else {
-                part += (w0 + w1) + (w2 + w3);
+                w[0] = pos < n.x ? w[0] : 0.0f;
+                w[1] = pos < n.y ? w[1] : 0.0f;
+                w[2] = pos < n.z ? w[2] : 0.0f;
+                w[3] = pos < n.w ? w[3] : 0.0f;
               }
+#pragma unroll
+              for (int k = 0; k < 4; ++k) part[k] += w[k];
             }
-            sum += part;
+            sum += (part[0] + part[1]) + (part[2] + part[3]);
           }
         }
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(dempty + 8 * buf);
+        if (lane == 0) arrive_cluster(lead_dempty + 8 * buf);
       }
-      if (ok) {
+      if (group == 1) ctl.sum[row] = sum;
+      asm volatile("bar.sync 1, 256;" ::: "memory");
+      if (group == 0) sum += ctl.sum[row];
+      if (ok && group == 0) {
         if (u0 == 0 && u1 == units) {
           if (pos < s.len) {
             const long long cap = (long long)a.c.columns * a.c.page_size;
             a.out[b * cap + pos] = (a.mass ? a.mass[b * a.mass_row + pos] : 0.0f) + sum;
           }
         } else {
-          a.part[(worker * 2 + (u0 == 0 ? 1 : 0)) * kMassPos + tid] = sum;
-          if (u0 == 0 && tid == 0) {   // the workers of this tile: up to the one that holds its last unit
+          a.part[(worker * 2 + (u0 == 0 ? 1 : 0)) * kMassPos + rank * 128 + row] = sum;
+          if (u0 == 0 && tid == 0 && rank == 0) {   // the workers of this tile: up to the one that holds its last unit
             int last = worker;
             while (sh.total * (last + 1) / sh.workers < at + units) ++last;
             a.meta[worker * 4] = b;
@@ -334,31 +429,86 @@ __global__ void __launch_bounds__(kMassThreads, 1) kk3_cache_mass_kernel(const M
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 8) tmem_dealloc(tmem, 2 * NR);
+  cluster_sync();   // neither CTA gives up its memory while the other's instructions may use it
+  if (warp == 9) pair_dealloc(tmem, 512);
 }
 
 __global__ void __launch_bounds__(kMassPos) kk3_cache_mass_join_kernel(const MassArgs a) {
+  cache_follow();
   const int worker = blockIdx.x, n = a.meta[worker * 4 + 2];
   if (n == 0) return;
   const int b = a.meta[worker * 4], pos = a.meta[worker * 4 + 1] * kMassPos + threadIdx.x;
   if (pos >= a.seq(b).len) return;
   float sum = 0.0f;
+#pragma unroll 4
   for (int w = 0; w < n; ++w) sum += a.part[((worker + w) * 2 + (w == 0 ? 1 : 0)) * kMassPos + threadIdx.x];
   const long long cap = (long long)a.c.columns * a.c.page_size;
   a.out[b * cap + pos] = (a.mass ? a.mass[b * a.mass_row + pos] : 0.0f) + sum;
 }
 
-template <int NR>
-static int mass_launch(const MassArgs& a, cudaStream_t st) {
-  const size_t smem = MassLayout<NR>::kCtl + sizeof(MassCtl) + 1024;
-  int r = cache_cuda(cudaFuncSetAttribute(kk3_cache_mass_kernel<NR>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem),
-                     "cudaFuncSetAttribute(kk3_cache_mass_kernel)");
-  if (r) return r;
-  kk3_cache_mass_kernel<NR><<<a.workers, kMassThreads, smem, st>>>(a);
-  r = cache_cuda(cudaGetLastError(), "kk3_cache_mass_kernel");
-  if (r) return r;
-  kk3_cache_mass_join_kernel<<<a.workers, kMassPos, 0, st>>>(a);
-  return cache_cuda(cudaGetLastError(), "kk3_cache_mass_join_kernel");
+// ---------------------------------------------------------------------------------------------
+// host side
+
+static int encode_rows(CUtensorMap* map, const void* base, int cols, int64_t rows, int64_t pitch, int box) {
+  static std::atomic<PFN_cuTensorMapEncodeTiled_v12000> known{nullptr};
+  PFN_cuTensorMapEncodeTiled_v12000 fn = known.load(std::memory_order_acquire);
+  if (!fn) {
+    cudaDriverEntryPointQueryResult qr;
+    const int rc = cache_cuda(cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", (void**)&fn, cudaEnableDefault, &qr),
+                              "cudaGetDriverEntryPoint(cuTensorMapEncodeTiled)");
+    if (rc) return rc;
+    if (qr != cudaDriverEntryPointSuccess || !fn) return KK3_ERR_CUDA;
+    known.store(fn, std::memory_order_release);
+  }
+  const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)pitch * 2};
+  const cuuint32_t boxes[2] = {64, (cuuint32_t)box}, steps[2] = {1, 1};
+  const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(base), dims, strides, boxes, steps,
+                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? KK3_OK : KK3_ERR_ARG;
+}
+
+// maps of all the rows of a [pages, page_size, cols] tensor: in boxes and row by row
+static int map_pages(CUtensorMap* by_box, CUtensorMap* by_row, int* ratio, int* end, const void* base, int cols,
+                     const kk3_cache* c, int64_t page_stride, int64_t row_stride, int box) {
+  const int64_t pages = c->num_pages;
+  if (c->page_size == 1 && pages > 1) row_stride = page_stride;
+  const int64_t r = pages > 1 ? page_stride / row_stride : c->page_size, rows = (pages - 1) * r + c->page_size;
+  if (row_stride < cols || (pages > 1 && page_stride % row_stride) || rows >= INT32_MAX) return KK3_ERR_UNSUPPORTED;
+  *ratio = (int)r;
+  *end = (int)rows;
+  const int rc = encode_rows(by_row, base, cols, rows, row_stride, 1);
+  return rc || !box ? rc : encode_rows(by_box, base, cols, rows, row_stride, box);
+}
+
+// map of the rows of a [tokens, heads, cols] tensor whose (token, head) rows lie at one pitch
+static int map_queries(CUtensorMap* map, const void* base, int cols, int64_t tokens, int64_t heads, int64_t tok_stride,
+                       int64_t head_stride, int box) {
+  if (heads == 1) head_stride = tokens == 1 ? cols : tok_stride;
+  if (head_stride < cols || (tokens > 1 && tok_stride != heads * head_stride)) return KK3_ERR_UNSUPPORTED;
+  return encode_rows(map, base, cols, tokens * heads, head_stride, box);
+}
+
+static int pair_maps(const kk3_cache* c, const void* q_latent, int64_t ql_token, int64_t ql_head, const void* q_pe,
+                     int64_t qp_token, int64_t qp_head, int tokens, int heads, int q_box, PairMaps* m, PairRows* r) {
+  memset(m, 0, sizeof(*m));
+  r->box = 64;
+  while (c->page_size % r->box) r->box /= 2;
+  if (r->box < 8) r->box = 0;
+  int rc = map_pages(&m->kv_box, &m->kv_row, &r->kv_ratio, &r->kv_end, c->kv, kLat, c, c->kv_page_stride, c->kv_row_stride, r->box);
+  if (!rc) rc = map_pages(&m->pe_box, &m->pe_row, &r->pe_ratio, &r->pe_end, c->pe, kRope, c, c->pe_page_stride, c->pe_row_stride, r->box);
+  if (!rc) rc = map_queries(&m->ql, q_latent, kLat, tokens, heads, ql_token, ql_head, q_box);
+  if (!rc) rc = map_queries(&m->qp, q_pe, kRope, tokens, heads, qp_token, qp_head, q_box);
+  return rc;
+}
+
+// rows of a matrix instruction for the average rows of a sequence: the smallest of 32, 64, 128 and 256 that holds
+// them (a unit costs the same shared-memory reads of the cache blocks whatever its rows; fewer leave more room in
+// the ring), 256 for more
+static int mass_rows(int64_t tokens, int64_t heads, int64_t batch) {
+  int rows = 32;
+  while (rows < 256 && (int64_t)rows * batch < tokens * heads) rows *= 2;
+  return rows;
 }
 
 }  // namespace kk3
@@ -369,7 +519,7 @@ extern "C" int64_t kk3_cache_mass_workspace(int batch, int tokens, int heads) {
   if (batch < 1 || tokens < 0 || heads < 1 || heads > kMaxHeads) return 0;
   int sms = 0;
   if (cache_sms(&sms)) return 0;
-  return (int64_t)sms * (16 + 2 * kMassPos * 4);
+  return (int64_t)(sms / 2) * (16 + 2 * kMassPos * 4);
 }
 
 extern "C" int kk3_cache_mass(const kk3_cache* cache, const void* q_latent, int64_t ql_token, int64_t ql_head,
@@ -405,11 +555,25 @@ extern "C" int kk3_cache_mass(const kk3_cache* cache, const void* q_latent, int6
   a.mass = mass;
   a.mass_row = mass_stride;
   a.out = new_mass;
-  a.workers = sms;
+  a.workers = sms / 2;
   a.meta = (int*)workspace;
-  a.part = (float*)((char*)workspace + (size_t)sms * 16);
-  // rows per unit: 32 where a sequence's rows fit (single tokens on a rank: the ring then holds more cache blocks in
-  // flight), 128 otherwise
-  const bool few = (int64_t)tokens * heads <= (int64_t)32 * a.c.batch;
-  return few ? mass_launch<32>(a, (cudaStream_t)stream) : mass_launch<128>(a, (cudaStream_t)stream);
+  a.part = (float*)((char*)workspace + (size_t)a.workers * 16);
+  PairMaps maps;
+  PairRows pr;
+  const int rows = mass_rows(tokens, heads, a.c.batch);
+  if (tokens > 0) {
+    const int r = pair_maps(cache, q_latent, ql_token, ql_head, q_pe, qp_token, qp_head, tokens, heads, rows / 2, &maps, &pr);
+    if (r) return r;
+  } else {
+    memset(&maps, 0, sizeof(maps));   // no tile reads them
+    memset(&pr, 0, sizeof(pr));
+  }
+  static std::atomic<bool> ready[kCacheMaxDevices];
+  int r = cache_allow_smem(kk3_cache_mass_kernel, kMassSmem, ready, "cudaFuncSetAttribute(kk3_cache_mass_kernel)");
+  if (r) return r;
+  const cudaStream_t st = (cudaStream_t)stream;
+  kk3_cache_mass_kernel<<<a.workers * 2, kMassThreads, kMassSmem, st>>>(a, pr, maps, rows);
+  r = cache_cuda(cudaGetLastError(), "kk3_cache_mass_kernel");
+  if (r) return r;
+  return cache_launch_after(kk3_cache_mass_join_kernel, dim3(a.workers), kMassPos, st, "kk3_cache_mass_join_kernel", a);
 }

@@ -18,6 +18,7 @@ these raise.
 from __future__ import annotations
 
 import ctypes
+import struct
 
 import torch
 
@@ -28,16 +29,13 @@ DEFAULT_SCALE = (128 + 64) ** -0.5      # (qk_nope_dim + qk_rope_dim) ** -0.5 (m
 MAX_SEQUENCES, MAX_HEADS, MAX_PAGE, MAX_POSITIONS = 4096, 128, 65536, 1 << 27
 
 
-class CacheDesc(ctypes.Structure):
-    """kk3_cache (include/kk3.h)."""
-    _fields_ = [("kv", ctypes.c_void_p), ("pe", ctypes.c_void_p), ("kv_page_stride", ctypes.c_int64),
-                ("kv_row_stride", ctypes.c_int64), ("pe_page_stride", ctypes.c_int64),
-                ("pe_row_stride", ctypes.c_int64), ("table", ctypes.c_void_p), ("table_stride", ctypes.c_int64),
-                ("num_pages", ctypes.c_int32), ("page_size", ctypes.c_int32), ("columns", ctypes.c_int32),
-                ("batch", ctypes.c_int32)]
+# kk3_cache (include/kk3.h) as bytes: kv, pe, their page and row strides, table, table_stride, num_pages, page_size,
+# columns, batch
+_DESC = struct.Struct("=QQqqqqQqiiii")
 
 
 _LIB = None
+_raw_stream = torch._C._cuda_getCurrentRawStream    # current_stream(device).cuda_stream without the Stream object
 
 
 def _lib() -> ctypes.CDLL:
@@ -45,7 +43,7 @@ def _lib() -> ctypes.CDLL:
     if _LIB is None:
         lib = load_library()
         vp, i32, i64, f32 = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_float
-        desc = ctypes.POINTER(CacheDesc)
+        desc = ctypes.c_char_p
         lib.kk3_cache_append.argtypes = [desc, vp, i64, vp, f32, vp, vp, i32, vp, vp, vp]
         lib.kk3_cache_attend_workspace.argtypes = [i32, i32, i32]
         lib.kk3_cache_attend_workspace.restype = i64
@@ -71,87 +69,149 @@ def paged_view(kv_cache: torch.Tensor, pe_cache: torch.Tensor, page_size: int):
 
 
 # --- argument checks -------------------------------------------------------------------------------------------
+# A decode step calls these operators once per layer, so the checks are written to cost little when they pass: one
+# comparison a line, and a message is only put together for a refusal.
+
+_BF16, _F32, _I32, _I64 = torch.bfloat16, torch.float32, torch.int32, torch.int64
+
 
 def _need(ok: bool, what: str) -> None:
     if not ok:
         raise ValueError(what)
 
 
-def _on(t, name: str, device: torch.device, dtype: torch.dtype, shape: tuple) -> torch.Tensor:
-    _need(isinstance(t, torch.Tensor), f"{name} must be a tensor")
-    _need(t.device == device, f"{name} must be on {device}, with the cache")
-    _need(t.dtype == dtype and tuple(t.shape) == shape, f"{name} must be {dtype} {list(shape)}")
-    return t
+def _check(t, name: str, device: torch.device, dtype: torch.dtype, shape: tuple) -> None:
+    """`t` is a contiguous tensor of this kind."""
+    _check_kind(t, name, device, dtype, shape)
+    if not t.is_contiguous():
+        raise ValueError(f"{name} must be contiguous")
 
 
-def _rows16(t: torch.Tensor, name: str) -> None:
-    """Vector loads: last dim contiguous, the other strides multiples of 8 elements, 16-byte aligned."""
-    _need(t.stride(-1) == 1 and all(s % 8 == 0 and s >= 0 for s, n in zip(t.stride()[:-1], t.shape[:-1]) if n > 1)
-          and t.data_ptr() % 16 == 0,
-          f"{name} needs a contiguous last dim, strides that are multiples of 8 elements and 16-byte alignment")
+def _check_kind(t, name: str, device: torch.device, dtype: torch.dtype, shape: tuple) -> None:
+    if not isinstance(t, torch.Tensor):
+        raise ValueError(f"{name} must be a tensor")
+    if t.dtype != dtype or t.shape != shape:
+        raise ValueError(f"{name} must be {dtype} {list(shape)}, not {t.dtype} {list(t.shape)}")
+    if t.device != device:
+        raise ValueError(f"{name} must be on {device}, with the cache")
 
 
-def _stride(t: torch.Tensor, dim: int) -> int:
-    """A stride for the kernels; that of a dim of one element means nothing and is made a valid one."""
-    return t.stride(dim) if t.shape[dim] > 1 else (t.shape[-1] + 7) // 8 * 8
+def _vector_rows(t, name: str) -> None:
+    """Refuse what 16-byte loads cannot read."""
+    if t.stride(-1) != 1 or t.data_ptr() % 16 or any(s % 8 or s < 0 for n, s in zip(t.shape[:-1], t.stride()) if n > 1):
+        raise ValueError(f"{name} needs a contiguous last dim, strides that are multiples of 8 elements and 16-byte "
+                         "alignment")
 
 
-def _cache(kv, pe, table) -> tuple[CacheDesc, torch.device, int]:
-    """(descriptor, device, positions per sequence)."""
-    for t, name in ((kv, "kv"), (pe, "pe"), (table, "table")):
-        _need(isinstance(t, torch.Tensor), f"{name} must be a tensor")
-    _need(kv.is_cuda, "the cache must be on a CUDA device (sm_100a kernels, no CPU path)")
-    _need(kv.dim() == 3 and kv.dtype == torch.bfloat16 and kv.shape[2] == LATENT and kv.shape[0] > 0 and kv.shape[1] > 0,
-          "kv must be bfloat16 [pages, page_size, 512]")
-    _on(pe, "pe", kv.device, torch.bfloat16, (kv.shape[0], kv.shape[1], ROPE))
-    _need(table.dim() == 2 and min(table.shape) > 0, "table must be int32 [B, columns], not empty")
-    _on(table, "table", kv.device, torch.int32, tuple(table.shape))
-    _need(table.stride(1) == 1 or table.shape[1] == 1, "table rows must be contiguous")
-    _rows16(kv, "kv")
-    _rows16(pe, "pe")
-    pages, page = kv.shape[:2]
+def _strides3(t, name: str) -> tuple[int, int, int]:
+    """(address, strides of the first two dims) of a three-dimensional tensor that the kernels read with 16-byte loads.
+    The stride of a dim of one element means nothing and is made a valid one."""
+    s0, s1, s2 = t.stride()
+    n0, n1, n2 = t.shape
+    at = t.data_ptr()
+    if s2 != 1 or (at | s0 * 2 | s1 * 2) & 15 or s0 < 0 or s1 < 0:
+        _vector_rows(t, name)
+    return at, s0 if n0 > 1 else n1 * n2, s1 if n1 > 1 else n2
+
+
+def _query_rows(t):
+    """(tensor, token stride, head stride) of queries [T, heads, n] whose (token, head) rows lie at one pitch, 16-byte
+    aligned, as the kernels' copies need; others are copied into that form."""
+    s0, s1, s2 = t.stride()
+    n0, n1, n2 = t.shape
+    if n1 == 1:
+        s1 = n2 if n0 == 1 else s0
+    if s2 != 1 or s1 < n2 or s1 % 8 or (n0 > 1 and s0 != n1 * s1) or t.data_ptr() % 16:
+        return t.clone(memory_format=torch.contiguous_format), n1 * n2, n2
+    return t, n1 * s1, s1
+
+
+def _cache(kv, pe, table):
+    """(kk3_cache bytes, device, sequences, positions per sequence)."""
+    if not isinstance(kv, torch.Tensor) or kv.dim() != 3 or kv.dtype != _BF16 or kv.shape[2] != LATENT or 0 in kv.shape:
+        raise ValueError("kv must be bfloat16 [pages, page_size, 512], not empty")
+    dev = kv.device
+    if dev.type != "cuda":
+        raise ValueError("the cache must be on a CUDA device (sm_100a kernels, no CPU path)")
+    pages, page, _ = kv.shape
+    _check_kind(pe, "pe", dev, _BF16, (pages, page, ROPE))
+    if not isinstance(table, torch.Tensor) or table.dim() != 2 or 0 in table.shape:
+        raise ValueError("table must be int32 [B, columns], not empty")
     B, columns = table.shape
-    _need(B <= MAX_SEQUENCES and page <= MAX_PAGE and columns * page <= MAX_POSITIONS and pages < 1 << 31,
-          f"at most {MAX_SEQUENCES} sequences, pages of {MAX_PAGE} and {MAX_POSITIONS} positions per sequence")
-    for t, name in ((kv, "kv"), (pe, "pe")):
-        _need(t.shape[1] == 1 or t.stride(1) >= t.shape[2], f"{name} rows must not overlap")
-    desc = CacheDesc(kv.data_ptr(), pe.data_ptr(), _stride(kv, 0), _stride(kv, 1), _stride(pe, 0), _stride(pe, 1),
-                     table.data_ptr(), table.stride(0) if B > 1 else columns, pages, page, columns, B)
-    return desc, kv.device, columns * page
+    _check_kind(table, "table", dev, _I32, (B, columns))
+    kv_at, kv_page, kv_row = _strides3(kv, "kv")
+    pe_at, pe_page, pe_row = _strides3(pe, "pe")
+    if kv_row < LATENT or pe_row < ROPE:
+        raise ValueError("the rows of kv and pe must not overlap")
+    if page > 1 and (kv_page % kv_row or pe_page % pe_row):
+        raise ValueError("the page strides of kv and pe must be multiples of their row strides")
+    if columns > 1 and table.stride(1) != 1:
+        raise ValueError("table rows must be contiguous")
+    if B > MAX_SEQUENCES or page > MAX_PAGE or columns * page > MAX_POSITIONS or pages >= 1 << 31:
+        raise ValueError(f"at most {MAX_SEQUENCES} sequences, pages of {MAX_PAGE} and {MAX_POSITIONS} positions per "
+                         "sequence")
+    desc = _DESC.pack(kv_at, pe_at, kv_page, kv_row, pe_page, pe_row, table.data_ptr(),
+                      table.stride(0) if B > 1 else columns, pages, page, columns, B)
+    return desc, dev, B, columns * page
 
 
 def _error(error_word, device) -> int | None:
     if error_word is None:
         return None
-    _need(isinstance(error_word, torch.Tensor) and error_word.device == device and error_word.dtype == torch.int32
+    _need(isinstance(error_word, torch.Tensor) and error_word.device == device and error_word.dtype == _I32
           and error_word.numel() == 1, "error_word must be one int32 on the cache's device")
     return error_word.data_ptr()
 
 
 def _queries(q_latent, q_pe, device, scale):
-    _need(isinstance(q_latent, torch.Tensor) and q_latent.dim() == 3, "q_latent must be bfloat16 [T, heads, 512]")
-    T, H = q_latent.shape[:2]
-    _need(1 <= H <= MAX_HEADS, f"heads must be 1..{MAX_HEADS}")
-    _need(T * H < 1 << 30, "too many query rows")
-    _on(q_latent, "q_latent", device, torch.bfloat16, (T, H, LATENT))
-    _on(q_pe, "q_pe", device, torch.bfloat16, (T, H, ROPE))
-    if T:
-        _rows16(q_latent, "q_latent")
-        _rows16(q_pe, "q_pe")
+    if not isinstance(q_latent, torch.Tensor) or q_latent.dim() != 3:
+        raise ValueError("q_latent must be bfloat16 [T, heads, 512]")
+    T, H, _ = q_latent.shape
+    if not 1 <= H <= MAX_HEADS or T * H >= 1 << 30:
+        raise ValueError(f"heads must be 1..{MAX_HEADS}, and T * heads below 2^30")
+    _check_kind(q_latent, "q_latent", device, _BF16, (T, H, LATENT))
+    _check_kind(q_pe, "q_pe", device, _BF16, (T, H, ROPE))
     scale = DEFAULT_SCALE if scale is None else float(scale)
-    _need(scale == scale and abs(scale) != float("inf"), "scale must be finite")
-    args = (q_latent.data_ptr(), _stride(q_latent, 0), _stride(q_latent, 1), q_pe.data_ptr(), _stride(q_pe, 0),
-            _stride(q_pe, 1))
-    return T, H, scale, args
+    if scale != scale or abs(scale) == float("inf"):
+        raise ValueError("scale must be finite")
+    if T:
+        q_latent, *ql = _query_rows(q_latent)
+        q_pe, *qp = _query_rows(q_pe)
+    else:
+        ql, qp = (LATENT, LATENT), (ROPE, ROPE)
+    return T, H, scale, (q_latent, q_pe), (q_latent.data_ptr(), *ql, q_pe.data_ptr(), *qp)
 
 
-def _call(rc: int, what: str) -> None:
+def _mass_stride(mass, name: str, device, B: int, capacity: int) -> int:
+    _check_kind(mass, name, device, _F32, (B, capacity))
+    row, one = mass.stride()
+    if (one != 1 and capacity > 1) or row < 0:
+        raise ValueError(f"{name} rows must be contiguous")
+    return row if B > 1 else capacity
+
+
+def _run(what: str, device: torch.device, *args) -> None:
+    """Call a C entry point on the cache's device and its current stream."""
+    fn, index = getattr(_lib(), what), device.index
+    if torch.cuda.current_device() == index:
+        rc = fn(*args, _raw_stream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = fn(*args, _raw_stream(index))
     if rc != 0:
         raise KK3Error(rc, what)
 
 
-def _stream(device) -> ctypes.c_void_p:
-    return ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
+def _workspace(what: str, device: torch.device, *args) -> torch.Tensor:
+    """A call's own workspace, from torch's allocator on the current stream."""
+    if torch.cuda.current_device() == device.index:
+        nbytes = getattr(_lib(), what)(*args)
+    else:
+        with torch.cuda.device(device):
+            nbytes = getattr(_lib(), what)(*args)
+    if nbytes <= 0:
+        raise KK3Error(-3, what)
+    return torch.empty(nbytes, dtype=torch.uint8, device=device)
 
 
 # --- the operators ---------------------------------------------------------------------------------------------
@@ -162,24 +222,24 @@ def append(raw, norm_weight, kv, pe, table, lengths, cu_new, *, eps: float = 1e-
     raw: bf16 [T, 576], the `ka` projection of the new tokens; its first 512 values are RMS-normalised with
     norm_weight (bf16 [512]) in FP32 and rounded once, the other 64 are stored as they are. lengths: positions cached
     before. A token behind the table's last column is not written and sets error_word."""
-    desc, dev, _ = _cache(kv, pe, table)
-    _need(isinstance(raw, torch.Tensor) and raw.dim() == 2, "raw must be bfloat16 [T, 576]")
+    desc, dev, B, _ = _cache(kv, pe, table)
+    if not isinstance(raw, torch.Tensor) or raw.dim() != 2:
+        raise ValueError("raw must be bfloat16 [T, 576]")
     T = raw.shape[0]
-    _on(raw, "raw", dev, torch.bfloat16, (T, LATENT + ROPE))
+    _check_kind(raw, "raw", dev, _BF16, (T, LATENT + ROPE))
+    _check(norm_weight, "norm_weight", dev, _BF16, (LATENT,))
+    _vector_rows(norm_weight, "norm_weight")
+    _check(lengths, "lengths", dev, _I64, (B,))
+    _check(cu_new, "cu_new", dev, _I32, (B + 1,))
+    if not eps >= 0:
+        raise ValueError("eps must not be negative")
+    row = LATENT + ROPE
     if T:
-        _rows16(raw, "raw")
-    _on(norm_weight, "norm_weight", dev, torch.bfloat16, (LATENT,))
-    _rows16(norm_weight, "norm_weight")
-    _on(lengths, "lengths", dev, torch.int64, (desc.batch,))
-    _on(cu_new, "cu_new", dev, torch.int32, (desc.batch + 1,))
-    _need(lengths.is_contiguous() and cu_new.is_contiguous(), "lengths and cu_new must be contiguous")
-    _need(eps >= 0, "eps must not be negative")
-    err = _error(error_word, dev)
-    with torch.cuda.device(dev):
-        out = torch.empty_like(lengths)
-        _call(_lib().kk3_cache_append(ctypes.byref(desc), raw.data_ptr(), _stride(raw, 0), norm_weight.data_ptr(), eps,
-                                      lengths.data_ptr(), cu_new.data_ptr(), T, out.data_ptr(), err, _stream(dev)),
-              "kk3_cache_append")
+        _vector_rows(raw, "raw")
+        row = raw.stride(0) if T > 1 else row
+    out = torch.empty_like(lengths)
+    _run("kk3_cache_append", dev, desc, raw.data_ptr(), row, norm_weight.data_ptr(), eps, lengths.data_ptr(),
+         cu_new.data_ptr(), T, out.data_ptr(), _error(error_word, dev))
     return out
 
 
@@ -188,33 +248,29 @@ def attend(q_latent, q_pe, kv, pe, table, lengths, cu_new, *, scale: float | Non
     """Attention of the new tokens over their sequences' caches, in the latent space: (out bf16 [T, heads, 512],
     lse f32 [T, heads]).
 
-    q_latent: bf16 [T, heads, 512] absorbed queries, q_pe: bf16 [T, heads, 64]; any strides that are multiples of 8.
+    q_latent: bf16 [T, heads, 512] absorbed queries, q_pe: bf16 [T, heads, 64], of any strides (unless
+    all (token, head) rows lie at one 16-byte aligned pitch, they are copied first).
     lengths: cached positions, the new tokens included (append's result): token i of n sees the first
     lengths - n + i + 1. A token that sees nothing gets zeros and -inf. Rows behind cu_new[B] are not written (pass
     `out` and `lse`, both contiguous, to keep theirs)."""
-    desc, dev, _ = _cache(kv, pe, table)
-    T, H, scale, q = _queries(q_latent, q_pe, dev, scale)
-    _on(lengths, "lengths", dev, torch.int64, (desc.batch,))
-    _on(cu_new, "cu_new", dev, torch.int32, (desc.batch + 1,))
-    _need(lengths.is_contiguous() and cu_new.is_contiguous(), "lengths and cu_new must be contiguous")
+    desc, dev, B, _ = _cache(kv, pe, table)
+    T, H, scale, _copies, q = _queries(q_latent, q_pe, dev, scale)
+    _check(lengths, "lengths", dev, _I64, (B,))
+    _check(cu_new, "cu_new", dev, _I32, (B + 1,))
+    if out is None:
+        out = torch.empty((T, H, LATENT), dtype=_BF16, device=dev)
+    else:
+        _check(out, "out", dev, _BF16, (T, H, LATENT))
+        _need(out.data_ptr() % 16 == 0, "out must be 16-byte aligned")
+    if lse is None:
+        lse = torch.empty((T, H), dtype=_F32, device=dev)
+    else:
+        _check(lse, "lse", dev, _F32, (T, H))
     err = _error(error_word, dev)
-    with torch.cuda.device(dev):
-        if out is None:
-            out = torch.empty((T, H, LATENT), dtype=torch.bfloat16, device=dev)
-        if lse is None:
-            lse = torch.empty((T, H), dtype=torch.float32, device=dev)
-        _on(out, "out", dev, torch.bfloat16, (T, H, LATENT))
-        _on(lse, "lse", dev, torch.float32, (T, H))
-        _need(out.is_contiguous() and lse.is_contiguous() and out.data_ptr() % 16 == 0,
-              "out and lse must be contiguous, out 16-byte aligned")
-        if T == 0:
-            return out, lse
-        lib = _lib()
-        nbytes = lib.kk3_cache_attend_workspace(desc.batch, T, H)
-        work = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=dev)
-        _call(lib.kk3_cache_attend(ctypes.byref(desc), *q, lengths.data_ptr(), cu_new.data_ptr(), T, H, scale,
-                                   out.data_ptr(), lse.data_ptr(), work.data_ptr(), nbytes, err, _stream(dev)),
-              "kk3_cache_attend")
+    if T:
+        work = _workspace("kk3_cache_attend_workspace", dev, B, T, H)
+        _run("kk3_cache_attend", dev, desc, *q, lengths.data_ptr(), cu_new.data_ptr(), T, H, scale, out.data_ptr(),
+             lse.data_ptr(), work.data_ptr(), work.numel(), err)
     return out, lse
 
 
@@ -225,29 +281,21 @@ def attention_mass(q_latent, q_pe, lse, kv, pe, table, lengths, cu_new, *, scale
 
     lse: attend's, with the same queries, lengths and scale. mass: what earlier calls accumulated (zeros if None);
     `out` may be mass itself. Positions at or behind a length keep their mass."""
-    desc, dev, capacity = _cache(kv, pe, table)
-    T, H, scale, q = _queries(q_latent, q_pe, dev, scale)
-    _on(lse, "lse", dev, torch.float32, (T, H))
-    _on(lengths, "lengths", dev, torch.int64, (desc.batch,))
-    _on(cu_new, "cu_new", dev, torch.int32, (desc.batch + 1,))
-    _need(lengths.is_contiguous() and cu_new.is_contiguous() and lse.is_contiguous(),
-          "lengths, cu_new and lse must be contiguous")
+    desc, dev, B, capacity = _cache(kv, pe, table)
+    T, H, scale, _copies, q = _queries(q_latent, q_pe, dev, scale)
+    _check(lse, "lse", dev, _F32, (T, H))
+    _check(lengths, "lengths", dev, _I64, (B,))
+    _check(cu_new, "cu_new", dev, _I32, (B + 1,))
+    row, before = 0, None
     if mass is not None:
-        _on(mass, "mass", dev, torch.float32, (desc.batch, capacity))
-        _need(mass.stride(1) == 1 or capacity == 1, "mass rows must be contiguous")
-    err = _error(error_word, dev)
-    with torch.cuda.device(dev):
-        if out is None:
-            out = torch.empty((desc.batch, capacity), dtype=torch.float32, device=dev)
-        _on(out, "out", dev, torch.float32, (desc.batch, capacity))
-        _need(out.is_contiguous(), "out must be contiguous")
-        lib = _lib()
-        nbytes = lib.kk3_cache_mass_workspace(desc.batch, T, H)
-        work = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=dev)
-        _call(lib.kk3_cache_mass(ctypes.byref(desc), *q, lse.data_ptr(), lengths.data_ptr(), cu_new.data_ptr(), T, H,
-                                 scale, None if mass is None else mass.data_ptr(),
-                                 0 if mass is None else (mass.stride(0) if desc.batch > 1 else capacity),
-                                 out.data_ptr(), work.data_ptr(), nbytes, err, _stream(dev)), "kk3_cache_mass")
+        row, before = _mass_stride(mass, "mass", dev, B, capacity), mass.data_ptr()
+    if out is None:
+        out = torch.empty((B, capacity), dtype=_F32, device=dev)
+    else:
+        _check(out, "out", dev, _F32, (B, capacity))
+    work = _workspace("kk3_cache_mass_workspace", dev, B, T, H)
+    _run("kk3_cache_mass", dev, desc, *q, lse.data_ptr(), lengths.data_ptr(), cu_new.data_ptr(), T, H, scale, before, row,
+         out.data_ptr(), work.data_ptr(), work.numel(), _error(error_word, dev))
     return out
 
 
@@ -260,29 +308,28 @@ def evict(kv, pe, table, lengths, mass, budget: int, *, sinks: int = 0, recent: 
     that none of the sequences uses, so that pages shared with others stay as they are), or in place (None). Returns
     (new lengths int64 [B], their mass f32 [B, columns * page_size] with zeros behind, their old positions int32
     [B, budget] with -1 behind)."""
-    desc, dev, capacity = _cache(kv, pe, table)
-    _on(lengths, "lengths", dev, torch.int64, (desc.batch,))
-    _need(lengths.is_contiguous(), "lengths must be contiguous")
-    _on(mass, "mass", dev, torch.float32, (desc.batch, capacity))
-    _need(mass.stride(1) == 1 or capacity == 1, "mass rows must be contiguous")
+    desc, dev, B, capacity = _cache(kv, pe, table)
+    _check(lengths, "lengths", dev, _I64, (B,))
+    row = _mass_stride(mass, "mass", dev, B, capacity)
     budget, sinks, recent = int(budget), int(sinks), int(recent)
-    _need(1 <= budget <= capacity, "budget must be 1 .. columns * page_size")
-    _need(sinks >= 0 and recent >= 0 and sinks + recent <= budget, "sinks + recent must not exceed the budget")
-    dst, dst_stride, dst_columns = None, 0, 0
+    if not 1 <= budget <= capacity:
+        raise ValueError("budget must be 1 .. columns * page_size")
+    if sinks < 0 or recent < 0 or sinks + recent > budget:
+        raise ValueError("sinks + recent must not exceed the budget")
+    dst, dst_row, dst_columns = None, 0, 0
     if dst_table is not None:
-        _need(isinstance(dst_table, torch.Tensor) and dst_table.dim() == 2, "dst_table must be int32 [B, columns]")
+        if not isinstance(dst_table, torch.Tensor) or dst_table.dim() != 2:
+            raise ValueError("dst_table must be int32 [B, columns]")
         dst_columns = dst_table.shape[1]
-        _on(dst_table, "dst_table", dev, torch.int32, (desc.batch, dst_columns))
-        _need(dst_table.stride(1) == 1 or dst_columns == 1, "dst_table rows must be contiguous")
-        _need(min(dst_columns * desc.page_size, MAX_POSITIONS) >= budget, "dst_table must hold the budget")
-        dst, dst_stride = dst_table.data_ptr(), dst_table.stride(0) if desc.batch > 1 else dst_columns
-    err = _error(error_word, dev)
-    with torch.cuda.device(dev):
-        new_lengths = torch.empty_like(lengths)
-        new_mass = torch.empty((desc.batch, capacity), dtype=torch.float32, device=dev)
-        kept = torch.empty((desc.batch, budget), dtype=torch.int32, device=dev)
-        _call(_lib().kk3_cache_evict(ctypes.byref(desc), lengths.data_ptr(), mass.data_ptr(),
-                                     mass.stride(0) if desc.batch > 1 else capacity, budget, sinks, recent, dst,
-                                     dst_stride, dst_columns, new_lengths.data_ptr(), new_mass.data_ptr(),
-                                     kept.data_ptr(), err, _stream(dev)), "kk3_cache_evict")
+        _check_kind(dst_table, "dst_table", dev, _I32, (B, dst_columns))
+        if dst_columns > 1 and dst_table.stride(1) != 1:
+            raise ValueError("dst_table rows must be contiguous")
+        if dst_columns * kv.shape[1] < budget:
+            raise ValueError("dst_table must hold the budget")
+        dst, dst_row = dst_table.data_ptr(), dst_table.stride(0) if B > 1 else dst_columns
+    new_lengths = torch.empty_like(lengths)
+    new_mass = torch.empty((B, capacity), dtype=_F32, device=dev)
+    kept = torch.empty((B, budget), dtype=_I32, device=dev)
+    _run("kk3_cache_evict", dev, desc, lengths.data_ptr(), mass.data_ptr(), row, budget, sinks, recent, dst, dst_row,
+         dst_columns, new_lengths.data_ptr(), new_mass.data_ptr(), kept.data_ptr(), _error(error_word, dev))
     return new_lengths, new_mass, kept
