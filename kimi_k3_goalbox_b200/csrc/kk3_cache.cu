@@ -126,6 +126,7 @@ constexpr int kWaPitch = kEntry + 8;      // 1168-byte rows: consecutive rows fa
 constexpr int kWaPPitch = kWaUnit + 8;
 constexpr int kWaThreads = 256;
 constexpr int kWaMinUnits = 4;
+constexpr int64_t kWarpRowsMost = 16;     // average rows of a sequence up to which this kernel is taken
 struct WaSmem {
   bf16 ring[kWaStages][kWaUnit][kWaPitch];
   bf16 q[kWaRows][kWaPitch];
@@ -329,54 +330,60 @@ __global__ void __launch_bounds__(kWaThreads, 1) kk3_cache_attend_warp_kernel(co
 
 // ---------------------------------------------------------------------------------------------
 // Join of a split tile: out = sum_w 2^(m_w - m) O_w / sum_w 2^(m_w - m) l_w over the tile's workers in order. One CTA
-// per (worker that begins a split tile, row); four groups of 128 threads (4 dims each) take a quarter of the workers'
+// per (worker that begins a split tile, every gridDim.y-th row); four groups of 128 threads (4 dims each) take a quarter of the workers'
 // sums each, so that the loads of many short pieces are in flight together.
 __global__ void __launch_bounds__(512) kk3_cache_join_kernel(const AttendArgs a, int tile_rows) {
-  const int worker = blockIdx.x, row = blockIdx.y;
+  const int worker = blockIdx.x;
   cache_follow();
   const int n = a.meta[worker * 4 + 2];
   if (n == 0) return;
   const int b = a.meta[worker * 4], t = a.meta[worker * 4 + 1];
   const Seq s = a.seq(b);
-  if ((long long)t * tile_rows + row >= (long long)s.n * a.heads) return;
+  const int rows = (int)min((long long)tile_rows, (long long)s.n * a.heads - (long long)t * tile_rows);
   __shared__ float4 sums[3][128];
   const int grp = threadIdx.x >> 7, i = threadIdx.x & 127;
-  const auto part = [&](int w) {
-    return a.part + (((long long)(worker + w) * 2 + (w == 0 ? 1 : 0)) * tile_rows + row) * kPartRow;
-  };
-  float top = -INFINITY;
-  for (int w = 0; w < n; ++w) top = fmaxf(top, part(w)[kLat]);
-  const float ref = top == -INFINITY ? 0.0f : top;
-  float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-  float l = 0.0f;
-  for (int w = 0; w < n; ++w) l += exp2f(part(w)[kLat] - ref) * part(w)[kLat + 1];
-  const int per = (n + 3) / 4;
+  for (int row = blockIdx.y; row < rows; row += gridDim.y) {
+    const auto part = [&](int w) {
+      return a.part + (((long long)(worker + w) * 2 + (w == 0 ? 1 : 0)) * tile_rows + row) * kPartRow;
+    };
+    float top = -INFINITY;
+    for (int w = 0; w < n; ++w) top = fmaxf(top, part(w)[kLat]);
+    const float ref = top == -INFINITY ? 0.0f : top;
+    float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    float l = 0.0f;
+    for (int w = 0; w < n; ++w) l += exp2f(part(w)[kLat] - ref) * part(w)[kLat + 1];
+    const int per = (n + 3) / 4;
 #pragma unroll 4
-  for (int w = grp * per; w < min(n, (grp + 1) * per); ++w) {
-    const float* p = part(w);
-    const float4 v = *reinterpret_cast<const float4*>(p + i * 4);
-    const float f = exp2f(p[kLat] - ref);
-    sum.x = fmaf(f, v.x, sum.x);
-    sum.y = fmaf(f, v.y, sum.y);
-    sum.z = fmaf(f, v.z, sum.z);
-    sum.w = fmaf(f, v.w, sum.w);
-  }
-  if (grp > 0) sums[grp - 1][i] = sum;
-  __syncthreads();
-  if (grp > 0) return;
+    for (int w = grp * per; w < min(n, (grp + 1) * per); ++w) {
+      const float* p = part(w);
+      const float4 v = *reinterpret_cast<const float4*>(p + i * 4);
+      const float f = exp2f(p[kLat] - ref);
+      sum.x = fmaf(f, v.x, sum.x);
+      sum.y = fmaf(f, v.y, sum.y);
+      sum.z = fmaf(f, v.z, sum.z);
+      sum.w = fmaf(f, v.w, sum.w);
+    }
+    if (grp > 0) sums[grp - 1][i] = sum;
+    __syncthreads();
+    if (grp > 0) {
+      __syncthreads();
+      continue;
+    }
 #pragma unroll
-  for (int k = 0; k < 3; ++k) {
-    sum.x += sums[k][i].x;
-    sum.y += sums[k][i].y;
-    sum.z += sums[k][i].z;
-    sum.w += sums[k][i].w;
+    for (int k = 0; k < 3; ++k) {
+      sum.x += sums[k][i].x;
+      sum.y += sums[k][i].y;
+      sum.z += sums[k][i].z;
+      sum.w += sums[k][i].w;
+    }
+    const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
+    const long long g = (long long)s.q0 * a.heads + (long long)t * tile_rows + row;
+    __nv_bfloat162* o = reinterpret_cast<__nv_bfloat162*>(a.out + g * kLat + i * 4);
+    o[0] = __floats2bfloat162_rn(sum.x * inv, sum.y * inv);
+    o[1] = __floats2bfloat162_rn(sum.z * inv, sum.w * inv);
+    if (i == 0) a.lse[g] = (ref + log2f(l)) * 0.69314718055994531f;
+    __syncthreads();   // sums is read
   }
-  const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
-  const long long g = (long long)s.q0 * a.heads + (long long)t * tile_rows + row;
-  __nv_bfloat162* o = reinterpret_cast<__nv_bfloat162*>(a.out + g * kLat + i * 4);
-  o[0] = __floats2bfloat162_rn(sum.x * inv, sum.y * inv);
-  o[1] = __floats2bfloat162_rn(sum.z * inv, sum.w * inv);
-  if (i == 0) a.lse[g] = (ref + log2f(l)) * 0.69314718055994531f;
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -665,11 +672,22 @@ extern "C" int kk3_cache_append(const kk3_cache* cache, const void* raw, int64_t
   return cache_cuda(cudaGetLastError(), "kk3_cache_append_kernel");
 }
 
+// The kernel for a call's average rows per sequence, and its workers.
+struct Plan {
+  bool pair;
+  int workers, rows;
+};
+static Plan attend_plan(int64_t batch, int64_t tokens, int64_t heads, int sms) {
+  const bool pair = tokens * heads > kWarpRowsMost * batch;
+  return pair ? Plan{true, sms / 2, kPairRows} : Plan{false, sms, kWaRows};
+}
+
 extern "C" int64_t kk3_cache_attend_workspace(int batch, int tokens, int heads) {
   if (batch < 1 || tokens < 0 || heads < 1 || heads > kMaxHeads) return 0;
   int sms = 0;
   if (cache_sms(&sms)) return 0;
-  return (int64_t)sms * 16 + (int64_t)sms * 2 * kWaRows * kPartRow * 4;
+  const Plan p = attend_plan(batch, tokens, heads, sms);
+  return (int64_t)p.workers * (16 + 2 * p.rows * kPartRow * 4);
 }
 
 extern "C" int kk3_cache_attend(const kk3_cache* cache, const void* q_latent, int64_t ql_token, int64_t ql_head,
@@ -703,16 +721,23 @@ extern "C" int kk3_cache_attend(const kk3_cache* cache, const void* q_latent, in
   a.scale_log2 = scale * 1.4426950408889634f;
   a.out = (bf16*)out;
   a.lse = lse;
-  a.workers = sms;
+  const Plan p = attend_plan(a.c.batch, tokens, heads, sms);
+  a.workers = p.workers;
   a.meta = (int*)workspace;
-  a.part = (float*)((char*)workspace + (size_t)sms * 16);
-  static std::atomic<bool> done[kCacheMaxDevices];
-  int r = cache_allow_smem(kk3_cache_attend_warp_kernel, sizeof(WaSmem), done, "cudaFuncSetAttribute(kk3_cache_attend_warp_kernel)");
+  a.part = (float*)((char*)workspace + (size_t)p.workers * 16);
+  const cudaStream_t st = (cudaStream_t)stream;
+  int r;
+  if (p.pair) {
+    r = attend_pair(cache, a, st);
+  } else {
+    static std::atomic<bool> done[kCacheMaxDevices];
+    r = cache_allow_smem(kk3_cache_attend_warp_kernel, sizeof(WaSmem), done, "cudaFuncSetAttribute(kk3_cache_attend_warp_kernel)");
+    if (r) return r;
+    kk3_cache_attend_warp_kernel<<<sms, kWaThreads, sizeof(WaSmem), st>>>(a);
+    r = cache_cuda(cudaGetLastError(), "kk3_cache_attend_warp_kernel");
+  }
   if (r) return r;
-  kk3_cache_attend_warp_kernel<<<sms, kWaThreads, sizeof(WaSmem), (cudaStream_t)stream>>>(a);
-  r = cache_cuda(cudaGetLastError(), "kk3_cache_attend_warp_kernel");
-  if (r) return r;
-  return cache_launch_after(kk3_cache_join_kernel, dim3(sms, kWaRows), 512, (cudaStream_t)stream, "kk3_cache_join_kernel", a, kWaRows);
+  return cache_launch_after(kk3_cache_join_kernel, dim3(p.workers, 16), 512, st, "kk3_cache_join_kernel", a, p.rows);
 }
 
 extern "C" int kk3_cache_evict(const kk3_cache* cache, const int64_t* lengths, const float* mass, int64_t mass_stride,

@@ -117,10 +117,12 @@ struct MassArgs : CallSeqs {
 struct AttendSplit {
   int rows, heads, unit;
   KK3_DEV int tiles(const Seq& s) const { return (int)(((long long)s.n * heads + rows - 1) / rows); }
+  KK3_DEV int sees(const Seq& s, int t) const {   // positions that the tile's last row sees, 0 or less: none
+    return s.len - s.n + min(s.n - 1, (int)((((long long)t + 1) * rows - 1) / heads)) + 1;
+  }
   KK3_DEV int units(const Seq& s, int t) const {
-    const int last = min(s.n - 1, (int)((((long long)t + 1) * rows - 1) / heads));
-    const int sees = s.len - s.n + last + 1;
-    return sees > unit ? (sees + unit - 1) / unit : 1;
+    const int n = sees(s, t);
+    return n > unit ? (n + unit - 1) / unit : 1;
   }
 };
 // Attention weight: a tile is `positions` positions of one sequence over the rows that see its first, a unit `rows`

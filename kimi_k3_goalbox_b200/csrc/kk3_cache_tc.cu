@@ -1,5 +1,5 @@
-// kk3_cache_tc.cu - tensor-core kernels of the paged latent cache (tcgen05 on CTA pairs, sm_100a): the accumulated
-// attention weight.
+// kk3_cache_tc.cu - tensor-core kernels of the paged latent cache (tcgen05 on CTA pairs, sm_100a): attention of new
+// tokens and the accumulated attention weight.
 //
 // Operands come through the page table by TMA, in blocks of 64 dims in the 128-byte swizzled form that the matrix
 // instructions read: boxes of as many rows as divide a page and a tile, or gathers of four rows where that is below
@@ -447,6 +447,392 @@ __global__ void __launch_bounds__(kMassPos) kk3_cache_mass_join_kernel(const Mas
 }
 
 // ---------------------------------------------------------------------------------------------
+// Attention: s = scale (q . e_p), running maximum m and sum l per row, O = O 2^(m - m') + sum_p 2^(s_p - m') c_p.
+//
+// A tile is 128 (token, head) rows of one sequence, 64 in each CTA, a unit 128 positions. The FP32 sums of 512 output
+// dims for 128 rows fill a whole TMEM, so the pair's M = 128 form carries them: 64 rows in either CTA, half of the
+// columns in lanes 0-63 and half in lanes 64-127, 256 columns in all, which leaves room for two score buffers. For the
+// scores each CTA loads 64 of the 128 positions (nine blocks of 8 KB), for the second product half of the output dims
+// of all 128 (four pieces of 16 KB, the same bytes in the other operand order); both rings hold one unit, and a block
+// is requested again as soon as its last instruction is done, a whole unit ahead of its use.
+//
+// Thread = row and half of a unit's positions. The running maximum moves only when it is exceeded by more than 2^8
+// (probabilities stay below 256, harmless in BF16 and FP32), so the sums in TMEM are rarely rescaled. Probabilities
+// are rounded to BF16 for the second product, the type that the instruction takes with BF16 latents; the running sum
+// adds them unrounded, since lse is an FP32 result.
+//
+// Bounds of a unit: 2176 clocks of tensor time (128 x 128 x 1088 products at 4096 a clock and SM), 1920 of
+// shared-memory reads, 139 KB of loads in each SM (64 bytes a clock, mostly from L2).
+
+constexpr int kPaRows = 128, kPaUnit = 128;
+constexpr int kPaThreads = 224;      // warps 0-3 softmax, 4 queries and score blocks, 5 value blocks, 6 instructions
+constexpr int kPaBlock = 64 * 128;   // 64 rows of 64 dims
+constexpr int kPaMinUnits = 2;
+constexpr float kPaSlack = 8.0f;
+struct PaCtl {
+  unsigned long long qfull, qempty, kfull[kBlocks], kempty[kBlocks], vfull[4], vempty[4], sfull[2], sfree[2], pfull, pvdone, done;
+  unsigned tmem;
+  int dead;
+  long long red[kPaThreads / 32 + 4];
+  float top[2][2][64];   // [unit parity][half][row]: row maxima of the halves
+  float sum[2][64];      // [half][row]
+};
+constexpr int kPaQ = 0, kPaK = kPaQ + kBlocks * kPaBlock, kPaV = kPaK + kBlocks * kPaBlock, kPaP = kPaV + 8 * kPaBlock,
+              kPaCtl = kPaP + 2 * kPaBlock;
+constexpr int kPaSmem = kPaCtl + (int)sizeof(PaCtl);
+static_assert(kPaSmem <= 232448, "shared memory of a CTA");
+
+// MN-major operand with the 128-byte swizzle: 64-element blocks `lbo` bytes apart, 8 K-rows in 1024 bytes
+KK3_DEV unsigned long long sdesc_mn(unsigned addr, unsigned lbo) {
+  return (unsigned long long)((addr & 0x3ffffu) >> 4) | ((unsigned long long)(lbo >> 4) << 16) |
+         ((unsigned long long)(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
+}
+KK3_DEV void tmem_st32(unsigned taddr, const float (&v)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,"
+      "%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};"
+      ::"r"(taddr), "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]), "f"(v[8]),
+        "f"(v[9]), "f"(v[10]), "f"(v[11]), "f"(v[12]), "f"(v[13]), "f"(v[14]), "f"(v[15]), "f"(v[16]), "f"(v[17]),
+        "f"(v[18]), "f"(v[19]), "f"(v[20]), "f"(v[21]), "f"(v[22]), "f"(v[23]), "f"(v[24]), "f"(v[25]), "f"(v[26]),
+        "f"(v[27]), "f"(v[28]), "f"(v[29]), "f"(v[30]), "f"(v[31])
+      : "memory");
+}
+KK3_DEV void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPaThreads, 1)
+    kk3_cache_attend_pair_kernel(const AttendArgs a, const PairRows pr, const __grid_constant__ PairMaps maps) {
+  extern __shared__ __align__(1024) unsigned char smem_raw[];
+  PaCtl& ctl = *reinterpret_cast<PaCtl*>(smem_raw + kPaCtl);
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, worker = blockIdx.x >> 1;
+  const unsigned rank = cluster_rank(), base = smem_u32(smem_raw);
+  const AttendSplit split{kPaRows, a.heads, kPaUnit};
+  const Share sh = plan_share<kPaThreads>(a, split, worker, kPaMinUnits, reinterpret_cast<int*>(smem_raw), ctl.red);
+  if (tid == 0 && rank == 0) a.meta[worker * 4 + 2] = 0;
+  if (base & 1023u) {   // the swizzled blocks need a 1024-byte boundary, which dynamic shared memory begins on
+    if (tid == 0) cache_error(a.c);
+    return;
+  }
+  if (worker >= sh.workers) return;   // both CTAs of the pair
+  const unsigned qfull = smem_u32(&ctl.qfull), qempty = smem_u32(&ctl.qempty), kfull = smem_u32(ctl.kfull),
+                 kempty = smem_u32(ctl.kempty), vfull = smem_u32(ctl.vfull), vempty = smem_u32(ctl.vempty),
+                 sfull = smem_u32(ctl.sfull), sfree = smem_u32(ctl.sfree), pfull = smem_u32(&ctl.pfull),
+                 pvdone = smem_u32(&ctl.pvdone), done = smem_u32(&ctl.done);
+  volatile int* dead = &ctl.dead;
+  if (tid == 0) {
+    mbar_init(qfull, 1);
+    mbar_init(qempty, 1);
+    for (int i = 0; i < kBlocks; ++i) {
+      mbar_init(kfull + 8 * i, 1);
+      mbar_init(kempty + 8 * i, 1);
+    }
+    for (int i = 0; i < 4; ++i) {
+      mbar_init(vfull + 8 * i, 1);
+      mbar_init(vempty + 8 * i, 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(sfull + 8 * i, 1);
+      mbar_init(sfree + 8 * i, 8);   // four warps of either CTA
+    }
+    mbar_init(pfull, 8);
+    mbar_init(pvdone, 1);
+    mbar_init(done, 1);
+    ctl.dead = 0;
+    fence_mbar_init();
+  }
+  if (warp == 6) pair_alloc(smem_u32(&ctl.tmem), 512);
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync();
+  tc_fence_after();
+  const unsigned tmem = *reinterpret_cast<volatile unsigned*>(&ctl.tmem);
+  const unsigned tmem_s = tmem + 256;
+
+  int b = sh.b, t = sh.t;
+  long long at = sh.at;
+  int n = 0, tile = 0;   // units and tiles so far
+  bool ok = true;
+  if (warp == 4) {
+    // ---- queries, and the positions' blocks for the scores
+    const unsigned lead_q = in_cta(qfull, 0), lead_k = in_cta(kfull, 0);
+    for (; ok && at < sh.end; ++t, ++tile) {
+      Seq s = a.seq(b);
+      for (; t >= split.tiles(s); t = 0) s = a.seq(++b);
+      const int units = split.units(s, t), end = split.sees(s, t);
+      const int u0 = (int)max(0ll, sh.begin - at), u1 = (int)min((long long)units, sh.end - at);
+      EntryRows er;
+      er.find(a.c, pr, b, u0 * kPaUnit + (int)rank * 64, 64, end);
+      ok = __all_sync(0xffffffffu, pair_wait(a.c, qempty, (tile & 1) ^ 1, dead));
+      if (!ok) break;
+      if (lane == 0) {
+        if (rank == 0) mbar_arrive_tx(qfull, 2 * kBlocks * kPaBlock);
+        const int q = s.q0 * a.heads + t * kPaRows + (int)rank * 64;   // rows behind the sequence's are not written
+        for (int d = 0; d < kBlocks - 1; ++d) load_box(base + kPaQ + d * kPaBlock, &maps.ql, d * 64, q, lead_q);
+        load_box(base + kPaQ + (kBlocks - 1) * kPaBlock, &maps.qp, 0, q, lead_q);
+      }
+      for (int u = u0; ok && u < u1; ++u, ++n) {
+        EntryRows next = er;
+        for (int d = 0; d < kBlocks; ++d) {
+          ok = __all_sync(0xffffffffu, pair_wait(a.c, kempty + 8 * d, (n & 1) ^ 1, dead));
+          if (!ok) break;
+          if (rank == 0 && lane == 0) mbar_arrive_tx(kfull + 8 * d, 2 * kPaBlock);
+          __syncwarp();
+          er.load(maps, pr, d, 64, base + kPaK + d * kPaBlock, lead_k + 8 * d);
+          if (d == 0 && u + 1 < u1) next.find(a.c, pr, b, (u + 1) * kPaUnit + (int)rank * 64, 64, end);
+        }
+        er = next;
+      }
+      at += units;
+    }
+    if (rank == 0 && lane == 0 && !ok) {   // after a failed wait: a bounded time for the copies in flight
+      mbar_wait_for(qfull, (tile & 1) ^ 1, kWaitNs);
+      for (int d = 0; d < kBlocks; ++d) mbar_wait_for(kfull + 8 * d, (n & 1) ^ 1, kWaitNs);
+    }
+    __syncwarp();
+  } else if (warp == 5) {
+    // ---- the positions' blocks for the second product: piece (h, p) is dims 256 h + 128 rank .. + 127 of positions
+    // 64 p .. + 63. Positions that no row sees have to be zeros, whatever the page holds there: row by row.
+    const unsigned lead_v = in_cta(vfull, 0);
+    PairRows one = pr;
+    one.box = 0;
+    for (; ok && at < sh.end; ++t) {
+      Seq s = a.seq(b);
+      for (; t >= split.tiles(s); t = 0) s = a.seq(++b);
+      const int units = split.units(s, t), end = split.sees(s, t);
+      const int u0 = (int)max(0ll, sh.begin - at), u1 = (int)min((long long)units, sh.end - at);
+      for (int u = u0; ok && u < u1; ++u, ++n) {
+        EntryRows er[2];
+        bool ragged[2];
+#pragma unroll
+        for (int p = 0; p < 2; ++p) {
+          const int pos = u * kPaUnit + p * 64;
+          ragged[p] = pos + 64 > end && pos < end;
+          er[p].find(a.c, ragged[p] ? one : pr, b, pos, 64, end);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int h = i >> 1, p = i & 1;
+          if (ok) ok = __all_sync(0xffffffffu, pair_wait(a.c, vempty + 8 * i, (n & 1) ^ 1, dead));
+          if (ok) {
+            if (rank == 0 && lane == 0) mbar_arrive_tx(vfull + 8 * i, 4 * kPaBlock);
+            __syncwarp();
+            const unsigned dst = base + kPaV + i * 2 * kPaBlock;
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+              er[p].load(maps, ragged[p] ? one : pr, 4 * h + 2 * (int)rank + j, 64, dst + j * kPaBlock, lead_v + 8 * i);
+          }
+        }
+      }
+      at += units;
+    }
+    if (rank == 0 && lane == 0 && !ok)
+      for (int i = 0; i < 4; ++i) mbar_wait_for(vfull + 8 * i, (n & 1) ^ 1, kWaitNs);
+    __syncwarp();
+  } else if (warp == 6) {
+    // ---- matrix instructions: one thread of the pair. Scores run one unit ahead of the second product.
+    if (lane == 0 && rank == 0) {
+      constexpr unsigned id_s = pair_idesc(128, 128), id_o = pair_idesc(128, 256) | (1u << 16);   // V is MN-major
+      const auto second = [&](int m, bool first) {   // unit number m of this worker; the first of its tile begins O
+        ok = pair_wait(a.c, pfull, m & 1, dead);
+        tc_fence_after();
+        for (int i = 0; ok && i < 4; ++i) {
+          ok = pair_wait(a.c, vfull + 8 * i, m & 1, dead);
+          if (!ok) break;
+          tc_fence_after();
+          const unsigned pa = base + kPaP + (i & 1) * kPaBlock, va = base + kPaV + i * 2 * kPaBlock;
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            pair_mma(tmem + (i >> 1) * 128, sdesc_sw128(pa + k * 32), sdesc_mn(va + k * 2048, kPaBlock), id_o,
+                     (unsigned)(!first || (i & 1) || k));
+          pair_commit(vempty + 8 * i);
+        }
+        if (ok) pair_commit(pvdone);
+      };
+      for (; ok && at < sh.end; ++t, ++tile) {
+        Seq s = a.seq(b);
+        for (; t >= split.tiles(s); t = 0) s = a.seq(++b);
+        const int units = split.units(s, t);
+        const int u0 = (int)max(0ll, sh.begin - at), u1 = (int)min((long long)units, sh.end - at);
+        ok = pair_wait(a.c, qfull, tile & 1, dead);
+        for (int u = u0; ok && u < u1; ++u, ++n) {
+          const int buf = n & 1;
+          ok = pair_wait(a.c, sfree + 8 * buf, ((n >> 1) & 1) ^ 1, dead);
+          tc_fence_after();
+          for (int d = 0; ok && d < kBlocks; ++d) {
+            ok = pair_wait(a.c, kfull + 8 * d, n & 1, dead);
+            if (!ok) break;
+            tc_fence_after();
+            const unsigned qa = base + kPaQ + d * kPaBlock, ka = base + kPaK + d * kPaBlock;
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              pair_mma(tmem_s + buf * 64, sdesc_sw128(qa + k * 32), sdesc_sw128(ka + k * 32), id_s, (unsigned)(d | k));
+            pair_commit(kempty + 8 * d);
+          }
+          if (ok) pair_commit(sfull + 8 * buf);
+          if (ok && u == u1 - 1) pair_commit(qempty);
+          if (ok && u > u0) second(n - 1, u - 1 == u0);
+        }
+        if (ok) second(n - 1, u1 - 1 == u0);
+        at += units;
+      }
+      pair_commit(done);   // all matrix instructions end before TMEM is given back
+      mbar_wait_for(done, 0, kWaitNs);
+    }
+    __syncwarp();
+  } else {
+    // ---- softmax: thread = row (64 in this CTA) and half of the positions; after a failed wait the rounds go on
+    // without work, since the warps of a row meet at barriers
+    const int half = warp >> 1, row = (warp & 1) * 32 + lane;
+    const unsigned tlane = (unsigned)(warp * 32) << 16;
+    const unsigned lead_sfree = in_cta(sfree, 0), lead_pfull = in_cta(pfull, 0);
+    const unsigned p_row = base + kPaP + half * kPaBlock + row * 128;
+    for (; at < sh.end; ++t) {
+      Seq s = a.seq(b);
+      for (; t >= split.tiles(s); t = 0) s = a.seq(++b);
+      const int units = split.units(s, t);
+      const int u0 = (int)max(0ll, sh.begin - at), u1 = (int)min((long long)units, sh.end - at);
+      const int row0 = t * kPaRows + (int)rank * 64, g = row0 + row;
+      const bool live = g < s.n * a.heads;
+      const int sees = live ? s.len - s.n + g / a.heads + 1 : 0;
+      float m = -INFINITY, l = 0.0f;
+      for (int u = u0; u < u1; ++u, ++n) {
+        const int buf = n & 1;
+        ok = __all_sync(0xffffffffu, pair_wait(a.c, sfull + 8 * buf, (n >> 1) & 1, dead)) && ok;
+        tc_fence_after();
+        float v[2][32];
+        tmem_ld32(tmem_s + buf * 64 + tlane, v[0]);
+        tmem_ld32(tmem_s + buf * 64 + tlane + 32, v[1]);
+        tmem_ld_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) arrive_cluster(lead_sfree + 8 * buf);
+        const int left = sees - u * kPaUnit - half * 64;   // positions of this thread's 64 that the row sees
+        if (!__all_sync(0xffffffffu, left >= 64)) {
+#pragma unroll
+          for (int i = 0; i < 64; ++i)
+            if (i >= left) v[i >> 5][i & 31] = -INFINITY;
+        }
+        float top = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < 64; ++i) top = fmaxf(top, v[i >> 5][i & 31]);
+        // the scale's sign decides which end of the scores is the largest
+        if (a.scale_log2 < 0.0f) {
+          top = -INFINITY;
+#pragma unroll
+          for (int i = 0; i < 64; ++i)
+            if (i < left) top = fmaxf(top, -v[i >> 5][i & 31]);
+        }
+        ctl.top[buf][half][row] = top;
+        asm volatile("bar.sync %0, 64;" ::"r"(1 + (warp & 1)) : "memory");
+        top = fmaxf(top, ctl.top[buf][half ^ 1][row]);
+        if (top != -INFINITY) top *= fabsf(a.scale_log2);
+        float alpha = 1.0f;
+        if (top > m + kPaSlack || m == -INFINITY) {
+          if (m != -INFINITY) alpha = ex2(m - top);
+          m = top;
+        }
+        const float ref = m == -INFINITY ? 0.0f : m;
+        float sum[4] = {};
+#pragma unroll
+        for (int i = 0; i < 64; ++i) {
+          float& x = v[i >> 5][i & 31];
+          x = ex2(fmaf(x, a.scale_log2, -ref));
+        }
+        if (a.scale_log2 < 0.0f || !__all_sync(0xffffffffu, left >= 64)) {
+#pragma unroll
+          for (int i = 0; i < 64; ++i)
+            if (i >= left) v[i >> 5][i & 31] = 0.0f;
+        }
+#pragma unroll
+        for (int i = 0; i < 64; ++i) sum[i & 3] += v[i >> 5][i & 31];
+        l = l * alpha + ((sum[0] + sum[1]) + (sum[2] + sum[3]));
+        // the second product of the unit before has read P and finished its sums
+        if (n > 0) ok = __all_sync(0xffffffffu, pair_wait(a.c, pvdone, (n - 1) & 1, dead)) && ok;
+        tc_fence_after();
+        if (u > u0 && __any_sync(0xffffffffu, alpha != 1.0f)) {
+#pragma unroll 1
+          for (int c = 0; c < 256; c += 32) {
+            float o[32];
+            tmem_ld32(tmem + tlane + c, o);
+            tmem_ld_wait();
+#pragma unroll
+            for (int i = 0; i < 32; ++i) o[i] *= alpha;
+            tmem_st32(tmem + tlane + c, o);
+          }
+          tmem_st_wait();
+        }
+#pragma unroll
+        for (int c = 0; c < 8; ++c) {
+          unsigned w[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int k = c * 8 + i * 2;
+            const __nv_bfloat162 h2 = __floats2bfloat162_rn(v[k >> 5][k & 31], v[k >> 5][(k & 31) + 1]);
+            w[i] = *reinterpret_cast<const unsigned*>(&h2);
+          }
+          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};"
+                       ::"r"(p_row + ((c ^ (row & 7)) << 4)), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
+        }
+        fence_async_smem();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) arrive_cluster(lead_pfull);
+      }
+      ok = __all_sync(0xffffffffu, pair_wait(a.c, pvdone, (n - 1) & 1, dead)) && ok;
+      tc_fence_after();
+      ctl.sum[half][row] = l;
+      asm volatile("bar.sync %0, 64;" ::"r"(1 + (warp & 1)) : "memory");
+      l += ctl.sum[half ^ 1][row];
+      const bool whole = u0 == 0 && u1 == units;
+      const long long out_row = (long long)s.q0 * a.heads + g;
+      float* part = a.part + (((long long)worker * 2 + (u0 == 0 ? 1 : 0)) * kPaRows + rank * 64 + row) * kPartRow;
+      const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
+#pragma unroll 1
+      for (int c = 0; c < 256; c += 32) {
+        const int dim = (c & 127) + half * 128 + (c >> 7) * 256;
+        float o[32];
+        tmem_ld32(tmem + tlane + c, o);
+        tmem_ld_wait();
+        if (!ok || !live) continue;
+        if (whole) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            __nv_bfloat162 w[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) w[k] = __floats2bfloat162_rn(o[i * 8 + k * 2] * inv, o[i * 8 + k * 2 + 1] * inv);
+            *reinterpret_cast<uint4*>(a.out + out_row * kLat + dim + i * 8) = *reinterpret_cast<const uint4*>(w);
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            *reinterpret_cast<float4*>(part + dim + i * 4) = make_float4(o[i * 4], o[i * 4 + 1], o[i * 4 + 2], o[i * 4 + 3]);
+        }
+      }
+      if (ok && live && half == 0) {
+        if (whole) {
+          a.lse[out_row] = (m + log2f(l)) * 0.69314718055994531f;
+        } else {
+          part[kLat] = m;
+          part[kLat + 1] = l;
+        }
+      }
+      if (ok && u0 == 0 && u1 < units && tid == 0 && rank == 0) {   // the workers of this tile: up to its last unit's
+        int last = worker;
+        while (sh.total * (last + 1) / sh.workers < at + units) ++last;
+        a.meta[worker * 4] = b;
+        a.meta[worker * 4 + 1] = t;
+        a.meta[worker * 4 + 2] = last - worker + 1;
+      }
+      at += units;
+      asm volatile("bar.sync %0, 64;" ::"r"(1 + (warp & 1)) : "memory");   // ctl.sum is read
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync();   // neither CTA gives up its memory while the other's instructions may use it
+  if (warp == 6) pair_dealloc(tmem, 512);
+}
+
+// ---------------------------------------------------------------------------------------------
 // host side
 
 static int encode_rows(CUtensorMap* map, const void* base, int cols, int64_t rows, int64_t pitch, int box) {
@@ -500,6 +886,18 @@ static int pair_maps(const kk3_cache* c, const void* q_latent, int64_t ql_token,
   if (!rc) rc = map_queries(&m->ql, q_latent, kLat, tokens, heads, ql_token, ql_head, q_box);
   if (!rc) rc = map_queries(&m->qp, q_pe, kRope, tokens, heads, qp_token, qp_head, q_box);
   return rc;
+}
+
+int attend_pair(const kk3_cache* c, const AttendArgs& a, cudaStream_t st) {
+  PairMaps maps;
+  PairRows pr;
+  int r = pair_maps(c, a.q_lat, a.ql_tok, a.ql_head, a.q_pe, a.qp_tok, a.qp_head, a.tokens, a.heads, 64, &maps, &pr);
+  if (r) return r;
+  static std::atomic<bool> ready[kCacheMaxDevices];
+  r = cache_allow_smem(kk3_cache_attend_pair_kernel, kPaSmem, ready, "cudaFuncSetAttribute(kk3_cache_attend_pair_kernel)");
+  if (r) return r;
+  kk3_cache_attend_pair_kernel<<<a.workers * 2, kPaThreads, kPaSmem, st>>>(a, pr, maps);
+  return cache_cuda(cudaGetLastError(), "kk3_cache_attend_pair_kernel");
 }
 
 // rows of a matrix instruction for the average rows of a sequence: the smallest of 32, 64, 128 and 256 that holds
