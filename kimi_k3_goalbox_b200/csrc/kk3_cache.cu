@@ -126,7 +126,7 @@ constexpr int kWaPitch = kEntry + 8;      // 1168-byte rows: consecutive rows fa
 constexpr int kWaPPitch = kWaUnit + 8;
 constexpr int kWaThreads = 256;
 constexpr int kWaMinUnits = 4;
-constexpr int64_t kWarpRowsMost = 16;     // average rows of a sequence up to which this kernel is taken
+constexpr int64_t kWarpRowsMost = 0;     // average rows of a sequence up to which this kernel is taken
 struct WaSmem {
   bf16 ring[kWaStages][kWaUnit][kWaPitch];
   bf16 q[kWaRows][kWaPitch];
@@ -678,8 +678,8 @@ struct Plan {
   int workers, rows;
 };
 static Plan attend_plan(int64_t batch, int64_t tokens, int64_t heads, int sms) {
-  const bool pair = tokens * heads > kWarpRowsMost * batch;
-  return pair ? Plan{true, sms / 2, kPairRows} : Plan{false, sms, kWaRows};
+  if (tokens * heads <= kWarpRowsMost * batch) return Plan{false, sms, kWaRows};
+  return Plan{true, sms / 2, kPairRows};
 }
 
 extern "C" int64_t kk3_cache_attend_workspace(int batch, int tokens, int heads) {

@@ -93,6 +93,7 @@ struct AttendArgs : CallSeqs {
   float* lse;            // [tokens, heads]
   float* part;           // [workers][2][tile rows][kPartRow]: running sums of tiles that several workers share
 };
+constexpr int kPairRows = 128;        // tile of the CTA-pair kernel
 constexpr int kPartRow = kLat + 4;   // 512 sums, running maximum, running sum, padding to 16 bytes
 
 struct MassArgs : CallSeqs {

@@ -16,8 +16,7 @@ int cache_cuda(cudaError_t e, const char* what);
 inline bool cache_aligned(const void* p, size_t n) { return p && (uintptr_t)p % n == 0; }
 // checks a kk3_cache and turns it into the kernels' form
 int cache_pages(const kk3_cache* c, CachePages* out, int* error_word);
-// attention by CTA pairs (kk3_cache_tc.cu): a.workers pairs, tiles of kPairRows rows
-constexpr int kPairRows = 128;
+// attention by CTA pairs (kk3_cache_tc.cu): a.workers pairs
 int attend_pair(const kk3_cache* c, const AttendArgs& a, cudaStream_t st);
 // SMs of the current device, looked up once per device
 int cache_sms(int* sms);

@@ -50,7 +50,10 @@ KK3_DEV void cluster_sync() {
 KK3_DEV void arrive_cluster(unsigned addr) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(addr) : "memory");
 }
-KK3_DEV bool pair_test(unsigned bar, unsigned parity) {
+// Bounded wait; false when it ran out or another role of the CTA gave up (*dead). For barriers that copies and matrix
+// instructions complete. A wait at cluster scope (pair_wait_peer) costs some hundred clocks more, so it is kept for
+// the barriers on which threads of the other CTA arrive.
+KK3_DEV bool pair_test_peer(unsigned bar, unsigned parity) {
   unsigned ok;
   asm volatile(
       "{\n .reg .pred p;\n mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n"
@@ -58,13 +61,13 @@ KK3_DEV bool pair_test(unsigned bar, unsigned parity) {
       : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
   return ok != 0;
 }
-// Bounded wait; false when it ran out or another role of the CTA gave up (*dead).
-KK3_DEV bool pair_wait(const CachePages& c, unsigned bar, unsigned parity, volatile int* dead) {
-  if (pair_test(bar, parity)) return true;
+template <bool PEER>
+KK3_DEV bool pair_wait_as(const CachePages& c, unsigned bar, unsigned parity, volatile int* dead) {
+  if (PEER ? pair_test_peer(bar, parity) : mbar_test(bar, parity)) return true;
   if (*dead) return false;
   const unsigned long long t0 = globaltimer();
   for (unsigned spin = 1;; ++spin) {
-    if (pair_test(bar, parity)) return true;
+    if (PEER ? pair_test_peer(bar, parity) : mbar_test(bar, parity)) return true;
     if ((spin & 15) == 0) {
       if (*dead) return false;
       if (globaltimer() - t0 > kWaitNs) {
@@ -74,6 +77,12 @@ KK3_DEV bool pair_wait(const CachePages& c, unsigned bar, unsigned parity, volat
       }
     }
   }
+}
+KK3_DEV bool pair_wait(const CachePages& c, unsigned bar, unsigned parity, volatile int* dead) {
+  return pair_wait_as<false>(c, bar, parity, dead);
+}
+KK3_DEV bool pair_wait_peer(const CachePages& c, unsigned bar, unsigned parity, volatile int* dead) {
+  return pair_wait_as<true>(c, bar, parity, dead);
 }
 // Rows row[0..3] of 64 elements from column x into 512 bytes of this CTA's shared memory; the bytes are counted on
 // `bar`, a barrier of either CTA of the pair.
@@ -317,7 +326,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMassThreads, 1)
         const int u0 = (int)max(0ll, sh.begin - at), u1 = (int)min((long long)units, sh.end - at);
         for (int u = u0; ok && u < u1; ++u, ++unit) {
           const int buf = unit & 1;
-          ok = pair_wait(a.c, dempty + 8 * buf, ((unit >> 1) & 1) ^ 1, dead);
+          ok = pair_wait_peer(a.c, dempty + 8 * buf, ((unit >> 1) & 1) ^ 1, dead);
           tc_fence_after();
           for (int d = 0; ok && d < kBlocks; ++d, ++job) {
             const int slot = job % slots;
@@ -449,36 +458,40 @@ __global__ void __launch_bounds__(kMassPos) kk3_cache_mass_join_kernel(const Mas
 // ---------------------------------------------------------------------------------------------
 // Attention: s = scale (q . e_p), running maximum m and sum l per row, O = O 2^(m - m') + sum_p 2^(s_p - m') c_p.
 //
-// A tile is 128 (token, head) rows of one sequence, 64 in each CTA, a unit 128 positions. The FP32 sums of 512 output
-// dims for 128 rows fill a whole TMEM, so the pair's M = 128 form carries them: 64 rows in either CTA, half of the
-// columns in lanes 0-63 and half in lanes 64-127, 256 columns in all, which leaves room for two score buffers. For the
-// scores each CTA loads 64 of the 128 positions (nine blocks of 8 KB), for the second product half of the output dims
-// of all 128 (four pieces of 16 KB, the same bytes in the other operand order); both rings hold one unit, and a block
-// is requested again as soon as its last instruction is done, a whole unit ahead of its use.
+// A tile is 128 (token, head) rows of one sequence, 64 in each CTA, a unit 256 positions. The FP32 sums of 512 output
+// dims for 128 rows would fill TMEM; the pair's M = 128 form spreads them over both CTAs (64 rows in either, half of
+// an instruction's columns in lanes 0-63 and half in lanes 64-127), 256 columns in all, next to two score buffers of
+// 128. Every instruction has 256 columns: one takes 64 clocks then, and about as much to issue whatever its size (57
+// clocks measured, 175 more for a commit), so narrower ones would leave the tensor cores waiting.
 //
-// Thread = row and half of a unit's positions. The running maximum moves only when it is exceeded by more than 2^8
-// (probabilities stay below 256, harmless in BF16 and FP32), so the sums in TMEM are rarely rescaled. Probabilities
-// are rounded to BF16 for the second product, the type that the instruction takes with BF16 latents; the running sum
-// adds them unrounded, since lse is an FP32 result.
+// Per unit each CTA loads 128 of the positions (nine blocks of 64 dims, 16 KB) for the scores, and half of the output
+// dims of all 256 (four stages of 64 positions x 2 x 128 dims) for the sums, through a ring of three 32 KB stages in the
+// order of their use; the rope block has a slot of its own. Scores run one unit ahead of sums.
 //
-// Bounds of a unit: 2176 clocks of tensor time (128 x 128 x 1088 products at 4096 a clock and SM), 1920 of
-// shared-memory reads, 139 KB of loads in each SM (64 bytes a clock, mostly from L2).
+// Softmax: four threads per row, 64 of a unit's positions each, that exchange maxima through shared memory. The running
+// maximum moves only when it is exceeded by more than 2^8 (probabilities stay below 256, harmless in BF16 and FP32), so
+// the sums in TMEM are rarely rescaled. Probabilities are rounded to BF16 for the second product, the type that the
+// instruction takes with BF16 latents; the running sum adds them unrounded, since lse is an FP32 result.
+//
+// Bounds of a unit: 4352 clocks of tensor time (128 x 256 x 1088 products at 4096 a clock and SM) and 9 commits, 278 KB
+// of loads in each SM (mostly from L2); for few rows the 294 KB per pair from HBM.
 
-constexpr int kPaRows = 128, kPaUnit = 128;
-constexpr int kPaThreads = 224;      // warps 0-3 softmax, 4 queries and score blocks, 5 value blocks, 6 instructions
-constexpr int kPaBlock = 64 * 128;   // 64 rows of 64 dims
-constexpr int kPaMinUnits = 2;
+constexpr int kPaUnit = 256;
+constexpr int kPaThreads = 320;        // warps 0-7 softmax, 8 copies, 9 instructions and TMEM
+constexpr int kPaQBlock = 64 * 128;    // 64 rows of 64 dims
+constexpr int kPaBlock = 128 * 128;    // 128 positions x 64 dims, or 64 positions x 128 dims
+constexpr int kPaStages = 3;
+constexpr int kPaMinUnits = 1;
 constexpr float kPaSlack = 8.0f;
 struct PaCtl {
-  unsigned long long qfull, qempty, kfull[kBlocks], kempty[kBlocks], vfull[4], vempty[4], sfull[2], sfree[2], pfull, pvdone, done;
+  unsigned long long qfull, qempty, full[kPaStages], empty[kPaStages], pefull, peempty, sfull[2], sfree[2], pfull, pvdone, done;
   unsigned tmem;
   int dead;
   long long red[kPaThreads / 32 + 4];
-  float top[2][2][64];   // [unit parity][half][row]: row maxima of the halves
-  float sum[2][64];      // [half][row]
+  float top[2][4][64];   // [unit parity][64 positions of 256][row]: maxima (at the end: sums) of a row's four threads
 };
-constexpr int kPaQ = 0, kPaK = kPaQ + kBlocks * kPaBlock, kPaV = kPaK + kBlocks * kPaBlock, kPaP = kPaV + 8 * kPaBlock,
-              kPaCtl = kPaP + 2 * kPaBlock;
+constexpr int kPaQ = 0, kPaP = kPaQ + kBlocks * kPaQBlock, kPaRing = kPaP + 4 * kPaQBlock,
+              kPaPe = kPaRing + kPaStages * 2 * kPaBlock, kPaCtl = kPaPe + kPaBlock;
 constexpr int kPaSmem = kPaCtl + (int)sizeof(PaCtl);
 static_assert(kPaSmem <= 232448, "shared memory of a CTA");
 
@@ -505,7 +518,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPaThreads, 1)
   PaCtl& ctl = *reinterpret_cast<PaCtl*>(smem_raw + kPaCtl);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, worker = blockIdx.x >> 1;
   const unsigned rank = cluster_rank(), base = smem_u32(smem_raw);
-  const AttendSplit split{kPaRows, a.heads, kPaUnit};
+  const AttendSplit split{kPairRows, a.heads, kPaUnit};
   const Share sh = plan_share<kPaThreads>(a, split, worker, kPaMinUnits, reinterpret_cast<int*>(smem_raw), ctl.red);
   if (tid == 0 && rank == 0) a.meta[worker * 4 + 2] = 0;
   if (base & 1023u) {   // the swizzled blocks need a 1024-byte boundary, which dynamic shared memory begins on
@@ -513,137 +526,146 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPaThreads, 1)
     return;
   }
   if (worker >= sh.workers) return;   // both CTAs of the pair
-  const unsigned qfull = smem_u32(&ctl.qfull), qempty = smem_u32(&ctl.qempty), kfull = smem_u32(ctl.kfull),
-                 kempty = smem_u32(ctl.kempty), vfull = smem_u32(ctl.vfull), vempty = smem_u32(ctl.vempty),
+  const unsigned qfull = smem_u32(&ctl.qfull), qempty = smem_u32(&ctl.qempty), full = smem_u32(ctl.full),
+                 empty = smem_u32(ctl.empty), pefull = smem_u32(&ctl.pefull), peempty = smem_u32(&ctl.peempty),
                  sfull = smem_u32(ctl.sfull), sfree = smem_u32(ctl.sfree), pfull = smem_u32(&ctl.pfull),
                  pvdone = smem_u32(&ctl.pvdone), done = smem_u32(&ctl.done);
   volatile int* dead = &ctl.dead;
   if (tid == 0) {
     mbar_init(qfull, 1);
     mbar_init(qempty, 1);
-    for (int i = 0; i < kBlocks; ++i) {
-      mbar_init(kfull + 8 * i, 1);
-      mbar_init(kempty + 8 * i, 1);
+    for (int i = 0; i < kPaStages; ++i) {
+      mbar_init(full + 8 * i, 1);
+      mbar_init(empty + 8 * i, 1);
     }
-    for (int i = 0; i < 4; ++i) {
-      mbar_init(vfull + 8 * i, 1);
-      mbar_init(vempty + 8 * i, 1);
-    }
+    mbar_init(pefull, 1);
+    mbar_init(peempty, 1);
     for (int i = 0; i < 2; ++i) {
       mbar_init(sfull + 8 * i, 1);
-      mbar_init(sfree + 8 * i, 8);   // four warps of either CTA
+      mbar_init(sfree + 8 * i, 16);   // the softmax warps of both CTAs
     }
-    mbar_init(pfull, 8);
+    mbar_init(pfull, 16);
     mbar_init(pvdone, 1);
     mbar_init(done, 1);
     ctl.dead = 0;
     fence_mbar_init();
   }
-  if (warp == 6) pair_alloc(smem_u32(&ctl.tmem), 512);
+  if (warp == 9) pair_alloc(smem_u32(&ctl.tmem), 512);
   tc_fence_before();
   __syncthreads();
   cluster_sync();
   tc_fence_after();
   const unsigned tmem = *reinterpret_cast<volatile unsigned*>(&ctl.tmem);
-  const unsigned tmem_s = tmem + 256;
+  const unsigned tmem_s = tmem + 256;   // two score buffers of 128 columns; the sums have 256 before them
 
   int b = sh.b, t = sh.t;
   long long at = sh.at;
-  int n = 0, tile = 0;   // units and tiles so far
+  int n = 0, tile = 0, job = 0;   // units, tiles and ring stages so far
   bool ok = true;
-  if (warp == 4) {
-    // ---- queries, and the positions' blocks for the scores
-    const unsigned lead_q = in_cta(qfull, 0), lead_k = in_cta(kfull, 0);
+  if (warp == 8) {
+    // ---- copies
+    const unsigned lead_q = in_cta(qfull, 0), lead_full = in_cta(full, 0), lead_pe = in_cta(pefull, 0);
+    PairRows single = pr;   // positions that no row sees must be zeros in the second product: row by row
+    single.box = 0;
+    const auto begin = [&](unsigned* bar) -> unsigned {   // the next stage, empty and expecting its bytes: its address
+      const int st = job % kPaStages;
+      ok = __all_sync(0xffffffffu, pair_wait(a.c, empty + 8 * st, ((job / kPaStages) & 1) ^ 1, dead));
+      if (ok && rank == 0 && lane == 0) mbar_arrive_tx(full + 8 * st, 4 * kPaBlock);
+      __syncwarp();
+      *bar = lead_full + 8 * st;
+      return base + kPaRing + st * 2 * kPaBlock;
+    };
     for (; ok && at < sh.end; ++t, ++tile) {
       Seq s = a.seq(b);
       for (; t >= split.tiles(s); t = 0) s = a.seq(++b);
       const int units = split.units(s, t), end = split.sees(s, t);
       const int u0 = (int)max(0ll, sh.begin - at), u1 = (int)min((long long)units, sh.end - at);
-      EntryRows er;
-      er.find(a.c, pr, b, u0 * kPaUnit + (int)rank * 64, 64, end);
+      // rows of a unit's entries, found one unit ahead: this CTA's 128 positions, and all 256 in groups of 64
+      EntryRows ek, ev[4], ek_next, ev_next[4];
+      unsigned cut = 0, cut_next = 0;   // groups that `end` cuts
+      const auto find = [&](int u) {
+        ek_next.find(a.c, pr, b, u * kPaUnit + (int)rank * 128, 128, end);
+        cut_next = 0;
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const int pos = u * kPaUnit + g * 64;
+          const bool c = pos < end && end < pos + 64;
+          ev_next[g].find(a.c, c ? single : pr, b, pos, 64, end);
+          cut_next |= (unsigned)c << g;
+        }
+      };
+      const auto values = [&]() {
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          unsigned bar;
+          const unsigned dst = begin(&bar);
+          if (!ok) break;
+#pragma unroll
+          for (int i = 0; i < 4; ++i)   // (dims 256 h + 128 rank + 64 j)
+            ev[g].load(maps, cut >> g & 1 ? single : pr, 4 * (i >> 1) + 2 * (int)rank + (i & 1), 64, dst + i * (kPaBlock / 2), bar);
+          ++job;
+        }
+      };
+      find(u0);
       ok = __all_sync(0xffffffffu, pair_wait(a.c, qempty, (tile & 1) ^ 1, dead));
       if (!ok) break;
       if (lane == 0) {
-        if (rank == 0) mbar_arrive_tx(qfull, 2 * kBlocks * kPaBlock);
-        const int q = s.q0 * a.heads + t * kPaRows + (int)rank * 64;   // rows behind the sequence's are not written
-        for (int d = 0; d < kBlocks - 1; ++d) load_box(base + kPaQ + d * kPaBlock, &maps.ql, d * 64, q, lead_q);
-        load_box(base + kPaQ + (kBlocks - 1) * kPaBlock, &maps.qp, 0, q, lead_q);
+        if (rank == 0) mbar_arrive_tx(qfull, 2 * kBlocks * kPaQBlock);
+        const int q = s.q0 * a.heads + t * kPairRows + (int)rank * 64;   // rows behind the sequence's are not written
+        for (int d = 0; d < kBlocks - 1; ++d) load_box(base + kPaQ + d * kPaQBlock, &maps.ql, d * 64, q, lead_q);
+        load_box(base + kPaQ + (kBlocks - 1) * kPaQBlock, &maps.qp, 0, q, lead_q);
       }
       for (int u = u0; ok && u < u1; ++u, ++n) {
-        EntryRows next = er;
-        for (int d = 0; d < kBlocks; ++d) {
-          ok = __all_sync(0xffffffffu, pair_wait(a.c, kempty + 8 * d, (n & 1) ^ 1, dead));
+        ek = ek_next;
+        for (int d = 0; d < kBlocks - 1; d += 2) {
+          unsigned bar;
+          const unsigned dst = begin(&bar);
           if (!ok) break;
-          if (rank == 0 && lane == 0) mbar_arrive_tx(kfull + 8 * d, 2 * kPaBlock);
-          __syncwarp();
-          er.load(maps, pr, d, 64, base + kPaK + d * kPaBlock, lead_k + 8 * d);
-          if (d == 0 && u + 1 < u1) next.find(a.c, pr, b, (u + 1) * kPaUnit + (int)rank * 64, 64, end);
+          ek.load(maps, pr, d, 128, dst, bar);
+          ek.load(maps, pr, d + 1, 128, dst + kPaBlock, bar);
+          ++job;
         }
-        er = next;
+        if (ok) ok = __all_sync(0xffffffffu, pair_wait(a.c, peempty, (n & 1) ^ 1, dead));
+        if (!ok) break;
+        if (rank == 0 && lane == 0) mbar_arrive_tx(pefull, 2 * kPaBlock);
+        __syncwarp();
+        ek.load(maps, pr, kBlocks - 1, 128, base + kPaPe, lead_pe);
+        if (u > u0) values();
+#pragma unroll
+        for (int g = 0; g < 4; ++g) ev[g] = ev_next[g];
+        cut = cut_next;
+        if (ok && u + 1 < u1) find(u + 1);
       }
+      if (ok) values();
       at += units;
     }
     if (rank == 0 && lane == 0 && !ok) {   // after a failed wait: a bounded time for the copies in flight
       mbar_wait_for(qfull, (tile & 1) ^ 1, kWaitNs);
-      for (int d = 0; d < kBlocks; ++d) mbar_wait_for(kfull + 8 * d, (n & 1) ^ 1, kWaitNs);
+      mbar_wait_for(pefull, (n & 1) ^ 1, kWaitNs);
+      for (int j = max(0, job - kPaStages); j < job; ++j)
+        mbar_wait_for(full + 8 * (j % kPaStages), (j / kPaStages) & 1, kWaitNs);
     }
     __syncwarp();
-  } else if (warp == 5) {
-    // ---- the positions' blocks for the second product: piece (h, p) is dims 256 h + 128 rank .. + 127 of positions
-    // 64 p .. + 63. Positions that no row sees have to be zeros, whatever the page holds there: row by row.
-    const unsigned lead_v = in_cta(vfull, 0);
-    PairRows one = pr;
-    one.box = 0;
-    for (; ok && at < sh.end; ++t) {
-      Seq s = a.seq(b);
-      for (; t >= split.tiles(s); t = 0) s = a.seq(++b);
-      const int units = split.units(s, t), end = split.sees(s, t);
-      const int u0 = (int)max(0ll, sh.begin - at), u1 = (int)min((long long)units, sh.end - at);
-      for (int u = u0; ok && u < u1; ++u, ++n) {
-        EntryRows er[2];
-        bool ragged[2];
-#pragma unroll
-        for (int p = 0; p < 2; ++p) {
-          const int pos = u * kPaUnit + p * 64;
-          ragged[p] = pos + 64 > end && pos < end;
-          er[p].find(a.c, ragged[p] ? one : pr, b, pos, 64, end);
-        }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int h = i >> 1, p = i & 1;
-          if (ok) ok = __all_sync(0xffffffffu, pair_wait(a.c, vempty + 8 * i, (n & 1) ^ 1, dead));
-          if (ok) {
-            if (rank == 0 && lane == 0) mbar_arrive_tx(vfull + 8 * i, 4 * kPaBlock);
-            __syncwarp();
-            const unsigned dst = base + kPaV + i * 2 * kPaBlock;
-#pragma unroll
-            for (int j = 0; j < 2; ++j)
-              er[p].load(maps, ragged[p] ? one : pr, 4 * h + 2 * (int)rank + j, 64, dst + j * kPaBlock, lead_v + 8 * i);
-          }
-        }
-      }
-      at += units;
-    }
-    if (rank == 0 && lane == 0 && !ok)
-      for (int i = 0; i < 4; ++i) mbar_wait_for(vfull + 8 * i, (n & 1) ^ 1, kWaitNs);
-    __syncwarp();
-  } else if (warp == 6) {
-    // ---- matrix instructions: one thread of the pair. Scores run one unit ahead of the second product.
+  } else if (warp == 9) {
+    // ---- matrix instructions: one thread of the pair
     if (lane == 0 && rank == 0) {
-      constexpr unsigned id_s = pair_idesc(128, 128), id_o = pair_idesc(128, 256) | (1u << 16);   // V is MN-major
-      const auto second = [&](int m, bool first) {   // unit number m of this worker; the first of its tile begins O
-        ok = pair_wait(a.c, pfull, m & 1, dead);
+      constexpr unsigned id_s = pair_idesc(128, 256), id_o = id_s | (1u << 16);   // values are MN-major
+      const auto sums = [&](int m, bool first) {   // unit number m of this worker; the first of its tile begins O
+        ok = pair_wait_peer(a.c, pfull, m & 1, dead);
         tc_fence_after();
-        for (int i = 0; ok && i < 4; ++i) {
-          ok = pair_wait(a.c, vfull + 8 * i, m & 1, dead);
+        for (int g = 0; ok && g < 4; ++g, ++job) {
+          const int st = job % kPaStages;
+          ok = pair_wait(a.c, full + 8 * st, (job / kPaStages) & 1, dead);
           if (!ok) break;
           tc_fence_after();
-          const unsigned pa = base + kPaP + (i & 1) * kPaBlock, va = base + kPaV + i * 2 * kPaBlock;
+          const unsigned va = base + kPaRing + st * 2 * kPaBlock, pa = base + kPaP + g * kPaQBlock;
 #pragma unroll
-          for (int k = 0; k < 4; ++k)
-            pair_mma(tmem + (i >> 1) * 128, sdesc_sw128(pa + k * 32), sdesc_mn(va + k * 2048, kPaBlock), id_o,
-                     (unsigned)(!first || (i & 1) || k));
-          pair_commit(vempty + 8 * i);
+          for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              pair_mma(tmem + h * 128, sdesc_sw128(pa + k * 32), sdesc_mn(va + h * kPaBlock + k * 2048, kPaBlock / 2), id_o,
+                       (unsigned)(!first || g || k));
+          pair_commit(empty + 8 * st);
         }
         if (ok) pair_commit(pvdone);
       };
@@ -655,23 +677,33 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPaThreads, 1)
         ok = pair_wait(a.c, qfull, tile & 1, dead);
         for (int u = u0; ok && u < u1; ++u, ++n) {
           const int buf = n & 1;
-          ok = pair_wait(a.c, sfree + 8 * buf, ((n >> 1) & 1) ^ 1, dead);
+          ok = pair_wait_peer(a.c, sfree + 8 * buf, ((n >> 1) & 1) ^ 1, dead);
           tc_fence_after();
-          for (int d = 0; ok && d < kBlocks; ++d) {
-            ok = pair_wait(a.c, kfull + 8 * d, n & 1, dead);
+          const unsigned d = tmem_s + buf * 128;
+          for (int i = 0; ok && i < (kBlocks - 1) / 2; ++i, ++job) {
+            const int st = job % kPaStages;
+            ok = pair_wait(a.c, full + 8 * st, (job / kPaStages) & 1, dead);
             if (!ok) break;
             tc_fence_after();
-            const unsigned qa = base + kPaQ + d * kPaBlock, ka = base + kPaK + d * kPaBlock;
+            const unsigned qa = base + kPaQ + i * 2 * kPaQBlock, ka = base + kPaRing + st * 2 * kPaBlock;
 #pragma unroll
-            for (int k = 0; k < 4; ++k)
-              pair_mma(tmem_s + buf * 64, sdesc_sw128(qa + k * 32), sdesc_sw128(ka + k * 32), id_s, (unsigned)(d | k));
-            pair_commit(kempty + 8 * d);
+            for (int k = 0; k < 8; ++k)
+              pair_mma(d, sdesc_sw128(qa + (k >> 2) * kPaQBlock + (k & 3) * 32),
+                       sdesc_sw128(ka + (k >> 2) * kPaBlock + (k & 3) * 32), id_s, (unsigned)(i | k));
+            pair_commit(empty + 8 * st);
           }
-          if (ok) pair_commit(sfull + 8 * buf);
-          if (ok && u == u1 - 1) pair_commit(qempty);
-          if (ok && u > u0) second(n - 1, u - 1 == u0);
+          if (ok) ok = pair_wait(a.c, pefull, n & 1, dead);
+          if (!ok) break;
+          tc_fence_after();
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            pair_mma(d, sdesc_sw128(base + kPaQ + (kBlocks - 1) * kPaQBlock + k * 32), sdesc_sw128(base + kPaPe + k * 32), id_s, 1u);
+          pair_commit(peempty);
+          pair_commit(sfull + 8 * buf);
+          if (u == u1 - 1) pair_commit(qempty);
+          if (u > u0) sums(n - 1, u - 1 == u0);
         }
-        if (ok) second(n - 1, u1 - 1 == u0);
+        if (ok) sums(n - 1, u1 - 1 == u0);
         at += units;
       }
       pair_commit(done);   // all matrix instructions end before TMEM is given back
@@ -679,18 +711,20 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPaThreads, 1)
     }
     __syncwarp();
   } else {
-    // ---- softmax: thread = row (64 in this CTA) and half of the positions; after a failed wait the rounds go on
-    // without work, since the warps of a row meet at barriers
-    const int half = warp >> 1, row = (warp & 1) * 32 + lane;
-    const unsigned tlane = (unsigned)(warp * 32) << 16;
+    // ---- softmax: a row's four threads are in the warps of equal parity, 64 positions of a unit each; after a failed
+    // wait the rounds go on without work, since they meet at barriers
+    const int wg = warp >> 2, quarter = warp & 3, row = (quarter & 1) * 32 + lane;
+    const int part64 = (quarter >> 1) * 2 + wg;   // which 64 positions of the unit
+    const unsigned tlane = (unsigned)(quarter * 32) << 16, meet = 1 + (quarter & 1);
     const unsigned lead_sfree = in_cta(sfree, 0), lead_pfull = in_cta(pfull, 0);
-    const unsigned p_row = base + kPaP + half * kPaBlock + row * 128;
+    const unsigned p_row = base + kPaP + part64 * kPaQBlock + row * 128;
+    const float sign = a.scale_log2 < 0.0f ? -1.0f : 1.0f, size = fabsf(a.scale_log2);
     for (; at < sh.end; ++t) {
       Seq s = a.seq(b);
       for (; t >= split.tiles(s); t = 0) s = a.seq(++b);
       const int units = split.units(s, t);
       const int u0 = (int)max(0ll, sh.begin - at), u1 = (int)min((long long)units, sh.end - at);
-      const int row0 = t * kPaRows + (int)rank * 64, g = row0 + row;
+      const int g = t * kPairRows + (int)rank * 64 + row;
       const bool live = g < s.n * a.heads;
       const int sees = live ? s.len - s.n + g / a.heads + 1 : 0;
       float m = -INFINITY, l = 0.0f;
@@ -699,64 +733,64 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPaThreads, 1)
         ok = __all_sync(0xffffffffu, pair_wait(a.c, sfull + 8 * buf, (n >> 1) & 1, dead)) && ok;
         tc_fence_after();
         float v[2][32];
-        tmem_ld32(tmem_s + buf * 64 + tlane, v[0]);
-        tmem_ld32(tmem_s + buf * 64 + tlane + 32, v[1]);
+        tmem_ld32(tmem_s + buf * 128 + wg * 64 + tlane, v[0]);
+        tmem_ld32(tmem_s + buf * 128 + wg * 64 + 32 + tlane, v[1]);
         tmem_ld_wait();
         tc_fence_before();
         __syncwarp();
         if (lane == 0) arrive_cluster(lead_sfree + 8 * buf);
-        const int left = sees - u * kPaUnit - half * 64;   // positions of this thread's 64 that the row sees
-        if (!__all_sync(0xffffffffu, left >= 64)) {
+        const int left = sees - u * kPaUnit - part64 * 64;   // positions of this thread's 64 that the row sees
+        const bool cut = !__all_sync(0xffffffffu, left >= 64);
+        if (a.scale_log2 < 0.0f) {
+#pragma unroll
+          for (int i = 0; i < 64; ++i) v[i >> 5][i & 31] *= sign;
+        }
+        if (cut) {
 #pragma unroll
           for (int i = 0; i < 64; ++i)
             if (i >= left) v[i >> 5][i & 31] = -INFINITY;
         }
-        float top = -INFINITY;
+        float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-        for (int i = 0; i < 64; ++i) top = fmaxf(top, v[i >> 5][i & 31]);
-        // the scale's sign decides which end of the scores is the largest
-        if (a.scale_log2 < 0.0f) {
-          top = -INFINITY;
+        for (int i = 0; i < 64; ++i) tops[i & 3] = fmaxf(tops[i & 3], v[i >> 5][i & 31]);
+        float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+        ctl.top[buf][part64][row] = top;
+        asm volatile("bar.sync %0, 128;" ::"r"(meet) : "memory");
 #pragma unroll
-          for (int i = 0; i < 64; ++i)
-            if (i < left) top = fmaxf(top, -v[i >> 5][i & 31]);
-        }
-        ctl.top[buf][half][row] = top;
-        asm volatile("bar.sync %0, 64;" ::"r"(1 + (warp & 1)) : "memory");
-        top = fmaxf(top, ctl.top[buf][half ^ 1][row]);
-        if (top != -INFINITY) top *= fabsf(a.scale_log2);
+        for (int i = 0; i < 4; ++i) top = fmaxf(top, ctl.top[buf][i][row]);
+        if (top != -INFINITY) top *= size;
         float alpha = 1.0f;
         if (top > m + kPaSlack || m == -INFINITY) {
           if (m != -INFINITY) alpha = ex2(m - top);
           m = top;
         }
         const float ref = m == -INFINITY ? 0.0f : m;
-        float sum[4] = {};
 #pragma unroll
         for (int i = 0; i < 64; ++i) {
           float& x = v[i >> 5][i & 31];
-          x = ex2(fmaf(x, a.scale_log2, -ref));
+          x = ex2(fmaf(x, size, -ref));
         }
-        if (a.scale_log2 < 0.0f || !__all_sync(0xffffffffu, left >= 64)) {
+        if (cut && size == 0.0f) {   // -infinity times a scale of zero is no -infinity
 #pragma unroll
           for (int i = 0; i < 64; ++i)
             if (i >= left) v[i >> 5][i & 31] = 0.0f;
         }
+        float sum[4] = {};
 #pragma unroll
         for (int i = 0; i < 64; ++i) sum[i & 3] += v[i >> 5][i & 31];
         l = l * alpha + ((sum[0] + sum[1]) + (sum[2] + sum[3]));
-        // the second product of the unit before has read P and finished its sums
+        // the sums of the unit before have read P and are done
         if (n > 0) ok = __all_sync(0xffffffffu, pair_wait(a.c, pvdone, (n - 1) & 1, dead)) && ok;
         tc_fence_after();
         if (u > u0 && __any_sync(0xffffffffu, alpha != 1.0f)) {
 #pragma unroll 1
-          for (int c = 0; c < 256; c += 32) {
+          for (int c = 0; c < 128; c += 32) {
             float o[32];
-            tmem_ld32(tmem + tlane + c, o);
+            tmem_ld32(tmem + wg * 128 + tlane + c, o);
             tmem_ld_wait();
 #pragma unroll
             for (int i = 0; i < 32; ++i) o[i] *= alpha;
-            tmem_st32(tmem + tlane + c, o);
+            tmem_st32(tmem + wg * 128 + tlane + c, o);
           }
           tmem_st_wait();
         }
@@ -779,18 +813,19 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPaThreads, 1)
       }
       ok = __all_sync(0xffffffffu, pair_wait(a.c, pvdone, (n - 1) & 1, dead)) && ok;
       tc_fence_after();
-      ctl.sum[half][row] = l;
-      asm volatile("bar.sync %0, 64;" ::"r"(1 + (warp & 1)) : "memory");
-      l += ctl.sum[half ^ 1][row];
+      asm volatile("bar.sync %0, 128;" ::"r"(meet) : "memory");   // the last maxima are read
+      ctl.top[0][part64][row] = l;
+      asm volatile("bar.sync %0, 128;" ::"r"(meet) : "memory");
+      l = (ctl.top[0][0][row] + ctl.top[0][1][row]) + (ctl.top[0][2][row] + ctl.top[0][3][row]);
       const bool whole = u0 == 0 && u1 == units;
       const long long out_row = (long long)s.q0 * a.heads + g;
-      float* part = a.part + (((long long)worker * 2 + (u0 == 0 ? 1 : 0)) * kPaRows + rank * 64 + row) * kPartRow;
+      float* part = a.part + (((long long)worker * 2 + (u0 == 0 ? 1 : 0)) * kPairRows + rank * 64 + row) * kPartRow;
       const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
 #pragma unroll 1
-      for (int c = 0; c < 256; c += 32) {
-        const int dim = (c & 127) + half * 128 + (c >> 7) * 256;
+      for (int c = 0; c < 128; c += 32) {
+        const int dim = wg * 256 + (quarter >> 1) * 128 + c;
         float o[32];
-        tmem_ld32(tmem + tlane + c, o);
+        tmem_ld32(tmem + wg * 128 + tlane + c, o);
         tmem_ld_wait();
         if (!ok || !live) continue;
         if (whole) {
@@ -807,7 +842,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPaThreads, 1)
             *reinterpret_cast<float4*>(part + dim + i * 4) = make_float4(o[i * 4], o[i * 4 + 1], o[i * 4 + 2], o[i * 4 + 3]);
         }
       }
-      if (ok && live && half == 0) {
+      if (ok && live && part64 == 0) {
         if (whole) {
           a.lse[out_row] = (m + log2f(l)) * 0.69314718055994531f;
         } else {
@@ -823,13 +858,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPaThreads, 1)
         a.meta[worker * 4 + 2] = last - worker + 1;
       }
       at += units;
-      asm volatile("bar.sync %0, 64;" ::"r"(1 + (warp & 1)) : "memory");   // ctl.sum is read
+      tc_fence_before();   // TMEM is read before the next tile's first sums, which wait for its probabilities
+      asm volatile("bar.sync %0, 128;" ::"r"(meet) : "memory");   // the sums are read before the next maxima
     }
   }
   tc_fence_before();
   __syncthreads();
   cluster_sync();   // neither CTA gives up its memory while the other's instructions may use it
-  if (warp == 6) pair_dealloc(tmem, 512);
+  if (warp == 9) pair_dealloc(tmem, 512);
 }
 
 // ---------------------------------------------------------------------------------------------
