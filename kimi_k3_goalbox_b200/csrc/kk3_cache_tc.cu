@@ -185,6 +185,49 @@ struct EntryRows {
   }
 };
 
+// The rows of 256 positions from `pos` on, one table lookup a lane: eight positions a lane, which lie in one page
+// unless pages have odd sizes (box 0).
+struct UnitRows {
+  int kv[8], pe[8];   // box > 0: [0] is the first position's
+  KK3_DEV void find(const CachePages& c, const PairRows& pr, int b, int pos, int end) {
+    pos += (threadIdx.x & 31) * 8;
+    if (pr.box) {
+      entry_row(c, pr, b, pos, end, &kv[0], &pe[0]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) entry_row(c, pr, b, pos + i, end, &kv[i], &pe[i]);
+    }
+  }
+  // a lane's part in loading `count` positions from `off` on (multiples of 64); single: row by row, zeros from `left`
+  // (counted from `off`) on
+  KK3_DEV EntryRows part(const PairRows& pr, int off, int count, bool single, int left) const {
+    const int lane = threadIdx.x & 31;
+    EntryRows e;
+    if (pr.box && !single) {
+      const int from = ((off + lane * pr.box) >> 3) & 31;
+      e.kv[0] = __shfl_sync(0xffffffffu, kv[0], from);
+      e.pe[0] = __shfl_sync(0xffffffffu, pe[0], from);
+    } else {
+      const int from = ((off + lane * 4) >> 3) & 31, up = (lane & 1) * 4;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (pr.box) {
+          const bool in = lane * 4 + i < left;
+          const int x = __shfl_sync(0xffffffffu, kv[0], from), y = __shfl_sync(0xffffffffu, pe[0], from);
+          e.kv[i] = in && x != pr.kv_end ? x + up + i : pr.kv_end;
+          e.pe[i] = in && y != pr.pe_end ? y + up + i : pr.pe_end;
+        } else {
+          const int x0 = __shfl_sync(0xffffffffu, kv[i], from), x1 = __shfl_sync(0xffffffffu, kv[i + 4], from);
+          const int y0 = __shfl_sync(0xffffffffu, pe[i], from), y1 = __shfl_sync(0xffffffffu, pe[i + 4], from);
+          e.kv[i] = up ? x1 : x0;
+          e.pe[i] = up ? y1 : y0;
+        }
+      }
+    }
+    return e;
+  }
+};
+
 // ---------------------------------------------------------------------------------------------
 // Attention weight of cached positions: w_p = sum over rows of 2^(s_p - lse), s_p = q . e_p.
 //
@@ -464,34 +507,35 @@ __global__ void __launch_bounds__(kMassPos) kk3_cache_mass_join_kernel(const Mas
 // 128. Every instruction has 256 columns: one takes 64 clocks then, and about as much to issue whatever its size (57
 // clocks measured, 175 more for a commit), so narrower ones would leave the tensor cores waiting.
 //
-// Per unit each CTA loads 128 of the positions (nine blocks of 64 dims, 16 KB) for the scores, and half of the output
-// dims of all 256 (four stages of 64 positions x 2 x 128 dims) for the sums, through a ring of three 32 KB stages in the
-// order of their use; the rope block has a slot of its own. Scores run one unit ahead of sums.
+// Per unit each CTA loads 128 of the positions (nine blocks of 64 dims) for the scores, and half of the output dims of
+// all 256 (eight pieces of 64 positions x 128 dims) for the sums, 16 KB each, through a ring of four and one of three.
+// Scores run one unit ahead of sums, and a thread each issues them: what one spends in commits is the other's.
 //
 // Softmax: four threads per row, 64 of a unit's positions each, that exchange maxima through shared memory. The running
 // maximum moves only when it is exceeded by more than 2^8 (probabilities stay below 256, harmless in BF16 and FP32), so
 // the sums in TMEM are rarely rescaled. Probabilities are rounded to BF16 for the second product, the type that the
 // instruction takes with BF16 latents; the running sum adds them unrounded, since lse is an FP32 result.
 //
-// Bounds of a unit: 4352 clocks of tensor time (128 x 256 x 1088 products at 4096 a clock and SM) and 9 commits, 278 KB
-// of loads in each SM (mostly from L2); for few rows the 294 KB per pair from HBM.
+// Bounds of a unit: 4352 clocks of tensor time (128 x 256 x 1088 products at 4096 a clock and SM), 4200 to issue its
+// scores, 278 KB of loads in each SM (mostly from L2); for few rows the 294 KB per pair from HBM.
 
 constexpr int kPaUnit = 256;
-constexpr int kPaThreads = 320;        // warps 0-7 softmax, 8 copies, 9 instructions and TMEM
+constexpr int kPaThreads = 384;        // warps 0-7 softmax, 8 and 9 copies and instructions of scores, 10 and 11 of sums
 constexpr int kPaQBlock = 64 * 128;    // 64 rows of 64 dims
 constexpr int kPaBlock = 128 * 128;    // 128 positions x 64 dims, or 64 positions x 128 dims
-constexpr int kPaStages = 3;
+constexpr int kPaKSlots = 4, kPaVSlots = 3;
 constexpr int kPaMinUnits = 1;
 constexpr float kPaSlack = 8.0f;
 struct PaCtl {
-  unsigned long long qfull, qempty, full[kPaStages], empty[kPaStages], pefull, peempty, sfull[2], sfree[2], pfull, pvdone, done;
+  unsigned long long qfull, qempty, kfull[kPaKSlots], kempty[kPaKSlots], vfull[kPaVSlots], vempty[kPaVSlots], sfull[2],
+      sfree[2], pfull, pvdone, done;
   unsigned tmem;
   int dead;
   long long red[kPaThreads / 32 + 4];
   float top[2][4][64];   // [unit parity][64 positions of 256][row]: maxima (at the end: sums) of a row's four threads
 };
-constexpr int kPaQ = 0, kPaP = kPaQ + kBlocks * kPaQBlock, kPaRing = kPaP + 4 * kPaQBlock,
-              kPaPe = kPaRing + kPaStages * 2 * kPaBlock, kPaCtl = kPaPe + kPaBlock;
+constexpr int kPaQ = 0, kPaP = kPaQ + kBlocks * kPaQBlock, kPaK = kPaP + 4 * kPaQBlock,
+              kPaV = kPaK + kPaKSlots * kPaBlock, kPaCtl = kPaV + kPaVSlots * kPaBlock;
 constexpr int kPaSmem = kPaCtl + (int)sizeof(PaCtl);
 static_assert(kPaSmem <= 232448, "shared memory of a CTA");
 
@@ -526,27 +570,29 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPaThreads, 1)
     return;
   }
   if (worker >= sh.workers) return;   // both CTAs of the pair
-  const unsigned qfull = smem_u32(&ctl.qfull), qempty = smem_u32(&ctl.qempty), full = smem_u32(ctl.full),
-                 empty = smem_u32(ctl.empty), pefull = smem_u32(&ctl.pefull), peempty = smem_u32(&ctl.peempty),
+  const unsigned qfull = smem_u32(&ctl.qfull), qempty = smem_u32(&ctl.qempty), kfull = smem_u32(ctl.kfull),
+                 kempty = smem_u32(ctl.kempty), vfull = smem_u32(ctl.vfull), vempty = smem_u32(ctl.vempty),
                  sfull = smem_u32(ctl.sfull), sfree = smem_u32(ctl.sfree), pfull = smem_u32(&ctl.pfull),
                  pvdone = smem_u32(&ctl.pvdone), done = smem_u32(&ctl.done);
   volatile int* dead = &ctl.dead;
   if (tid == 0) {
     mbar_init(qfull, 1);
     mbar_init(qempty, 1);
-    for (int i = 0; i < kPaStages; ++i) {
-      mbar_init(full + 8 * i, 1);
-      mbar_init(empty + 8 * i, 1);
+    for (int i = 0; i < kPaKSlots; ++i) {
+      mbar_init(kfull + 8 * i, 1);
+      mbar_init(kempty + 8 * i, 1);
     }
-    mbar_init(pefull, 1);
-    mbar_init(peempty, 1);
+    for (int i = 0; i < kPaVSlots; ++i) {
+      mbar_init(vfull + 8 * i, 1);
+      mbar_init(vempty + 8 * i, 1);
+    }
     for (int i = 0; i < 2; ++i) {
       mbar_init(sfull + 8 * i, 1);
       mbar_init(sfree + 8 * i, 16);   // the softmax warps of both CTAs
     }
     mbar_init(pfull, 16);
     mbar_init(pvdone, 1);
-    mbar_init(done, 1);
+    mbar_init(done, 2);
     ctl.dead = 0;
     fence_mbar_init();
   }
@@ -560,53 +606,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPaThreads, 1)
 
   int b = sh.b, t = sh.t;
   long long at = sh.at;
-  int n = 0, tile = 0, job = 0;   // units, tiles and ring stages so far
+  int n = 0, tile = 0, job = 0;   // units, tiles and ring slots so far
   bool ok = true;
   if (warp == 8) {
-    // ---- copies
-    const unsigned lead_q = in_cta(qfull, 0), lead_full = in_cta(full, 0), lead_pe = in_cta(pefull, 0);
-    PairRows single = pr;   // positions that no row sees must be zeros in the second product: row by row
-    single.box = 0;
-    const auto begin = [&](unsigned* bar) -> unsigned {   // the next stage, empty and expecting its bytes: its address
-      const int st = job % kPaStages;
-      ok = __all_sync(0xffffffffu, pair_wait(a.c, empty + 8 * st, ((job / kPaStages) & 1) ^ 1, dead));
-      if (ok && rank == 0 && lane == 0) mbar_arrive_tx(full + 8 * st, 4 * kPaBlock);
-      __syncwarp();
-      *bar = lead_full + 8 * st;
-      return base + kPaRing + st * 2 * kPaBlock;
-    };
+    // ---- queries, and the entries' blocks for the scores
+    const unsigned lead_q = in_cta(qfull, 0), lead_k = in_cta(kfull, 0);
     for (; ok && at < sh.end; ++t, ++tile) {
       Seq s = a.seq(b);
       for (; t >= split.tiles(s); t = 0) s = a.seq(++b);
       const int units = split.units(s, t), end = split.sees(s, t);
       const int u0 = (int)max(0ll, sh.begin - at), u1 = (int)min((long long)units, sh.end - at);
-      // rows of a unit's entries, found one unit ahead: this CTA's 128 positions, and all 256 in groups of 64
-      EntryRows ek, ev[4], ek_next, ev_next[4];
-      unsigned cut = 0, cut_next = 0;   // groups that `end` cuts
-      const auto find = [&](int u) {
-        ek_next.find(a.c, pr, b, u * kPaUnit + (int)rank * 128, 128, end);
-        cut_next = 0;
-#pragma unroll
-        for (int g = 0; g < 4; ++g) {
-          const int pos = u * kPaUnit + g * 64;
-          const bool c = pos < end && end < pos + 64;
-          ev_next[g].find(a.c, c ? single : pr, b, pos, 64, end);
-          cut_next |= (unsigned)c << g;
-        }
-      };
-      const auto values = [&]() {
-#pragma unroll
-        for (int g = 0; g < 4; ++g) {
-          unsigned bar;
-          const unsigned dst = begin(&bar);
-          if (!ok) break;
-#pragma unroll
-          for (int i = 0; i < 4; ++i)   // (dims 256 h + 128 rank + 64 j)
-            ev[g].load(maps, cut >> g & 1 ? single : pr, 4 * (i >> 1) + 2 * (int)rank + (i & 1), 64, dst + i * (kPaBlock / 2), bar);
-          ++job;
-        }
-      };
-      find(u0);
+      UnitRows next;   // looked up one unit ahead
+      next.find(a.c, pr, b, u0 * kPaUnit, end);
       ok = __all_sync(0xffffffffu, pair_wait(a.c, qempty, (tile & 1) ^ 1, dead));
       if (!ok) break;
       if (lane == 0) {
@@ -615,95 +626,109 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPaThreads, 1)
         for (int d = 0; d < kBlocks - 1; ++d) load_box(base + kPaQ + d * kPaQBlock, &maps.ql, d * 64, q, lead_q);
         load_box(base + kPaQ + (kBlocks - 1) * kPaQBlock, &maps.qp, 0, q, lead_q);
       }
-      for (int u = u0; ok && u < u1; ++u, ++n) {
-        ek = ek_next;
-        for (int d = 0; d < kBlocks - 1; d += 2) {
-          unsigned bar;
-          const unsigned dst = begin(&bar);
+      for (int u = u0; ok && u < u1; ++u) {
+        const EntryRows ek = next.part(pr, (int)rank * 128, 128, false, 0);
+        for (int d = 0; d < kBlocks; ++d, ++job) {
+          const int slot = job % kPaKSlots;
+          ok = __all_sync(0xffffffffu, pair_wait(a.c, kempty + 8 * slot, ((job / kPaKSlots) & 1) ^ 1, dead));
           if (!ok) break;
-          ek.load(maps, pr, d, 128, dst, bar);
-          ek.load(maps, pr, d + 1, 128, dst + kPaBlock, bar);
-          ++job;
+          if (rank == 0 && lane == 0) mbar_arrive_tx(kfull + 8 * slot, 2 * kPaBlock);
+          __syncwarp();
+          ek.load(maps, pr, d, 128, base + kPaK + slot * kPaBlock, lead_k + 8 * slot);
+          if (d == 0 && u + 1 < u1) next.find(a.c, pr, b, (u + 1) * kPaUnit, end);
         }
-        if (ok) ok = __all_sync(0xffffffffu, pair_wait(a.c, peempty, (n & 1) ^ 1, dead));
-        if (!ok) break;
-        if (rank == 0 && lane == 0) mbar_arrive_tx(pefull, 2 * kPaBlock);
-        __syncwarp();
-        ek.load(maps, pr, kBlocks - 1, 128, base + kPaPe, lead_pe);
-        if (u > u0) values();
-#pragma unroll
-        for (int g = 0; g < 4; ++g) ev[g] = ev_next[g];
-        cut = cut_next;
-        if (ok && u + 1 < u1) find(u + 1);
       }
-      if (ok) values();
       at += units;
     }
     if (rank == 0 && lane == 0 && !ok) {   // after a failed wait: a bounded time for the copies in flight
       mbar_wait_for(qfull, (tile & 1) ^ 1, kWaitNs);
-      mbar_wait_for(pefull, (n & 1) ^ 1, kWaitNs);
-      for (int j = max(0, job - kPaStages); j < job; ++j)
-        mbar_wait_for(full + 8 * (j % kPaStages), (j / kPaStages) & 1, kWaitNs);
+      for (int j = max(0, job - kPaKSlots); j < job; ++j)
+        mbar_wait_for(kfull + 8 * (j % kPaKSlots), (j / kPaKSlots) & 1, kWaitNs);
     }
     __syncwarp();
-  } else if (warp == 9) {
-    // ---- matrix instructions: one thread of the pair
+  } else if (warp == 10) {
+    // ---- the entries' pieces for the sums: piece (g, h) is dims 256 h + 128 rank .. + 127 of positions 64 g .. + 63 of
+    // the unit. Positions that no row sees must be zeros, whatever the page holds there: row by row.
+    const unsigned lead_v = in_cta(vfull, 0);
+    PairRows single = pr;
+    single.box = 0;
+    for (; ok && at < sh.end; ++t) {
+      Seq s = a.seq(b);
+      for (; t >= split.tiles(s); t = 0) s = a.seq(++b);
+      const int units = split.units(s, t), end = split.sees(s, t);
+      const int u0 = (int)max(0ll, sh.begin - at), u1 = (int)min((long long)units, sh.end - at);
+      UnitRows next, now;
+      next.find(a.c, pr, b, u0 * kPaUnit, end);
+      for (int u = u0; ok && u < u1; ++u) {
+        now = next;
+        for (int i = 0; i < 8; ++i, ++job) {
+          const int g = i >> 1, h = i & 1, left = end - (u * kPaUnit + g * 64);
+          const bool cut = left > 0 && left < 64;
+          const EntryRows ev = now.part(pr, g * 64, 64, cut, left);
+          const int slot = job % kPaVSlots;
+          ok = __all_sync(0xffffffffu, pair_wait(a.c, vempty + 8 * slot, ((job / kPaVSlots) & 1) ^ 1, dead));
+          if (!ok) break;
+          if (rank == 0 && lane == 0) mbar_arrive_tx(vfull + 8 * slot, 2 * kPaBlock);
+          __syncwarp();
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
+            ev.load(maps, cut ? single : pr, 4 * h + 2 * (int)rank + j, 64, base + kPaV + slot * kPaBlock + j * (kPaBlock / 2),
+                    lead_v + 8 * slot);
+          if (i == 0 && u + 1 < u1) next.find(a.c, pr, b, (u + 1) * kPaUnit, end);
+        }
+      }
+      at += units;
+    }
+    if (rank == 0 && lane == 0 && !ok)
+      for (int j = max(0, job - kPaVSlots); j < job; ++j)
+        mbar_wait_for(vfull + 8 * (j % kPaVSlots), (j / kPaVSlots) & 1, kWaitNs);
+    __syncwarp();
+  } else if (warp == 9 || warp == 11) {
+    // ---- matrix instructions: two threads of the pair
     if (lane == 0 && rank == 0) {
       constexpr unsigned id_s = pair_idesc(128, 256), id_o = id_s | (1u << 16);   // values are MN-major
-      const auto sums = [&](int m, bool first) {   // unit number m of this worker; the first of its tile begins O
-        ok = pair_wait_peer(a.c, pfull, m & 1, dead);
-        tc_fence_after();
-        for (int g = 0; ok && g < 4; ++g, ++job) {
-          const int st = job % kPaStages;
-          ok = pair_wait(a.c, full + 8 * st, (job / kPaStages) & 1, dead);
-          if (!ok) break;
-          tc_fence_after();
-          const unsigned va = base + kPaRing + st * 2 * kPaBlock, pa = base + kPaP + g * kPaQBlock;
-#pragma unroll
-          for (int h = 0; h < 2; ++h)
-#pragma unroll
-            for (int k = 0; k < 4; ++k)
-              pair_mma(tmem + h * 128, sdesc_sw128(pa + k * 32), sdesc_mn(va + h * kPaBlock + k * 2048, kPaBlock / 2), id_o,
-                       (unsigned)(!first || g || k));
-          pair_commit(empty + 8 * st);
-        }
-        if (ok) pair_commit(pvdone);
-      };
       for (; ok && at < sh.end; ++t, ++tile) {
         Seq s = a.seq(b);
         for (; t >= split.tiles(s); t = 0) s = a.seq(++b);
         const int units = split.units(s, t);
         const int u0 = (int)max(0ll, sh.begin - at), u1 = (int)min((long long)units, sh.end - at);
-        ok = pair_wait(a.c, qfull, tile & 1, dead);
-        for (int u = u0; ok && u < u1; ++u, ++n) {
-          const int buf = n & 1;
-          ok = pair_wait_peer(a.c, sfree + 8 * buf, ((n >> 1) & 1) ^ 1, dead);
-          tc_fence_after();
-          const unsigned d = tmem_s + buf * 128;
-          for (int i = 0; ok && i < (kBlocks - 1) / 2; ++i, ++job) {
-            const int st = job % kPaStages;
-            ok = pair_wait(a.c, full + 8 * st, (job / kPaStages) & 1, dead);
-            if (!ok) break;
-            tc_fence_after();
-            const unsigned qa = base + kPaQ + i * 2 * kPaQBlock, ka = base + kPaRing + st * 2 * kPaBlock;
+        if (warp == 9) {
+          ok = pair_wait(a.c, qfull, tile & 1, dead);
+          for (int u = u0; ok && u < u1; ++u, ++n) {
+            const int buf = n & 1;
+            ok = pair_wait_peer(a.c, sfree + 8 * buf, ((n >> 1) & 1) ^ 1, dead);
+            for (int d = 0; ok && d < kBlocks; ++d, ++job) {
+              const int slot = job % kPaKSlots;
+              ok = pair_wait(a.c, kfull + 8 * slot, (job / kPaKSlots) & 1, dead);
+              if (!ok) break;
+              tc_fence_after();
+              const unsigned qa = base + kPaQ + d * kPaQBlock, ka = base + kPaK + slot * kPaBlock;
 #pragma unroll
-            for (int k = 0; k < 8; ++k)
-              pair_mma(d, sdesc_sw128(qa + (k >> 2) * kPaQBlock + (k & 3) * 32),
-                       sdesc_sw128(ka + (k >> 2) * kPaBlock + (k & 3) * 32), id_s, (unsigned)(i | k));
-            pair_commit(empty + 8 * st);
+              for (int k = 0; k < 4; ++k)
+                pair_mma(tmem_s + buf * 128, sdesc_sw128(qa + k * 32), sdesc_sw128(ka + k * 32), id_s, (unsigned)(d | k));
+              pair_commit(kempty + 8 * slot);
+            }
+            if (ok) pair_commit(sfull + 8 * buf);
           }
-          if (ok) ok = pair_wait(a.c, pefull, n & 1, dead);
-          if (!ok) break;
-          tc_fence_after();
+          if (ok) pair_commit(qempty);
+        } else {
+          for (int u = u0; ok && u < u1; ++u, ++n) {
+            ok = pair_wait_peer(a.c, pfull, n & 1, dead);
+            for (int i = 0; ok && i < 8; ++i, ++job) {
+              const int slot = job % kPaVSlots;
+              ok = pair_wait(a.c, vfull + 8 * slot, (job / kPaVSlots) & 1, dead);
+              if (!ok) break;
+              tc_fence_after();
+              const unsigned va = base + kPaV + slot * kPaBlock, pa = base + kPaP + (i >> 1) * kPaQBlock;
 #pragma unroll
-          for (int k = 0; k < 4; ++k)
-            pair_mma(d, sdesc_sw128(base + kPaQ + (kBlocks - 1) * kPaQBlock + k * 32), sdesc_sw128(base + kPaPe + k * 32), id_s, 1u);
-          pair_commit(peempty);
-          pair_commit(sfull + 8 * buf);
-          if (u == u1 - 1) pair_commit(qempty);
-          if (u > u0) sums(n - 1, u - 1 == u0);
+              for (int k = 0; k < 4; ++k)
+                pair_mma(tmem + (i & 1) * 128, sdesc_sw128(pa + k * 32), sdesc_mn(va + k * 2048, kPaBlock / 2), id_o,
+                         (unsigned)(u > u0 || i > 1 || k));
+              pair_commit(vempty + 8 * slot);
+            }
+            if (ok) pair_commit(pvdone);
+          }
         }
-        if (ok) sums(n - 1, u1 - 1 == u0);
         at += units;
       }
       pair_commit(done);   // all matrix instructions end before TMEM is given back
@@ -779,6 +804,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPaThreads, 1)
 #pragma unroll
         for (int i = 0; i < 64; ++i) sum[i & 3] += v[i >> 5][i & 31];
         l = l * alpha + ((sum[0] + sum[1]) + (sum[2] + sum[3]));
+        unsigned w[32];
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+          const __nv_bfloat162 h2 = __floats2bfloat162_rn(v[i >> 4][(i & 15) * 2], v[i >> 4][(i & 15) * 2 + 1]);
+          w[i] = *reinterpret_cast<const unsigned*>(&h2);
+        }
         // the sums of the unit before have read P and are done
         if (n > 0) ok = __all_sync(0xffffffffu, pair_wait(a.c, pvdone, (n - 1) & 1, dead)) && ok;
         tc_fence_after();
@@ -795,17 +826,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPaThreads, 1)
           tmem_st_wait();
         }
 #pragma unroll
-        for (int c = 0; c < 8; ++c) {
-          unsigned w[4];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int k = c * 8 + i * 2;
-            const __nv_bfloat162 h2 = __floats2bfloat162_rn(v[k >> 5][k & 31], v[k >> 5][(k & 31) + 1]);
-            w[i] = *reinterpret_cast<const unsigned*>(&h2);
-          }
+        for (int c = 0; c < 8; ++c)
           asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};"
-                       ::"r"(p_row + ((c ^ (row & 7)) << 4)), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
-        }
+                       ::"r"(p_row + ((c ^ (row & 7)) << 4)), "r"(w[c * 4]), "r"(w[c * 4 + 1]), "r"(w[c * 4 + 2]), "r"(w[c * 4 + 3])
+                       : "memory");
         fence_async_smem();
         tc_fence_before();
         __syncwarp();
