@@ -47,27 +47,20 @@ KK3_DEV unsigned in_cta(unsigned addr, unsigned rank) {
 KK3_DEV void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
+// Arrival on a barrier of either CTA. What these arrivals hand over stays in this SM: tensor memory that was read or
+// written to the end (tcgen05.wait, tcgen05.fence) and shared memory that was fenced towards the matrix instructions
+// (fence.proxy.async), both of which this SM's half of the instruction then uses; no other CTA reads it. So they are
+// released at CTA scope: at cluster scope an arrival waits about 1800 clocks for all of the thread's memory traffic.
 KK3_DEV void arrive_cluster(unsigned addr) {
-  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(addr) : "memory");
+  asm volatile("mbarrier.arrive.release.cta.shared::cluster.b64 _, [%0];" ::"r"(addr) : "memory");
 }
-// Bounded wait; false when it ran out or another role of the CTA gave up (*dead). For barriers that copies and matrix
-// instructions complete. A wait at cluster scope (pair_wait_peer) costs some hundred clocks more, so it is kept for
-// the barriers on which threads of the other CTA arrive.
-KK3_DEV bool pair_test_peer(unsigned bar, unsigned parity) {
-  unsigned ok;
-  asm volatile(
-      "{\n .reg .pred p;\n mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n"
-      " selp.u32 %0, 1, 0, p;\n}"
-      : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
-  return ok != 0;
-}
-template <bool PEER>
-KK3_DEV bool pair_wait_as(const CachePages& c, unsigned bar, unsigned parity, volatile int* dead) {
-  if (PEER ? pair_test_peer(bar, parity) : mbar_test(bar, parity)) return true;
+// Bounded wait; false when it ran out or another role of the CTA gave up (*dead).
+KK3_DEV bool pair_wait(const CachePages& c, unsigned bar, unsigned parity, volatile int* dead) {
+  if (mbar_test(bar, parity)) return true;
   if (*dead) return false;
   const unsigned long long t0 = globaltimer();
   for (unsigned spin = 1;; ++spin) {
-    if (PEER ? pair_test_peer(bar, parity) : mbar_test(bar, parity)) return true;
+    if (mbar_test(bar, parity)) return true;
     if ((spin & 15) == 0) {
       if (*dead) return false;
       if (globaltimer() - t0 > kWaitNs) {
@@ -77,12 +70,6 @@ KK3_DEV bool pair_wait_as(const CachePages& c, unsigned bar, unsigned parity, vo
       }
     }
   }
-}
-KK3_DEV bool pair_wait(const CachePages& c, unsigned bar, unsigned parity, volatile int* dead) {
-  return pair_wait_as<false>(c, bar, parity, dead);
-}
-KK3_DEV bool pair_wait_peer(const CachePages& c, unsigned bar, unsigned parity, volatile int* dead) {
-  return pair_wait_as<true>(c, bar, parity, dead);
 }
 // Rows row[0..3] of 64 elements from column x into 512 bytes of this CTA's shared memory; the bytes are counted on
 // `bar`, a barrier of either CTA of the pair.
@@ -369,7 +356,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMassThreads, 1)
         const int u0 = (int)max(0ll, sh.begin - at), u1 = (int)min((long long)units, sh.end - at);
         for (int u = u0; ok && u < u1; ++u, ++unit) {
           const int buf = unit & 1;
-          ok = pair_wait_peer(a.c, dempty + 8 * buf, ((unit >> 1) & 1) ^ 1, dead);
+          ok = pair_wait(a.c, dempty + 8 * buf, ((unit >> 1) & 1) ^ 1, dead);
           tc_fence_after();
           for (int d = 0; ok && d < kBlocks; ++d, ++job) {
             const int slot = job % slots;
@@ -528,7 +515,7 @@ constexpr int kPaMinUnits = 1;
 constexpr float kPaSlack = 8.0f;
 struct PaCtl {
   unsigned long long qfull, qempty, kfull[kPaKSlots], kempty[kPaKSlots], vfull[kPaVSlots], vempty[kPaVSlots], sfull[2],
-      sfree[2], pfull, pvdone, done;
+      sfree[2], oready, pfull[4], pfree[4], pvdone, done;
   unsigned tmem;
   int dead;
   long long red[kPaThreads / 32 + 4];
@@ -572,8 +559,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPaThreads, 1)
   if (worker >= sh.workers) return;   // both CTAs of the pair
   const unsigned qfull = smem_u32(&ctl.qfull), qempty = smem_u32(&ctl.qempty), kfull = smem_u32(ctl.kfull),
                  kempty = smem_u32(ctl.kempty), vfull = smem_u32(ctl.vfull), vempty = smem_u32(ctl.vempty),
-                 sfull = smem_u32(ctl.sfull), sfree = smem_u32(ctl.sfree), pfull = smem_u32(&ctl.pfull),
-                 pvdone = smem_u32(&ctl.pvdone), done = smem_u32(&ctl.done);
+                 sfull = smem_u32(ctl.sfull), sfree = smem_u32(ctl.sfree), oready = smem_u32(&ctl.oready),
+                 pfull = smem_u32(ctl.pfull), pfree = smem_u32(ctl.pfree), pvdone = smem_u32(&ctl.pvdone), done = smem_u32(&ctl.done);
   volatile int* dead = &ctl.dead;
   if (tid == 0) {
     mbar_init(qfull, 1);
@@ -590,7 +577,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPaThreads, 1)
       mbar_init(sfull + 8 * i, 1);
       mbar_init(sfree + 8 * i, 16);   // the softmax warps of both CTAs
     }
-    mbar_init(pfull, 16);
+    mbar_init(oready, 16);
+    for (int i = 0; i < 4; ++i) {
+      mbar_init(pfull + 8 * i, 4);   // the warps of these 64 positions, of both CTAs
+      mbar_init(pfree + 8 * i, 1);
+    }
     mbar_init(pvdone, 1);
     mbar_init(done, 2);
     ctl.dead = 0;
@@ -696,7 +687,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPaThreads, 1)
           ok = pair_wait(a.c, qfull, tile & 1, dead);
           for (int u = u0; ok && u < u1; ++u, ++n) {
             const int buf = n & 1;
-            ok = pair_wait_peer(a.c, sfree + 8 * buf, ((n >> 1) & 1) ^ 1, dead);
+            ok = pair_wait(a.c, sfree + 8 * buf, ((n >> 1) & 1) ^ 1, dead);
             for (int d = 0; ok && d < kBlocks; ++d, ++job) {
               const int slot = job % kPaKSlots;
               ok = pair_wait(a.c, kfull + 8 * slot, (job / kPaKSlots) & 1, dead);
@@ -713,10 +704,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPaThreads, 1)
           if (ok) pair_commit(qempty);
         } else {
           for (int u = u0; ok && u < u1; ++u, ++n) {
-            ok = pair_wait_peer(a.c, pfull, n & 1, dead);
+            ok = pair_wait(a.c, oready, n & 1, dead);
             for (int i = 0; ok && i < 8; ++i, ++job) {
               const int slot = job % kPaVSlots;
-              ok = pair_wait(a.c, vfull + 8 * slot, (job / kPaVSlots) & 1, dead);
+              ok = (i & 1) || pair_wait(a.c, pfull + 4 * i, n & 1, dead);
+              if (ok) ok = pair_wait(a.c, vfull + 8 * slot, (job / kPaVSlots) & 1, dead);
               if (!ok) break;
               tc_fence_after();
               const unsigned va = base + kPaV + slot * kPaBlock, pa = base + kPaP + (i >> 1) * kPaQBlock;
@@ -725,6 +717,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPaThreads, 1)
                 pair_mma(tmem + (i & 1) * 128, sdesc_sw128(pa + k * 32), sdesc_mn(va + k * 2048, kPaBlock / 2), id_o,
                          (unsigned)(u > u0 || i > 1 || k));
               pair_commit(vempty + 8 * slot);
+              if (i & 1) pair_commit(pfree + 4 * (i - 1));
             }
             if (ok) pair_commit(pvdone);
           }
@@ -741,7 +734,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPaThreads, 1)
     const int wg = warp >> 2, quarter = warp & 3, row = (quarter & 1) * 32 + lane;
     const int part64 = (quarter >> 1) * 2 + wg;   // which 64 positions of the unit
     const unsigned tlane = (unsigned)(quarter * 32) << 16, meet = 1 + (quarter & 1);
-    const unsigned lead_sfree = in_cta(sfree, 0), lead_pfull = in_cta(pfull, 0);
+    const unsigned lead_sfree = in_cta(sfree, 0), lead_oready = in_cta(oready, 0),
+                   lead_pfull = in_cta(pfull + 8 * part64, 0);
     const unsigned p_row = base + kPaP + part64 * kPaQBlock + row * 128;
     const float sign = a.scale_log2 < 0.0f ? -1.0f : 1.0f, size = fabsf(a.scale_log2);
     for (; at < sh.end; ++t) {
@@ -790,6 +784,23 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPaThreads, 1)
           m = top;
         }
         const float ref = m == -INFINITY ? 0.0f : m;
+        if (u > u0 && __any_sync(0xffffffffu, alpha != 1.0f)) {   // rescale, once the unit before has been added
+          ok = __all_sync(0xffffffffu, pair_wait(a.c, pvdone, (n - 1) & 1, dead)) && ok;
+          tc_fence_after();
+#pragma unroll 1
+          for (int c = 0; c < 128; c += 32) {
+            float o[32];
+            tmem_ld32(tmem + wg * 128 + tlane + c, o);
+            tmem_ld_wait();
+#pragma unroll
+            for (int i = 0; i < 32; ++i) o[i] *= alpha;
+            tmem_st32(tmem + wg * 128 + tlane + c, o);
+          }
+          tmem_st_wait();
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) arrive_cluster(lead_oready);
 #pragma unroll
         for (int i = 0; i < 64; ++i) {
           float& x = v[i >> 5][i & 31];
@@ -810,28 +821,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPaThreads, 1)
           const __nv_bfloat162 h2 = __floats2bfloat162_rn(v[i >> 4][(i & 15) * 2], v[i >> 4][(i & 15) * 2 + 1]);
           w[i] = *reinterpret_cast<const unsigned*>(&h2);
         }
-        // the sums of the unit before have read P and are done
-        if (n > 0) ok = __all_sync(0xffffffffu, pair_wait(a.c, pvdone, (n - 1) & 1, dead)) && ok;
-        tc_fence_after();
-        if (u > u0 && __any_sync(0xffffffffu, alpha != 1.0f)) {
-#pragma unroll 1
-          for (int c = 0; c < 128; c += 32) {
-            float o[32];
-            tmem_ld32(tmem + wg * 128 + tlane + c, o);
-            tmem_ld_wait();
-#pragma unroll
-            for (int i = 0; i < 32; ++i) o[i] *= alpha;
-            tmem_st32(tmem + wg * 128 + tlane + c, o);
-          }
-          tmem_st_wait();
-        }
+        // the sums of the unit before have read this part of P
+        if (n > 0) ok = __all_sync(0xffffffffu, pair_wait(a.c, pfree + 8 * part64, (n - 1) & 1, dead)) && ok;
 #pragma unroll
         for (int c = 0; c < 8; ++c)
           asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};"
                        ::"r"(p_row + ((c ^ (row & 7)) << 4)), "r"(w[c * 4]), "r"(w[c * 4 + 1]), "r"(w[c * 4 + 2]), "r"(w[c * 4 + 3])
                        : "memory");
         fence_async_smem();
-        tc_fence_before();
         __syncwarp();
         if (lane == 0) arrive_cluster(lead_pfull);
       }
