@@ -88,6 +88,15 @@ KK3_DEV void load_box(unsigned dst, const CUtensorMap* map, int x, int row, unsi
       ::"r"(dst), "l"(map), "r"(x), "r"(row), "r"(bar)
       : "memory");
 }
+// whether a phase has completed, without the wait that try_wait may make
+KK3_DEV bool pair_seen(unsigned bar, unsigned parity) {
+  unsigned ok;
+  asm volatile(
+      "{\n .reg .pred p;\n mbarrier.test_wait.parity.acquire.cta.shared::cta.b64 p, [%1], %2;\n"
+      " selp.u32 %0, 1, 0, p;\n}"
+      : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+  return ok != 0;
+}
 KK3_DEV void pair_mma(unsigned d, unsigned long long a, unsigned long long b, unsigned idesc, unsigned accumulate) {
   asm volatile(
       "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
@@ -675,48 +684,63 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPaThreads, 1)
         mbar_wait_for(vfull + 8 * (j % kPaVSlots), (j / kPaVSlots) & 1, kWaitNs);
     __syncwarp();
   } else if (warp == 9 || warp == 11) {
-    // ---- matrix instructions: two threads of the pair
+    // ---- matrix instructions: two threads of the pair. Issuing costs as much as the instructions take, so the next
+    // slot's barrier is tested before the current slot's instructions (its answer is there when they are out) and the
+    // descriptors are sums of 16-byte offsets.
     if (lane == 0 && rank == 0) {
       constexpr unsigned id_s = pair_idesc(128, 256), id_o = id_s | (1u << 16);   // values are MN-major
+      const int slots = warp == 9 ? kPaKSlots : kPaVSlots;
+      const unsigned fullb = warp == 9 ? kfull : vfull, emptyb = warp == 9 ? kempty : vempty;
+      int slot = 0, phase = 0;
+      bool there = false;   // whether the slot's data were seen already
+      const auto take = [&]() {   // waits for the slot; looks at the next one
+        if (!there) ok = pair_wait(a.c, fullb + 8 * slot, phase, dead);
+        tc_fence_after();
+        const int ns = slot + 1 == slots ? 0 : slot + 1;
+        there = pair_seen(fullb + 8 * ns, ns ? phase : phase ^ 1);
+      };
+      const auto give = [&]() {
+        pair_commit(emptyb + 8 * slot);
+        if (++slot == slots) {
+          slot = 0;
+          phase ^= 1;
+        }
+      };
       for (; ok && at < sh.end; ++t, ++tile) {
         Seq s = a.seq(b);
         for (; t >= split.tiles(s); t = 0) s = a.seq(++b);
         const int units = split.units(s, t);
         const int u0 = (int)max(0ll, sh.begin - at), u1 = (int)min((long long)units, sh.end - at);
         if (warp == 9) {
+          const unsigned long long qd = sdesc_sw128(base + kPaQ), kd = sdesc_sw128(base + kPaK);
           ok = pair_wait(a.c, qfull, tile & 1, dead);
           for (int u = u0; ok && u < u1; ++u, ++n) {
             const int buf = n & 1;
             ok = pair_wait(a.c, sfree + 8 * buf, ((n >> 1) & 1) ^ 1, dead);
-            for (int d = 0; ok && d < kBlocks; ++d, ++job) {
-              const int slot = job % kPaKSlots;
-              ok = pair_wait(a.c, kfull + 8 * slot, (job / kPaKSlots) & 1, dead);
+            for (int d = 0; ok && d < kBlocks; ++d) {
+              take();
               if (!ok) break;
-              tc_fence_after();
-              const unsigned qa = base + kPaQ + d * kPaQBlock, ka = base + kPaK + slot * kPaBlock;
+              const unsigned long long qa = qd + d * (kPaQBlock >> 4), ka = kd + slot * (kPaBlock >> 4);
 #pragma unroll
-              for (int k = 0; k < 4; ++k)
-                pair_mma(tmem_s + buf * 128, sdesc_sw128(qa + k * 32), sdesc_sw128(ka + k * 32), id_s, (unsigned)(d | k));
-              pair_commit(kempty + 8 * slot);
+              for (int k = 0; k < 4; ++k) pair_mma(tmem_s + buf * 128, qa + k * 2, ka + k * 2, id_s, (unsigned)(d | k));
+              give();
             }
             if (ok) pair_commit(sfull + 8 * buf);
           }
           if (ok) pair_commit(qempty);
         } else {
+          const unsigned long long pd = sdesc_sw128(base + kPaP), vd = sdesc_mn(base + kPaV, kPaBlock / 2);
           for (int u = u0; ok && u < u1; ++u, ++n) {
             ok = pair_wait(a.c, oready, n & 1, dead);
-            for (int i = 0; ok && i < 8; ++i, ++job) {
-              const int slot = job % kPaVSlots;
-              ok = (i & 1) || pair_wait(a.c, pfull + 4 * i, n & 1, dead);
-              if (ok) ok = pair_wait(a.c, vfull + 8 * slot, (job / kPaVSlots) & 1, dead);
+            for (int i = 0; ok && i < 8; ++i) {
+              if (!(i & 1)) ok = pair_wait(a.c, pfull + 4 * i, n & 1, dead);
+              if (ok) take();
               if (!ok) break;
-              tc_fence_after();
-              const unsigned va = base + kPaV + slot * kPaBlock, pa = base + kPaP + (i >> 1) * kPaQBlock;
+              const unsigned long long pa = pd + (i >> 1) * (kPaQBlock >> 4), va = vd + slot * (kPaBlock >> 4);
 #pragma unroll
               for (int k = 0; k < 4; ++k)
-                pair_mma(tmem + (i & 1) * 128, sdesc_sw128(pa + k * 32), sdesc_mn(va + k * 2048, kPaBlock / 2), id_o,
-                         (unsigned)(u > u0 || i > 1 || k));
-              pair_commit(vempty + 8 * slot);
+                pair_mma(tmem + (i & 1) * 128, pa + k * 2, va + k * 128, id_o, (unsigned)(u > u0 || i > 1 || k));
+              give();
               if (i & 1) pair_commit(pfree + 4 * (i - 1));
             }
             if (ok) pair_commit(pvdone);
