@@ -141,88 +141,68 @@ KK3_DEV constexpr unsigned pair_idesc(int m, int n) {
   return (1u << 4) | (1u << 7) | (1u << 10) | ((unsigned)(n >> 3) << 17) | ((unsigned)(m >> 4) << 24);
 }
 
-// row numbers of the cached position `pos` of sequence `b`; at or behind `end`, or without a page: past the pool
-KK3_DEV void entry_row(const CachePages& c, const PairRows& pr, int b, int pos, int end, int* kv, int* pe) {
-  *kv = pr.kv_end;
-  *pe = pr.pe_end;
-  if (pos < end) {
-    int slot;
-    const int page = page_at(c, b, pos, &slot);
-    if (page >= 0) {
-      *kv = page * pr.kv_ratio + slot;
-      *pe = page * pr.pe_ratio + slot;
-    }
-  }
-}
-// A warp's part in loading `count` (64 or 128) cached positions from `pos` on: the row of a lane's box or gather.
-struct EntryRows {
-  int kv[4], pe[4];
-  KK3_DEV void find(const CachePages& c, const PairRows& pr, int b, int pos, int count, int end) {
-    const int lane = threadIdx.x & 31;
-    if (pr.box) {
-      if (lane * pr.box < count) entry_row(c, pr, b, pos + lane * pr.box, end, &kv[0], &pe[0]);
-    } else if (lane * 4 < count) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) entry_row(c, pr, b, pos + lane * 4 + i, end, &kv[i], &pe[i]);
-    }
-  }
-  // 64-dim block `d` of the positions into [count][64] at `dst`
-  KK3_DEV void load(const PairMaps& m, const PairRows& pr, int d, int count, unsigned dst, unsigned bar) const {
-    const int lane = threadIdx.x & 31;
-    if (pr.box) {
-      if (lane * pr.box < count) {
-        if (d < kBlocks - 1) load_box(dst + lane * pr.box * 128, &m.kv_box, d * 64, kv[0], bar);
-        else load_box(dst + lane * pr.box * 128, &m.pe_box, 0, pe[0], bar);
-      }
-    } else if (lane * 4 < count) {
-      if (d < kBlocks - 1) gather4(dst + lane * 512, &m.kv_row, d * 64, kv, bar);
-      else gather4(dst + lane * 512, &m.pe_row, 0, pe, bar);
-    }
-  }
+// The rows of 256 cached positions of a sequence, behind `end` or without a page: the first past the pool. A copying
+// warp looks them up together (eight positions a lane, which lie in one page unless pages have odd sizes), one table
+// ahead: fetch() only reads the page table, write() turns what came into rows. One lane then issues all copies from the
+// table: a copy is one instruction for the whole warp, and going through the lanes one by one took 300 clocks each.
+struct RowTab {
+  alignas(16) int kv[256];
+  alignas(16) int pe[256];
 };
-
-// The rows of 256 positions from `pos` on, one table lookup a lane: eight positions a lane, which lie in one page
-// unless pages have odd sizes (box 0).
-struct UnitRows {
-  int kv[8], pe[8];   // box > 0: [0] is the first position's
-  KK3_DEV void find(const CachePages& c, const PairRows& pr, int b, int pos, int end) {
+struct PageIds {
+  int id[8];
+  KK3_DEV void fetch(const CachePages& c, const PairRows& pr, int b, int pos, int end) {
     pos += (threadIdx.x & 31) * 8;
-    if (pr.box) {
-      entry_row(c, pr, b, pos, end, &kv[0], &pe[0]);
-    } else {
+    const int* table = c.table + (long long)b * c.table_stride;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) entry_row(c, pr, b, pos + i, end, &kv[i], &pe[i]);
-    }
+    for (int i = 0; i < 8; ++i)
+      if ((i == 0 || !pr.box) && pos + i < end) id[i] = table[page_of(c, pos + i)];
   }
-  // a lane's part in loading `count` positions from `off` on (multiples of 64); single: row by row, zeros from `left`
-  // (counted from `off`) on
-  KK3_DEV EntryRows part(const PairRows& pr, int off, int count, bool single, int left) const {
+  KK3_DEV void write(const CachePages& c, const PairRows& pr, int pos, int end, RowTab& tab) const {
     const int lane = threadIdx.x & 31;
-    EntryRows e;
-    if (pr.box && !single) {
-      const int from = ((off + lane * pr.box) >> 3) & 31;
-      e.kv[0] = __shfl_sync(0xffffffffu, kv[0], from);
-      e.pe[0] = __shfl_sync(0xffffffffu, pe[0], from);
-    } else {
-      const int from = ((off + lane * 4) >> 3) & 31, up = (lane & 1) * 4;
+    pos += lane * 8;
+    int kv[8], pe[8];
+    const int slot = pos - page_of(c, pos) * c.page_size;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        if (pr.box) {
-          const bool in = lane * 4 + i < left;
-          const int x = __shfl_sync(0xffffffffu, kv[0], from), y = __shfl_sync(0xffffffffu, pe[0], from);
-          e.kv[i] = in && x != pr.kv_end ? x + up + i : pr.kv_end;
-          e.pe[i] = in && y != pr.pe_end ? y + up + i : pr.pe_end;
+    for (int i = 0; i < 8; ++i) {
+      kv[i] = pr.kv_end;
+      pe[i] = pr.pe_end;
+      if (pos + i < end) {
+        const int page = pr.box ? id[0] : id[i];
+        const int in = pr.box ? slot + i : pos + i - page_of(c, pos + i) * c.page_size;
+        if ((unsigned)page < (unsigned)c.num_pages) {
+          kv[i] = page * pr.kv_ratio + in;
+          pe[i] = page * pr.pe_ratio + in;
         } else {
-          const int x0 = __shfl_sync(0xffffffffu, kv[i], from), x1 = __shfl_sync(0xffffffffu, kv[i + 4], from);
-          const int y0 = __shfl_sync(0xffffffffu, pe[i], from), y1 = __shfl_sync(0xffffffffu, pe[i + 4], from);
-          e.kv[i] = up ? x1 : x0;
-          e.pe[i] = up ? y1 : y0;
+          cache_error(c);
         }
       }
     }
-    return e;
+#pragma unroll
+    for (int i = 0; i < 8; i += 4) {
+      *reinterpret_cast<int4*>(&tab.kv[lane * 8 + i]) = make_int4(kv[i], kv[i + 1], kv[i + 2], kv[i + 3]);
+      *reinterpret_cast<int4*>(&tab.pe[lane * 8 + i]) = make_int4(pe[i], pe[i + 1], pe[i + 2], pe[i + 3]);
+    }
   }
 };
+// One thread: 64-dim block `d` of the `count` positions from number `off` of the table on into [count][64] at `dst`;
+// box 0: row by row.
+KK3_DEV void load_entries(const PairMaps& m, const RowTab& tab, int box, int d, int off, int count, unsigned dst, unsigned bar) {
+  const bool rope = d == kBlocks - 1;
+  const int* rows = (rope ? tab.pe : tab.kv) + off;
+  const int x = rope ? 0 : d * 64;
+  if (box) {
+    const CUtensorMap* map = rope ? &m.pe_box : &m.kv_box;
+    for (int k = 0; k < count; k += box) load_box(dst + k * 128, map, x, rows[k], bar);
+  } else {
+    const CUtensorMap* map = rope ? &m.pe_row : &m.kv_row;
+    for (int k = 0; k < count; k += 4) {
+      const int4 r = *reinterpret_cast<const int4*>(&rows[k]);
+      const int four[4] = {r.x, r.y, r.z, r.w};
+      gather4(dst + k * 128, map, x, four, bar);
+    }
+  }
+}
 
 // ---------------------------------------------------------------------------------------------
 // Attention weight of cached positions: w_p = sum over rows of 2^(s_p - lse), s_p = q . e_p.
@@ -250,6 +230,7 @@ struct MassCtl {
   alignas(16) float lse[2][256];   // read four at a time
   alignas(16) int sees[2][256];
   float sum[128];
+  RowTab rows;
 };
 constexpr int kMassSmem = kBlocks * kMassKBlock + kMassRing + (int)sizeof(MassCtl) + 1024;
 static_assert(kMassSmem <= 232448, "shared memory of a CTA");
@@ -314,44 +295,47 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMassThreads, 1)
   if (warp == 8) {
     // ---- copies
     const unsigned lead_full = in_cta(full, 0);
-    int job = 0, tile = 0;
+    int slot = 0, phase = 0, tile = 0, ahead_b = -1, ahead_t = -1;   // the tile whose page ids are there
+    PageIds ids;
     bool ok = true;
     while (ok && at < sh.end) {
       Seq s = a.seq(b);
       for (; t >= split.tiles(s); t = 0) s = a.seq(++b);
       const int units = split.units(s, t), first = split.first_unit(s, t);
       const int u0 = (int)max(0ll, sh.begin - at), u1 = (int)min((long long)units, sh.end - at);
-      EntryRows er;
-      er.find(a.c, pr, b, t * kMassPos + (int)rank * 128, 128, s.len);
-      for (int u = u0; ok && u < u1; ++u) {
-        const int q = s.q0 * a.heads + (first + u) * rows + (int)rank * half;   // rows behind the sequence's: masked
-        for (int d = 0; d < kBlocks; ++d, ++job) {
-          const int slot = job % slots;
-          const unsigned bar = lead_full + 8 * slot;
-          ok = pair_wait(a.c, empty + 8 * slot, ((job / slots) & 1) ^ 1, dead);
-          if (ok && u == u0) ok = pair_wait(a.c, kempty + 8 * d, (tile & 1) ^ 1, dead);
-          ok = __all_sync(0xffffffffu, ok);
-          if (!ok) break;
-          if (rank == 0 && lane == 0)
-            mbar_arrive_tx(full + 8 * slot, 2 * (slot_bytes + (u == u0 ? kMassKBlock : 0)));
-          __syncwarp();
-          if (u == u0) er.load(maps, pr, d, 128, kbase + d * kMassKBlock, bar);
-          if (lane == 0) {
-            const unsigned qd = qbase + slot * slot_bytes;
+      if (ahead_b != b || ahead_t != t) ids.fetch(a.c, pr, b, t * kMassPos, s.len);
+      ids.write(a.c, pr, t * kMassPos, s.len, ctl.rows);
+      __syncwarp();
+      ids.fetch(a.c, pr, b, (t + 1) * kMassPos, s.len);
+      ahead_b = b;
+      ahead_t = t + 1;
+      if (lane == 0) {
+        for (int u = u0; ok && u < u1; ++u) {
+          const int q = s.q0 * a.heads + (first + u) * rows + (int)rank * half;   // rows behind the sequence's: masked
+          for (int d = 0; d < kBlocks; ++d) {
+            const unsigned bar = lead_full + 8 * slot, qd = qbase + slot * slot_bytes;
+            ok = pair_wait(a.c, empty + 8 * slot, phase ^ 1, dead);
+            if (ok && u == u0) ok = pair_wait(a.c, kempty + 8 * d, (tile & 1) ^ 1, dead);
+            if (!ok) break;
+            if (rank == 0) mbar_arrive_tx(full + 8 * slot, 2 * (slot_bytes + (u == u0 ? kMassKBlock : 0)));
+            if (u == u0) load_entries(maps, ctl.rows, pr.box, d, (int)rank * 128, 128, kbase + d * kMassKBlock, bar);
             if (d < kBlocks - 1) load_box(qd, &maps.ql, d * 64, q, bar);
             else load_box(qd, &maps.qp, 0, q, bar);
+            if (++slot == slots) {
+              slot = 0;
+              phase ^= 1;
+            }
           }
         }
+        // after a failed wait: a bounded time for the copies in flight (else their consumers waited for them)
+        if (!ok && rank == 0)
+          for (int i = 0; i < slots; ++i) mbar_wait_for(full + 8 * i, i < slot ? phase : phase ^ 1, kWaitNs);
       }
+      ok = __shfl_sync(0xffffffffu, ok, 0);
       at += units;
       ++t;
       ++tile;
     }
-    // the last copies have landed before the CTA can leave: their consumers waited for them, or (after a failed
-    // wait) the slots' barriers are given a bounded time here
-    if (!ok && rank == 0 && lane == 0)
-      for (int j = max(0, job - slots); j < job; ++j) mbar_wait_for(full + 8 * (j % slots), (j / slots) & 1, kWaitNs);
-    __syncwarp();
   } else if (warp == 9) {
     // ---- matrix instructions: one thread of the pair
     if (lane == 0 && rank == 0) {
@@ -372,10 +356,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMassThreads, 1)
             ok = pair_wait(a.c, full + 8 * slot, (job / slots) & 1, dead);
             if (!ok) break;
             tc_fence_after();
-            const unsigned ka = kbase + d * kMassKBlock, qa = qbase + slot * slot_bytes;
+            const unsigned long long ka = sdesc_sw128(kbase + d * kMassKBlock), qa = sdesc_sw128(qbase + slot * slot_bytes);
 #pragma unroll
-            for (int k = 0; k < 4; ++k)
-              pair_mma(tmem + buf * 256, sdesc_sw128(ka + k * 32), sdesc_sw128(qa + k * 32), idesc, (unsigned)(d | k));
+            for (int k = 0; k < 4; ++k) pair_mma(tmem + buf * 256, ka + k * 2, qa + k * 2, idesc, (unsigned)(d | k));
             pair_commit(empty + 8 * slot);
             if (u == u1 - 1) pair_commit(kempty + 8 * d);
           }
@@ -528,6 +511,7 @@ struct PaCtl {
   unsigned tmem;
   int dead;
   long long red[kPaThreads / 32 + 4];
+  RowTab rows[2];        // entries of the scores' and of the sums' unit
   float top[2][4][64];   // [unit parity][64 positions of 256][row]: maxima (at the end: sums) of a row's four threads
 };
 constexpr int kPaQ = 0, kPaP = kPaQ + kBlocks * kPaQBlock, kPaK = kPaP + 4 * kPaQBlock,
@@ -606,18 +590,19 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPaThreads, 1)
 
   int b = sh.b, t = sh.t;
   long long at = sh.at;
-  int n = 0, tile = 0, job = 0;   // units, tiles and ring slots so far
+  int n = 0, tile = 0;   // units and tiles so far
   bool ok = true;
   if (warp == 8) {
     // ---- queries, and the entries' blocks for the scores
     const unsigned lead_q = in_cta(qfull, 0), lead_k = in_cta(kfull, 0);
+    int slot = 0, phase = 0;
     for (; ok && at < sh.end; ++t, ++tile) {
       Seq s = a.seq(b);
       for (; t >= split.tiles(s); t = 0) s = a.seq(++b);
       const int units = split.units(s, t), end = split.sees(s, t);
       const int u0 = (int)max(0ll, sh.begin - at), u1 = (int)min((long long)units, sh.end - at);
-      UnitRows next;   // looked up one unit ahead
-      next.find(a.c, pr, b, u0 * kPaUnit, end);
+      PageIds ids;
+      ids.fetch(a.c, pr, b, u0 * kPaUnit, end);
       ok = __all_sync(0xffffffffu, pair_wait(a.c, qempty, (tile & 1) ^ 1, dead));
       if (!ok) break;
       if (lane == 0) {
@@ -627,61 +612,70 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPaThreads, 1)
         load_box(base + kPaQ + (kBlocks - 1) * kPaQBlock, &maps.qp, 0, q, lead_q);
       }
       for (int u = u0; ok && u < u1; ++u) {
-        const EntryRows ek = next.part(pr, (int)rank * 128, 128, false, 0);
-        for (int d = 0; d < kBlocks; ++d, ++job) {
-          const int slot = job % kPaKSlots;
-          ok = __all_sync(0xffffffffu, pair_wait(a.c, kempty + 8 * slot, ((job / kPaKSlots) & 1) ^ 1, dead));
-          if (!ok) break;
-          if (rank == 0 && lane == 0) mbar_arrive_tx(kfull + 8 * slot, 2 * kPaBlock);
-          __syncwarp();
-          ek.load(maps, pr, d, 128, base + kPaK + slot * kPaBlock, lead_k + 8 * slot);
-          if (d == 0 && u + 1 < u1) next.find(a.c, pr, b, (u + 1) * kPaUnit, end);
+        ids.write(a.c, pr, u * kPaUnit, end, ctl.rows[0]);
+        __syncwarp();
+        ids.fetch(a.c, pr, b, (u + 1) * kPaUnit, end);
+        if (lane == 0) {
+          for (int d = 0; d < kBlocks; ++d) {
+            ok = pair_wait(a.c, kempty + 8 * slot, phase ^ 1, dead);
+            if (!ok) break;
+            if (rank == 0) mbar_arrive_tx(kfull + 8 * slot, 2 * kPaBlock);
+            load_entries(maps, ctl.rows[0], pr.box, d, (int)rank * 128, 128, base + kPaK + slot * kPaBlock, lead_k + 8 * slot);
+            if (++slot == kPaKSlots) {
+              slot = 0;
+              phase ^= 1;
+            }
+          }
         }
+        ok = __shfl_sync(0xffffffffu, ok, 0);
       }
       at += units;
     }
     if (rank == 0 && lane == 0 && !ok) {   // after a failed wait: a bounded time for the copies in flight
       mbar_wait_for(qfull, (tile & 1) ^ 1, kWaitNs);
-      for (int j = max(0, job - kPaKSlots); j < job; ++j)
-        mbar_wait_for(kfull + 8 * (j % kPaKSlots), (j / kPaKSlots) & 1, kWaitNs);
+      for (int i = 0; i < kPaKSlots; ++i) mbar_wait_for(kfull + 8 * i, i < slot ? phase : phase ^ 1, kWaitNs);
     }
     __syncwarp();
   } else if (warp == 10) {
     // ---- the entries' pieces for the sums: piece (g, h) is dims 256 h + 128 rank .. + 127 of positions 64 g .. + 63 of
-    // the unit. Positions that no row sees must be zeros, whatever the page holds there: row by row.
+    // the unit. Positions that no row sees must be zeros, whatever the page holds there: a group that `end` cuts comes
+    // row by row.
     const unsigned lead_v = in_cta(vfull, 0);
-    PairRows single = pr;
-    single.box = 0;
+    int slot = 0, phase = 0;
     for (; ok && at < sh.end; ++t) {
       Seq s = a.seq(b);
       for (; t >= split.tiles(s); t = 0) s = a.seq(++b);
       const int units = split.units(s, t), end = split.sees(s, t);
       const int u0 = (int)max(0ll, sh.begin - at), u1 = (int)min((long long)units, sh.end - at);
-      UnitRows next, now;
-      next.find(a.c, pr, b, u0 * kPaUnit, end);
+      PageIds ids;
+      ids.fetch(a.c, pr, b, u0 * kPaUnit, end);
       for (int u = u0; ok && u < u1; ++u) {
-        now = next;
-        for (int i = 0; i < 8; ++i, ++job) {
-          const int g = i >> 1, h = i & 1, left = end - (u * kPaUnit + g * 64);
-          const bool cut = left > 0 && left < 64;
-          const EntryRows ev = now.part(pr, g * 64, 64, cut, left);
-          const int slot = job % kPaVSlots;
-          ok = __all_sync(0xffffffffu, pair_wait(a.c, vempty + 8 * slot, ((job / kPaVSlots) & 1) ^ 1, dead));
-          if (!ok) break;
-          if (rank == 0 && lane == 0) mbar_arrive_tx(vfull + 8 * slot, 2 * kPaBlock);
-          __syncwarp();
+        ids.write(a.c, pr, u * kPaUnit, end, ctl.rows[1]);
+        __syncwarp();
+        ids.fetch(a.c, pr, b, (u + 1) * kPaUnit, end);
+        if (lane == 0) {
+          for (int i = 0; i < 8; ++i) {
+            const int g = i >> 1, h = i & 1, left = end - (u * kPaUnit + g * 64);
+            const unsigned dst = base + kPaV + slot * kPaBlock, bar = lead_v + 8 * slot;
+            ok = pair_wait(a.c, vempty + 8 * slot, phase ^ 1, dead);
+            if (!ok) break;
+            if (rank == 0) mbar_arrive_tx(vfull + 8 * slot, 2 * kPaBlock);
 #pragma unroll
-          for (int j = 0; j < 2; ++j)
-            ev.load(maps, cut ? single : pr, 4 * h + 2 * (int)rank + j, 64, base + kPaV + slot * kPaBlock + j * (kPaBlock / 2),
-                    lead_v + 8 * slot);
-          if (i == 0 && u + 1 < u1) next.find(a.c, pr, b, (u + 1) * kPaUnit, end);
+            for (int j = 0; j < 2; ++j)
+              load_entries(maps, ctl.rows[1], left > 0 && left < 64 ? 0 : pr.box, 4 * h + 2 * (int)rank + j, g * 64, 64,
+                           dst + j * (kPaBlock / 2), bar);
+            if (++slot == kPaVSlots) {
+              slot = 0;
+              phase ^= 1;
+            }
+          }
         }
+        ok = __shfl_sync(0xffffffffu, ok, 0);
       }
       at += units;
     }
     if (rank == 0 && lane == 0 && !ok)
-      for (int j = max(0, job - kPaVSlots); j < job; ++j)
-        mbar_wait_for(vfull + 8 * (j % kPaVSlots), (j / kPaVSlots) & 1, kWaitNs);
+      for (int i = 0; i < kPaVSlots; ++i) mbar_wait_for(vfull + 8 * i, i < slot ? phase : phase ^ 1, kWaitNs);
     __syncwarp();
   } else if (warp == 9 || warp == 11) {
     // ---- matrix instructions: two threads of the pair. Issuing costs as much as the instructions take, so the next
