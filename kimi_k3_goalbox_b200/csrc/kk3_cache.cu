@@ -329,60 +329,86 @@ __global__ void __launch_bounds__(kWaThreads, 1) kk3_cache_attend_warp_kernel(co
 }
 
 // ---------------------------------------------------------------------------------------------
-// Join of a split tile: out = sum_w 2^(m_w - m) O_w / sum_w 2^(m_w - m) l_w over the tile's workers in order. One CTA
-// per (worker that begins a split tile, every gridDim.y-th row); four groups of 128 threads (4 dims each) take a quarter of the workers'
-// sums each, so that the loads of many short pieces are in flight together.
-__global__ void __launch_bounds__(512) kk3_cache_join_kernel(const AttendArgs a, int tile_rows) {
-  const int worker = blockIdx.x;
+// Join of a split tile: out = sum_w 2^(m_w - m) O_w / sum_w 2^(m_w - m) l_w over the tile's workers in order. grid.x is
+// the worker that begins the tile, grid.y deals out its rows. Bound by the pieces' bytes in flight: a warp takes a row
+// of few pieces (16 dims a lane, four pieces at a time), the eight warps of a CTA share a row of many.
+constexpr int kJoinThreads = 256, kJoinFew = 8;
+
+// sums of pieces w0 .. w1 - 1 of a row, weighted; dims 4 lane + 128 j .. + 3 in sum[j]
+KK3_DEV void join_pieces(const float* first, const float* rest, long long pitch, int w0, int w1, float ref, float4 (&sum)[4]) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) sum[j] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 4
+  for (int w = w0; w < w1; ++w) {
+    const float* p = w == 0 ? first : rest + (w - 1) * pitch;
+    const float f = exp2f(p[kLat] - ref);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float4 v = *reinterpret_cast<const float4*>(p + j * 128 + lane * 4);
+      sum[j].x = fmaf(f, v.x, sum[j].x);
+      sum[j].y = fmaf(f, v.y, sum[j].y);
+      sum[j].z = fmaf(f, v.z, sum[j].z);
+      sum[j].w = fmaf(f, v.w, sum[j].w);
+    }
+  }
+}
+
+__global__ void __launch_bounds__(kJoinThreads) kk3_cache_join_kernel(const AttendArgs a, int tile_rows) {
+  __shared__ float4 shared_sum[kJoinThreads / 32][4][32];
+  const int worker = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  constexpr int kWarps = kJoinThreads / 32;
   cache_follow();
   const int n = a.meta[worker * 4 + 2];
   if (n == 0) return;
   const int b = a.meta[worker * 4], t = a.meta[worker * 4 + 1];
   const Seq s = a.seq(b);
   const int rows = (int)min((long long)tile_rows, (long long)s.n * a.heads - (long long)t * tile_rows);
-  __shared__ float4 sums[3][128];
-  const int grp = threadIdx.x >> 7, i = threadIdx.x & 127;
-  for (int row = blockIdx.y; row < rows; row += gridDim.y) {
-    const auto part = [&](int w) {
-      return a.part + (((long long)(worker + w) * 2 + (w == 0 ? 1 : 0)) * tile_rows + row) * kPartRow;
-    };
+  const bool few = n <= kJoinFew;
+  const long long pitch = 2ll * tile_rows * kPartRow;   // from one worker's piece to the next one's
+  for (int row = few ? blockIdx.y * kWarps + warp : blockIdx.y; row < rows; row += gridDim.y * (few ? kWarps : 1)) {
+    // the piece of the worker that begins the tile, and those of the workers that it continues into
+    const float* first = a.part + (worker * 2ll + 1) * tile_rows * kPartRow + (long long)row * kPartRow;
+    const float* rest = a.part + (worker + 1) * pitch + (long long)row * kPartRow;
+    const auto piece = [&](int w) { return w == 0 ? first : rest + (w - 1) * pitch; };
     float top = -INFINITY;
-    for (int w = 0; w < n; ++w) top = fmaxf(top, part(w)[kLat]);
+    for (int w = lane; w < n; w += 32) top = fmaxf(top, piece(w)[kLat]);
+    top = warp_max(top);
     const float ref = top == -INFINITY ? 0.0f : top;
-    float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     float l = 0.0f;
-    for (int w = 0; w < n; ++w) l += exp2f(part(w)[kLat] - ref) * part(w)[kLat + 1];
-    const int per = (n + 3) / 4;
-#pragma unroll 4
-    for (int w = grp * per; w < min(n, (grp + 1) * per); ++w) {
-      const float* p = part(w);
-      const float4 v = *reinterpret_cast<const float4*>(p + i * 4);
-      const float f = exp2f(p[kLat] - ref);
-      sum.x = fmaf(f, v.x, sum.x);
-      sum.y = fmaf(f, v.y, sum.y);
-      sum.z = fmaf(f, v.z, sum.z);
-      sum.w = fmaf(f, v.w, sum.w);
-    }
-    if (grp > 0) sums[grp - 1][i] = sum;
-    __syncthreads();
-    if (grp > 0) {
-      __syncthreads();
-      continue;
-    }
+    for (int w = lane; w < n; w += 32) l += exp2f(piece(w)[kLat] - ref) * piece(w)[kLat + 1];
+    l = warp_sum(l);
+    float4 sum[4];
+    if (few) {
+      join_pieces(first, rest, pitch, 0, n, ref, sum);
+    } else {
+      const int per = (n + kWarps - 1) / kWarps;
+      join_pieces(first, rest, pitch, min(n, warp * per), min(n, (warp + 1) * per), ref, sum);
 #pragma unroll
-    for (int k = 0; k < 3; ++k) {
-      sum.x += sums[k][i].x;
-      sum.y += sums[k][i].y;
-      sum.z += sums[k][i].z;
-      sum.w += sums[k][i].w;
+      for (int j = 0; j < 4; ++j) shared_sum[warp][j][lane] = sum[j];
+      __syncthreads();
+      if (warp < 4) {   // warp j adds up dims 128 j .. 128 j + 127
+        sum[0] = shared_sum[0][warp][lane];
+#pragma unroll
+        for (int w = 1; w < kWarps; ++w) {
+          const float4 v = shared_sum[w][warp][lane];
+          sum[0].x += v.x;
+          sum[0].y += v.y;
+          sum[0].z += v.z;
+          sum[0].w += v.w;
+        }
+      }
+      __syncthreads();
     }
     const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
     const long long g = (long long)s.q0 * a.heads + (long long)t * tile_rows + row;
-    __nv_bfloat162* o = reinterpret_cast<__nv_bfloat162*>(a.out + g * kLat + i * 4);
-    o[0] = __floats2bfloat162_rn(sum.x * inv, sum.y * inv);
-    o[1] = __floats2bfloat162_rn(sum.z * inv, sum.w * inv);
-    if (i == 0) a.lse[g] = (ref + log2f(l)) * 0.69314718055994531f;
-    __syncthreads();   // sums is read
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (!few && (j > 0 || warp >= 4)) break;
+      __nv_bfloat162 o[2] = {__floats2bfloat162_rn(sum[j].x * inv, sum[j].y * inv), __floats2bfloat162_rn(sum[j].z * inv, sum[j].w * inv)};
+      *reinterpret_cast<uint2*>(a.out + g * kLat + (few ? j : warp) * 128 + lane * 4) = *reinterpret_cast<const uint2*>(o);
+    }
+    if (lane == 0 && (few || warp == 0)) a.lse[g] = (ref + log2f(l)) * 0.69314718055994531f;
   }
 }
 
@@ -737,7 +763,7 @@ extern "C" int kk3_cache_attend(const kk3_cache* cache, const void* q_latent, in
     r = cache_cuda(cudaGetLastError(), "kk3_cache_attend_warp_kernel");
   }
   if (r) return r;
-  return cache_launch_after(kk3_cache_join_kernel, dim3(p.workers, 16), 512, st, "kk3_cache_join_kernel", a, p.rows);
+  return cache_launch_after(kk3_cache_join_kernel, dim3(p.workers, 16), kJoinThreads, st, "kk3_cache_join_kernel", a, p.rows);
 }
 
 extern "C" int kk3_cache_evict(const kk3_cache* cache, const int64_t* lengths, const float* mass, int64_t mass_stride,
