@@ -71,21 +71,30 @@ KK3_DEV bool pair_wait(const CachePages& c, unsigned bar, unsigned parity, volat
     }
   }
 }
+// Copies are issued by one lane (`me`) of a converged warp: 50 clocks each, against 90 in a branch of one lane, where
+// every operand moves to the uniform registers anew.
+KK3_DEV bool elect_one() {
+  unsigned p;
+  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.b32 %0, 1, 0, p;\n}" : "=r"(p));
+  return p != 0;
+}
 // Rows row[0..3] of 64 elements from column x into 512 bytes of this CTA's shared memory; the bytes are counted on
 // `bar`, a barrier of either CTA of the pair.
-KK3_DEV void gather4(unsigned dst, const CUtensorMap* map, int x, const int (&row)[4], unsigned bar) {
+KK3_DEV void gather4(bool me, unsigned dst, const CUtensorMap* map, int x, const int4& row, unsigned bar) {
   asm volatile(
-      "cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes.cta_group::2 [%0], "
-      "[%1, {%2, %3, %4, %5, %6}], [%7];"
-      ::"r"(dst), "l"(map), "r"(x), "r"(row[0]), "r"(row[1]), "r"(row[2]), "r"(row[3]), "r"(bar)
+      "{\n .reg .pred p;\n setp.ne.b32 p, %8, 0;\n"
+      " @p cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes.cta_group::2 [%0], "
+      "[%1, {%2, %3, %4, %5, %6}], [%7];\n}"
+      ::"r"(dst), "l"(map), "r"(x), "r"(row.x), "r"(row.y), "r"(row.z), "r"(row.w), "r"(bar), "r"((unsigned)me)
       : "memory");
 }
 // A box of the map's rows from `row` on, likewise.
-KK3_DEV void load_box(unsigned dst, const CUtensorMap* map, int x, int row, unsigned bar) {
+KK3_DEV void load_box(bool me, unsigned dst, const CUtensorMap* map, int x, int row, unsigned bar) {
   asm volatile(
-      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 [%0], "
-      "[%1, {%2, %3}], [%4];"
-      ::"r"(dst), "l"(map), "r"(x), "r"(row), "r"(bar)
+      "{\n .reg .pred p;\n setp.ne.b32 p, %5, 0;\n"
+      " @p cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 [%0], "
+      "[%1, {%2, %3}], [%4];\n}"
+      ::"r"(dst), "l"(map), "r"(x), "r"(row), "r"(bar), "r"((unsigned)me)
       : "memory");
 }
 // whether a phase has completed, without the wait that try_wait may make
@@ -143,8 +152,7 @@ KK3_DEV constexpr unsigned pair_idesc(int m, int n) {
 
 // The rows of 256 cached positions of a sequence, behind `end` or without a page: the first past the pool. A copying
 // warp looks them up together (eight positions a lane, which lie in one page unless pages have odd sizes), one table
-// ahead: fetch() only reads the page table, write() turns what came into rows. One lane then issues all copies from the
-// table: a copy is one instruction for the whole warp, and going through the lanes one by one took 300 clocks each.
+// ahead: fetch() only reads the page table, write() turns what came into rows, from which all copies are issued.
 struct RowTab {
   alignas(16) int kv[256];
   alignas(16) int pe[256];
@@ -185,22 +193,31 @@ struct PageIds {
     }
   }
 };
-// One thread: 64-dim block `d` of the `count` positions from number `off` of the table on into [count][64] at `dst`;
-// box 0: row by row.
-KK3_DEV void load_entries(const PairMaps& m, const RowTab& tab, int box, int d, int off, int count, unsigned dst, unsigned bar) {
+// 64-dim block `d` of COUNT positions from number `off` of the table on into [COUNT][64] at `dst`; BOX 0: row by row.
+template <int COUNT, int BOX>
+KK3_DEV void load_entries_as(bool me, const PairMaps& m, const RowTab& tab, int d, int off, unsigned dst, unsigned bar) {
   const bool rope = d == kBlocks - 1;
   const int* rows = (rope ? tab.pe : tab.kv) + off;
   const int x = rope ? 0 : d * 64;
-  if (box) {
+  if (BOX) {
+    constexpr int kBox = BOX ? BOX : 1;
     const CUtensorMap* map = rope ? &m.pe_box : &m.kv_box;
-    for (int k = 0; k < count; k += box) load_box(dst + k * 128, map, x, rows[k], bar);
+#pragma unroll
+    for (int k = 0; k < COUNT; k += kBox) load_box(me, dst + k * 128, map, x, rows[k], bar);
   } else {
     const CUtensorMap* map = rope ? &m.pe_row : &m.kv_row;
-    for (int k = 0; k < count; k += 4) {
-      const int4 r = *reinterpret_cast<const int4*>(&rows[k]);
-      const int four[4] = {r.x, r.y, r.z, r.w};
-      gather4(dst + k * 128, map, x, four, bar);
-    }
+#pragma unroll 4
+    for (int k = 0; k < COUNT; k += 4) gather4(me, dst + k * 128, map, x, *reinterpret_cast<const int4*>(&rows[k]), bar);
+  }
+}
+template <int COUNT>
+KK3_DEV void load_entries(bool me, const PairMaps& m, const RowTab& tab, int box, int d, int off, unsigned dst, unsigned bar) {
+  switch (box) {
+    case 64: return load_entries_as<COUNT, 64>(me, m, tab, d, off, dst, bar);
+    case 32: return load_entries_as<COUNT, 32>(me, m, tab, d, off, dst, bar);
+    case 16: return load_entries_as<COUNT, 16>(me, m, tab, d, off, dst, bar);
+    case 8: return load_entries_as<COUNT, 8>(me, m, tab, d, off, dst, bar);
+    default: return load_entries_as<COUNT, 0>(me, m, tab, d, off, dst, bar);
   }
 }
 
@@ -295,6 +312,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMassThreads, 1)
   if (warp == 8) {
     // ---- copies
     const unsigned lead_full = in_cta(full, 0);
+    const bool me = elect_one();
     int slot = 0, phase = 0, tile = 0, ahead_b = -1, ahead_t = -1;   // the tile whose page ids are there
     PageIds ids;
     bool ok = true;
@@ -309,33 +327,32 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMassThreads, 1)
       ids.fetch(a.c, pr, b, (t + 1) * kMassPos, s.len);
       ahead_b = b;
       ahead_t = t + 1;
-      if (lane == 0) {
-        for (int u = u0; ok && u < u1; ++u) {
-          const int q = s.q0 * a.heads + (first + u) * rows + (int)rank * half;   // rows behind the sequence's: masked
-          for (int d = 0; d < kBlocks; ++d) {
-            const unsigned bar = lead_full + 8 * slot, qd = qbase + slot * slot_bytes;
-            ok = pair_wait(a.c, empty + 8 * slot, phase ^ 1, dead);
-            if (ok && u == u0) ok = pair_wait(a.c, kempty + 8 * d, (tile & 1) ^ 1, dead);
-            if (!ok) break;
-            if (rank == 0) mbar_arrive_tx(full + 8 * slot, 2 * (slot_bytes + (u == u0 ? kMassKBlock : 0)));
-            if (u == u0) load_entries(maps, ctl.rows, pr.box, d, (int)rank * 128, 128, kbase + d * kMassKBlock, bar);
-            if (d < kBlocks - 1) load_box(qd, &maps.ql, d * 64, q, bar);
-            else load_box(qd, &maps.qp, 0, q, bar);
-            if (++slot == slots) {
-              slot = 0;
-              phase ^= 1;
-            }
+      for (int u = u0; ok && u < u1; ++u) {
+        const int q = s.q0 * a.heads + (first + u) * rows + (int)rank * half;   // rows behind the sequence's: masked
+        for (int d = 0; d < kBlocks; ++d) {
+          const unsigned bar = lead_full + 8 * slot, qd = qbase + slot * slot_bytes;
+          ok = pair_wait(a.c, empty + 8 * slot, phase ^ 1, dead);
+          if (u == u0) ok = pair_wait(a.c, kempty + 8 * d, (tile & 1) ^ 1, dead) && ok;
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
+          if (rank == 0 && me) mbar_arrive_tx(full + 8 * slot, 2 * (slot_bytes + (u == u0 ? kMassKBlock : 0)));
+          __syncwarp();
+          if (u == u0) load_entries<128>(me, maps, ctl.rows, pr.box, d, (int)rank * 128, kbase + d * kMassKBlock, bar);
+          load_box(me, qd, d < kBlocks - 1 ? &maps.ql : &maps.qp, d < kBlocks - 1 ? d * 64 : 0, q, bar);
+          if (++slot == slots) {
+            slot = 0;
+            phase ^= 1;
           }
         }
-        // after a failed wait: a bounded time for the copies in flight (else their consumers waited for them)
-        if (!ok && rank == 0)
-          for (int i = 0; i < slots; ++i) mbar_wait_for(full + 8 * i, i < slot ? phase : phase ^ 1, kWaitNs);
       }
-      ok = __shfl_sync(0xffffffffu, ok, 0);
       at += units;
       ++t;
       ++tile;
     }
+    // after a failed wait: a bounded time for the copies in flight (else their consumers waited for them)
+    if (!ok && rank == 0 && lane == 0)
+      for (int i = 0; i < slots; ++i) mbar_wait_for(full + 8 * i, i < slot ? phase : phase ^ 1, kWaitNs);
+    __syncwarp();
   } else if (warp == 9) {
     // ---- matrix instructions: one thread of the pair
     if (lane == 0 && rank == 0) {
@@ -595,6 +612,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPaThreads, 1)
   if (warp == 8) {
     // ---- queries, and the entries' blocks for the scores
     const unsigned lead_q = in_cta(qfull, 0), lead_k = in_cta(kfull, 0);
+    const bool me = elect_one();
     int slot = 0, phase = 0;
     for (; ok && at < sh.end; ++t, ++tile) {
       Seq s = a.seq(b);
@@ -605,29 +623,30 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPaThreads, 1)
       ids.fetch(a.c, pr, b, u0 * kPaUnit, end);
       ok = __all_sync(0xffffffffu, pair_wait(a.c, qempty, (tile & 1) ^ 1, dead));
       if (!ok) break;
-      if (lane == 0) {
-        if (rank == 0) mbar_arrive_tx(qfull, 2 * kBlocks * kPaQBlock);
+      {
+        if (rank == 0 && me) mbar_arrive_tx(qfull, 2 * kBlocks * kPaQBlock);
+        __syncwarp();
         const int q = s.q0 * a.heads + t * kPairRows + (int)rank * 64;   // rows behind the sequence's are not written
-        for (int d = 0; d < kBlocks - 1; ++d) load_box(base + kPaQ + d * kPaQBlock, &maps.ql, d * 64, q, lead_q);
-        load_box(base + kPaQ + (kBlocks - 1) * kPaQBlock, &maps.qp, 0, q, lead_q);
+#pragma unroll
+        for (int d = 0; d < kBlocks; ++d)
+          load_box(me, base + kPaQ + d * kPaQBlock, d < kBlocks - 1 ? &maps.ql : &maps.qp, d < kBlocks - 1 ? d * 64 : 0, q, lead_q);
       }
       for (int u = u0; ok && u < u1; ++u) {
         ids.write(a.c, pr, u * kPaUnit, end, ctl.rows[0]);
         __syncwarp();
         ids.fetch(a.c, pr, b, (u + 1) * kPaUnit, end);
-        if (lane == 0) {
-          for (int d = 0; d < kBlocks; ++d) {
-            ok = pair_wait(a.c, kempty + 8 * slot, phase ^ 1, dead);
-            if (!ok) break;
-            if (rank == 0) mbar_arrive_tx(kfull + 8 * slot, 2 * kPaBlock);
-            load_entries(maps, ctl.rows[0], pr.box, d, (int)rank * 128, 128, base + kPaK + slot * kPaBlock, lead_k + 8 * slot);
-            if (++slot == kPaKSlots) {
-              slot = 0;
-              phase ^= 1;
-            }
+        for (int d = 0; d < kBlocks; ++d) {
+          ok = __all_sync(0xffffffffu, pair_wait(a.c, kempty + 8 * slot, phase ^ 1, dead));
+          if (!ok) break;
+          if (rank == 0 && me) mbar_arrive_tx(kfull + 8 * slot, 2 * kPaBlock);
+          __syncwarp();
+          load_entries<128>(me, maps, ctl.rows[0], pr.box, d, (int)rank * 128, base + kPaK + slot * kPaBlock, lead_k + 8 * slot);
+          if (++slot == kPaKSlots) {
+            slot = 0;
+            phase ^= 1;
           }
         }
-        ok = __shfl_sync(0xffffffffu, ok, 0);
+        __syncwarp();   // the table is read
       }
       at += units;
     }
@@ -641,6 +660,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPaThreads, 1)
     // the unit. Positions that no row sees must be zeros, whatever the page holds there: a group that `end` cuts comes
     // row by row.
     const unsigned lead_v = in_cta(vfull, 0);
+    const bool me = elect_one();
     int slot = 0, phase = 0;
     for (; ok && at < sh.end; ++t) {
       Seq s = a.seq(b);
@@ -653,24 +673,23 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPaThreads, 1)
         ids.write(a.c, pr, u * kPaUnit, end, ctl.rows[1]);
         __syncwarp();
         ids.fetch(a.c, pr, b, (u + 1) * kPaUnit, end);
-        if (lane == 0) {
-          for (int i = 0; i < 8; ++i) {
-            const int g = i >> 1, h = i & 1, left = end - (u * kPaUnit + g * 64);
-            const unsigned dst = base + kPaV + slot * kPaBlock, bar = lead_v + 8 * slot;
-            ok = pair_wait(a.c, vempty + 8 * slot, phase ^ 1, dead);
-            if (!ok) break;
-            if (rank == 0) mbar_arrive_tx(vfull + 8 * slot, 2 * kPaBlock);
+        for (int i = 0; i < 8; ++i) {
+          const int g = i >> 1, h = i & 1, left = end - (u * kPaUnit + g * 64);
+          const unsigned dst = base + kPaV + slot * kPaBlock, bar = lead_v + 8 * slot;
+          ok = __all_sync(0xffffffffu, pair_wait(a.c, vempty + 8 * slot, phase ^ 1, dead));
+          if (!ok) break;
+          if (rank == 0 && me) mbar_arrive_tx(vfull + 8 * slot, 2 * kPaBlock);
+          __syncwarp();
+          const int box = left > 0 && left < 64 ? 0 : pr.box;
 #pragma unroll
-            for (int j = 0; j < 2; ++j)
-              load_entries(maps, ctl.rows[1], left > 0 && left < 64 ? 0 : pr.box, 4 * h + 2 * (int)rank + j, g * 64, 64,
-                           dst + j * (kPaBlock / 2), bar);
-            if (++slot == kPaVSlots) {
-              slot = 0;
-              phase ^= 1;
-            }
+          for (int j = 0; j < 2; ++j)
+            load_entries<64>(me, maps, ctl.rows[1], box, 4 * h + 2 * (int)rank + j, g * 64, dst + j * (kPaBlock / 2), bar);
+          if (++slot == kPaVSlots) {
+            slot = 0;
+            phase ^= 1;
           }
         }
-        ok = __shfl_sync(0xffffffffu, ok, 0);
+        __syncwarp();   // the table is read
       }
       at += units;
     }
@@ -860,26 +879,36 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPaThreads, 1)
       const long long out_row = (long long)s.q0 * a.heads + g;
       float* part = a.part + (((long long)worker * 2 + (u0 == 0 ? 1 : 0)) * kPairRows + rank * 64 + row) * kPartRow;
       const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
+      // through this warp's 4 KB of P, which the instructions have read: 32 rows x 32 dims, so that a row's dims leave
+      // in one piece
+      float* stage = reinterpret_cast<float*>(smem_raw + kPaP + warp * 4096);
+      const float factor = whole ? inv : 1.0f;
 #pragma unroll 1
       for (int c = 0; c < 128; c += 32) {
-        const int dim = wg * 256 + (quarter >> 1) * 128 + c;
+        const int dim = wg * 256 + (quarter >> 1) * 128 + c + (lane & 7) * 4;
         float o[32];
         tmem_ld32(tmem + wg * 128 + tlane + c, o);
         tmem_ld_wait();
-        if (!ok || !live) continue;
-        if (whole) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            __nv_bfloat162 w[4];
+        for (int i = 0; i < 8; ++i)
+          *reinterpret_cast<float4*>(stage + lane * 32 + ((i ^ (lane & 7)) * 4)) =
+              make_float4(o[i * 4] * factor, o[i * 4 + 1] * factor, o[i * 4 + 2] * factor, o[i * 4 + 3] * factor);
+        __syncwarp();
 #pragma unroll
-            for (int k = 0; k < 4; ++k) w[k] = __floats2bfloat162_rn(o[i * 8 + k * 2] * inv, o[i * 8 + k * 2 + 1] * inv);
-            *reinterpret_cast<uint4*>(a.out + out_row * kLat + dim + i * 8) = *reinterpret_cast<const uint4*>(w);
+        for (int i = 0; i < 8; ++i) {
+          const int r = i * 4 + (lane >> 3);
+          const float4 v = *reinterpret_cast<const float4*>(stage + r * 32 + (((lane & 7) ^ (r & 7)) * 4));
+          const int gr = g - lane + r;   // row r of this warp's 32
+          if (ok && gr < s.n * a.heads) {
+            if (whole) {
+              const __nv_bfloat162 w[2] = {__floats2bfloat162_rn(v.x, v.y), __floats2bfloat162_rn(v.z, v.w)};
+              *reinterpret_cast<uint2*>(a.out + ((long long)s.q0 * a.heads + gr) * kLat + dim) = *reinterpret_cast<const uint2*>(w);
+            } else {
+              *reinterpret_cast<float4*>(part + (long long)(r - lane) * kPartRow + dim) = v;
+            }
           }
-        } else {
-#pragma unroll
-          for (int i = 0; i < 8; ++i)
-            *reinterpret_cast<float4*>(part + dim + i * 4) = make_float4(o[i * 4], o[i * 4 + 1], o[i * 4 + 2], o[i * 4 + 3]);
         }
+        __syncwarp();
       }
       if (ok && live && part64 == 0) {
         if (whole) {
