@@ -169,7 +169,7 @@ __global__ void __launch_bounds__(kWaThreads, 1) kk3_cache_attend_warp_kernel(co
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int worker = blockIdx.x;
   static_assert(sizeof(sm.ring) >= (kMaxSeqs + 1) * sizeof(int), "the sequences' tile prefix lies in the ring");
-  const AttendSplit split{kWaRows, a.heads, kWaUnit};
+  const AttendSplit split{kWaRows, a.heads, kWaUnit, 0};
   const Share sh = plan_share<kWaThreads>(a, split, worker, kWaMinUnits, reinterpret_cast<int*>(&sm.ring[0][0][0]),
                                           sm.red);
   if (tid == 0) a.meta[worker * 4 + 2] = 0;

@@ -112,19 +112,32 @@ struct MassArgs : CallSeqs {
 // The work of one call is cut into tiles, laid end to end; a tile takes a number of units, one at least, and every
 // worker takes an equal run of units, so that short and long sequences, one token and many, all fill the GPU. A tile
 // that is cut is joined afterwards from the sums of its workers, in their order.
-//
+
+// One worker's run of units [begin, end) of the call's `total`, and the tile it begins in.
+struct Share {
+  long long begin, end, total;
+  long long at;      // units before the first tile
+  int b, t;          // first tile: its sequence and its number within it
+  int workers;       // workers that take part (this one does not when its number is not below)
+};
+
 // Attention: a tile is `rows` (token, head) rows of one sequence over the positions that its last row sees, a unit
 // `unit` positions.
 struct AttendSplit {
   int rows, heads, unit;
-  KK3_DEV int tiles(const Seq& s) const { return (int)(((long long)s.n * heads + rows - 1) / rows); }
+  int cost;   // what a tile costs besides its units, in units: they lie before the tile's own
+  KK3_DEV int tiles(const Seq& s) const { return (s.n * heads + rows - 1) / rows; }
   KK3_DEV int sees(const Seq& s, int t) const {   // positions that the tile's last row sees, 0 or less: none
-    return s.len - s.n + min(s.n - 1, (int)((((long long)t + 1) * rows - 1) / heads)) + 1;
+    return s.len - s.n + min(s.n - 1, (int)(((unsigned)(t + 1) * rows - 1) / (unsigned)heads)) + 1;
   }
   KK3_DEV int units(const Seq& s, int t) const {
     const int n = sees(s, t);
     return n > unit ? (n + unit - 1) / unit : 1;
   }
+  KK3_DEV int size(const Seq& s, int t) const { return units(s, t) + cost; }
+  // the tile's units that a worker takes, of a tile that begins at `at`
+  KK3_DEV int from(const Share& sh, long long at, int units) const { return (int)min((long long)units, max(0ll, sh.begin - at - cost)); }
+  KK3_DEV int to(const Share& sh, long long at, int units) const { return (int)min((long long)units, max(0ll, sh.end - at - cost)); }
 };
 // Attention weight: a tile is `positions` positions of one sequence over the rows that see its first, a unit `rows`
 // (token, head) rows.
@@ -132,11 +145,10 @@ struct MassSplit {
   int positions, rows, heads;
   KK3_DEV int tiles(const Seq& s) const { return s.n > 0 ? (s.len + positions - 1) / positions : 0; }
   KK3_DEV int first_unit(const Seq& s, int t) const {   // first rows that see position t * positions
-    return (int)((long long)max(0, t * positions - (s.len - s.n)) * heads / rows);
+    return max(0, t * positions - (s.len - s.n)) * heads / rows;
   }
-  KK3_DEV int units(const Seq& s, int t) const {
-    return (int)(((long long)s.n * heads + rows - 1) / rows) - first_unit(s, t);
-  }
+  KK3_DEV int units(const Seq& s, int t) const { return (s.n * heads + rows - 1) / rows - first_unit(s, t); }
+  KK3_DEV int size(const Seq& s, int t) const { return units(s, t); }
 };
 
 // Sum over the threads of a block of NT (a multiple of 32) threads before this one; *total over all of them. `red`
@@ -162,14 +174,6 @@ KK3_DEV long long block_scan(long long mine, long long* red, long long* total) {
   *total = all;
   return before;
 }
-
-// One worker's run of units [begin, end) of the call's `total`, and the tile it begins in.
-struct Share {
-  long long begin, end, total;
-  long long at;      // units before the first tile
-  int b, t;          // first tile: its sequence and its number within it
-  int workers;       // workers that take part (this one does not when its number is not below)
-};
 
 // Computed by every CTA for itself; all NT threads take part. `prefix` is shared memory of batch + 1 ints, `red` of
 // NT / 32 + 4 long longs. A worker takes min_units units at least: shorter pieces cost more to join than they save.
@@ -203,7 +207,7 @@ KK3_DEV Share plan_share(const CallSeqs& a, const Split& split, int worker, int 
     Seq s = a.seq(b);
     for (int g = g0; g < g1; ++g) {
       while (g >= prefix[b + 1]) s = a.seq(++b);
-      mine += split.units(s, g - prefix[b]);
+      mine += split.size(s, g - prefix[b]);
     }
   }
   Share sh;
@@ -222,7 +226,7 @@ KK3_DEV Share plan_share(const CallSeqs& a, const Split& split, int worker, int 
     Seq s = a.seq(b);
     for (int g = g0; g < g1; ++g) {
       while (g >= prefix[b + 1]) s = a.seq(++b);
-      const int k = split.units(s, g - prefix[b]);
+      const int k = split.size(s, g - prefix[b]);
       if (u + k > sh.begin) {
         found[0] = b;
         found[1] = g - prefix[b];

@@ -10,6 +10,7 @@
 #include <cuda.h>
 #include <cuda_runtime.h>
 #include <cudaTypedefs.h>
+#include <limits.h>
 #include <string.h>
 
 #include "kk3_cache.cuh"
@@ -44,6 +45,8 @@ KK3_DEV unsigned in_cta(unsigned addr, unsigned rank) {
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
   return r;
 }
+KK3_DEV void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+KK3_DEV void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 KK3_DEV void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
@@ -219,6 +222,17 @@ KK3_DEV void load_entries(bool me, const PairMaps& m, const RowTab& tab, int box
     case 8: return load_entries_as<COUNT, 8>(me, m, tab, d, off, dst, bar);
     default: return load_entries_as<COUNT, 0>(me, m, tab, d, off, dst, bar);
   }
+}
+
+// Bring 128 positions from number `off` of the table on into L2, for loads one unit later: HBM's latency is longer than
+// what the ring holds. One instruction per box, where a box's rows lie without gaps.
+KK3_DEV void prefetch_entries(const CachePages& c, const PairRows& pr, const RowTab& tab, int off) {
+  const int lane = threadIdx.x & 31;
+  if (!pr.box || c.kv_row != kLat || c.pe_row != kRope || lane * pr.box >= 128) return;
+  const int kv = tab.kv[off + lane * pr.box], pe = tab.pe[off + lane * pr.box];
+  if (kv == pr.kv_end) return;
+  asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(c.kv + (long long)kv * kLat), "r"(pr.box * kLat * 2) : "memory");
+  asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(c.pe + (long long)pe * kRope), "r"(pr.box * kRope * 2) : "memory");
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -520,7 +534,8 @@ constexpr int kPaThreads = 384;        // warps 0-7 softmax, 8 and 9 copies and 
 constexpr int kPaQBlock = 64 * 128;    // 64 rows of 64 dims
 constexpr int kPaBlock = 128 * 128;    // 128 positions x 64 dims, or 64 positions x 128 dims
 constexpr int kPaKSlots = 4, kPaVSlots = 3;
-constexpr int kPaMinUnits = 1;
+constexpr int kPaMinUnits = 3;
+constexpr int kPaTileCost = 2;   // what a tile costs besides its units, in units: query load, first and last latencies
 constexpr float kPaSlack = 8.0f;
 struct PaCtl {
   unsigned long long qfull, qempty, kfull[kPaKSlots], kempty[kPaKSlots], vfull[kPaVSlots], vempty[kPaVSlots], sfull[2],
@@ -528,7 +543,7 @@ struct PaCtl {
   unsigned tmem;
   int dead;
   long long red[kPaThreads / 32 + 4];
-  RowTab rows[2];        // entries of the scores' and of the sums' unit
+  RowTab rows[3];        // entries of a unit: the scores' (two, in turn) and the sums'
   float top[2][4][64];   // [unit parity][64 positions of 256][row]: maxima (at the end: sums) of a row's four threads
 };
 constexpr int kPaQ = 0, kPaP = kPaQ + kBlocks * kPaQBlock, kPaK = kPaP + 4 * kPaQBlock,
@@ -559,18 +574,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPaThreads, 1)
   PaCtl& ctl = *reinterpret_cast<PaCtl*>(smem_raw + kPaCtl);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, worker = blockIdx.x >> 1;
   const unsigned rank = cluster_rank(), base = smem_u32(smem_raw);
-  const AttendSplit split{kPairRows, a.heads, kPaUnit};
-  const Share sh = plan_share<kPaThreads>(a, split, worker, kPaMinUnits, reinterpret_cast<int*>(smem_raw), ctl.red);
-  if (tid == 0 && rank == 0) a.meta[worker * 4 + 2] = 0;
-  if (base & 1023u) {   // the swizzled blocks need a 1024-byte boundary, which dynamic shared memory begins on
-    if (tid == 0) cache_error(a.c);
-    return;
-  }
-  if (worker >= sh.workers) return;   // both CTAs of the pair
   const unsigned qfull = smem_u32(&ctl.qfull), qempty = smem_u32(&ctl.qempty), kfull = smem_u32(ctl.kfull),
                  kempty = smem_u32(ctl.kempty), vfull = smem_u32(ctl.vfull), vempty = smem_u32(ctl.vempty),
                  sfull = smem_u32(ctl.sfull), sfree = smem_u32(ctl.sfree), oready = smem_u32(&ctl.oready),
-                 pfull = smem_u32(ctl.pfull), pfree = smem_u32(ctl.pfree), pvdone = smem_u32(&ctl.pvdone), done = smem_u32(&ctl.done);
+                 pfull = smem_u32(ctl.pfull), pfree = smem_u32(ctl.pfree), pvdone = smem_u32(&ctl.pvdone),
+                 done = smem_u32(&ctl.done);
   volatile int* dead = &ctl.dead;
   if (tid == 0) {
     mbar_init(qfull, 1);
@@ -598,18 +606,26 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPaThreads, 1)
     fence_mbar_init();
   }
   if (warp == 9) pair_alloc(smem_u32(&ctl.tmem), 512);
+  __syncwarp();
+  cluster_arrive();   // the peer's barriers are needed after the plan
+  const AttendSplit split{kPairRows, a.heads, kPaUnit, kPaTileCost};
+  const Share sh = plan_share<kPaThreads>(a, split, worker, kPaMinUnits, reinterpret_cast<int*>(smem_raw), ctl.red);
+  if (tid == 0 && rank == 0) a.meta[worker * 4 + 2] = 0;
   tc_fence_before();
   __syncthreads();
-  cluster_sync();
+  cluster_wait();
   tc_fence_after();
   const unsigned tmem = *reinterpret_cast<volatile unsigned*>(&ctl.tmem);
   const unsigned tmem_s = tmem + 256;   // two score buffers of 128 columns; the sums have 256 before them
+  if ((base & 1023u) && tid == 0) cache_error(a.c);   // dynamic shared memory begins on the swizzled blocks' boundary
+  const bool takes_part = worker < sh.workers && (base & 1023u) == 0;   // alike in both CTAs of the pair
 
   int b = sh.b, t = sh.t;
   long long at = sh.at;
   int n = 0, tile = 0;   // units and tiles so far
   bool ok = true;
-  if (warp == 8) {
+  if (!takes_part) {
+  } else if (warp == 8) {
     // ---- queries, and the entries' blocks for the scores
     const unsigned lead_q = in_cta(qfull, 0), lead_k = in_cta(kfull, 0);
     const bool me = elect_one();
@@ -618,9 +634,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPaThreads, 1)
       Seq s = a.seq(b);
       for (; t >= split.tiles(s); t = 0) s = a.seq(++b);
       const int units = split.units(s, t), end = split.sees(s, t);
-      const int u0 = (int)max(0ll, sh.begin - at), u1 = (int)min((long long)units, sh.end - at);
+      const int u0 = split.from(sh, at, units), u1 = split.to(sh, at, units);
+      if (u0 == u1) break;   // only a tile's cost is left: the next worker's
       PageIds ids;
       ids.fetch(a.c, pr, b, u0 * kPaUnit, end);
+      const bool once = s.n * a.heads <= kPairRows;   // the cache is read by this tile alone: it comes from HBM
       ok = __all_sync(0xffffffffu, pair_wait(a.c, qempty, (tile & 1) ^ 1, dead));
       if (!ok) break;
       {
@@ -631,16 +649,21 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPaThreads, 1)
         for (int d = 0; d < kBlocks; ++d)
           load_box(me, base + kPaQ + d * kPaQBlock, d < kBlocks - 1 ? &maps.ql : &maps.qp, d < kBlocks - 1 ? d * 64 : 0, q, lead_q);
       }
+      ids.write(a.c, pr, u0 * kPaUnit, end, ctl.rows[0]);
+      ids.fetch(a.c, pr, b, (u0 + 1) * kPaUnit, end);
       for (int u = u0; ok && u < u1; ++u) {
-        ids.write(a.c, pr, u * kPaUnit, end, ctl.rows[0]);
+        const RowTab& tab = ctl.rows[(u - u0) & 1];
+        RowTab& tab_next = ctl.rows[((u - u0) & 1) ^ 1];
+        ids.write(a.c, pr, (u + 1) * kPaUnit, end, tab_next);
         __syncwarp();
-        ids.fetch(a.c, pr, b, (u + 1) * kPaUnit, end);
+        ids.fetch(a.c, pr, b, (u + 2) * kPaUnit, end);
+        if (once && u + 1 < u1) prefetch_entries(a.c, pr, tab_next, (int)rank * 128);
         for (int d = 0; d < kBlocks; ++d) {
           ok = __all_sync(0xffffffffu, pair_wait(a.c, kempty + 8 * slot, phase ^ 1, dead));
           if (!ok) break;
           if (rank == 0 && me) mbar_arrive_tx(kfull + 8 * slot, 2 * kPaBlock);
           __syncwarp();
-          load_entries<128>(me, maps, ctl.rows[0], pr.box, d, (int)rank * 128, base + kPaK + slot * kPaBlock, lead_k + 8 * slot);
+          load_entries<128>(me, maps, tab, pr.box, d, (int)rank * 128, base + kPaK + slot * kPaBlock, lead_k + 8 * slot);
           if (++slot == kPaKSlots) {
             slot = 0;
             phase ^= 1;
@@ -648,7 +671,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPaThreads, 1)
         }
         __syncwarp();   // the table is read
       }
-      at += units;
+      at += units + kPaTileCost;
     }
     if (rank == 0 && lane == 0 && !ok) {   // after a failed wait: a bounded time for the copies in flight
       mbar_wait_for(qfull, (tile & 1) ^ 1, kWaitNs);
@@ -666,11 +689,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPaThreads, 1)
       Seq s = a.seq(b);
       for (; t >= split.tiles(s); t = 0) s = a.seq(++b);
       const int units = split.units(s, t), end = split.sees(s, t);
-      const int u0 = (int)max(0ll, sh.begin - at), u1 = (int)min((long long)units, sh.end - at);
+      const int u0 = split.from(sh, at, units), u1 = split.to(sh, at, units);
+      if (u0 == u1) break;
       PageIds ids;
       ids.fetch(a.c, pr, b, u0 * kPaUnit, end);
       for (int u = u0; ok && u < u1; ++u) {
-        ids.write(a.c, pr, u * kPaUnit, end, ctl.rows[1]);
+        ids.write(a.c, pr, u * kPaUnit, end, ctl.rows[2]);
         __syncwarp();
         ids.fetch(a.c, pr, b, (u + 1) * kPaUnit, end);
         for (int i = 0; i < 8; ++i) {
@@ -683,7 +707,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPaThreads, 1)
           const int box = left > 0 && left < 64 ? 0 : pr.box;
 #pragma unroll
           for (int j = 0; j < 2; ++j)
-            load_entries<64>(me, maps, ctl.rows[1], box, 4 * h + 2 * (int)rank + j, g * 64, dst + j * (kPaBlock / 2), bar);
+            load_entries<64>(me, maps, ctl.rows[2], box, 4 * h + 2 * (int)rank + j, g * 64, dst + j * (kPaBlock / 2), bar);
           if (++slot == kPaVSlots) {
             slot = 0;
             phase ^= 1;
@@ -691,7 +715,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPaThreads, 1)
         }
         __syncwarp();   // the table is read
       }
-      at += units;
+      at += units + kPaTileCost;
     }
     if (rank == 0 && lane == 0 && !ok)
       for (int i = 0; i < kPaVSlots; ++i) mbar_wait_for(vfull + 8 * i, i < slot ? phase : phase ^ 1, kWaitNs);
@@ -723,7 +747,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPaThreads, 1)
         Seq s = a.seq(b);
         for (; t >= split.tiles(s); t = 0) s = a.seq(++b);
         const int units = split.units(s, t);
-        const int u0 = (int)max(0ll, sh.begin - at), u1 = (int)min((long long)units, sh.end - at);
+        const int u0 = split.from(sh, at, units), u1 = split.to(sh, at, units);
+        if (u0 == u1) break;
         if (warp == 9) {
           const unsigned long long qd = sdesc_sw128(base + kPaQ), kd = sdesc_sw128(base + kPaK);
           ok = pair_wait(a.c, qfull, tile & 1, dead);
@@ -759,7 +784,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPaThreads, 1)
             if (ok) pair_commit(pvdone);
           }
         }
-        at += units;
+        at += units + kPaTileCost;
       }
       pair_commit(done);   // all matrix instructions end before TMEM is given back
       mbar_wait_for(done, 0, kWaitNs);
@@ -774,15 +799,26 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPaThreads, 1)
     const unsigned lead_sfree = in_cta(sfree, 0), lead_oready = in_cta(oready, 0),
                    lead_pfull = in_cta(pfull + 8 * part64, 0);
     const unsigned p_row = base + kPaP + part64 * kPaQBlock + row * 128;
+    // Units before number m have been added to O. Where this thread stands, the one three before is known to be added
+    // (this thread's part of P was free again for the one two before); a barrier only tells a phase from its neighbours,
+    // so the last two are waited for one after the other.
+    const auto all_added = [&](int m) {
+      bool done = true;
+      if (m > 1) done = pair_wait(a.c, pvdone, (m - 2) & 1, dead);
+      if (m > 0) done = pair_wait(a.c, pvdone, (m - 1) & 1, dead) && done;
+      return __all_sync(0xffffffffu, done) != 0;
+    };
     const float sign = a.scale_log2 < 0.0f ? -1.0f : 1.0f, size = fabsf(a.scale_log2);
     for (; at < sh.end; ++t) {
       Seq s = a.seq(b);
       for (; t >= split.tiles(s); t = 0) s = a.seq(++b);
       const int units = split.units(s, t);
-      const int u0 = (int)max(0ll, sh.begin - at), u1 = (int)min((long long)units, sh.end - at);
+      const int u0 = split.from(sh, at, units), u1 = split.to(sh, at, units);
+      if (u0 == u1) break;
       const int g = t * kPairRows + (int)rank * 64 + row;
       const bool live = g < s.n * a.heads;
-      const int sees = live ? s.len - s.n + g / a.heads + 1 : 0;
+      // rows behind the last are computed without a mask (it would cost every unit) and not written
+      const int sees = live ? s.len - s.n + g / a.heads + 1 : INT_MAX;
       float m = -INFINITY, l = 0.0f;
       for (int u = u0; u < u1; ++u, ++n) {
         const int buf = n & 1;
@@ -822,7 +858,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPaThreads, 1)
         }
         const float ref = m == -INFINITY ? 0.0f : m;
         if (u > u0 && __any_sync(0xffffffffu, alpha != 1.0f)) {   // rescale, once the unit before has been added
-          ok = __all_sync(0xffffffffu, pair_wait(a.c, pvdone, (n - 1) & 1, dead)) && ok;
+          ok = all_added(n) && ok;
           tc_fence_after();
 #pragma unroll 1
           for (int c = 0; c < 128; c += 32) {
@@ -869,7 +905,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPaThreads, 1)
         __syncwarp();
         if (lane == 0) arrive_cluster(lead_pfull);
       }
-      ok = __all_sync(0xffffffffu, pair_wait(a.c, pvdone, (n - 1) & 1, dead)) && ok;
+      ok = all_added(n) && ok;
       tc_fence_after();
       asm volatile("bar.sync %0, 128;" ::"r"(meet) : "memory");   // the last maxima are read
       ctl.top[0][part64][row] = l;
@@ -879,33 +915,37 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPaThreads, 1)
       const long long out_row = (long long)s.q0 * a.heads + g;
       float* part = a.part + (((long long)worker * 2 + (u0 == 0 ? 1 : 0)) * kPairRows + rank * 64 + row) * kPartRow;
       const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
-      // through this warp's 4 KB of P, which the instructions have read: 32 rows x 32 dims, so that a row's dims leave
-      // in one piece
-      float* stage = reinterpret_cast<float*>(smem_raw + kPaP + warp * 4096);
-      const float factor = whole ? inv : 1.0f;
+      // through this warp's 4 KB of P, which the instructions have read, so that a row's dims leave in pieces of 128 bytes:
+      // 32 rows x 64 dims of results, 32 dims of running sums
+      unsigned char* stage = smem_raw + kPaP + warp * 4096;
+      const int mine = lane & 7, dim0 = wg * 256 + (quarter >> 1) * 128, rows_here = s.n * a.heads - (g - lane);
 #pragma unroll 1
       for (int c = 0; c < 128; c += 32) {
-        const int dim = wg * 256 + (quarter >> 1) * 128 + c + (lane & 7) * 4;
         float o[32];
         tmem_ld32(tmem + wg * 128 + tlane + c, o);
         tmem_ld_wait();
+        if (whole) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-          *reinterpret_cast<float4*>(stage + lane * 32 + ((i ^ (lane & 7)) * 4)) =
-              make_float4(o[i * 4] * factor, o[i * 4 + 1] * factor, o[i * 4 + 2] * factor, o[i * 4 + 3] * factor);
+          for (int i = 0; i < 4; ++i) {
+            __nv_bfloat162 w[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) w[k] = __floats2bfloat162_rn(o[i * 8 + k * 2] * inv, o[i * 8 + k * 2 + 1] * inv);
+            *reinterpret_cast<uint4*>(stage + lane * 128 + ((((c >> 3) & 4) + i) ^ mine) * 16) = *reinterpret_cast<const uint4*>(w);
+          }
+          if (!(c & 32)) continue;
+        } else {
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            *reinterpret_cast<float4*>(stage + lane * 128 + (i ^ mine) * 16) = make_float4(o[i * 4], o[i * 4 + 1], o[i * 4 + 2], o[i * 4 + 3]);
+        }
         __syncwarp();
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          const int r = i * 4 + (lane >> 3);
-          const float4 v = *reinterpret_cast<const float4*>(stage + r * 32 + (((lane & 7) ^ (r & 7)) * 4));
-          const int gr = g - lane + r;   // row r of this warp's 32
-          if (ok && gr < s.n * a.heads) {
-            if (whole) {
-              const __nv_bfloat162 w[2] = {__floats2bfloat162_rn(v.x, v.y), __floats2bfloat162_rn(v.z, v.w)};
-              *reinterpret_cast<uint2*>(a.out + ((long long)s.q0 * a.heads + gr) * kLat + dim) = *reinterpret_cast<const uint2*>(w);
-            } else {
-              *reinterpret_cast<float4*>(part + (long long)(r - lane) * kPartRow + dim) = v;
-            }
+          const int r = i * 4 + (lane >> 3);   // row of this warp's 32
+          const uint4 v = *reinterpret_cast<const uint4*>(stage + r * 128 + (mine ^ (r & 7)) * 16);
+          if (ok && r < rows_here) {
+            if (whole) *reinterpret_cast<uint4*>(a.out + (out_row - lane + r) * kLat + dim0 + (c & 64) + mine * 8) = v;
+            else *reinterpret_cast<uint4*>(part + (long long)(r - lane) * kPartRow + dim0 + c + mine * 4) = v;
           }
         }
         __syncwarp();
@@ -920,12 +960,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPaThreads, 1)
       }
       if (ok && u0 == 0 && u1 < units && tid == 0 && rank == 0) {   // the workers of this tile: up to its last unit's
         int last = worker;
-        while (sh.total * (last + 1) / sh.workers < at + units) ++last;
+        while (sh.total * (last + 1) / sh.workers < at + kPaTileCost + units) ++last;
         a.meta[worker * 4] = b;
         a.meta[worker * 4 + 1] = t;
         a.meta[worker * 4 + 2] = last - worker + 1;
       }
-      at += units;
+      at += units + kPaTileCost;
       tc_fence_before();   // TMEM is read before the next tile's first sums, which wait for its probabilities
       asm volatile("bar.sync %0, 128;" ::"r"(meet) : "memory");   // the sums are read before the next maxima
     }
