@@ -30,6 +30,7 @@ struct PairMaps {
 struct PairRows {
   int kv_ratio, pe_ratio;   // rows from one page to the next
   int kv_end, pe_end;       // number of the first row behind the pool: reads as zeros
+  long long kv_pitch, pe_pitch;   // elements from one row to the next
   int box;                  // rows of a box: divides a page and 64, 8 at least; 0: gathers only
 };
 
@@ -57,22 +58,24 @@ KK3_DEV void cluster_sync() {
 KK3_DEV void arrive_cluster(unsigned addr) {
   asm volatile("mbarrier.arrive.release.cta.shared::cluster.b64 _, [%0];" ::"r"(addr) : "memory");
 }
-// Bounded wait; false when it ran out or another role of the CTA gave up (*dead).
-KK3_DEV bool pair_wait(const CachePages& c, unsigned bar, unsigned parity, volatile int* dead) {
-  if (mbar_test(bar, parity)) return true;
-  if (*dead) return false;
+// Bounded wait; false when it ran out or another role of the CTA gave up (*dead). The part that waits is not inlined:
+// the roles' loops stay short.
+static __device__ __noinline__ bool pair_wait_on(int* error_word, unsigned bar, unsigned parity, volatile int* dead) {
   const unsigned long long t0 = globaltimer();
   for (unsigned spin = 1;; ++spin) {
     if (mbar_test(bar, parity)) return true;
-    if ((spin & 15) == 0) {
+    if ((spin & 15) == 0 || spin == 1) {
       if (*dead) return false;
       if (globaltimer() - t0 > kWaitNs) {
         *dead = 1;
-        if (c.error_word) *reinterpret_cast<volatile int*>(c.error_word) = kErrTimeout;
+        if (error_word) *reinterpret_cast<volatile int*>(error_word) = kErrTimeout;
         return false;
       }
     }
   }
+}
+KK3_DEV bool pair_wait(const CachePages& c, unsigned bar, unsigned parity, volatile int* dead) {
+  return mbar_test(bar, parity) || pair_wait_on(c.error_word, bar, parity, dead);
 }
 // Copies are issued by one lane (`me`) of a converged warp: 50 clocks each, against 90 in a branch of one lane, where
 // every operand moves to the uniform registers anew.
@@ -99,15 +102,6 @@ KK3_DEV void load_box(bool me, unsigned dst, const CUtensorMap* map, int x, int 
       "[%1, {%2, %3}], [%4];\n}"
       ::"r"(dst), "l"(map), "r"(x), "r"(row), "r"(bar), "r"((unsigned)me)
       : "memory");
-}
-// whether a phase has completed, without the wait that try_wait may make
-KK3_DEV bool pair_seen(unsigned bar, unsigned parity) {
-  unsigned ok;
-  asm volatile(
-      "{\n .reg .pred p;\n mbarrier.test_wait.parity.acquire.cta.shared::cta.b64 p, [%1], %2;\n"
-      " selp.u32 %0, 1, 0, p;\n}"
-      : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
-  return ok != 0;
 }
 KK3_DEV void pair_mma(unsigned d, unsigned long long a, unsigned long long b, unsigned idesc, unsigned accumulate) {
   asm volatile(
@@ -224,15 +218,20 @@ KK3_DEV void load_entries(bool me, const PairMaps& m, const RowTab& tab, int box
   }
 }
 
-// Bring 128 positions from number `off` of the table on into L2, for loads one unit later: HBM's latency is longer than
-// what the ring holds. One instruction per box, where a box's rows lie without gaps.
+// Bring 128 positions from number `off` of the table on into L2, for copies one unit later: HBM's latency is longer than
+// what the ring holds. By plain prefetches of 128 bytes: bulk ones queue up before the copies (single tokens of 64
+// sequences over 8192 positions took 205 us with them, 152 without).
 KK3_DEV void prefetch_entries(const CachePages& c, const PairRows& pr, const RowTab& tab, int off) {
   const int lane = threadIdx.x & 31;
-  if (!pr.box || c.kv_row != kLat || c.pe_row != kRope || lane * pr.box >= 128) return;
-  const int kv = tab.kv[off + lane * pr.box], pe = tab.pe[off + lane * pr.box];
-  if (kv == pr.kv_end) return;
-  asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(c.kv + (long long)kv * kLat), "r"(pr.box * kLat * 2) : "memory");
-  asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(c.pe + (long long)pe * kRope), "r"(pr.box * kRope * 2) : "memory");
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int kv = tab.kv[off + i * 32 + lane], pe = tab.pe[off + i * 32 + lane];
+    if (kv == pr.kv_end) continue;
+    const bf16* row = c.kv + (long long)kv * pr.kv_pitch;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) asm volatile("prefetch.global.L2 [%0];" ::"l"(row + k * 64));
+    asm volatile("prefetch.global.L2 [%0];" ::"l"(c.pe + (long long)pe * pr.pe_pitch));
+  }
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -518,7 +517,7 @@ __global__ void __launch_bounds__(kMassPos) kk3_cache_mass_join_kernel(const Mas
 // clocks measured, 175 more for a commit), so narrower ones would leave the tensor cores waiting.
 //
 // Per unit each CTA loads 128 of the positions (nine blocks of 64 dims) for the scores, and half of the output dims of
-// all 256 (eight pieces of 64 positions x 128 dims) for the sums, 16 KB each, through a ring of four and one of three.
+// all 256 (four stages of 64 positions x 2 x 128 dims, 32 KB) for the sums, through a ring of 48 KB and one of 64 KB.
 // Scores run one unit ahead of sums, and a thread each issues them: what one spends in commits is the other's.
 //
 // Softmax: four threads per row, 64 of a unit's positions each, that exchange maxima through shared memory. The running
@@ -533,13 +532,14 @@ constexpr int kPaUnit = 256;
 constexpr int kPaThreads = 384;        // warps 0-7 softmax, 8 and 9 copies and instructions of scores, 10 and 11 of sums
 constexpr int kPaQBlock = 64 * 128;    // 64 rows of 64 dims
 constexpr int kPaBlock = 128 * 128;    // 128 positions x 64 dims, or 64 positions x 128 dims
-constexpr int kPaKSlots = 4, kPaVSlots = 3;
+constexpr int kPaKSlots = 3;           // 16 KB each; nine blocks a unit: block d is in slot d % 3
+constexpr int kPaVSlots = 2;           // 32 KB each; four stages a unit: stage g is in slot g % 2
 constexpr int kPaMinUnits = 3;
 constexpr int kPaTileCost = 2;   // what a tile costs besides its units, in units: query load, first and last latencies
 constexpr float kPaSlack = 8.0f;
 struct PaCtl {
   unsigned long long qfull, qempty, kfull[kPaKSlots], kempty[kPaKSlots], vfull[kPaVSlots], vempty[kPaVSlots], sfull[2],
-      sfree[2], oready, pfull[4], pfree[4], pvdone, done;
+      sfree[2], oready[2], pfull[4], pfree[4], pvdone[2], done;
   unsigned tmem;
   int dead;
   long long red[kPaThreads / 32 + 4];
@@ -547,7 +547,7 @@ struct PaCtl {
   float top[2][4][64];   // [unit parity][64 positions of 256][row]: maxima (at the end: sums) of a row's four threads
 };
 constexpr int kPaQ = 0, kPaP = kPaQ + kBlocks * kPaQBlock, kPaK = kPaP + 4 * kPaQBlock,
-              kPaV = kPaK + kPaKSlots * kPaBlock, kPaCtl = kPaV + kPaVSlots * kPaBlock;
+              kPaV = kPaK + kPaKSlots * kPaBlock, kPaCtl = kPaV + kPaVSlots * 2 * kPaBlock;
 constexpr int kPaSmem = kPaCtl + (int)sizeof(PaCtl);
 static_assert(kPaSmem <= 232448, "shared memory of a CTA");
 
@@ -576,8 +576,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPaThreads, 1)
   const unsigned rank = cluster_rank(), base = smem_u32(smem_raw);
   const unsigned qfull = smem_u32(&ctl.qfull), qempty = smem_u32(&ctl.qempty), kfull = smem_u32(ctl.kfull),
                  kempty = smem_u32(ctl.kempty), vfull = smem_u32(ctl.vfull), vempty = smem_u32(ctl.vempty),
-                 sfull = smem_u32(ctl.sfull), sfree = smem_u32(ctl.sfree), oready = smem_u32(&ctl.oready),
-                 pfull = smem_u32(ctl.pfull), pfree = smem_u32(ctl.pfree), pvdone = smem_u32(&ctl.pvdone),
+                 sfull = smem_u32(ctl.sfull), sfree = smem_u32(ctl.sfree), oready = smem_u32(ctl.oready),
+                 pfull = smem_u32(ctl.pfull), pfree = smem_u32(ctl.pfree), pvdone = smem_u32(ctl.pvdone),
                  done = smem_u32(&ctl.done);
   volatile int* dead = &ctl.dead;
   if (tid == 0) {
@@ -595,12 +595,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPaThreads, 1)
       mbar_init(sfull + 8 * i, 1);
       mbar_init(sfree + 8 * i, 16);   // the softmax warps of both CTAs
     }
-    mbar_init(oready, 16);
+    mbar_init(oready, 16);   // units in turn: one CTA's warps may be a unit ahead of the other's, never two
+    mbar_init(oready + 8, 16);
     for (int i = 0; i < 4; ++i) {
       mbar_init(pfull + 8 * i, 4);   // the warps of these 64 positions, of both CTAs
       mbar_init(pfree + 8 * i, 1);
     }
-    mbar_init(pvdone, 1);
+    mbar_init(pvdone, 1);   // units in turn
+    mbar_init(pvdone + 8, 1);
     mbar_init(done, 2);
     ctl.dead = 0;
     fence_mbar_init();
@@ -629,7 +631,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPaThreads, 1)
     // ---- queries, and the entries' blocks for the scores
     const unsigned lead_q = in_cta(qfull, 0), lead_k = in_cta(kfull, 0);
     const bool me = elect_one();
-    int slot = 0, phase = 0;
     for (; ok && at < sh.end; ++t, ++tile) {
       Seq s = a.seq(b);
       for (; t >= split.tiles(s); t = 0) s = a.seq(++b);
@@ -659,32 +660,29 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPaThreads, 1)
         ids.fetch(a.c, pr, b, (u + 2) * kPaUnit, end);
         if (once && u + 1 < u1) prefetch_entries(a.c, pr, tab_next, (int)rank * 128);
         for (int d = 0; d < kBlocks; ++d) {
-          ok = __all_sync(0xffffffffu, pair_wait(a.c, kempty + 8 * slot, phase ^ 1, dead));
+          const int slot = d % kPaKSlots, use = n + d / kPaKSlots;   // (three uses a unit: their parity)
+          ok = __all_sync(0xffffffffu, pair_wait(a.c, kempty + 8 * slot, (use & 1) ^ 1, dead));
           if (!ok) break;
           if (rank == 0 && me) mbar_arrive_tx(kfull + 8 * slot, 2 * kPaBlock);
           __syncwarp();
           load_entries<128>(me, maps, tab, pr.box, d, (int)rank * 128, base + kPaK + slot * kPaBlock, lead_k + 8 * slot);
-          if (++slot == kPaKSlots) {
-            slot = 0;
-            phase ^= 1;
-          }
         }
+        ++n;
         __syncwarp();   // the table is read
       }
       at += units + kPaTileCost;
     }
     if (rank == 0 && lane == 0 && !ok) {   // after a failed wait: a bounded time for the copies in flight
       mbar_wait_for(qfull, (tile & 1) ^ 1, kWaitNs);
-      for (int i = 0; i < kPaKSlots; ++i) mbar_wait_for(kfull + 8 * i, i < slot ? phase : phase ^ 1, kWaitNs);
+      for (int i = 0; i < 2 * kPaKSlots; ++i) mbar_wait_for(kfull + 8 * (i / 2), i & 1, kWaitNs / 8);
     }
     __syncwarp();
   } else if (warp == 10) {
-    // ---- the entries' pieces for the sums: piece (g, h) is dims 256 h + 128 rank .. + 127 of positions 64 g .. + 63 of
-    // the unit. Positions that no row sees must be zeros, whatever the page holds there: a group that `end` cuts comes
-    // row by row.
+    // ---- the entries' stages for the sums: stage g is dims 256 h + 128 rank .. + 127, h = 0 and 1, of positions 64 g ..
+    // + 63 of the unit. Positions that no row sees must be zeros, whatever the page holds there: a stage that `end` cuts
+    // comes row by row.
     const unsigned lead_v = in_cta(vfull, 0);
     const bool me = elect_one();
-    int slot = 0, phase = 0;
     for (; ok && at < sh.end; ++t) {
       Seq s = a.seq(b);
       for (; t >= split.tiles(s); t = 0) s = a.seq(++b);
@@ -697,52 +695,30 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPaThreads, 1)
         ids.write(a.c, pr, u * kPaUnit, end, ctl.rows[2]);
         __syncwarp();
         ids.fetch(a.c, pr, b, (u + 1) * kPaUnit, end);
-        for (int i = 0; i < 8; ++i) {
-          const int g = i >> 1, h = i & 1, left = end - (u * kPaUnit + g * 64);
-          const unsigned dst = base + kPaV + slot * kPaBlock, bar = lead_v + 8 * slot;
-          ok = __all_sync(0xffffffffu, pair_wait(a.c, vempty + 8 * slot, phase ^ 1, dead));
+        for (int g = 0; g < 4; ++g) {
+          const int slot = g % kPaVSlots, left = end - (u * kPaUnit + g * 64);   // two uses a unit
+          const unsigned dst = base + kPaV + slot * 2 * kPaBlock, bar = lead_v + 8 * slot;
+          ok = __all_sync(0xffffffffu, pair_wait(a.c, vempty + 8 * slot, (g / kPaVSlots) ^ 1, dead));
           if (!ok) break;
-          if (rank == 0 && me) mbar_arrive_tx(vfull + 8 * slot, 2 * kPaBlock);
+          if (rank == 0 && me) mbar_arrive_tx(vfull + 8 * slot, 4 * kPaBlock);
           __syncwarp();
           const int box = left > 0 && left < 64 ? 0 : pr.box;
-#pragma unroll
-          for (int j = 0; j < 2; ++j)
-            load_entries<64>(me, maps, ctl.rows[2], box, 4 * h + 2 * (int)rank + j, g * 64, dst + j * (kPaBlock / 2), bar);
-          if (++slot == kPaVSlots) {
-            slot = 0;
-            phase ^= 1;
-          }
+#pragma unroll 1
+          for (int j = 0; j < 4; ++j)
+            load_entries<64>(me, maps, ctl.rows[2], box, 4 * (j >> 1) + 2 * (int)rank + (j & 1), g * 64, dst + j * (kPaBlock / 2), bar);
         }
         __syncwarp();   // the table is read
       }
       at += units + kPaTileCost;
     }
     if (rank == 0 && lane == 0 && !ok)
-      for (int i = 0; i < kPaVSlots; ++i) mbar_wait_for(vfull + 8 * i, i < slot ? phase : phase ^ 1, kWaitNs);
+      for (int i = 0; i < 2 * kPaVSlots; ++i) mbar_wait_for(vfull + 8 * (i / 2), i & 1, kWaitNs / 8);
     __syncwarp();
   } else if (warp == 9 || warp == 11) {
-    // ---- matrix instructions: two threads of the pair. Issuing costs as much as the instructions take, so the next
-    // slot's barrier is tested before the current slot's instructions (its answer is there when they are out) and the
-    // descriptors are sums of 16-byte offsets.
+    // ---- matrix instructions: two threads of the pair. Issuing costs as much as the instructions take, so the loops are
+    // unrolled over the slots and the descriptors are sums of 16-byte offsets.
     if (lane == 0 && rank == 0) {
       constexpr unsigned id_s = pair_idesc(128, 256), id_o = id_s | (1u << 16);   // values are MN-major
-      const int slots = warp == 9 ? kPaKSlots : kPaVSlots;
-      const unsigned fullb = warp == 9 ? kfull : vfull, emptyb = warp == 9 ? kempty : vempty;
-      int slot = 0, phase = 0;
-      bool there = false;   // whether the slot's data were seen already
-      const auto take = [&]() {   // waits for the slot; looks at the next one
-        if (!there) ok = pair_wait(a.c, fullb + 8 * slot, phase, dead);
-        tc_fence_after();
-        const int ns = slot + 1 == slots ? 0 : slot + 1;
-        there = pair_seen(fullb + 8 * ns, ns ? phase : phase ^ 1);
-      };
-      const auto give = [&]() {
-        pair_commit(emptyb + 8 * slot);
-        if (++slot == slots) {
-          slot = 0;
-          phase ^= 1;
-        }
-      };
       for (; ok && at < sh.end; ++t, ++tile) {
         Seq s = a.seq(b);
         for (; t >= split.tiles(s); t = 0) s = a.seq(++b);
@@ -754,14 +730,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPaThreads, 1)
           ok = pair_wait(a.c, qfull, tile & 1, dead);
           for (int u = u0; ok && u < u1; ++u, ++n) {
             const int buf = n & 1;
+            const unsigned d = tmem_s + buf * 128;
             ok = pair_wait(a.c, sfree + 8 * buf, ((n >> 1) & 1) ^ 1, dead);
-            for (int d = 0; ok && d < kBlocks; ++d) {
-              take();
-              if (!ok) break;
-              const unsigned long long qa = qd + d * (kPaQBlock >> 4), ka = kd + slot * (kPaBlock >> 4);
 #pragma unroll
-              for (int k = 0; k < 4; ++k) pair_mma(tmem_s + buf * 128, qa + k * 2, ka + k * 2, id_s, (unsigned)(d | k));
-              give();
+            for (int i = 0; i < kBlocks; ++i) {
+              const int slot = i % kPaKSlots;
+              if (ok) ok = pair_wait(a.c, kfull + 8 * slot, (n + i / kPaKSlots) & 1, dead);
+              if (!ok) break;
+              tc_fence_after();
+#pragma unroll
+              for (int k = 0; k < 4; ++k)
+                pair_mma(d, qd + i * (kPaQBlock >> 4) + k * 2, kd + slot * (kPaBlock >> 4) + k * 2, id_s, (unsigned)(i | k));
+              pair_commit(kempty + 8 * slot);
             }
             if (ok) pair_commit(sfull + 8 * buf);
           }
@@ -769,19 +749,21 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPaThreads, 1)
         } else {
           const unsigned long long pd = sdesc_sw128(base + kPaP), vd = sdesc_mn(base + kPaV, kPaBlock / 2);
           for (int u = u0; ok && u < u1; ++u, ++n) {
-            ok = pair_wait(a.c, oready, n & 1, dead);
-            for (int i = 0; ok && i < 8; ++i) {
-              if (!(i & 1)) ok = pair_wait(a.c, pfull + 4 * i, n & 1, dead);
-              if (ok) take();
-              if (!ok) break;
-              const unsigned long long pa = pd + (i >> 1) * (kPaQBlock >> 4), va = vd + slot * (kPaBlock >> 4);
+            ok = pair_wait(a.c, oready + 8 * (n & 1), (n >> 1) & 1, dead);
 #pragma unroll
-              for (int k = 0; k < 4; ++k)
-                pair_mma(tmem + (i & 1) * 128, pa + k * 2, va + k * 128, id_o, (unsigned)(u > u0 || i > 1 || k));
-              give();
-              if (i & 1) pair_commit(pfree + 4 * (i - 1));
+            for (int g = 0; g < 4; ++g) {
+              const int slot = g % kPaVSlots;
+              if (ok) ok = pair_wait(a.c, pfull + 8 * g, n & 1, dead) && pair_wait(a.c, vfull + 8 * slot, g / kPaVSlots, dead);
+              if (!ok) break;
+              tc_fence_after();
+#pragma unroll
+              for (int k = 0; k < 8; ++k)
+                pair_mma(tmem + (k >> 2) * 128, pd + g * (kPaQBlock >> 4) + (k & 3) * 2,
+                         vd + (slot * 2 + (k >> 2)) * (kPaBlock >> 4) + (k & 3) * 128, id_o, (unsigned)(u > u0 || g || (k & 3)));
+              pair_commit(vempty + 8 * slot);
+              pair_commit(pfree + 8 * g);
             }
-            if (ok) pair_commit(pvdone);
+            if (ok) pair_commit(pvdone + 8 * (n & 1));
           }
         }
         at += units + kPaTileCost;
@@ -799,14 +781,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPaThreads, 1)
     const unsigned lead_sfree = in_cta(sfree, 0), lead_oready = in_cta(oready, 0),
                    lead_pfull = in_cta(pfull + 8 * part64, 0);
     const unsigned p_row = base + kPaP + part64 * kPaQBlock + row * 128;
-    // Units before number m have been added to O. Where this thread stands, the one three before is known to be added
-    // (this thread's part of P was free again for the one two before); a barrier only tells a phase from its neighbours,
-    // so the last two are waited for one after the other.
+    // Units before number m have been added to O. A barrier's parity only tells a phase from its neighbours: each of the
+    // two has every other unit, and where this is asked, the unit three before is known to be added (this thread's part
+    // of P was free again from the one two before) and the next one waits for this thread.
     const auto all_added = [&](int m) {
-      bool done = true;
-      if (m > 1) done = pair_wait(a.c, pvdone, (m - 2) & 1, dead);
-      if (m > 0) done = pair_wait(a.c, pvdone, (m - 1) & 1, dead) && done;
-      return __all_sync(0xffffffffu, done) != 0;
+      return __all_sync(0xffffffffu, m == 0 || pair_wait(a.c, pvdone + 8 * ((m - 1) & 1), ((m - 1) >> 1) & 1, dead)) != 0;
     };
     const float sign = a.scale_log2 < 0.0f ? -1.0f : 1.0f, size = fabsf(a.scale_log2);
     for (; at < sh.end; ++t) {
@@ -873,7 +852,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPaThreads, 1)
         }
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) arrive_cluster(lead_oready);
+        if (lane == 0) arrive_cluster(lead_oready + 8 * buf);
 #pragma unroll
         for (int i = 0; i < 64; ++i) {
           float& x = v[i >> 5][i & 31];
@@ -999,7 +978,7 @@ static int encode_rows(CUtensorMap* map, const void* base, int cols, int64_t row
 }
 
 // maps of all the rows of a [pages, page_size, cols] tensor: in boxes and row by row
-static int map_pages(CUtensorMap* by_box, CUtensorMap* by_row, int* ratio, int* end, const void* base, int cols,
+static int map_pages(CUtensorMap* by_box, CUtensorMap* by_row, int* ratio, int* end, long long* pitch, const void* base, int cols,
                      const kk3_cache* c, int64_t page_stride, int64_t row_stride, int box) {
   const int64_t pages = c->num_pages;
   if (c->page_size == 1 && pages > 1) row_stride = page_stride;
@@ -1007,6 +986,7 @@ static int map_pages(CUtensorMap* by_box, CUtensorMap* by_row, int* ratio, int* 
   if (row_stride < cols || (pages > 1 && page_stride % row_stride) || rows >= INT32_MAX) return KK3_ERR_UNSUPPORTED;
   *ratio = (int)r;
   *end = (int)rows;
+  *pitch = row_stride;
   const int rc = encode_rows(by_row, base, cols, rows, row_stride, 1);
   return rc || !box ? rc : encode_rows(by_box, base, cols, rows, row_stride, box);
 }
@@ -1025,8 +1005,8 @@ static int pair_maps(const kk3_cache* c, const void* q_latent, int64_t ql_token,
   r->box = 64;
   while (c->page_size % r->box) r->box /= 2;
   if (r->box < 8) r->box = 0;
-  int rc = map_pages(&m->kv_box, &m->kv_row, &r->kv_ratio, &r->kv_end, c->kv, kLat, c, c->kv_page_stride, c->kv_row_stride, r->box);
-  if (!rc) rc = map_pages(&m->pe_box, &m->pe_row, &r->pe_ratio, &r->pe_end, c->pe, kRope, c, c->pe_page_stride, c->pe_row_stride, r->box);
+  int rc = map_pages(&m->kv_box, &m->kv_row, &r->kv_ratio, &r->kv_end, &r->kv_pitch, c->kv, kLat, c, c->kv_page_stride, c->kv_row_stride, r->box);
+  if (!rc) rc = map_pages(&m->pe_box, &m->pe_row, &r->pe_ratio, &r->pe_end, &r->pe_pitch, c->pe, kRope, c, c->pe_page_stride, c->pe_row_stride, r->box);
   if (!rc) rc = map_queries(&m->ql, q_latent, kLat, tokens, heads, ql_token, ql_head, q_box);
   if (!rc) rc = map_queries(&m->qp, q_pe, kRope, tokens, heads, qp_token, qp_head, q_box);
   return rc;
