@@ -13,6 +13,8 @@
 #include <limits.h>
 #include <string.h>
 
+#include <type_traits>
+
 #include "kk3_cache.cuh"
 #include "kk3_cache_host.h"
 #include "kk3_tcgen05.cuh"
@@ -190,31 +192,47 @@ struct PageIds {
     }
   }
 };
-// 64-dim block `d` of COUNT positions from number `off` of the table on into [COUNT][64] at `dst`; BOX 0: row by row.
+// COUNT positions of the table in boxes of BOX rows, their row numbers in registers; BOX 0: row by row, from the table.
 template <int COUNT, int BOX>
-KK3_DEV void load_entries_as(bool me, const PairMaps& m, const RowTab& tab, int d, int off, unsigned dst, unsigned bar) {
-  const bool rope = d == kBlocks - 1;
-  const int* rows = (rope ? tab.pe : tab.kv) + off;
-  const int x = rope ? 0 : d * 64;
-  if (BOX) {
-    constexpr int kBox = BOX ? BOX : 1;
-    const CUtensorMap* map = rope ? &m.pe_box : &m.kv_box;
+struct Boxes {
+  static constexpr int kMany = BOX ? COUNT / (BOX ? BOX : 1) : 1;
+  int kv[kMany], pe[kMany];
+  const RowTab* tab;
+  int off;
+  KK3_DEV void take(const RowTab& t, int from) {
+    tab = &t;
+    off = from;
 #pragma unroll
-    for (int k = 0; k < COUNT; k += kBox) load_box(me, dst + k * 128, map, x, rows[k], bar);
-  } else {
-    const CUtensorMap* map = rope ? &m.pe_row : &m.kv_row;
-#pragma unroll 4
-    for (int k = 0; k < COUNT; k += 4) gather4(me, dst + k * 128, map, x, *reinterpret_cast<const int4*>(&rows[k]), bar);
+    for (int i = 0; i < kMany; ++i) {
+      kv[i] = t.kv[from + i * BOX];
+      pe[i] = t.pe[from + i * BOX];
+    }
   }
-}
-template <int COUNT>
-KK3_DEV void load_entries(bool me, const PairMaps& m, const RowTab& tab, int box, int d, int off, unsigned dst, unsigned bar) {
+  // 64-dim block `d` of them into [COUNT][64] at `dst`
+  KK3_DEV void load(bool me, const PairMaps& m, int d, unsigned dst, unsigned bar) const {
+    const bool rope = d == kBlocks - 1;
+    const int x = rope ? 0 : d * 64;
+    if (BOX) {
+#pragma unroll
+      for (int i = 0; i < kMany; ++i)
+        load_box(me, dst + i * BOX * 128, rope ? &m.pe_box : &m.kv_box, x, rope ? pe[i] : kv[i], bar);
+    } else {
+      const int* rows = (rope ? tab->pe : tab->kv) + off;
+#pragma unroll 4
+      for (int k = 0; k < COUNT; k += 4)
+        gather4(me, dst + k * 128, rope ? &m.pe_row : &m.kv_row, x, *reinterpret_cast<const int4*>(&rows[k]), bar);
+    }
+  }
+};
+// f(integral constant of the call's box)
+template <class F>
+KK3_DEV void with_box(int box, const F& f) {
   switch (box) {
-    case 64: return load_entries_as<COUNT, 64>(me, m, tab, d, off, dst, bar);
-    case 32: return load_entries_as<COUNT, 32>(me, m, tab, d, off, dst, bar);
-    case 16: return load_entries_as<COUNT, 16>(me, m, tab, d, off, dst, bar);
-    case 8: return load_entries_as<COUNT, 8>(me, m, tab, d, off, dst, bar);
-    default: return load_entries_as<COUNT, 0>(me, m, tab, d, off, dst, bar);
+    case 64: return f(std::integral_constant<int, 64>());
+    case 32: return f(std::integral_constant<int, 32>());
+    case 16: return f(std::integral_constant<int, 16>());
+    case 8: return f(std::integral_constant<int, 8>());
+    default: return f(std::integral_constant<int, 0>());
   }
 }
 
@@ -340,24 +358,29 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMassThreads, 1)
       ids.fetch(a.c, pr, b, (t + 1) * kMassPos, s.len);
       ahead_b = b;
       ahead_t = t + 1;
-      for (int u = u0; ok && u < u1; ++u) {
-        const int q = s.q0 * a.heads + (first + u) * rows + (int)rank * half;   // rows behind the sequence's: masked
-        for (int d = 0; d < kBlocks; ++d) {
-          const unsigned bar = lead_full + 8 * slot, qd = qbase + slot * slot_bytes;
-          ok = pair_wait(a.c, empty + 8 * slot, phase ^ 1, dead);
-          if (u == u0) ok = pair_wait(a.c, kempty + 8 * d, (tile & 1) ^ 1, dead) && ok;
-          ok = __all_sync(0xffffffffu, ok);
-          if (!ok) break;
-          if (rank == 0 && me) mbar_arrive_tx(full + 8 * slot, 2 * (slot_bytes + (u == u0 ? kMassKBlock : 0)));
-          __syncwarp();
-          if (u == u0) load_entries<128>(me, maps, ctl.rows, pr.box, d, (int)rank * 128, kbase + d * kMassKBlock, bar);
-          load_box(me, qd, d < kBlocks - 1 ? &maps.ql : &maps.qp, d < kBlocks - 1 ? d * 64 : 0, q, bar);
-          if (++slot == slots) {
-            slot = 0;
-            phase ^= 1;
+      with_box(pr.box, [&](auto box) {
+        Boxes<128, decltype(box)::value> boxes;
+        boxes.take(ctl.rows, (int)rank * 128);
+        for (int u = u0; ok && u < u1; ++u) {
+          const int q = s.q0 * a.heads + (first + u) * rows + (int)rank * half;   // rows behind the sequence's: masked
+#pragma unroll 1
+          for (int d = 0; d < kBlocks; ++d) {
+            const unsigned bar = lead_full + 8 * slot, qd = qbase + slot * slot_bytes;
+            ok = pair_wait(a.c, empty + 8 * slot, phase ^ 1, dead);
+            if (u == u0) ok = pair_wait(a.c, kempty + 8 * d, (tile & 1) ^ 1, dead) && ok;
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+            if (rank == 0 && me) mbar_arrive_tx(full + 8 * slot, 2 * (slot_bytes + (u == u0 ? kMassKBlock : 0)));
+            __syncwarp();
+            if (u == u0) boxes.load(me, maps, d, kbase + d * kMassKBlock, bar);
+            load_box(me, qd, d < kBlocks - 1 ? &maps.ql : &maps.qp, d < kBlocks - 1 ? d * 64 : 0, q, bar);
+            if (++slot == slots) {
+              slot = 0;
+              phase ^= 1;
+            }
           }
         }
-      }
+      });
       at += units;
       ++t;
       ++tile;
@@ -517,7 +540,7 @@ __global__ void __launch_bounds__(kMassPos) kk3_cache_mass_join_kernel(const Mas
 // clocks measured, 175 more for a commit), so narrower ones would leave the tensor cores waiting.
 //
 // Per unit each CTA loads 128 of the positions (nine blocks of 64 dims) for the scores, and half of the output dims of
-// all 256 (four stages of 64 positions x 2 x 128 dims, 32 KB) for the sums, through a ring of 48 KB and one of 64 KB.
+// all 256 (four stages of 64 positions x 2 x 128 dims, 32 KB) for the sums, through two rings of 64 KB.
 // Scores run one unit ahead of sums, and a thread each issues them: what one spends in commits is the other's.
 //
 // Softmax: four threads per row, 64 of a unit's positions each, that exchange maxima through shared memory. The running
@@ -532,7 +555,7 @@ constexpr int kPaUnit = 256;
 constexpr int kPaThreads = 384;        // warps 0-7 softmax, 8 and 9 copies and instructions of scores, 10 and 11 of sums
 constexpr int kPaQBlock = 64 * 128;    // 64 rows of 64 dims
 constexpr int kPaBlock = 128 * 128;    // 128 positions x 64 dims, or 64 positions x 128 dims
-constexpr int kPaKSlots = 3;           // 16 KB each; nine blocks a unit: block d is in slot d % 3
+constexpr int kPaKSlots = 4;           // 16 KB each; nine blocks a unit
 constexpr int kPaVSlots = 2;           // 32 KB each; four stages a unit: stage g is in slot g % 2
 constexpr int kPaMinUnits = 3;
 constexpr int kPaTileCost = 2;   // what a tile costs besides its units, in units: query load, first and last latencies
@@ -546,7 +569,7 @@ struct PaCtl {
   RowTab rows[3];        // entries of a unit: the scores' (two, in turn) and the sums'
   float top[2][4][64];   // [unit parity][64 positions of 256][row]: maxima (at the end: sums) of a row's four threads
 };
-constexpr int kPaQ = 0, kPaP = kPaQ + kBlocks * kPaQBlock, kPaK = kPaP + 4 * kPaQBlock,
+constexpr int kPaQ = 0, kPaP = kPaQ + kBlocks * kPaQBlock, kPaK = kPaP + 2 * kPaQBlock,
               kPaV = kPaK + kPaKSlots * kPaBlock, kPaCtl = kPaV + kPaVSlots * 2 * kPaBlock;
 constexpr int kPaSmem = kPaCtl + (int)sizeof(PaCtl);
 static_assert(kPaSmem <= 232448, "shared memory of a CTA");
@@ -631,47 +654,53 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPaThreads, 1)
     // ---- queries, and the entries' blocks for the scores
     const unsigned lead_q = in_cta(qfull, 0), lead_k = in_cta(kfull, 0);
     const bool me = elect_one();
-    for (; ok && at < sh.end; ++t, ++tile) {
-      Seq s = a.seq(b);
-      for (; t >= split.tiles(s); t = 0) s = a.seq(++b);
-      const int units = split.units(s, t), end = split.sees(s, t);
-      const int u0 = split.from(sh, at, units), u1 = split.to(sh, at, units);
-      if (u0 == u1) break;   // only a tile's cost is left: the next worker's
-      PageIds ids;
-      ids.fetch(a.c, pr, b, u0 * kPaUnit, end);
-      const bool once = s.n * a.heads <= kPairRows;   // the cache is read by this tile alone: it comes from HBM
-      ok = __all_sync(0xffffffffu, pair_wait(a.c, qempty, (tile & 1) ^ 1, dead));
-      if (!ok) break;
-      {
+    with_box(pr.box, [&](auto box) {
+      int slot = 0, phase = 0;
+      for (; ok && at < sh.end; ++t, ++tile) {
+        Seq s = a.seq(b);
+        for (; t >= split.tiles(s); t = 0) s = a.seq(++b);
+        const int units = split.units(s, t), end = split.sees(s, t);
+        const int u0 = split.from(sh, at, units), u1 = split.to(sh, at, units);
+        if (u0 == u1) break;   // only a tile's cost is left: the next worker's
+        PageIds ids;
+        ids.fetch(a.c, pr, b, u0 * kPaUnit, end);
+        const bool once = s.n * a.heads <= kPairRows;   // the cache is read by this tile alone: it comes from HBM
+        ok = __all_sync(0xffffffffu, pair_wait(a.c, qempty, (tile & 1) ^ 1, dead));
+        if (!ok) break;
         if (rank == 0 && me) mbar_arrive_tx(qfull, 2 * kBlocks * kPaQBlock);
         __syncwarp();
         const int q = s.q0 * a.heads + t * kPairRows + (int)rank * 64;   // rows behind the sequence's are not written
 #pragma unroll
         for (int d = 0; d < kBlocks; ++d)
           load_box(me, base + kPaQ + d * kPaQBlock, d < kBlocks - 1 ? &maps.ql : &maps.qp, d < kBlocks - 1 ? d * 64 : 0, q, lead_q);
-      }
-      ids.write(a.c, pr, u0 * kPaUnit, end, ctl.rows[0]);
-      ids.fetch(a.c, pr, b, (u0 + 1) * kPaUnit, end);
-      for (int u = u0; ok && u < u1; ++u) {
-        const RowTab& tab = ctl.rows[(u - u0) & 1];
-        RowTab& tab_next = ctl.rows[((u - u0) & 1) ^ 1];
-        ids.write(a.c, pr, (u + 1) * kPaUnit, end, tab_next);
-        __syncwarp();
-        ids.fetch(a.c, pr, b, (u + 2) * kPaUnit, end);
-        if (once && u + 1 < u1) prefetch_entries(a.c, pr, tab_next, (int)rank * 128);
-        for (int d = 0; d < kBlocks; ++d) {
-          const int slot = d % kPaKSlots, use = n + d / kPaKSlots;   // (three uses a unit: their parity)
-          ok = __all_sync(0xffffffffu, pair_wait(a.c, kempty + 8 * slot, (use & 1) ^ 1, dead));
-          if (!ok) break;
-          if (rank == 0 && me) mbar_arrive_tx(kfull + 8 * slot, 2 * kPaBlock);
+        ids.write(a.c, pr, u0 * kPaUnit, end, ctl.rows[0]);
+        ids.fetch(a.c, pr, b, (u0 + 1) * kPaUnit, end);
+        for (int u = u0; ok && u < u1; ++u) {
+          const RowTab& tab = ctl.rows[(u - u0) & 1];
+          RowTab& tab_next = ctl.rows[((u - u0) & 1) ^ 1];
+          ids.write(a.c, pr, (u + 1) * kPaUnit, end, tab_next);
           __syncwarp();
-          load_entries<128>(me, maps, tab, pr.box, d, (int)rank * 128, base + kPaK + slot * kPaBlock, lead_k + 8 * slot);
+          ids.fetch(a.c, pr, b, (u + 2) * kPaUnit, end);
+          if (once && u + 1 < u1) prefetch_entries(a.c, pr, tab_next, (int)rank * 128);
+          Boxes<128, decltype(box)::value> boxes;
+          boxes.take(tab, (int)rank * 128);
+#pragma unroll 1
+          for (int d = 0; d < kBlocks; ++d) {
+            ok = __all_sync(0xffffffffu, pair_wait(a.c, kempty + 8 * slot, phase ^ 1, dead));
+            if (!ok) break;
+            if (rank == 0 && me) mbar_arrive_tx(kfull + 8 * slot, 2 * kPaBlock);
+            __syncwarp();
+            boxes.load(me, maps, d, base + kPaK + slot * kPaBlock, lead_k + 8 * slot);
+            if (++slot == kPaKSlots) {
+              slot = 0;
+              phase ^= 1;
+            }
+          }
+          __syncwarp();   // the table is read
         }
-        ++n;
-        __syncwarp();   // the table is read
+        at += units + kPaTileCost;
       }
-      at += units + kPaTileCost;
-    }
+    });
     if (rank == 0 && lane == 0 && !ok) {   // after a failed wait: a bounded time for the copies in flight
       mbar_wait_for(qfull, (tile & 1) ^ 1, kWaitNs);
       for (int i = 0; i < 2 * kPaKSlots; ++i) mbar_wait_for(kfull + 8 * (i / 2), i & 1, kWaitNs / 8);
@@ -683,34 +712,42 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPaThreads, 1)
     // comes row by row.
     const unsigned lead_v = in_cta(vfull, 0);
     const bool me = elect_one();
-    for (; ok && at < sh.end; ++t) {
-      Seq s = a.seq(b);
-      for (; t >= split.tiles(s); t = 0) s = a.seq(++b);
-      const int units = split.units(s, t), end = split.sees(s, t);
-      const int u0 = split.from(sh, at, units), u1 = split.to(sh, at, units);
-      if (u0 == u1) break;
-      PageIds ids;
-      ids.fetch(a.c, pr, b, u0 * kPaUnit, end);
-      for (int u = u0; ok && u < u1; ++u) {
-        ids.write(a.c, pr, u * kPaUnit, end, ctl.rows[2]);
-        __syncwarp();
-        ids.fetch(a.c, pr, b, (u + 1) * kPaUnit, end);
-        for (int g = 0; g < 4; ++g) {
-          const int slot = g % kPaVSlots, left = end - (u * kPaUnit + g * 64);   // two uses a unit
-          const unsigned dst = base + kPaV + slot * 2 * kPaBlock, bar = lead_v + 8 * slot;
-          ok = __all_sync(0xffffffffu, pair_wait(a.c, vempty + 8 * slot, (g / kPaVSlots) ^ 1, dead));
-          if (!ok) break;
-          if (rank == 0 && me) mbar_arrive_tx(vfull + 8 * slot, 4 * kPaBlock);
+    with_box(pr.box, [&](auto box) {
+      for (; ok && at < sh.end; ++t) {
+        Seq s = a.seq(b);
+        for (; t >= split.tiles(s); t = 0) s = a.seq(++b);
+        const int units = split.units(s, t), end = split.sees(s, t);
+        const int u0 = split.from(sh, at, units), u1 = split.to(sh, at, units);
+        if (u0 == u1) break;
+        PageIds ids;
+        ids.fetch(a.c, pr, b, u0 * kPaUnit, end);
+        for (int u = u0; ok && u < u1; ++u) {
+          ids.write(a.c, pr, u * kPaUnit, end, ctl.rows[2]);
           __syncwarp();
-          const int box = left > 0 && left < 64 ? 0 : pr.box;
+          ids.fetch(a.c, pr, b, (u + 1) * kPaUnit, end);
 #pragma unroll 1
-          for (int j = 0; j < 4; ++j)
-            load_entries<64>(me, maps, ctl.rows[2], box, 4 * (j >> 1) + 2 * (int)rank + (j & 1), g * 64, dst + j * (kPaBlock / 2), bar);
+          for (int g = 0; g < 4; ++g) {
+            const int slot = g % kPaVSlots, left = end - (u * kPaUnit + g * 64);   // two uses a unit
+            const unsigned dst = base + kPaV + slot * 2 * kPaBlock, bar = lead_v + 8 * slot;
+            const auto stage = [&](auto boxes) {
+              boxes.take(ctl.rows[2], g * 64);
+              ok = __all_sync(0xffffffffu, pair_wait(a.c, vempty + 8 * slot, (g / kPaVSlots) ^ 1, dead));
+              if (!ok) return;
+              if (rank == 0 && me) mbar_arrive_tx(vfull + 8 * slot, 4 * kPaBlock);
+              __syncwarp();
+#pragma unroll
+              for (int j = 0; j < 4; ++j)
+                boxes.load(me, maps, 4 * (j >> 1) + 2 * (int)rank + (j & 1), dst + j * (kPaBlock / 2), bar);
+            };
+            if (left > 0 && left < 64) stage(Boxes<64, 0>());
+            else stage(Boxes<64, decltype(box)::value>());
+            if (!ok) break;
+          }
+          __syncwarp();   // the table is read
         }
-        __syncwarp();   // the table is read
+        at += units + kPaTileCost;
       }
-      at += units + kPaTileCost;
-    }
+    });
     if (rank == 0 && lane == 0 && !ok)
       for (int i = 0; i < 2 * kPaVSlots; ++i) mbar_wait_for(vfull + 8 * (i / 2), i & 1, kWaitNs / 8);
     __syncwarp();
@@ -734,13 +771,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPaThreads, 1)
             ok = pair_wait(a.c, sfree + 8 * buf, ((n >> 1) & 1) ^ 1, dead);
 #pragma unroll
             for (int i = 0; i < kBlocks; ++i) {
-              const int slot = i % kPaKSlots;
-              if (ok) ok = pair_wait(a.c, kfull + 8 * slot, (n + i / kPaKSlots) & 1, dead);
+              const int use = n * kBlocks + i, slot = use % kPaKSlots;
+              if (ok) ok = pair_wait(a.c, kfull + 8 * slot, (use / kPaKSlots) & 1, dead);
               if (!ok) break;
               tc_fence_after();
+              const unsigned long long ka = kd + slot * (kPaBlock >> 4);
 #pragma unroll
-              for (int k = 0; k < 4; ++k)
-                pair_mma(d, qd + i * (kPaQBlock >> 4) + k * 2, kd + slot * (kPaBlock >> 4) + k * 2, id_s, (unsigned)(i | k));
+              for (int k = 0; k < 4; ++k) pair_mma(d, qd + i * (kPaQBlock >> 4) + k * 2, ka + k * 2, id_s, (unsigned)(i | k));
               pair_commit(kempty + 8 * slot);
             }
             if (ok) pair_commit(sfull + 8 * buf);
@@ -758,7 +795,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPaThreads, 1)
               tc_fence_after();
 #pragma unroll
               for (int k = 0; k < 8; ++k)
-                pair_mma(tmem + (k >> 2) * 128, pd + g * (kPaQBlock >> 4) + (k & 3) * 2,
+                pair_mma(tmem + (k >> 2) * 128, pd + (g & 1) * (kPaQBlock >> 4) + (k & 3) * 2,
                          vd + (slot * 2 + (k >> 2)) * (kPaBlock >> 4) + (k & 3) * 128, id_o, (unsigned)(u > u0 || g || (k & 3)));
               pair_commit(vempty + 8 * slot);
               pair_commit(pfree + 8 * g);
@@ -780,7 +817,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPaThreads, 1)
     const unsigned tlane = (unsigned)(quarter * 32) << 16, meet = 1 + (quarter & 1);
     const unsigned lead_sfree = in_cta(sfree, 0), lead_oready = in_cta(oready, 0),
                    lead_pfull = in_cta(pfull + 8 * part64, 0);
-    const unsigned p_row = base + kPaP + part64 * kPaQBlock + row * 128;
+    const unsigned p_row = base + kPaP + (part64 & 1) * kPaQBlock + row * 128;
     // Units before number m have been added to O. A barrier's parity only tells a phase from its neighbours: each of the
     // two has every other unit, and where this is asked, the unit three before is known to be added (this thread's part
     // of P was free again from the one two before) and the next one waits for this thread.
@@ -873,8 +910,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPaThreads, 1)
           const __nv_bfloat162 h2 = __floats2bfloat162_rn(v[i >> 4][(i & 15) * 2], v[i >> 4][(i & 15) * 2 + 1]);
           w[i] = *reinterpret_cast<const unsigned*>(&h2);
         }
-        // the sums of the unit before have read this part of P
-        if (n > 0) ok = __all_sync(0xffffffffu, pair_wait(a.c, pfree + 8 * part64, (n - 1) & 1, dead)) && ok;
+        // the sums have read what was in this half of P: the second halves of the unit before, the first of this one
+        if (part64 >= 2) ok = __all_sync(0xffffffffu, pair_wait(a.c, pfree + 8 * (part64 - 2), n & 1, dead)) && ok;
+        else if (n > 0) ok = __all_sync(0xffffffffu, pair_wait(a.c, pfree + 8 * (part64 + 2), (n - 1) & 1, dead)) && ok;
 #pragma unroll
         for (int c = 0; c < 8; ++c)
           asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};"
@@ -894,40 +932,45 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPaThreads, 1)
       const long long out_row = (long long)s.q0 * a.heads + g;
       float* part = a.part + (((long long)worker * 2 + (u0 == 0 ? 1 : 0)) * kPairRows + rank * 64 + row) * kPartRow;
       const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
-      // through this warp's 4 KB of P, which the instructions have read, so that a row's dims leave in pieces of 128 bytes:
-      // 32 rows x 64 dims of results, 32 dims of running sums
-      unsigned char* stage = smem_raw + kPaP + warp * 4096;
-      const int mine = lane & 7, dim0 = wg * 256 + (quarter >> 1) * 128, rows_here = s.n * a.heads - (g - lane);
+      // through this warp's 2 KB of P, which the instructions have read, so that a row's dims leave in pieces of 64 bytes:
+      // 32 rows x 32 dims of results, 16 dims of running sums
+      unsigned char* stage = smem_raw + kPaP + warp * 2048;
+      const int dim0 = wg * 256 + (quarter >> 1) * 128, rows_here = s.n * a.heads - (g - lane);
+      const int put = lane * 64, turn = (lane >> 1) & 3;
 #pragma unroll 1
       for (int c = 0; c < 128; c += 32) {
         float o[32];
         tmem_ld32(tmem + wg * 128 + tlane + c, o);
         tmem_ld_wait();
-        if (whole) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          if (whole) {
+            if (h) break;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              __nv_bfloat162 w[4];
+#pragma unroll
+              for (int k = 0; k < 4; ++k) w[k] = __floats2bfloat162_rn(o[i * 8 + k * 2] * inv, o[i * 8 + k * 2 + 1] * inv);
+              *reinterpret_cast<uint4*>(stage + put + (i ^ turn) * 16) = *reinterpret_cast<const uint4*>(w);
+            }
+          } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              *reinterpret_cast<float4*>(stage + put + (i ^ turn) * 16) =
+                  make_float4(o[h * 16 + i * 4], o[h * 16 + i * 4 + 1], o[h * 16 + i * 4 + 2], o[h * 16 + i * 4 + 3]);
+          }
+          __syncwarp();
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            __nv_bfloat162 w[4];
-#pragma unroll
-            for (int k = 0; k < 4; ++k) w[k] = __floats2bfloat162_rn(o[i * 8 + k * 2] * inv, o[i * 8 + k * 2 + 1] * inv);
-            *reinterpret_cast<uint4*>(stage + lane * 128 + ((((c >> 3) & 4) + i) ^ mine) * 16) = *reinterpret_cast<const uint4*>(w);
+            const int r = i * 8 + (lane >> 2), ch = lane & 3;   // row of this warp's 32, and 16 bytes of it
+            const uint4 v = *reinterpret_cast<const uint4*>(stage + r * 64 + (ch ^ ((r >> 1) & 3)) * 16);
+            if (ok && r < rows_here) {
+              if (whole) *reinterpret_cast<uint4*>(a.out + (out_row - lane + r) * kLat + dim0 + c + ch * 8) = v;
+              else *reinterpret_cast<uint4*>(part + (long long)(r - lane) * kPartRow + dim0 + c + h * 16 + ch * 4) = v;
+            }
           }
-          if (!(c & 32)) continue;
-        } else {
-#pragma unroll
-          for (int i = 0; i < 8; ++i)
-            *reinterpret_cast<float4*>(stage + lane * 128 + (i ^ mine) * 16) = make_float4(o[i * 4], o[i * 4 + 1], o[i * 4 + 2], o[i * 4 + 3]);
+          __syncwarp();
         }
-        __syncwarp();
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const int r = i * 4 + (lane >> 3);   // row of this warp's 32
-          const uint4 v = *reinterpret_cast<const uint4*>(stage + r * 128 + (mine ^ (r & 7)) * 16);
-          if (ok && r < rows_here) {
-            if (whole) *reinterpret_cast<uint4*>(a.out + (out_row - lane + r) * kLat + dim0 + (c & 64) + mine * 8) = v;
-            else *reinterpret_cast<uint4*>(part + (long long)(r - lane) * kPartRow + dim0 + c + mine * 4) = v;
-          }
-        }
-        __syncwarp();
       }
       if (ok && live && part64 == 0) {
         if (whole) {
