@@ -157,7 +157,7 @@ struct RowTab {
   alignas(16) int pe[256];
 };
 struct PageIds {
-  int id[8];
+  int id[8] = {};
   KK3_DEV void fetch(const CachePages& c, const PairRows& pr, int b, int pos, int end) {
     pos += (threadIdx.x & 31) * 8;
     const int* table = c.table + (long long)b * c.table_stride;
@@ -165,23 +165,34 @@ struct PageIds {
     for (int i = 0; i < 8; ++i)
       if ((i == 0 || !pr.box) && pos + i < end) id[i] = table[page_of(c, pos + i)];
   }
+  template <bool BOXED>
   KK3_DEV void write(const CachePages& c, const PairRows& pr, int pos, int end, RowTab& tab) const {
     const int lane = threadIdx.x & 31;
     pos += lane * 8;
     int kv[8], pe[8];
-    const int slot = pos - page_of(c, pos) * c.page_size;
+    if (BOXED) {
+      const bool fine = (unsigned)id[0] < (unsigned)c.num_pages;
+      const int slot = pos - page_of(c, pos) * c.page_size, left = fine ? end - pos : 0;
+      const int kv0 = id[0] * pr.kv_ratio + slot, pe0 = id[0] * pr.pe_ratio + slot;
+      if (!fine && pos < end) cache_error(c);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      kv[i] = pr.kv_end;
-      pe[i] = pr.pe_end;
-      if (pos + i < end) {
-        const int page = pr.box ? id[0] : id[i];
-        const int in = pr.box ? slot + i : pos + i - page_of(c, pos + i) * c.page_size;
-        if ((unsigned)page < (unsigned)c.num_pages) {
-          kv[i] = page * pr.kv_ratio + in;
-          pe[i] = page * pr.pe_ratio + in;
-        } else {
-          cache_error(c);
+      for (int i = 0; i < 8; ++i) {
+        kv[i] = i < left ? kv0 + i : pr.kv_end;
+        pe[i] = i < left ? pe0 + i : pr.pe_end;
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        kv[i] = pr.kv_end;
+        pe[i] = pr.pe_end;
+        if (pos + i < end) {
+          const int in = pos + i - page_of(c, pos + i) * c.page_size;
+          if ((unsigned)id[i] < (unsigned)c.num_pages) {
+            kv[i] = id[i] * pr.kv_ratio + in;
+            pe[i] = id[i] * pr.pe_ratio + in;
+          } else {
+            cache_error(c);
+          }
         }
       }
     }
@@ -353,7 +364,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMassThreads, 1)
       const int units = split.units(s, t), first = split.first_unit(s, t);
       const int u0 = (int)max(0ll, sh.begin - at), u1 = (int)min((long long)units, sh.end - at);
       if (ahead_b != b || ahead_t != t) ids.fetch(a.c, pr, b, t * kMassPos, s.len);
-      ids.write(a.c, pr, t * kMassPos, s.len, ctl.rows);
+      if (pr.box) ids.write<true>(a.c, pr, t * kMassPos, s.len, ctl.rows);
+      else ids.write<false>(a.c, pr, t * kMassPos, s.len, ctl.rows);
       __syncwarp();
       ids.fetch(a.c, pr, b, (t + 1) * kMassPos, s.len);
       ahead_b = b;
@@ -540,7 +552,7 @@ __global__ void __launch_bounds__(kMassPos) kk3_cache_mass_join_kernel(const Mas
 // clocks measured, 175 more for a commit), so narrower ones would leave the tensor cores waiting.
 //
 // Per unit each CTA loads 128 of the positions (nine blocks of 64 dims) for the scores, and half of the output dims of
-// all 256 (four stages of 64 positions x 2 x 128 dims, 32 KB) for the sums, through two rings of 64 KB.
+// all 256 (eight pieces of 64 positions x 128 dims) for the sums, 16 KB each, through a ring of four and one of three.
 // Scores run one unit ahead of sums, and a thread each issues them: what one spends in commits is the other's.
 //
 // Softmax: four threads per row, 64 of a unit's positions each, that exchange maxima through shared memory. The running
@@ -555,8 +567,7 @@ constexpr int kPaUnit = 256;
 constexpr int kPaThreads = 384;        // warps 0-7 softmax, 8 and 9 copies and instructions of scores, 10 and 11 of sums
 constexpr int kPaQBlock = 64 * 128;    // 64 rows of 64 dims
 constexpr int kPaBlock = 128 * 128;    // 128 positions x 64 dims, or 64 positions x 128 dims
-constexpr int kPaKSlots = 4;           // 16 KB each; nine blocks a unit
-constexpr int kPaVSlots = 2;           // 32 KB each; four stages a unit: stage g is in slot g % 2
+constexpr int kPaKSlots = 4, kPaVSlots = 3;   // 16 KB each: nine blocks and eight pieces a unit
 constexpr int kPaMinUnits = 3;
 constexpr int kPaTileCost = 2;   // what a tile costs besides its units, in units: query load, first and last latencies
 constexpr float kPaSlack = 8.0f;
@@ -566,11 +577,11 @@ struct PaCtl {
   unsigned tmem;
   int dead;
   long long red[kPaThreads / 32 + 4];
-  RowTab rows[3];        // entries of a unit: the scores' (two, in turn) and the sums'
+  RowTab rows[4];        // entries of a unit: the scores' (two, in turn) and the sums' (two)
   float top[2][4][64];   // [unit parity][64 positions of 256][row]: maxima (at the end: sums) of a row's four threads
 };
-constexpr int kPaQ = 0, kPaP = kPaQ + kBlocks * kPaQBlock, kPaK = kPaP + 2 * kPaQBlock,
-              kPaV = kPaK + kPaKSlots * kPaBlock, kPaCtl = kPaV + kPaVSlots * 2 * kPaBlock;
+constexpr int kPaQ = 0, kPaP = kPaQ + kBlocks * kPaQBlock, kPaK = kPaP + 4 * kPaQBlock,
+              kPaV = kPaK + kPaKSlots * kPaBlock, kPaCtl = kPaV + kPaVSlots * kPaBlock;
 constexpr int kPaSmem = kPaCtl + (int)sizeof(PaCtl);
 static_assert(kPaSmem <= 232448, "shared memory of a CTA");
 
@@ -673,17 +684,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPaThreads, 1)
 #pragma unroll
         for (int d = 0; d < kBlocks; ++d)
           load_box(me, base + kPaQ + d * kPaQBlock, d < kBlocks - 1 ? &maps.ql : &maps.qp, d < kBlocks - 1 ? d * 64 : 0, q, lead_q);
-        ids.write(a.c, pr, u0 * kPaUnit, end, ctl.rows[0]);
+        ids.write<decltype(box)::value != 0>(a.c, pr, u0 * kPaUnit, end, ctl.rows[0]);
+        __syncwarp();
         ids.fetch(a.c, pr, b, (u0 + 1) * kPaUnit, end);
+        Boxes<128, decltype(box)::value> boxes, next;
+        next.take(ctl.rows[0], (int)rank * 128);
         for (int u = u0; ok && u < u1; ++u) {
-          const RowTab& tab = ctl.rows[(u - u0) & 1];
-          RowTab& tab_next = ctl.rows[((u - u0) & 1) ^ 1];
-          ids.write(a.c, pr, (u + 1) * kPaUnit, end, tab_next);
-          __syncwarp();
-          ids.fetch(a.c, pr, b, (u + 2) * kPaUnit, end);
-          if (once && u + 1 < u1) prefetch_entries(a.c, pr, tab_next, (int)rank * 128);
-          Boxes<128, decltype(box)::value> boxes;
-          boxes.take(tab, (int)rank * 128);
+          boxes = next;
 #pragma unroll 1
           for (int d = 0; d < kBlocks; ++d) {
             ok = __all_sync(0xffffffffu, pair_wait(a.c, kempty + 8 * slot, phase ^ 1, dead));
@@ -695,9 +702,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPaThreads, 1)
               slot = 0;
               phase ^= 1;
             }
+            if (d == 3 && u + 1 < u1) {   // the next unit's rows, while copies are on their way
+              RowTab& tab = ctl.rows[(u + 1 - u0) & 1];
+              ids.write<decltype(box)::value != 0>(a.c, pr, (u + 1) * kPaUnit, end, tab);
+              __syncwarp();
+              ids.fetch(a.c, pr, b, (u + 2) * kPaUnit, end);
+              next.take(tab, (int)rank * 128);
+              if (once) prefetch_entries(a.c, pr, tab, (int)rank * 128);
+            }
           }
-          __syncwarp();   // the table is read
         }
+        __syncwarp();   // the tables are read
         at += units + kPaTileCost;
       }
     });
@@ -707,12 +722,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPaThreads, 1)
     }
     __syncwarp();
   } else if (warp == 10) {
-    // ---- the entries' stages for the sums: stage g is dims 256 h + 128 rank .. + 127, h = 0 and 1, of positions 64 g ..
-    // + 63 of the unit. Positions that no row sees must be zeros, whatever the page holds there: a stage that `end` cuts
-    // comes row by row.
+    // ---- the entries' pieces for the sums: piece (g, h) is dims 256 h + 128 rank .. + 127 of positions 64 g .. + 63 of
+    // the unit. Positions that no row sees must be zeros, whatever the page holds there: a group that `end` cuts comes
+    // row by row.
     const unsigned lead_v = in_cta(vfull, 0);
     const bool me = elect_one();
     with_box(pr.box, [&](auto box) {
+      int slot = 0, phase = 0;
       for (; ok && at < sh.end; ++t) {
         Seq s = a.seq(b);
         for (; t >= split.tiles(s); t = 0) s = a.seq(++b);
@@ -721,30 +737,42 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPaThreads, 1)
         if (u0 == u1) break;
         PageIds ids;
         ids.fetch(a.c, pr, b, u0 * kPaUnit, end);
+        ids.write<decltype(box)::value != 0>(a.c, pr, u0 * kPaUnit, end, ctl.rows[2]);
+        __syncwarp();
+        ids.fetch(a.c, pr, b, (u0 + 1) * kPaUnit, end);
         for (int u = u0; ok && u < u1; ++u) {
-          ids.write(a.c, pr, u * kPaUnit, end, ctl.rows[2]);
-          __syncwarp();
-          ids.fetch(a.c, pr, b, (u + 1) * kPaUnit, end);
+          const RowTab& tab = ctl.rows[2 + ((u - u0) & 1)];
 #pragma unroll 1
           for (int g = 0; g < 4; ++g) {
-            const int slot = g % kPaVSlots, left = end - (u * kPaUnit + g * 64);   // two uses a unit
-            const unsigned dst = base + kPaV + slot * 2 * kPaBlock, bar = lead_v + 8 * slot;
-            const auto stage = [&](auto boxes) {
-              boxes.take(ctl.rows[2], g * 64);
-              ok = __all_sync(0xffffffffu, pair_wait(a.c, vempty + 8 * slot, (g / kPaVSlots) ^ 1, dead));
-              if (!ok) return;
-              if (rank == 0 && me) mbar_arrive_tx(vfull + 8 * slot, 4 * kPaBlock);
-              __syncwarp();
+            const int left = end - (u * kPaUnit + g * 64);
+            const auto pieces = [&](auto boxes) {
+              boxes.take(tab, g * 64);
 #pragma unroll
-              for (int j = 0; j < 4; ++j)
-                boxes.load(me, maps, 4 * (j >> 1) + 2 * (int)rank + (j & 1), dst + j * (kPaBlock / 2), bar);
+              for (int h = 0; h < 2; ++h) {
+                const unsigned dst = base + kPaV + slot * kPaBlock, bar = lead_v + 8 * slot;
+                ok = ok && __all_sync(0xffffffffu, pair_wait(a.c, vempty + 8 * slot, phase ^ 1, dead));
+                if (!ok) return;
+                if (rank == 0 && me) mbar_arrive_tx(vfull + 8 * slot, 2 * kPaBlock);
+                __syncwarp();
+#pragma unroll
+                for (int j = 0; j < 2; ++j) boxes.load(me, maps, 4 * h + 2 * (int)rank + j, dst + j * (kPaBlock / 2), bar);
+                if (++slot == kPaVSlots) {
+                  slot = 0;
+                  phase ^= 1;
+                }
+              }
             };
-            if (left > 0 && left < 64) stage(Boxes<64, 0>());
-            else stage(Boxes<64, decltype(box)::value>());
+            if (left > 0 && left < 64) pieces(Boxes<64, 0>());
+            else pieces(Boxes<64, decltype(box)::value>());
             if (!ok) break;
+            if (g == 1 && u + 1 < u1) {   // the next unit's rows, while copies are on their way
+              ids.write<decltype(box)::value != 0>(a.c, pr, (u + 1) * kPaUnit, end, ctl.rows[2 + ((u + 1 - u0) & 1)]);
+              __syncwarp();
+              ids.fetch(a.c, pr, b, (u + 2) * kPaUnit, end);
+            }
           }
-          __syncwarp();   // the table is read
         }
+        __syncwarp();   // the tables are read
         at += units + kPaTileCost;
       }
     });
@@ -788,17 +816,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPaThreads, 1)
           for (int u = u0; ok && u < u1; ++u, ++n) {
             ok = pair_wait(a.c, oready + 8 * (n & 1), (n >> 1) & 1, dead);
 #pragma unroll
-            for (int g = 0; g < 4; ++g) {
-              const int slot = g % kPaVSlots;
-              if (ok) ok = pair_wait(a.c, pfull + 8 * g, n & 1, dead) && pair_wait(a.c, vfull + 8 * slot, g / kPaVSlots, dead);
+            for (int i = 0; i < 8; ++i) {
+              const int use = n * 8 + i, slot = use % kPaVSlots;
+              if (ok && !(i & 1)) ok = pair_wait(a.c, pfull + 4 * i, n & 1, dead);
+              if (ok) ok = pair_wait(a.c, vfull + 8 * slot, (use / kPaVSlots) & 1, dead);
               if (!ok) break;
               tc_fence_after();
+              const unsigned long long va = vd + slot * (kPaBlock >> 4);
 #pragma unroll
-              for (int k = 0; k < 8; ++k)
-                pair_mma(tmem + (k >> 2) * 128, pd + (g & 1) * (kPaQBlock >> 4) + (k & 3) * 2,
-                         vd + (slot * 2 + (k >> 2)) * (kPaBlock >> 4) + (k & 3) * 128, id_o, (unsigned)(u > u0 || g || (k & 3)));
+              for (int k = 0; k < 4; ++k)
+                pair_mma(tmem + (i & 1) * 128, pd + (i >> 1) * (kPaQBlock >> 4) + k * 2, va + k * 128, id_o, (unsigned)(u > u0 || i > 1 || k));
               pair_commit(vempty + 8 * slot);
-              pair_commit(pfree + 8 * g);
+              if (i & 1) pair_commit(pfree + 4 * (i - 1));
             }
             if (ok) pair_commit(pvdone + 8 * (n & 1));
           }
@@ -817,7 +846,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPaThreads, 1)
     const unsigned tlane = (unsigned)(quarter * 32) << 16, meet = 1 + (quarter & 1);
     const unsigned lead_sfree = in_cta(sfree, 0), lead_oready = in_cta(oready, 0),
                    lead_pfull = in_cta(pfull + 8 * part64, 0);
-    const unsigned p_row = base + kPaP + (part64 & 1) * kPaQBlock + row * 128;
+    const unsigned p_row = base + kPaP + part64 * kPaQBlock + row * 128;
     // Units before number m have been added to O. A barrier's parity only tells a phase from its neighbours: each of the
     // two has every other unit, and where this is asked, the unit three before is known to be added (this thread's part
     // of P was free again from the one two before) and the next one waits for this thread.
@@ -910,9 +939,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPaThreads, 1)
           const __nv_bfloat162 h2 = __floats2bfloat162_rn(v[i >> 4][(i & 15) * 2], v[i >> 4][(i & 15) * 2 + 1]);
           w[i] = *reinterpret_cast<const unsigned*>(&h2);
         }
-        // the sums have read what was in this half of P: the second halves of the unit before, the first of this one
-        if (part64 >= 2) ok = __all_sync(0xffffffffu, pair_wait(a.c, pfree + 8 * (part64 - 2), n & 1, dead)) && ok;
-        else if (n > 0) ok = __all_sync(0xffffffffu, pair_wait(a.c, pfree + 8 * (part64 + 2), (n - 1) & 1, dead)) && ok;
+        // the sums of the unit before have read this part of P
+        if (n > 0) ok = __all_sync(0xffffffffu, pair_wait(a.c, pfree + 8 * part64, (n - 1) & 1, dead)) && ok;
 #pragma unroll
         for (int c = 0; c < 8; ++c)
           asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};"
