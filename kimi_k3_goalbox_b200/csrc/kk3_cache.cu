@@ -126,7 +126,7 @@ constexpr int kWaPitch = kEntry + 8;      // 1168-byte rows: consecutive rows fa
 constexpr int kWaPPitch = kWaUnit + 8;
 constexpr int kWaThreads = 256;
 constexpr int kWaMinUnits = 4;
-constexpr int64_t kWarpRowsMost = 0;     // average rows of a sequence up to which this kernel is taken
+constexpr int64_t kWarpRowsMost = 16;     // average rows of a sequence up to which this kernel is taken
 struct WaSmem {
   bf16 ring[kWaStages][kWaUnit][kWaPitch];
   bf16 q[kWaRows][kWaPitch];

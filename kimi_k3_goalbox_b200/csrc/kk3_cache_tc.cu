@@ -32,7 +32,6 @@ struct PairMaps {
 struct PairRows {
   int kv_ratio, pe_ratio;   // rows from one page to the next
   int kv_end, pe_end;       // number of the first row behind the pool: reads as zeros
-  long long kv_pitch, pe_pitch;   // elements from one row to the next
   int box;                  // rows of a box: divides a page and 64, 8 at least; 0: gathers only
 };
 
@@ -244,22 +243,6 @@ KK3_DEV void with_box(int box, const F& f) {
     case 16: return f(std::integral_constant<int, 16>());
     case 8: return f(std::integral_constant<int, 8>());
     default: return f(std::integral_constant<int, 0>());
-  }
-}
-
-// Bring 128 positions from number `off` of the table on into L2, for copies one unit later: HBM's latency is longer than
-// what the ring holds. By plain prefetches of 128 bytes: bulk ones queue up before the copies (single tokens of 64
-// sequences over 8192 positions took 205 us with them, 152 without).
-KK3_DEV void prefetch_entries(const CachePages& c, const PairRows& pr, const RowTab& tab, int off) {
-  const int lane = threadIdx.x & 31;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int kv = tab.kv[off + i * 32 + lane], pe = tab.pe[off + i * 32 + lane];
-    if (kv == pr.kv_end) continue;
-    const bf16* row = c.kv + (long long)kv * pr.kv_pitch;
-#pragma unroll
-    for (int k = 0; k < 8; ++k) asm volatile("prefetch.global.L2 [%0];" ::"l"(row + k * 64));
-    asm volatile("prefetch.global.L2 [%0];" ::"l"(c.pe + (long long)pe * pr.pe_pitch));
   }
 }
 
@@ -675,7 +658,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPaThreads, 1)
         if (u0 == u1) break;   // only a tile's cost is left: the next worker's
         PageIds ids;
         ids.fetch(a.c, pr, b, u0 * kPaUnit, end);
-        const bool once = s.n * a.heads <= kPairRows;   // the cache is read by this tile alone: it comes from HBM
         ok = __all_sync(0xffffffffu, pair_wait(a.c, qempty, (tile & 1) ^ 1, dead));
         if (!ok) break;
         if (rank == 0 && me) mbar_arrive_tx(qfull, 2 * kBlocks * kPaQBlock);
@@ -708,7 +690,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPaThreads, 1)
               __syncwarp();
               ids.fetch(a.c, pr, b, (u + 2) * kPaUnit, end);
               next.take(tab, (int)rank * 128);
-              if (once) prefetch_entries(a.c, pr, tab, (int)rank * 128);
             }
           }
         }
@@ -1049,7 +1030,7 @@ static int encode_rows(CUtensorMap* map, const void* base, int cols, int64_t row
 }
 
 // maps of all the rows of a [pages, page_size, cols] tensor: in boxes and row by row
-static int map_pages(CUtensorMap* by_box, CUtensorMap* by_row, int* ratio, int* end, long long* pitch, const void* base, int cols,
+static int map_pages(CUtensorMap* by_box, CUtensorMap* by_row, int* ratio, int* end, const void* base, int cols,
                      const kk3_cache* c, int64_t page_stride, int64_t row_stride, int box) {
   const int64_t pages = c->num_pages;
   if (c->page_size == 1 && pages > 1) row_stride = page_stride;
@@ -1057,7 +1038,6 @@ static int map_pages(CUtensorMap* by_box, CUtensorMap* by_row, int* ratio, int* 
   if (row_stride < cols || (pages > 1 && page_stride % row_stride) || rows >= INT32_MAX) return KK3_ERR_UNSUPPORTED;
   *ratio = (int)r;
   *end = (int)rows;
-  *pitch = row_stride;
   const int rc = encode_rows(by_row, base, cols, rows, row_stride, 1);
   return rc || !box ? rc : encode_rows(by_box, base, cols, rows, row_stride, box);
 }
@@ -1076,8 +1056,8 @@ static int pair_maps(const kk3_cache* c, const void* q_latent, int64_t ql_token,
   r->box = 64;
   while (c->page_size % r->box) r->box /= 2;
   if (r->box < 8) r->box = 0;
-  int rc = map_pages(&m->kv_box, &m->kv_row, &r->kv_ratio, &r->kv_end, &r->kv_pitch, c->kv, kLat, c, c->kv_page_stride, c->kv_row_stride, r->box);
-  if (!rc) rc = map_pages(&m->pe_box, &m->pe_row, &r->pe_ratio, &r->pe_end, &r->pe_pitch, c->pe, kRope, c, c->pe_page_stride, c->pe_row_stride, r->box);
+  int rc = map_pages(&m->kv_box, &m->kv_row, &r->kv_ratio, &r->kv_end, c->kv, kLat, c, c->kv_page_stride, c->kv_row_stride, r->box);
+  if (!rc) rc = map_pages(&m->pe_box, &m->pe_row, &r->pe_ratio, &r->pe_end, c->pe, kRope, c, c->pe_page_stride, c->pe_row_stride, r->box);
   if (!rc) rc = map_queries(&m->ql, q_latent, kLat, tokens, heads, ql_token, ql_head, q_box);
   if (!rc) rc = map_queries(&m->qp, q_pe, kRope, tokens, heads, qp_token, qp_head, q_box);
   return rc;
