@@ -194,45 +194,97 @@ typedef struct kk3_cache {
  * raw[t] (bf16 [tokens, 576], the step's `ka` product): latent = x / sqrt(mean(x^2) + eps) * norm_weight over the
  * first 512 values (FP32, one rounding), rope part as it is. new_lengths[b] = lengths[b] + new tokens (another buffer
  * than lengths). A token that does not fit behind the last column is not written. */
-int kk3_cache_append(const kk3_cache* cache, const void* raw, int64_t raw_stride, const void* norm_weight, float eps,
-                     const int64_t* lengths, const int32_t* cu_new, int tokens, int64_t* new_lengths, int* error_word,
-                     void* stream);
+typedef struct kk3_cache_append_args {
+    kk3_cache cache;
+    const void* raw;             /* bf16 [tokens, 576], row stride raw_stride */
+    int64_t raw_stride;
+    const void* norm_weight;     /* bf16 [512] */
+    const int64_t* lengths;      /* [batch] positions cached before */
+    const int32_t* cu_new;       /* [batch + 1] */
+    int64_t* new_lengths;        /* [batch] */
+    int32_t* error_word;         /* optional */
+    int32_t tokens;
+    float eps;
+} kk3_cache_append_args;
+int kk3_cache_append(const kk3_cache_append_args* args, void* stream);
 
 /* Attention of the new tokens over their sequence's cache in the latent space. `lengths` includes the new tokens
  * (already appended): token i of n sees the first lengths[b] - n + i + 1 positions. Per token and head
  *   s_p = scale * (q_latent . c_p + q_pe . r_p),  out = sum_p softmax(s)_p c_p  (bf16 [tokens, heads, 512]),
  *   lse = log sum_p exp(s_p)  (f32 [tokens, heads]).
  * A token that sees nothing gets out = 0 and lse = -infinity. Queries: bf16, last dim contiguous, all (token,
- * head) rows at one pitch: the token stride is heads times the head stride (KK3_ERR_UNSUPPORTED otherwise). Sums and softmax statistics are FP32, probabilities are rounded to bf16 for the second product. The
+ * head) rows at one pitch: the token stride is heads times the head stride (KK3_ERR_UNSUPPORTED otherwise).
+ * Sums and softmax statistics are FP32, probabilities are rounded to bf16 for the second product. The
  * positions that a sequence holds must be finite for its tokens' results to be. workspace: 16-byte aligned,
- * kk3_cache_attend_workspace bytes (0: bad arguments or no device), used until the call's kernels end: calls that may
- * overlap need one each. Results do not depend on the order in which CTAs run. */
-int64_t kk3_cache_attend_workspace(int batch, int tokens, int heads);
-int kk3_cache_attend(const kk3_cache* cache, const void* q_latent, int64_t ql_token, int64_t ql_head, const void* q_pe,
-                     int64_t qp_token, int64_t qp_head, const int64_t* lengths, const int32_t* cu_new, int tokens,
-                     int heads, float scale, void* out, float* lse, void* workspace, int64_t workspace_bytes,
-                     int* error_word, void* stream);
+ * kk3_cache_attend_workspace() bytes (the same for every call on a device; 0: no device), used until the call's kernels
+ * end: calls that may overlap need one each. Results do not depend on the order in which CTAs run. */
+typedef struct kk3_cache_attend_args {
+    kk3_cache cache;
+    const void* q_latent;        /* bf16 [tokens, heads, 512] */
+    int64_t ql_token, ql_head;   /* strides */
+    const void* q_pe;            /* bf16 [tokens, heads, 64] */
+    int64_t qp_token, qp_head;
+    const int64_t* lengths;      /* [batch] */
+    const int32_t* cu_new;       /* [batch + 1] */
+    void* out;
+    float* lse;
+    void* workspace;
+    int64_t workspace_bytes;
+    int32_t* error_word;         /* optional */
+    int32_t tokens, heads;
+    float scale;
+    int32_t reserved;
+} kk3_cache_attend_args;
+int64_t kk3_cache_attend_workspace(void);
+int kk3_cache_attend(const kk3_cache_attend_args* args, void* stream);
 
 /* Accumulated attention weight: new_mass[b][p] = mass[b][p] + sum over the sequence's new tokens that see p and over
  * heads of exp(s_p - lse), with kk3_cache_attend's lse (rows with lse = -infinity add nothing). mass (optional, NULL:
  * zeros) and new_mass are f32 [batch, columns * page_size], mass with its own row stride; they may be the same buffer.
- * Positions at or behind the length keep their mass. FP32 sums in a fixed order. */
-int64_t kk3_cache_mass_workspace(int batch, int tokens, int heads);
-int kk3_cache_mass(const kk3_cache* cache, const void* q_latent, int64_t ql_token, int64_t ql_head, const void* q_pe,
-                   int64_t qp_token, int64_t qp_head, const float* lse, const int64_t* lengths, const int32_t* cu_new,
-                   int tokens, int heads, float scale, const float* mass, int64_t mass_stride, float* new_mass,
-                   void* workspace, int64_t workspace_bytes, int* error_word, void* stream);
+ * Positions at or behind the length keep their mass. FP32 sums in a fixed order. Workspace as above, of
+ * kk3_cache_mass_workspace() bytes. */
+typedef struct kk3_cache_mass_args {
+    kk3_cache cache;
+    const void* q_latent;        /* as for kk3_cache_attend */
+    int64_t ql_token, ql_head;
+    const void* q_pe;
+    int64_t qp_token, qp_head;
+    const float* lse;            /* [tokens, heads] */
+    const int64_t* lengths;
+    const int32_t* cu_new;
+    const float* mass;           /* optional */
+    int64_t mass_stride;
+    float* new_mass;
+    void* workspace;
+    int64_t workspace_bytes;
+    int32_t* error_word;         /* optional */
+    int32_t tokens, heads;
+    float scale;
+    int32_t reserved;
+} kk3_cache_mass_args;
+int64_t kk3_cache_mass_workspace(void);
+int kk3_cache_mass(const kk3_cache_mass_args* args, void* stream);
 
 /* Eviction: each sequence keeps min(lengths[b], budget) positions: its first `sinks`, its last `recent`
- * (sinks + recent <= budget), and of the others those of the largest mass (f32 [batch, columns * page_size] with a
- * row stride; equal ones: the lowest position; a NaN counts as the largest). The kept entries move, in ascending
- * order, to positions 0, 1, ... of dst_table's pages (int32 [batch, dst_columns], pages that no listed sequence
- * uses: shared pages stay as they are), or in place (dst_table = NULL). new_lengths, new_mass [batch,
- * columns * page_size] (the kept positions' mass, zeros behind) and kept [batch, budget] (their old positions, -1
- * behind) are other buffers than the inputs. */
-int kk3_cache_evict(const kk3_cache* cache, const int64_t* lengths, const float* mass, int64_t mass_stride, int budget,
-                    int sinks, int recent, const int32_t* dst_table, int64_t dst_stride, int dst_columns,
-                    int64_t* new_lengths, float* new_mass, int32_t* kept, int* error_word, void* stream);
+ * (sinks + recent <= budget), and of the others those of the largest mass (equal ones: the lowest position; a NaN
+ * counts as the largest). The kept entries move, in ascending order, to positions 0, 1, ... of dst_table's pages
+ * (pages that no listed sequence uses: shared pages stay as they are), or in place (dst_table = NULL). new_lengths,
+ * new_mass (the kept positions' mass, zeros behind) and kept (their old positions, -1 behind) are other buffers than
+ * the inputs. */
+typedef struct kk3_cache_evict_args {
+    kk3_cache cache;
+    const int64_t* lengths;      /* [batch] */
+    const float* mass;           /* [batch, columns * page_size], row stride mass_stride */
+    int64_t mass_stride;
+    const int32_t* dst_table;    /* [batch, dst_columns], or NULL */
+    int64_t dst_stride;
+    int64_t* new_lengths;        /* [batch] */
+    float* new_mass;             /* [batch, columns * page_size] */
+    int32_t* kept;               /* [batch, budget] */
+    int32_t* error_word;         /* optional */
+    int32_t budget, sinks, recent, dst_columns;
+} kk3_cache_evict_args;
+int kk3_cache_evict(const kk3_cache_evict_args* args, void* stream);
 
 /* Human-readable text for a return code. */
 const char* kk3_error_string(int code);

@@ -425,7 +425,6 @@ struct EvictArgs {
   int budget, sinks, recent;
   const int* dst;          // destination table, or null: in place
   long long dst_row;
-  int dst_columns;
   long long* new_lengths;
   float* new_mass;         // [batch, columns * page_size]
   int* kept;               // [batch, budget]
@@ -675,25 +674,24 @@ int cache_sms(int* sms) {
 
 }  // namespace kk3
 
-extern "C" int kk3_cache_append(const kk3_cache* cache, const void* raw, int64_t raw_stride, const void* norm_weight,
-                                float eps, const int64_t* lengths, const int32_t* cu_new, int tokens,
-                                int64_t* new_lengths, int* error_word, void* stream) {
+extern "C" int kk3_cache_append(const kk3_cache_append_args* x, void* stream) {
+  if (!x) return KK3_ERR_ARG;
   AppendArgs a;
-  const int rc = cache_pages(cache, &a.c, error_word);
+  const int rc = cache_pages(&x->cache, &a.c, x->error_word);
   if (rc) return rc;
-  if (tokens < 0 || (tokens > 0 && !cache_aligned(raw, 16)) || raw_stride % 8 || raw_stride < kEntry ||
-      !cache_aligned(norm_weight, 16) || !cache_aligned(lengths, 8) || !cache_aligned(cu_new, 4) || !cache_aligned(new_lengths, 8) ||
-      lengths == new_lengths || !(eps >= 0.0f))
+  if (x->tokens < 0 || (x->tokens > 0 && !cache_aligned(x->raw, 16)) || x->raw_stride % 8 || x->raw_stride < kEntry ||
+      !cache_aligned(x->norm_weight, 16) || !cache_aligned(x->lengths, 8) || !cache_aligned(x->cu_new, 4) ||
+      !cache_aligned(x->new_lengths, 8) || x->lengths == x->new_lengths || !(x->eps >= 0.0f))
     return KK3_ERR_ARG;
-  a.raw = (const bf16*)raw;
-  a.raw_row = raw_stride;
-  a.weight = (const bf16*)norm_weight;
-  a.lengths = (const long long*)lengths;
-  a.new_lengths = (long long*)new_lengths;
-  a.cu_new = cu_new;
-  a.tokens = tokens;
-  a.eps = eps;
-  const int grid = tokens > 0 ? (tokens + kAppendWarps - 1) / kAppendWarps : 1;
+  a.raw = (const bf16*)x->raw;
+  a.raw_row = x->raw_stride;
+  a.weight = (const bf16*)x->norm_weight;
+  a.lengths = (const long long*)x->lengths;
+  a.new_lengths = (long long*)x->new_lengths;
+  a.cu_new = x->cu_new;
+  a.tokens = x->tokens;
+  a.eps = x->eps;
+  const int grid = x->tokens > 0 ? (x->tokens + kAppendWarps - 1) / kAppendWarps : 1;
   kk3_cache_append_kernel<<<grid, kAppendWarps * 32, 0, (cudaStream_t)stream>>>(a);
   return cache_cuda(cudaGetLastError(), "kk3_cache_append_kernel");
 }
@@ -708,53 +706,50 @@ static Plan attend_plan(int64_t batch, int64_t tokens, int64_t heads, int sms) {
   return Plan{true, sms / 2, kPairRows};
 }
 
-extern "C" int64_t kk3_cache_attend_workspace(int batch, int tokens, int heads) {
-  if (batch < 1 || tokens < 0 || heads < 1 || heads > kMaxHeads) return 0;
+extern "C" int64_t kk3_cache_attend_workspace(void) {
   int sms = 0;
   if (cache_sms(&sms)) return 0;
-  const Plan p = attend_plan(batch, tokens, heads, sms);
-  return (int64_t)p.workers * (16 + 2 * p.rows * kPartRow * 4);
+  const int64_t pair = (int64_t)(sms / 2) * (16 + 2 * kPairRows * kPartRow * 4), warp = (int64_t)sms * (16 + 2 * kWaRows * kPartRow * 4);
+  return pair > warp ? pair : warp;
 }
 
-extern "C" int kk3_cache_attend(const kk3_cache* cache, const void* q_latent, int64_t ql_token, int64_t ql_head,
-                                const void* q_pe, int64_t qp_token, int64_t qp_head, const int64_t* lengths,
-                                const int32_t* cu_new, int tokens, int heads, float scale, void* out, float* lse,
-                                void* workspace, int64_t workspace_bytes, int* error_word, void* stream) {
+extern "C" int kk3_cache_attend(const kk3_cache_attend_args* x, void* stream) {
+  if (!x) return KK3_ERR_ARG;
   AttendArgs a;
-  const int rc = cache_pages(cache, &a.c, error_word);
+  const int rc = cache_pages(&x->cache, &a.c, x->error_word);
   if (rc) return rc;
-  if (tokens < 0 || heads < 1 || !cache_aligned(lengths, 8) || !cache_aligned(cu_new, 4) || !(scale == scale)) return KK3_ERR_ARG;
+  const int tokens = x->tokens, heads = x->heads;
+  if (tokens < 0 || heads < 1 || !cache_aligned(x->lengths, 8) || !cache_aligned(x->cu_new, 4) || !(x->scale == x->scale))
+    return KK3_ERR_ARG;
   if (heads > kMaxHeads || (int64_t)tokens * heads > INT32_MAX / 2) return KK3_ERR_UNSUPPORTED;
   if (tokens == 0) return KK3_OK;
-  if (!cache_aligned(q_latent, 16) || !cache_aligned(q_pe, 16) || !cache_aligned(out, 16) || !cache_aligned(lse, 4) || ql_token % 8 ||
-      ql_head % 8 || qp_token % 8 || qp_head % 8 || ql_token < 0 || ql_head < 0 || qp_token < 0 || qp_head < 0)
+  if (!cache_queries(x->q_latent, x->ql_token, x->ql_head, x->q_pe, x->qp_token, x->qp_head) || !cache_aligned(x->out, 16) ||
+      !cache_aligned(x->lse, 4))
     return KK3_ERR_ARG;
-  const int64_t need = kk3_cache_attend_workspace(a.c.batch, tokens, heads);
-  if (need == 0) return KK3_ERR_CUDA;
-  if (!cache_aligned(workspace, 16) || workspace_bytes < need) return KK3_ERR_ARG;
   int sms = 0;
   if (cache_sms(&sms)) return KK3_ERR_CUDA;
-  a.q_lat = (const bf16*)q_latent;
-  a.q_pe = (const bf16*)q_pe;
-  a.ql_tok = ql_token;
-  a.ql_head = ql_head;
-  a.qp_tok = qp_token;
-  a.qp_head = qp_head;
-  a.lengths = (const long long*)lengths;
-  a.cu_new = cu_new;
+  if (!cache_aligned(x->workspace, 16) || x->workspace_bytes < kk3_cache_attend_workspace()) return KK3_ERR_ARG;
+  a.q_lat = (const bf16*)x->q_latent;
+  a.q_pe = (const bf16*)x->q_pe;
+  a.ql_tok = x->ql_token;
+  a.ql_head = x->ql_head;
+  a.qp_tok = x->qp_token;
+  a.qp_head = x->qp_head;
+  a.lengths = (const long long*)x->lengths;
+  a.cu_new = x->cu_new;
   a.tokens = tokens;
   a.heads = heads;
-  a.scale_log2 = scale * 1.4426950408889634f;
-  a.out = (bf16*)out;
-  a.lse = lse;
+  a.scale_log2 = x->scale * 1.4426950408889634f;
+  a.out = (bf16*)x->out;
+  a.lse = x->lse;
   const Plan p = attend_plan(a.c.batch, tokens, heads, sms);
   a.workers = p.workers;
-  a.meta = (int*)workspace;
-  a.part = (float*)((char*)workspace + (size_t)p.workers * 16);
+  a.meta = (int*)x->workspace;
+  a.part = (float*)((char*)x->workspace + (size_t)p.workers * 16);
   const cudaStream_t st = (cudaStream_t)stream;
   int r;
   if (p.pair) {
-    r = attend_pair(cache, a, st);
+    r = attend_pair(&x->cache, a, st);
   } else {
     static std::atomic<bool> done[kCacheMaxDevices];
     r = cache_allow_smem(kk3_cache_attend_warp_kernel, sizeof(WaSmem), done, "cudaFuncSetAttribute(kk3_cache_attend_warp_kernel)");
@@ -766,41 +761,38 @@ extern "C" int kk3_cache_attend(const kk3_cache* cache, const void* q_latent, in
   return cache_launch_after(kk3_cache_join_kernel, dim3(p.workers, 16), kJoinThreads, st, "kk3_cache_join_kernel", a, p.rows);
 }
 
-extern "C" int kk3_cache_evict(const kk3_cache* cache, const int64_t* lengths, const float* mass, int64_t mass_stride,
-                               int budget, int sinks, int recent, const int32_t* dst_table, int64_t dst_stride,
-                               int dst_columns, int64_t* new_lengths, float* new_mass, int32_t* kept, int* error_word,
-                               void* stream) {
+extern "C" int kk3_cache_evict(const kk3_cache_evict_args* x, void* stream) {
+  if (!x) return KK3_ERR_ARG;
   EvictArgs a;
-  const int rc = cache_pages(cache, &a.c, error_word);
+  const int rc = cache_pages(&x->cache, &a.c, x->error_word);
   if (rc) return rc;
-  if (!cache_aligned(lengths, 8) || !cache_aligned(mass, 4) || mass_stride < 0 || budget < 1 || sinks < 0 || recent < 0 ||
-      (int64_t)sinks + recent > budget || !cache_aligned(new_lengths, 8) || !cache_aligned(new_mass, 4) || !cache_aligned(kept, 4) ||
-      lengths == new_lengths || mass == new_mass)
+  const int budget = x->budget;
+  if (!cache_aligned(x->lengths, 8) || !cache_aligned(x->mass, 4) || x->mass_stride < 0 || budget < 1 || x->sinks < 0 ||
+      x->recent < 0 || (int64_t)x->sinks + x->recent > budget || !cache_aligned(x->new_lengths, 8) ||
+      !cache_aligned(x->new_mass, 4) || !cache_aligned(x->kept, 4) || x->lengths == x->new_lengths || x->mass == x->new_mass)
     return KK3_ERR_ARG;
-  const int64_t cap = (int64_t)cache->columns * cache->page_size;
+  const int64_t cap = (int64_t)x->cache.columns * x->cache.page_size;
   if (budget > cap) return KK3_ERR_ARG;
-  if (dst_table && (((uintptr_t)dst_table % 4) || dst_stride < 0 || (int64_t)dst_columns * cache->page_size < budget))
+  if (x->dst_table && (((uintptr_t)x->dst_table % 4) || x->dst_stride < 0 || (int64_t)x->dst_columns * x->cache.page_size < budget))
     return KK3_ERR_ARG;
-  a.lengths = (const long long*)lengths;
-  a.mass = mass;
-  a.mass_row = mass_stride;
+  a.lengths = (const long long*)x->lengths;
+  a.mass = x->mass;
+  a.mass_row = x->mass_stride;
   a.budget = budget;
-  a.sinks = sinks;
-  a.recent = recent;
-  a.dst = dst_table;
-  a.dst_row = dst_stride;
-  a.dst_columns = dst_columns;
-  a.new_lengths = (long long*)new_lengths;
-  a.new_mass = new_mass;
-  a.kept = kept;
+  a.sinks = x->sinks;
+  a.recent = x->recent;
+  a.dst = x->dst_table;
+  a.dst_row = x->dst_stride;
+  a.new_lengths = (long long*)x->new_lengths;
+  a.new_mass = x->new_mass;
+  a.kept = x->kept;
   const cudaStream_t st = (cudaStream_t)stream;
   kk3_cache_select_kernel<<<a.c.batch, kEvThreads, 0, st>>>(a);
   int r = cache_cuda(cudaGetLastError(), "kk3_cache_select_kernel");
   if (r) return r;
-  if (dst_table) {
+  if (x->dst_table)
     return cache_launch_after(kk3_cache_move_kernel, dim3((budget + kMoveWarps - 1) / kMoveWarps, a.c.batch),
                               kMoveWarps * 32, st, "kk3_cache_move_kernel", a);
-  }
   return cache_launch_after(kk3_cache_slide_kernel, dim3(kEntry / 32, a.c.batch), kSlideThreads, st,
                             "kk3_cache_slide_kernel", a);
 }

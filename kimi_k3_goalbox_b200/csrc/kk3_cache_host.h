@@ -14,6 +14,11 @@ namespace kk3 {
 int cache_cuda(cudaError_t e, const char* what);
 // a non-null pointer on an n-byte boundary
 inline bool cache_aligned(const void* p, size_t n) { return p && (uintptr_t)p % n == 0; }
+// queries that the kernels can read: 16-byte aligned rows
+inline bool cache_queries(const void* ql, int64_t ql_token, int64_t ql_head, const void* qp, int64_t qp_token, int64_t qp_head) {
+  return cache_aligned(ql, 16) && cache_aligned(qp, 16) && ((ql_token | ql_head | qp_token | qp_head) & 7) == 0 && ql_token >= 0 &&
+         ql_head >= 0 && qp_token >= 0 && qp_head >= 0;
+}
 // checks a kk3_cache and turns it into the kernels' form
 int cache_pages(const kk3_cache* c, CachePages* out, int* error_word);
 // attention by CTA pairs (kk3_cache_tc.cu): a.workers pairs

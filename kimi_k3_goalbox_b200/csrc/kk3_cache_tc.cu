@@ -1088,54 +1088,51 @@ static int mass_rows(int64_t tokens, int64_t heads, int64_t batch) {
 
 using namespace kk3;
 
-extern "C" int64_t kk3_cache_mass_workspace(int batch, int tokens, int heads) {
-  if (batch < 1 || tokens < 0 || heads < 1 || heads > kMaxHeads) return 0;
+extern "C" int64_t kk3_cache_mass_workspace(void) {
   int sms = 0;
   if (cache_sms(&sms)) return 0;
   return (int64_t)(sms / 2) * (16 + 2 * kMassPos * 4);
 }
 
-extern "C" int kk3_cache_mass(const kk3_cache* cache, const void* q_latent, int64_t ql_token, int64_t ql_head,
-                              const void* q_pe, int64_t qp_token, int64_t qp_head, const float* lse,
-                              const int64_t* lengths, const int32_t* cu_new, int tokens, int heads, float scale,
-                              const float* mass, int64_t mass_stride, float* new_mass, void* workspace,
-                              int64_t workspace_bytes, int* error_word, void* stream) {
+extern "C" int kk3_cache_mass(const kk3_cache_mass_args* x, void* stream) {
+  if (!x) return KK3_ERR_ARG;
   MassArgs a;
-  const int rc = cache_pages(cache, &a.c, error_word);
+  const int rc = cache_pages(&x->cache, &a.c, x->error_word);
   if (rc) return rc;
-  if (tokens < 0 || heads < 1 || !cache_aligned(lengths, 8) || !cache_aligned(cu_new, 4) || !(scale == scale) ||
-      !cache_aligned(new_mass, 4) || (mass && ((uintptr_t)mass % 4 || mass_stride < 0)))
+  const int tokens = x->tokens, heads = x->heads;
+  if (tokens < 0 || heads < 1 || !cache_aligned(x->lengths, 8) || !cache_aligned(x->cu_new, 4) || !(x->scale == x->scale) ||
+      !cache_aligned(x->new_mass, 4) || (x->mass && ((uintptr_t)x->mass % 4 || x->mass_stride < 0)))
     return KK3_ERR_ARG;
   if (heads > kMaxHeads || (int64_t)tokens * heads > INT32_MAX / 2) return KK3_ERR_UNSUPPORTED;
-  if (tokens > 0 && (!cache_aligned(q_latent, 16) || !cache_aligned(q_pe, 16) || !cache_aligned(lse, 4) || ql_token % 8 ||
-                     ql_head % 8 || qp_token % 8 || qp_head % 8 || ql_token < 0 || ql_head < 0 || qp_token < 0 || qp_head < 0))
+  if (tokens > 0 && (!cache_queries(x->q_latent, x->ql_token, x->ql_head, x->q_pe, x->qp_token, x->qp_head) ||
+                     !cache_aligned(x->lse, 4)))
     return KK3_ERR_ARG;
   int sms = 0;
   if (cache_sms(&sms)) return KK3_ERR_CUDA;
-  if (!cache_aligned(workspace, 16) || workspace_bytes < kk3_cache_mass_workspace(a.c.batch, tokens, heads)) return KK3_ERR_ARG;
-  a.q_lat = (const bf16*)q_latent;
-  a.q_pe = (const bf16*)q_pe;
-  a.ql_tok = ql_token;
-  a.ql_head = ql_head;
-  a.qp_tok = qp_token;
-  a.qp_head = qp_head;
-  a.lse = lse;
-  a.lengths = (const long long*)lengths;
-  a.cu_new = cu_new;
+  if (!cache_aligned(x->workspace, 16) || x->workspace_bytes < kk3_cache_mass_workspace()) return KK3_ERR_ARG;
+  a.q_lat = (const bf16*)x->q_latent;
+  a.q_pe = (const bf16*)x->q_pe;
+  a.ql_tok = x->ql_token;
+  a.ql_head = x->ql_head;
+  a.qp_tok = x->qp_token;
+  a.qp_head = x->qp_head;
+  a.lse = x->lse;
+  a.lengths = (const long long*)x->lengths;
+  a.cu_new = x->cu_new;
   a.tokens = tokens;
   a.heads = heads;
-  a.scale_log2 = scale * 1.4426950408889634f;
-  a.mass = mass;
-  a.mass_row = mass_stride;
-  a.out = new_mass;
+  a.scale_log2 = x->scale * 1.4426950408889634f;
+  a.mass = x->mass;
+  a.mass_row = x->mass_stride;
+  a.out = x->new_mass;
   a.workers = sms / 2;
-  a.meta = (int*)workspace;
-  a.part = (float*)((char*)workspace + (size_t)a.workers * 16);
+  a.meta = (int*)x->workspace;
+  a.part = (float*)((char*)x->workspace + (size_t)a.workers * 16);
   PairMaps maps;
   PairRows pr;
   const int rows = mass_rows(tokens, heads, a.c.batch);
   if (tokens > 0) {
-    const int r = pair_maps(cache, q_latent, ql_token, ql_head, q_pe, qp_token, qp_head, tokens, heads, rows / 2, &maps, &pr);
+    const int r = pair_maps(&x->cache, x->q_latent, x->ql_token, x->ql_head, x->q_pe, x->qp_token, x->qp_head, tokens, heads, rows / 2, &maps, &pr);
     if (r) return r;
   } else {
     memset(&maps, 0, sizeof(maps));   // no tile reads them

@@ -29,12 +29,16 @@ DEFAULT_SCALE = (128 + 64) ** -0.5      # (qk_nope_dim + qk_rope_dim) ** -0.5 (m
 MAX_SEQUENCES, MAX_HEADS, MAX_PAGE, MAX_POSITIONS = 4096, 128, 65536, 1 << 27
 
 
-# kk3_cache (include/kk3.h) as bytes: kv, pe, their page and row strides, table, table_stride, num_pages, page_size,
-# columns, batch
-_DESC = struct.Struct("=QQqqqqQqiiii")
-
+# The argument blocks of include/kk3.h as bytes. kk3_cache: kv, pe, their page and row strides, table, table_stride,
+# num_pages, page_size, columns, batch; then each operator's own fields in their order.
+_CACHE = "QQqqqqQqiiii"
+_APPEND = struct.Struct("=" + _CACHE + "QqQQQQQif")
+_ATTEND = struct.Struct("=" + _CACHE + "QqqQqqQQQQQqQiifi")
+_MASS = struct.Struct("=" + _CACHE + "QqqQqqQQQQqQQqQiifi")
+_EVICT = struct.Struct("=" + _CACHE + "QQqQqQQQQiiii")
 
 _LIB = None
+_WORKSPACE: dict = {}       # (operator, device index) -> bytes, the same for every call on a device
 _raw_stream = torch._C._cuda_getCurrentRawStream    # current_stream(device).cuda_stream without the Stream object
 
 
@@ -42,17 +46,11 @@ def _lib() -> ctypes.CDLL:
     global _LIB
     if _LIB is None:
         lib = load_library()
-        vp, i32, i64, f32 = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_float
-        desc = ctypes.c_char_p
-        lib.kk3_cache_append.argtypes = [desc, vp, i64, vp, f32, vp, vp, i32, vp, vp, vp]
-        lib.kk3_cache_attend_workspace.argtypes = [i32, i32, i32]
-        lib.kk3_cache_attend_workspace.restype = i64
-        lib.kk3_cache_attend.argtypes = [desc, vp, i64, i64, vp, i64, i64, vp, vp, i32, i32, f32, vp, vp, vp, i64, vp, vp]
-        lib.kk3_cache_mass_workspace.argtypes = [i32, i32, i32]
-        lib.kk3_cache_mass_workspace.restype = i64
-        lib.kk3_cache_mass.argtypes = [desc, vp, i64, i64, vp, i64, i64, vp, vp, vp, i32, i32, f32, vp, i64, vp, vp, i64,
-                                       vp, vp]
-        lib.kk3_cache_evict.argtypes = [desc, vp, vp, i64, i32, i32, i32, vp, i64, i32, vp, vp, vp, vp, vp]
+        for name in ("append", "attend", "mass", "evict"):
+            getattr(lib, f"kk3_cache_{name}").argtypes = [ctypes.c_char_p, ctypes.c_void_p]
+        for name in ("attend", "mass"):
+            getattr(lib, f"kk3_cache_{name}_workspace").argtypes = []
+            getattr(lib, f"kk3_cache_{name}_workspace").restype = ctypes.c_int64
         _LIB = lib
     return _LIB
 
@@ -69,49 +67,81 @@ def paged_view(kv_cache: torch.Tensor, pe_cache: torch.Tensor, page_size: int):
 
 
 # --- argument checks -------------------------------------------------------------------------------------------
-# A decode step calls these operators once per layer, so the checks are written to cost little when they pass: one
-# comparison a line, and a message is only put together for a refusal.
+# A decode step calls these operators once per layer, so a check that passes is one expression; what is wrong is only
+# looked for, and put into words, when it fails.
 
 _BF16, _F32, _I32, _I64 = torch.bfloat16, torch.float32, torch.int32, torch.int64
 
 
-def _need(ok: bool, what: str) -> None:
-    if not ok:
-        raise ValueError(what)
+def _explain(device, *expected) -> None:
+    """Raise for the first of (tensor, name, dtype, shape or None, contiguous) that is not what it should be."""
+    for t, name, dtype, shape, contiguous in expected:
+        if not isinstance(t, torch.Tensor):
+            raise ValueError(f"{name} must be a tensor")
+        if t.dtype != dtype or (shape is not None and t.shape != shape):
+            raise ValueError(f"{name} must be {dtype}{'' if shape is None else ' ' + str(list(shape))}, not {t.dtype} "
+                             f"{list(t.shape)}")
+        if not t.is_cuda:
+            raise ValueError(f"{name} must be on a CUDA device (sm_100a kernels, no CPU path)")
+        if t.get_device() != device:
+            raise ValueError(f"{name} must be on cuda:{device}, with the cache")
+        if contiguous and not t.is_contiguous():
+            raise ValueError(f"{name} must be contiguous")
+    raise ValueError("arguments do not fit together")
 
 
-def _check(t, name: str, device: torch.device, dtype: torch.dtype, shape: tuple) -> None:
-    """`t` is a contiguous tensor of this kind."""
-    _check_kind(t, name, device, dtype, shape)
-    if not t.is_contiguous():
-        raise ValueError(f"{name} must be contiguous")
+def _explain_rows(*tensors) -> None:
+    for t, name in tensors:
+        if t.stride(-1) != 1 or t.data_ptr() % 16 or any(s % 8 or s < 0 for n, s in zip(t.shape[:-1], t.stride()) if n > 1):
+            raise ValueError(f"{name} needs a contiguous last dim, strides that are multiples of 8 elements and 16-byte "
+                             "alignment")
+    raise ValueError("the rows of kv and pe must not overlap, and their page strides must be multiples of their row strides")
 
 
-def _check_kind(t, name: str, device: torch.device, dtype: torch.dtype, shape: tuple) -> None:
-    if not isinstance(t, torch.Tensor):
-        raise ValueError(f"{name} must be a tensor")
-    if t.dtype != dtype or t.shape != shape:
-        raise ValueError(f"{name} must be {dtype} {list(shape)}, not {t.dtype} {list(t.shape)}")
-    if t.device != device:
-        raise ValueError(f"{name} must be on {device}, with the cache")
+def _cache(kv, pe, table):
+    """(the fields of kk3_cache, device index, sequences, positions per sequence)."""
+    try:
+        ks, ts, dev = kv.shape, table.shape, kv.get_device()
+        fine = (len(ks) == 3 and len(ts) == 2 and ks[2] == LATENT and kv.dtype is _BF16 and pe.dtype is _BF16
+                and table.dtype is _I32 and dev >= 0 and pe.get_device() == dev and table.get_device() == dev
+                and pe.shape == (ks[0], ks[1], ROPE) and ks[0] > 0 and ks[1] > 0 and ts[0] > 0 and ts[1] > 0)
+    except AttributeError:
+        fine = False
+    if not fine:
+        for t, name, n in ((kv, "kv", 3), (pe, "pe", 3), (table, "table", 2)):
+            if not isinstance(t, torch.Tensor) or t.dim() != n or 0 in t.shape:
+                raise ValueError(f"{name} must be a tensor of {n} dims, not empty")
+        _explain(kv.get_device(), (kv, "kv", _BF16, (kv.shape[0], kv.shape[1], LATENT), False),
+                 (pe, "pe", _BF16, (kv.shape[0], kv.shape[1], ROPE), False), (table, "table", _I32, None, False))
+    pages, page, _ = ks
+    B, columns = ts
+    kv_at, pe_at = kv.data_ptr(), pe.data_ptr()
+    k0, k1, k2 = kv.stride()
+    p0, p1, p2 = pe.stride()
+    # the stride of a dim of one element means nothing
+    if page == 1:
+        k1, p1 = LATENT, ROPE
+    if pages == 1:
+        k0, p0 = page * k1, page * p1
+    if (k2 != 1 or p2 != 1 or (kv_at | pe_at) & 15 or (k0 | k1 | p0 | p1) & 7 or k1 < LATENT or p1 < ROPE or k0 < 0 or p0 < 0
+            or k0 % k1 or p0 % p1):
+        _explain_rows((kv, "kv"), (pe, "pe"))
+    t0, t1 = table.stride()
+    if (t1 != 1 and columns > 1) or t0 < 0:
+        raise ValueError("table rows must be contiguous")
+    if B > MAX_SEQUENCES or page > MAX_PAGE or columns * page > MAX_POSITIONS or pages >= 1 << 31:
+        raise ValueError(f"at most {MAX_SEQUENCES} sequences, pages of {MAX_PAGE} and {MAX_POSITIONS} positions per "
+                         "sequence")
+    return (kv_at, pe_at, k0, k1, p0, p1, table.data_ptr(), t0 if B > 1 else columns, pages, page, columns, B), dev, B, columns * page
 
 
-def _vector_rows(t, name: str) -> None:
-    """Refuse what 16-byte loads cannot read."""
-    if t.stride(-1) != 1 or t.data_ptr() % 16 or any(s % 8 or s < 0 for n, s in zip(t.shape[:-1], t.stride()) if n > 1):
-        raise ValueError(f"{name} needs a contiguous last dim, strides that are multiples of 8 elements and 16-byte "
-                         "alignment")
-
-
-def _strides3(t, name: str) -> tuple[int, int, int]:
-    """(address, strides of the first two dims) of a three-dimensional tensor that the kernels read with 16-byte loads.
-    The stride of a dim of one element means nothing and is made a valid one."""
-    s0, s1, s2 = t.stride()
-    n0, n1, n2 = t.shape
-    at = t.data_ptr()
-    if s2 != 1 or (at | s0 * 2 | s1 * 2) & 15 or s0 < 0 or s1 < 0:
-        _vector_rows(t, name)
-    return at, s0 if n0 > 1 else n1 * n2, s1 if n1 > 1 else n2
+def _error(error_word, device: int) -> int:
+    if error_word is None:
+        return 0
+    if (not isinstance(error_word, torch.Tensor) or error_word.get_device() != device or error_word.dtype != _I32
+            or error_word.numel() != 1):
+        raise ValueError("error_word must be one int32 on the cache's device")
+    return error_word.data_ptr()
 
 
 def _query_rows(t):
@@ -126,92 +156,71 @@ def _query_rows(t):
     return t, n1 * s1, s1
 
 
-def _cache(kv, pe, table):
-    """(kk3_cache bytes, device, sequences, positions per sequence)."""
-    if not isinstance(kv, torch.Tensor) or kv.dim() != 3 or kv.dtype != _BF16 or kv.shape[2] != LATENT or 0 in kv.shape:
-        raise ValueError("kv must be bfloat16 [pages, page_size, 512], not empty")
-    dev = kv.device
-    if dev.type != "cuda":
-        raise ValueError("the cache must be on a CUDA device (sm_100a kernels, no CPU path)")
-    pages, page, _ = kv.shape
-    _check_kind(pe, "pe", dev, _BF16, (pages, page, ROPE))
-    if not isinstance(table, torch.Tensor) or table.dim() != 2 or 0 in table.shape:
-        raise ValueError("table must be int32 [B, columns], not empty")
-    B, columns = table.shape
-    _check_kind(table, "table", dev, _I32, (B, columns))
-    kv_at, kv_page, kv_row = _strides3(kv, "kv")
-    pe_at, pe_page, pe_row = _strides3(pe, "pe")
-    if kv_row < LATENT or pe_row < ROPE:
-        raise ValueError("the rows of kv and pe must not overlap")
-    if page > 1 and (kv_page % kv_row or pe_page % pe_row):
-        raise ValueError("the page strides of kv and pe must be multiples of their row strides")
-    if columns > 1 and table.stride(1) != 1:
-        raise ValueError("table rows must be contiguous")
-    if B > MAX_SEQUENCES or page > MAX_PAGE or columns * page > MAX_POSITIONS or pages >= 1 << 31:
-        raise ValueError(f"at most {MAX_SEQUENCES} sequences, pages of {MAX_PAGE} and {MAX_POSITIONS} positions per "
-                         "sequence")
-    desc = _DESC.pack(kv_at, pe_at, kv_page, kv_row, pe_page, pe_row, table.data_ptr(),
-                      table.stride(0) if B > 1 else columns, pages, page, columns, B)
-    return desc, dev, B, columns * page
-
-
-def _error(error_word, device) -> int | None:
-    if error_word is None:
-        return None
-    _need(isinstance(error_word, torch.Tensor) and error_word.device == device and error_word.dtype == _I32
-          and error_word.numel() == 1, "error_word must be one int32 on the cache's device")
-    return error_word.data_ptr()
-
-
-def _queries(q_latent, q_pe, device, scale):
-    if not isinstance(q_latent, torch.Tensor) or q_latent.dim() != 3:
-        raise ValueError("q_latent must be bfloat16 [T, heads, 512]")
-    T, H, _ = q_latent.shape
+def _queries(q_latent, q_pe, lengths, cu_new, dev: int, B: int, scale):
+    """(T, heads, scale, tensors to keep until the launch, q_latent and its strides, q_pe and its strides)."""
+    try:
+        qs = q_latent.shape
+        fine = (len(qs) == 3 and qs[2] == LATENT and q_pe.shape == (qs[0], qs[1], ROPE) and q_latent.dtype is _BF16
+                and q_pe.dtype is _BF16 and q_latent.get_device() == dev and q_pe.get_device() == dev
+                and lengths.dtype is _I64 and cu_new.dtype is _I32 and lengths.shape == (B,) and cu_new.shape == (B + 1,)
+                and lengths.get_device() == dev and cu_new.get_device() == dev
+                and lengths.is_contiguous() and cu_new.is_contiguous())
+    except AttributeError:
+        fine = False
+    if not fine:
+        if not isinstance(q_latent, torch.Tensor) or q_latent.dim() != 3:
+            raise ValueError("q_latent must be bfloat16 [T, heads, 512]")
+        T, H = q_latent.shape[:2]
+        _explain(dev, (q_latent, "q_latent", _BF16, (T, H, LATENT), False), (q_pe, "q_pe", _BF16, (T, H, ROPE), False),
+                 (lengths, "lengths", _I64, (B,), True), (cu_new, "cu_new", _I32, (B + 1,), True))
+    T, H, _ = qs
     if not 1 <= H <= MAX_HEADS or T * H >= 1 << 30:
         raise ValueError(f"heads must be 1..{MAX_HEADS}, and T * heads below 2^30")
-    _check_kind(q_latent, "q_latent", device, _BF16, (T, H, LATENT))
-    _check_kind(q_pe, "q_pe", device, _BF16, (T, H, ROPE))
-    scale = DEFAULT_SCALE if scale is None else float(scale)
-    if scale != scale or abs(scale) == float("inf"):
-        raise ValueError("scale must be finite")
-    if T:
-        q_latent, *ql = _query_rows(q_latent)
-        q_pe, *qp = _query_rows(q_pe)
+    if scale is None:
+        scale = DEFAULT_SCALE
     else:
-        ql, qp = (LATENT, LATENT), (ROPE, ROPE)
-    return T, H, scale, (q_latent, q_pe), (q_latent.data_ptr(), *ql, q_pe.data_ptr(), *qp)
+        scale = float(scale)
+        if scale != scale or abs(scale) == float("inf"):
+            raise ValueError("scale must be finite")
+    if T:
+        q_latent, l0, l1 = _query_rows(q_latent)
+        q_pe, p0, p1 = _query_rows(q_pe)
+    else:
+        l0, l1, p0, p1 = LATENT, LATENT, ROPE, ROPE
+    return T, H, scale, (q_latent, q_pe), (q_latent.data_ptr(), l0, l1, q_pe.data_ptr(), p0, p1)
 
 
-def _mass_stride(mass, name: str, device, B: int, capacity: int) -> int:
-    _check_kind(mass, name, device, _F32, (B, capacity))
+def _mass_stride(mass, name: str, dev: int, B: int, capacity: int) -> int:
+    if not isinstance(mass, torch.Tensor) or mass.dtype is not _F32 or mass.shape != (B, capacity) or mass.get_device() != dev:
+        _explain(dev, (mass, name, _F32, (B, capacity), False))
     row, one = mass.stride()
     if (one != 1 and capacity > 1) or row < 0:
         raise ValueError(f"{name} rows must be contiguous")
     return row if B > 1 else capacity
 
 
-def _run(what: str, device: torch.device, *args) -> None:
+def _run(what: str, dev: int, args: bytes) -> None:
     """Call a C entry point on the cache's device and its current stream."""
-    fn, index = getattr(_lib(), what), device.index
-    if torch.cuda.current_device() == index:
-        rc = fn(*args, _raw_stream(index))
+    fn = getattr(_LIB or _lib(), what)
+    if torch.cuda.current_device() == dev:
+        rc = fn(args, _raw_stream(dev))
     else:
-        with torch.cuda.device(index):
-            rc = fn(*args, _raw_stream(index))
+        with torch.cuda.device(dev):
+            rc = fn(args, _raw_stream(dev))
     if rc != 0:
         raise KK3Error(rc, what)
 
 
-def _workspace(what: str, device: torch.device, *args) -> torch.Tensor:
-    """A call's own workspace, from torch's allocator on the current stream."""
-    if torch.cuda.current_device() == device.index:
-        nbytes = getattr(_lib(), what)(*args)
-    else:
+def _workspace(what: str, device: torch.device) -> tuple[torch.Tensor, int]:
+    """A call's own workspace, from torch's allocator on the current stream, and its size."""
+    nbytes = _WORKSPACE.get((what, device.index))
+    if nbytes is None:
         with torch.cuda.device(device):
-            nbytes = getattr(_lib(), what)(*args)
-    if nbytes <= 0:
-        raise KK3Error(-3, what)
-    return torch.empty(nbytes, dtype=torch.uint8, device=device)
+            nbytes = getattr(_lib(), what)()
+        if nbytes <= 0:
+            raise KK3Error(-3, what)
+        _WORKSPACE[what, device.index] = nbytes
+    return torch.empty(nbytes, dtype=torch.uint8, device=device), nbytes
 
 
 # --- the operators ---------------------------------------------------------------------------------------------
@@ -222,24 +231,33 @@ def append(raw, norm_weight, kv, pe, table, lengths, cu_new, *, eps: float = 1e-
     raw: bf16 [T, 576], the `ka` projection of the new tokens; its first 512 values are RMS-normalised with
     norm_weight (bf16 [512]) in FP32 and rounded once, the other 64 are stored as they are. lengths: positions cached
     before. A token behind the table's last column is not written and sets error_word."""
-    desc, dev, B, _ = _cache(kv, pe, table)
-    if not isinstance(raw, torch.Tensor) or raw.dim() != 2:
-        raise ValueError("raw must be bfloat16 [T, 576]")
-    T = raw.shape[0]
-    _check_kind(raw, "raw", dev, _BF16, (T, LATENT + ROPE))
-    _check(norm_weight, "norm_weight", dev, _BF16, (LATENT,))
-    _vector_rows(norm_weight, "norm_weight")
-    _check(lengths, "lengths", dev, _I64, (B,))
-    _check(cu_new, "cu_new", dev, _I32, (B + 1,))
+    cache, dev, B, _ = _cache(kv, pe, table)
+    try:
+        rs = raw.shape
+        fine = (len(rs) == 2 and rs[1] == LATENT + ROPE and raw.dtype is _BF16 and norm_weight.dtype is _BF16
+                and norm_weight.shape == (LATENT,) and raw.get_device() == dev and norm_weight.get_device() == dev
+                and norm_weight.is_contiguous() and lengths.dtype is _I64 and cu_new.dtype is _I32 and lengths.shape == (B,)
+                and cu_new.shape == (B + 1,) and lengths.get_device() == dev and cu_new.get_device() == dev
+                and lengths.is_contiguous() and cu_new.is_contiguous())
+    except AttributeError:
+        fine = False
+    if not fine:
+        if not isinstance(raw, torch.Tensor) or raw.dim() != 2:
+            raise ValueError("raw must be bfloat16 [T, 576]")
+        _explain(dev, (raw, "raw", _BF16, (raw.shape[0], LATENT + ROPE), False), (norm_weight, "norm_weight", _BF16, (LATENT,), True),
+                 (lengths, "lengths", _I64, (B,), True), (cu_new, "cu_new", _I32, (B + 1,), True))
+    T = rs[0]
+    row, one = raw.stride()
+    if T <= 1:
+        row = LATENT + ROPE
+    at, weight = raw.data_ptr(), norm_weight.data_ptr()
+    if T and (one != 1 or at & 15 or row & 7 or row < LATENT + ROPE) or weight & 15:
+        raise ValueError("raw and norm_weight need 16-byte aligned rows with a contiguous last dim")
     if not eps >= 0:
         raise ValueError("eps must not be negative")
-    row = LATENT + ROPE
-    if T:
-        _vector_rows(raw, "raw")
-        row = raw.stride(0) if T > 1 else row
     out = torch.empty_like(lengths)
-    _run("kk3_cache_append", dev, desc, raw.data_ptr(), row, norm_weight.data_ptr(), eps, lengths.data_ptr(),
-         cu_new.data_ptr(), T, out.data_ptr(), _error(error_word, dev))
+    _run("kk3_cache_append", dev, _APPEND.pack(*cache, at, row, weight, lengths.data_ptr(), cu_new.data_ptr(), out.data_ptr(),
+                                               _error(error_word, dev), T, eps))
     return out
 
 
@@ -253,24 +271,22 @@ def attend(q_latent, q_pe, kv, pe, table, lengths, cu_new, *, scale: float | Non
     lengths: cached positions, the new tokens included (append's result): token i of n sees the first
     lengths - n + i + 1. A token that sees nothing gets zeros and -inf. Rows behind cu_new[B] are not written (pass
     `out` and `lse`, both contiguous, to keep theirs)."""
-    desc, dev, B, _ = _cache(kv, pe, table)
-    T, H, scale, _copies, q = _queries(q_latent, q_pe, dev, scale)
-    _check(lengths, "lengths", dev, _I64, (B,))
-    _check(cu_new, "cu_new", dev, _I32, (B + 1,))
+    cache, dev, B, _ = _cache(kv, pe, table)
+    T, H, scale, _keep, q = _queries(q_latent, q_pe, lengths, cu_new, dev, B, scale)
+    device = kv.device
     if out is None:
-        out = torch.empty((T, H, LATENT), dtype=_BF16, device=dev)
-    else:
-        _check(out, "out", dev, _BF16, (T, H, LATENT))
-        _need(out.data_ptr() % 16 == 0, "out must be 16-byte aligned")
+        out = torch.empty((T, H, LATENT), dtype=_BF16, device=device)
+    elif out.dtype != _BF16 or out.shape != (T, H, LATENT) or out.get_device() != dev or not out.is_contiguous() or out.data_ptr() % 16:
+        raise ValueError(f"out must be contiguous bfloat16 {[T, H, LATENT]} on the cache's device, 16-byte aligned")
     if lse is None:
-        lse = torch.empty((T, H), dtype=_F32, device=dev)
-    else:
-        _check(lse, "lse", dev, _F32, (T, H))
+        lse = torch.empty((T, H), dtype=_F32, device=device)
+    elif lse.dtype != _F32 or lse.shape != (T, H) or lse.get_device() != dev or not lse.is_contiguous():
+        raise ValueError(f"lse must be contiguous float32 {[T, H]} on the cache's device")
     err = _error(error_word, dev)
     if T:
-        work = _workspace("kk3_cache_attend_workspace", dev, B, T, H)
-        _run("kk3_cache_attend", dev, desc, *q, lengths.data_ptr(), cu_new.data_ptr(), T, H, scale, out.data_ptr(),
-             lse.data_ptr(), work.data_ptr(), work.numel(), err)
+        work, nbytes = _workspace("kk3_cache_attend_workspace", device)
+        _run("kk3_cache_attend", dev, _ATTEND.pack(*cache, *q, lengths.data_ptr(), cu_new.data_ptr(), out.data_ptr(),
+                                                   lse.data_ptr(), work.data_ptr(), nbytes, err, T, H, scale, 0))
     return out, lse
 
 
@@ -281,21 +297,21 @@ def attention_mass(q_latent, q_pe, lse, kv, pe, table, lengths, cu_new, *, scale
 
     lse: attend's, with the same queries, lengths and scale. mass: what earlier calls accumulated (zeros if None);
     `out` may be mass itself. Positions at or behind a length keep their mass."""
-    desc, dev, B, capacity = _cache(kv, pe, table)
-    T, H, scale, _copies, q = _queries(q_latent, q_pe, dev, scale)
-    _check(lse, "lse", dev, _F32, (T, H))
-    _check(lengths, "lengths", dev, _I64, (B,))
-    _check(cu_new, "cu_new", dev, _I32, (B + 1,))
-    row, before = 0, None
+    cache, dev, B, capacity = _cache(kv, pe, table)
+    T, H, scale, _keep, q = _queries(q_latent, q_pe, lengths, cu_new, dev, B, scale)
+    if not isinstance(lse, torch.Tensor) or lse.dtype is not _F32 or lse.shape != (T, H) or lse.get_device() != dev or not lse.is_contiguous():
+        _explain(dev, (lse, "lse", _F32, (T, H), True))
+    row, before = 0, 0
     if mass is not None:
         row, before = _mass_stride(mass, "mass", dev, B, capacity), mass.data_ptr()
+    device = kv.device
     if out is None:
-        out = torch.empty((B, capacity), dtype=_F32, device=dev)
-    else:
-        _check(out, "out", dev, _F32, (B, capacity))
-    work = _workspace("kk3_cache_mass_workspace", dev, B, T, H)
-    _run("kk3_cache_mass", dev, desc, *q, lse.data_ptr(), lengths.data_ptr(), cu_new.data_ptr(), T, H, scale, before, row,
-         out.data_ptr(), work.data_ptr(), work.numel(), _error(error_word, dev))
+        out = torch.empty((B, capacity), dtype=_F32, device=device)
+    elif out.dtype != _F32 or out.shape != (B, capacity) or out.get_device() != dev or not out.is_contiguous():
+        raise ValueError(f"out must be contiguous float32 {[B, capacity]} on the cache's device")
+    work, nbytes = _workspace("kk3_cache_mass_workspace", device)
+    _run("kk3_cache_mass", dev, _MASS.pack(*cache, *q, lse.data_ptr(), lengths.data_ptr(), cu_new.data_ptr(), before, row,
+                                           out.data_ptr(), work.data_ptr(), nbytes, _error(error_word, dev), T, H, scale, 0))
     return out
 
 
@@ -308,28 +324,34 @@ def evict(kv, pe, table, lengths, mass, budget: int, *, sinks: int = 0, recent: 
     that none of the sequences uses, so that pages shared with others stay as they are), or in place (None). Returns
     (new lengths int64 [B], their mass f32 [B, columns * page_size] with zeros behind, their old positions int32
     [B, budget] with -1 behind)."""
-    desc, dev, B, capacity = _cache(kv, pe, table)
-    _check(lengths, "lengths", dev, _I64, (B,))
+    cache, dev, B, capacity = _cache(kv, pe, table)
+    if (not isinstance(lengths, torch.Tensor) or lengths.dtype is not _I64 or lengths.shape != (B,) or lengths.get_device() != dev
+            or not lengths.is_contiguous()):
+        _explain(dev, (lengths, "lengths", _I64, (B,), True))
     row = _mass_stride(mass, "mass", dev, B, capacity)
     budget, sinks, recent = int(budget), int(sinks), int(recent)
     if not 1 <= budget <= capacity:
         raise ValueError("budget must be 1 .. columns * page_size")
     if sinks < 0 or recent < 0 or sinks + recent > budget:
         raise ValueError("sinks + recent must not exceed the budget")
-    dst, dst_row, dst_columns = None, 0, 0
+    dst, dst_row, dst_columns = 0, 0, 0
     if dst_table is not None:
         if not isinstance(dst_table, torch.Tensor) or dst_table.dim() != 2:
             raise ValueError("dst_table must be int32 [B, columns]")
         dst_columns = dst_table.shape[1]
-        _check_kind(dst_table, "dst_table", dev, _I32, (B, dst_columns))
-        if dst_columns > 1 and dst_table.stride(1) != 1:
+        if dst_table.dtype is not _I32 or dst_table.shape[0] != B or dst_table.get_device() != dev:
+            _explain(dev, (dst_table, "dst_table", _I32, (B, dst_columns), False))
+        dst_row, one = dst_table.stride()
+        if (one != 1 and dst_columns > 1) or dst_row < 0:
             raise ValueError("dst_table rows must be contiguous")
         if dst_columns * kv.shape[1] < budget:
             raise ValueError("dst_table must hold the budget")
-        dst, dst_row = dst_table.data_ptr(), dst_table.stride(0) if B > 1 else dst_columns
+        dst, dst_row = dst_table.data_ptr(), dst_row if B > 1 else dst_columns
+    device = kv.device
     new_lengths = torch.empty_like(lengths)
-    new_mass = torch.empty((B, capacity), dtype=_F32, device=dev)
-    kept = torch.empty((B, budget), dtype=_I32, device=dev)
-    _run("kk3_cache_evict", dev, desc, lengths.data_ptr(), mass.data_ptr(), row, budget, sinks, recent, dst, dst_row,
-         dst_columns, new_lengths.data_ptr(), new_mass.data_ptr(), kept.data_ptr(), _error(error_word, dev))
+    new_mass = torch.empty((B, capacity), dtype=_F32, device=device)
+    kept = torch.empty((B, budget), dtype=_I32, device=device)
+    _run("kk3_cache_evict", dev, _EVICT.pack(*cache, lengths.data_ptr(), mass.data_ptr(), row, dst, dst_row,
+                                             new_lengths.data_ptr(), new_mass.data_ptr(), kept.data_ptr(),
+                                             _error(error_word, dev), budget, sinks, recent, dst_columns))
     return new_lengths, new_mass, kept
