@@ -1,29 +1,11 @@
-// kk3_cache.cu - kernels and C entry points of the paged latent cache (include/kk3.h, kk3_cache_*): append, attention
-// of new tokens at warp level, the join of split attention tiles, eviction.
+// kk3_cache.cu - kernels and C entry points of the paged latent cache (include/kk3.h, kk3_cache_*): append, the
+// join of split attention tiles, eviction.
 #include <cuda_runtime.h>
 
 #include "kk3_cache.cuh"
 #include "kk3_cache_host.h"
 
 namespace kk3 {
-
-KK3_DEV void cp_async16_zfill(void* smem, const void* src, bool live) {
-  const unsigned dst = (unsigned)__cvta_generic_to_shared(smem);
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(live ? 16 : 0) : "memory");
-}
-KK3_DEV void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-KK3_DEV void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
-KK3_DEV void ldsm4(unsigned (&r)[4], const void* p) {
-  const unsigned a = (unsigned)__cvta_generic_to_shared(p);
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a) : "memory");
-}
-KK3_DEV void ldsm4t(unsigned (&r)[4], const void* p) {
-  const unsigned a = (unsigned)__cvta_generic_to_shared(p);
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a) : "memory");
-}
 
 // ---------------------------------------------------------------------------------------------
 // append: latent = x[:512] / rms(x[:512]) * weight (FP32, rounded to BF16 once), rope = x[512:], into the page of the
@@ -104,288 +86,6 @@ __global__ void __launch_bounds__(kAppendWarps * 32) kk3_cache_append_kernel(con
   }
   if (lane < 8)
     *reinterpret_cast<uint4*>(a.c.pe + (long long)page * a.c.pe_page + (long long)slot * a.c.pe_row + lane * 8) = rope;
-}
-
-// ---------------------------------------------------------------------------------------------
-// Attention at warp level: a tile is 16 or 32 (MT = 1, 2) (token, head) rows, a unit 64 cached positions.
-//
-//   s = scale (q . e_p), running maximum m and sum l per row, O = O 2^(m - m') + sum_p 2^(s - m') c_p
-//
-// Each cached entry is read once per tile and serves both products from shared memory, so few rows per sequence leave
-// the call bound by the cache's bytes: 64 positions are 73.7 KB, 3200 clocks at one SM's share of HBM, against some
-// 1400 (MT = 1) of work. 8 warps; the query's fragments stay in registers (each warp holds one half of the 576 dims: 18
-// k-steps) and 16 of the unit's positions are a warp's in the first product; warp w owns the output dims
-// 64 w .. 64 w + 63 in the second. Stages of 32 positions (36.5 KB) arrive by cp.async, three and more ahead; the page
-// numbers they need are looked up one unit before that.
-// Probabilities are rounded to BF16 for the second product, the type that the instruction takes with BF16 latents; the
-// running sum adds them unrounded, since lse is an FP32 result.
-
-constexpr int kWaUnit = 64, kWaStage = 32;
-constexpr int kWaPitch = kEntry + 8;      // 1168-byte rows: consecutive rows fall on different banks (ldmatrix)
-constexpr int kWaPPitch = kWaUnit + 8;
-constexpr int kWaThreads = 256;
-constexpr int kWaMinUnits = 2;
-template <int MT>
-struct WaSmem {
-  static constexpr int kRows = 16 * MT, kStages = MT == 1 ? 5 : 4;
-  bf16 ring[kStages][kWaStage][kWaPitch];
-  bf16 q[kRows][kWaPitch];
-  float s[2][kRows][kWaUnit + 4];
-  bf16 p[kRows][kWaPPitch];
-  float alpha[kRows];
-  float m[kRows], l[kRows];
-  long long red[kWaThreads / 32 + 4];
-};
-static_assert(sizeof(WaSmem<1>) <= 232448 && sizeof(WaSmem<2>) <= 232448, "shared memory of a CTA");
-
-// Page of this lane's position (lanes 0 .. 3: the warp's four) of stage `st`, -1 where the tile sees none.
-KK3_DEV int wa_page(const CachePages& c, int b, int st, int sees) {
-  const int lane = threadIdx.x & 31, pos = st * kWaStage + (threadIdx.x >> 5) * 4 + lane;
-  return lane < 4 && pos < sees ? c.table[(long long)b * c.table_stride + page_of(c, pos)] : -1;
-}
-// Copy stage `st` into `ring`, rows without a page as zeros. `page`: wa_page's.
-KK3_DEV void wa_load(const CachePages& c, bf16 (*ring)[kWaPitch], int st, int sees, int page) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  long long kv = -1, pe = -1;
-  if (lane < 4) {
-    const int pos = st * kWaStage + warp * 4 + lane;
-    if (pos < sees) {
-      if ((unsigned)page < (unsigned)c.num_pages) {
-        const int slot = pos - page_of(c, pos) * c.page_size;
-        kv = (long long)page * c.kv_page + (long long)slot * c.kv_row;
-        pe = (long long)page * c.pe_page + (long long)slot * c.pe_row;
-      } else {
-        cache_error(c);
-      }
-    }
-  }
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int row = i >> 1, chunk = (i & 1) * 32 + lane;
-    const long long o = __shfl_sync(0xffffffffu, kv, row);
-    cp_async16_zfill(&ring[warp * 4 + row][chunk * 8], o >= 0 ? c.kv + o + chunk * 8 : c.kv, o >= 0);
-  }
-  const long long o = __shfl_sync(0xffffffffu, pe, lane >> 3);
-  cp_async16_zfill(&ring[warp * 4 + (lane >> 3)][kLat + (lane & 7) * 8], o >= 0 ? c.pe + o + (lane & 7) * 8 : c.pe, o >= 0);
-}
-
-template <int MT>
-__global__ void __launch_bounds__(kWaThreads, 1) kk3_cache_attend_warp_kernel(const AttendArgs a) {
-  constexpr int kRows = 16 * MT, kStages = WaSmem<MT>::kStages;
-  extern __shared__ __align__(128) unsigned char smem_raw[];
-  WaSmem<MT>& sm = *reinterpret_cast<WaSmem<MT>*>(smem_raw);
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int worker = blockIdx.x;
-  static_assert(sizeof(sm.ring) >= (kMaxSeqs + 1) * sizeof(int), "the sequences' tile prefix lies in the ring");
-  const AttendSplit split{kRows, a.heads, kWaUnit, 0};
-  const Share sh = plan_share<kWaThreads>(a, split, worker, kWaMinUnits, reinterpret_cast<int*>(&sm.ring[0][0][0]),
-                                          sm.red);
-  if (tid == 0) a.meta[worker * 4 + 2] = 0;
-  if (worker >= sh.workers) return;
-  int b = sh.b, t = sh.t;
-  long long at = sh.at;
-  while (at < sh.end) {
-    Seq s = a.seq(b);
-    for (; t >= split.tiles(s); t = 0) s = a.seq(++b);
-    const int units = split.units(s, t);
-    const int u0 = split.from(sh, at, units), u1 = split.to(sh, at, units);
-    const bool whole = u0 == 0 && u1 == units;
-    const int row0 = t * kRows, rows = min(kRows, s.n * a.heads - row0);
-    const int sees_max = split.sees(s, t);
-    __syncthreads();   // the previous tile's readers are done with q, p and the ring
-    // stages 2 u0 .. 2 u1 - 1; stage st is in slot (st - 2 u0) % kStages
-    const int st0 = 2 * u0, st1 = 2 * u1;
-    int page[2] = {wa_page(a.c, b, st0, sees_max), wa_page(a.c, b, st0 + 1, sees_max)};
-    // query rows, zeros below the last
-    for (int i = tid; i < kRows * (kEntry / 8); i += kWaThreads) {
-      const int r = i / (kEntry / 8), ch = i % (kEntry / 8);
-      const int g = row0 + min(r, rows - 1), tok = s.q0 + g / a.heads, head = g % a.heads;
-      const bf16* src = ch < kLat / 8 ? a.q_lat + tok * a.ql_tok + head * a.ql_head + ch * 8
-                                      : a.q_pe + tok * a.qp_tok + head * a.qp_head + (ch - kLat / 8) * 8;
-      cp_async16_zfill(&sm.q[r][ch * 8], src, r < rows);
-    }
-    cp_async_commit();
-#pragma unroll
-    for (int i = 0; i < kStages - 2; ++i) {
-      if (st0 + i < st1) wa_load(a.c, sm.ring[i], st0 + i, sees_max, page[i & 1]);
-      cp_async_commit();
-      if (st0 + i + 2 < st1) page[i & 1] = wa_page(a.c, b, st0 + i + 2, sees_max);
-    }
-    cp_async_wait<kStages - 2>();
-    __syncthreads();
-    // this warp's query fragments: k-steps 18 (warp / 4) .. + 17
-    const int ntile = warp & 3, khalf = warp >> 2;
-    unsigned qf[MT][18][4];
-#pragma unroll
-    for (int h = 0; h < MT; ++h)
-#pragma unroll
-      for (int k = 0; k < 18; ++k)
-        ldsm4(qf[h][k], &sm.q[h * 16 + (lane & 15)][(khalf * 18 + k) * 16 + (lane >> 4) * 8]);
-    float acc[MT][8][4] = {};
-    // softmax rows of this warp: 2 MT warp .. + 2 MT - 1, two positions a lane
-    float m[2 * MT], l[2 * MT];
-    int sees[2 * MT];
-#pragma unroll
-    for (int j = 0; j < 2 * MT; ++j) {
-      const int r = warp * 2 * MT + j;
-      m[j] = -INFINITY;
-      l[j] = 0.0f;
-      sees[j] = r < rows ? s.len - s.n + (row0 + r) / a.heads + 1 : 0;
-    }
-    int slot = 0;   // of the unit's first stage
-    for (int u = u0; u < u1; ++u) {
-      // copies so far: stages up to 2 u + kStages - 3; those of this unit are in when kStages - 4 are left
-      cp_async_wait<kStages - 4>();
-      __syncthreads();   // and every warp is done with the unit before, whose slots are filled again
-      const int next = 2 * u + kStages - 2;
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int st = next + i, sl = (slot + kStages - 2 + i) % kStages;
-        constexpr int kTurn = kStages & 1;   // page[] holds stages in turn
-        if (st < st1) wa_load(a.c, sm.ring[sl], st, sees_max, page[(i + kTurn) & 1]);
-        cp_async_commit();
-        if (st + 2 < st1) page[(i + kTurn) & 1] = wa_page(a.c, b, st + 2, sees_max);
-      }
-      const int slot1 = (slot + 1) % kStages;
-      {
-        float c[MT][2][2][4] = {};   // [16 rows][8 positions][chain]
-        const bf16(*ring)[kWaPitch] = sm.ring[ntile < 2 ? slot : slot1];
-        const int prow = (ntile & 1) * 16;
-#pragma unroll
-        for (int k = 0; k < 18; k += 2) {
-#pragma unroll
-          for (int n = 0; n < 2; ++n) {
-            unsigned bf[4];
-            ldsm4(bf, &ring[prow + n * 8 + (lane & 7)][(khalf * 18 + k) * 16 + (lane >> 3) * 8]);
-#pragma unroll
-            for (int h = 0; h < MT; ++h) {
-              mma_bf16(c[h][n][0], qf[h][k][0], qf[h][k][1], qf[h][k][2], qf[h][k][3], bf[0], bf[1]);
-              mma_bf16(c[h][n][1], qf[h][k + 1][0], qf[h][k + 1][1], qf[h][k + 1][2], qf[h][k + 1][3], bf[2], bf[3]);
-            }
-          }
-        }
-#pragma unroll
-        for (int h = 0; h < MT; ++h)
-#pragma unroll
-          for (int n = 0; n < 2; ++n) {
-            const int r = h * 16 + (lane >> 2), col = ntile * 16 + n * 8 + (lane & 3) * 2;
-            const float(*x)[4] = c[h][n];
-            *reinterpret_cast<float2*>(&sm.s[khalf][r][col]) = make_float2(x[0][0] + x[1][0], x[0][1] + x[1][1]);
-            *reinterpret_cast<float2*>(&sm.s[khalf][r + 8][col]) = make_float2(x[0][2] + x[1][2], x[0][3] + x[1][3]);
-          }
-      }
-      __syncthreads();
-      {
-        float v[2 * MT][2], top[2 * MT];
-#pragma unroll
-        for (int j = 0; j < 2 * MT; ++j) {
-          const int r = warp * 2 * MT + j;
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const int col = i * 32 + lane;
-            v[j][i] = (sm.s[0][r][col] + sm.s[1][r][col]) * a.scale_log2;
-            if (u * kWaUnit + col >= sees[j]) v[j][i] = -INFINITY;
-          }
-          top[j] = fmaxf(v[j][0], v[j][1]);
-        }
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1)
-#pragma unroll
-          for (int j = 0; j < 2 * MT; ++j) top[j] = fmaxf(top[j], __shfl_xor_sync(0xffffffffu, top[j], o));
-#pragma unroll
-        for (int j = 0; j < 2 * MT; ++j) {
-          const int r = warp * 2 * MT + j;
-          top[j] = fmaxf(m[j], top[j]);
-          const float ref = top[j] == -INFINITY ? 0.0f : top[j];
-          const float al = exp2f(m[j] - ref);
-          const float p0 = exp2f(v[j][0] - ref), p1 = exp2f(v[j][1] - ref);
-          l[j] = l[j] * al + (p0 + p1);
-          m[j] = top[j];
-          sm.p[r][lane] = f2bf(p0);
-          sm.p[r][32 + lane] = f2bf(p1);
-          if (lane == 0) sm.alpha[r] = al;
-        }
-      }
-      __syncthreads();
-#pragma unroll
-      for (int h = 0; h < MT; ++h) {
-        const float a0 = sm.alpha[h * 16 + (lane >> 2)], a1 = sm.alpha[h * 16 + (lane >> 2) + 8];
-#pragma unroll
-        for (int n = 0; n < 8; ++n) {
-          acc[h][n][0] *= a0;
-          acc[h][n][1] *= a0;
-          acc[h][n][2] *= a1;
-          acc[h][n][3] *= a1;
-        }
-      }
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        unsigned pf[MT][4];
-#pragma unroll
-        for (int h = 0; h < MT; ++h) ldsm4(pf[h], &sm.p[h * 16 + (lane & 15)][k * 16 + (lane >> 4) * 8]);
-        const bf16(*ring)[kWaPitch] = sm.ring[k < 2 ? slot : slot1];
-#pragma unroll
-        for (int n = 0; n < 8; n += 2) {
-          unsigned bf[4];
-          ldsm4t(bf, &ring[(k & 1) * 16 + (lane & 15)][warp * 64 + n * 8 + (lane >> 4) * 8]);
-#pragma unroll
-          for (int h = 0; h < MT; ++h) {
-            mma_bf16(acc[h][n], pf[h][0], pf[h][1], pf[h][2], pf[h][3], bf[0], bf[1]);
-            mma_bf16(acc[h][n + 1], pf[h][0], pf[h][1], pf[h][2], pf[h][3], bf[2], bf[3]);
-          }
-        }
-      }
-      slot = (slot + 2) % kStages;
-    }
-    cp_async_wait<0>();
-#pragma unroll
-    for (int j = 0; j < 2 * MT; ++j) {
-      l[j] = warp_sum(l[j]);
-      if (lane == 0) {
-        sm.m[warp * 2 * MT + j] = m[j];
-        sm.l[warp * 2 * MT + j] = l[j];
-      }
-    }
-    __syncthreads();
-    const long long g = (long long)s.q0 * a.heads + row0;
-    // running sums for the join: slot 1 for the tile this worker begins and leaves, slot 0 for one it comes into
-    float* part = a.part + ((long long)worker * 2 + (u0 == 0 ? 1 : 0)) * kRows * kPartRow;
-#pragma unroll
-    for (int h = 0; h < 2 * MT; ++h) {
-      const int rr = (h >> 1) * 16 + (h & 1) * 8 + (lane >> 2);
-      if (rr < rows) {
-        const float(*x)[4] = acc[h >> 1];
-        if (whole) {
-          const float lr = sm.l[rr], inv = lr > 0.0f || lr != lr ? 1.0f / lr : 0.0f;
-          bf16* o = a.out + (g + rr) * kLat + warp * 64 + (lane & 3) * 2;
-#pragma unroll
-          for (int n = 0; n < 8; ++n)
-            *reinterpret_cast<__nv_bfloat162*>(o + n * 8) = __floats2bfloat162_rn(x[n][(h & 1) * 2] * inv, x[n][(h & 1) * 2 + 1] * inv);
-        } else {
-          float* o = part + rr * kPartRow + warp * 64 + (lane & 3) * 2;
-#pragma unroll
-          for (int n = 0; n < 8; ++n) *reinterpret_cast<float2*>(o + n * 8) = make_float2(x[n][(h & 1) * 2], x[n][(h & 1) * 2 + 1]);
-        }
-      }
-    }
-    if (tid < rows) {
-      if (whole) {
-        a.lse[g + tid] = (sm.m[tid] + log2f(sm.l[tid])) * 0.69314718055994531f;
-      } else {
-        part[tid * kPartRow + kLat] = sm.m[tid];
-        part[tid * kPartRow + kLat + 1] = sm.l[tid];
-      }
-    }
-    if (!whole && u0 == 0 && tid == 0) {   // the workers of this tile: up to the one that holds its last unit
-      int last = worker;
-      while (sh.total * (last + 1) / sh.workers < at + units) ++last;
-      a.meta[worker * 4] = b;
-      a.meta[worker * 4 + 1] = t;
-      a.meta[worker * 4 + 2] = last - worker + 1;
-    }
-    at += units;
-    ++t;
-  }
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -756,32 +456,19 @@ extern "C" int kk3_cache_append(const kk3_cache_append_args* x, void* stream) {
   return cache_cuda(cudaGetLastError(), "kk3_cache_append_kernel");
 }
 
-// The kernel for a call's average rows per sequence, and its workers: the warp-level ones up to 16 and 32 rows, CTA pairs
-// above.
+// The kernel for a call's average rows per sequence, and its workers: warp-level products up to 16 rows, CTA pairs above.
 struct Plan {
   int workers, rows;
 };
 static Plan attend_plan(int64_t batch, int64_t tokens, int64_t heads, int sms) {
-  const int64_t total = tokens * heads;
-  if (total <= 16 * batch) return Plan{sms, 16};
-  if (total <= 32 * batch) return Plan{sms, 32};
-  return Plan{sms / 2, kPairRows};
-}
-template <int MT>
-static int attend_warp(const AttendArgs& a, cudaStream_t st) {
-  static std::atomic<bool> done[kCacheMaxDevices];
-  const int r = cache_allow_smem(kk3_cache_attend_warp_kernel<MT>, sizeof(WaSmem<MT>), done,
-                                 "cudaFuncSetAttribute(kk3_cache_attend_warp_kernel)");
-  if (r) return r;
-  kk3_cache_attend_warp_kernel<MT><<<a.workers, kWaThreads, sizeof(WaSmem<MT>), st>>>(a);
-  return cache_cuda(cudaGetLastError(), "kk3_cache_attend_warp_kernel");
+  return tokens * heads <= kFewRows * batch ? Plan{sms, kFewRows} : Plan{sms / 2, kPairRows};
 }
 
 extern "C" int64_t kk3_cache_attend_workspace(void) {
   int sms = 0;
   if (cache_sms(&sms)) return 0;
-  const int64_t pair = (int64_t)(sms / 2) * (16 + 2 * kPairRows * kPartRow * 4), warp = (int64_t)sms * (16 + 2 * 32 * kPartRow * 4);
-  return pair > warp ? pair : warp;
+  const int64_t pair = (int64_t)(sms / 2) * (16 + 2 * kPairRows * kPartRow * 4), few = (int64_t)sms * (16 + 2 * kFewRows * kPartRow * 4);
+  return pair > few ? pair : few;
 }
 
 extern "C" int kk3_cache_attend(const kk3_cache_attend_args* x, void* stream) {
@@ -818,7 +505,7 @@ extern "C" int kk3_cache_attend(const kk3_cache_attend_args* x, void* stream) {
   a.meta = (int*)x->workspace;
   a.part = (float*)((char*)x->workspace + (size_t)p.workers * 16);
   const cudaStream_t st = (cudaStream_t)stream;
-  const int r = p.rows == 16 ? attend_warp<1>(a, st) : p.rows == 32 ? attend_warp<2>(a, st) : attend_pair(&x->cache, a, st);
+  const int r = p.rows == kFewRows ? attend_few(&x->cache, a, st) : attend_pair(&x->cache, a, st);
   if (r) return r;
   return cache_launch_after(kk3_cache_join_kernel, dim3(p.workers, 16), kJoinThreads, st, "kk3_cache_join_kernel", a, p.rows);
 }

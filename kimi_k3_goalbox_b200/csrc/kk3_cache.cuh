@@ -1,6 +1,6 @@
 // kk3_cache.cuh - the paged latent cache of the MLA layers: argument blocks, address arithmetic and the work split
-// shared by its kernels (kk3_cache.cu: append, evict, warp-level attention, joins; kk3_cache_tc.cu: tensor-core
-// attention and attention weight).
+// shared by its kernels (kk3_cache.cu: append, evict, the join of attention tiles; kk3_cache_tc.cu: attention and
+// attention weight).
 //
 // A cached position is 512 latent values and 64 rope values (BF16), in a page of `page_size` positions found
 // through the sequence's row of the page table. Everything a kernel reads from the device (lengths, cu_new, the
@@ -93,7 +93,7 @@ struct AttendArgs : CallSeqs {
   float* lse;            // [tokens, heads]
   float* part;           // [workers][2][tile rows][kPartRow]: running sums of tiles that several workers share
 };
-constexpr int kPairRows = 128;        // tile of the CTA-pair kernel
+constexpr int kFewRows = 16, kPairRows = 128;   // tiles of the two attention kernels
 constexpr int kPartRow = kLat + 4;   // 512 sums, running maximum, running sum, padding to 16 bytes
 
 struct MassArgs : CallSeqs {
@@ -175,19 +175,25 @@ KK3_DEV long long block_scan(long long mine, long long* red, long long* total) {
   return before;
 }
 
-// Computed by every CTA for itself; all NT threads take part. `prefix` is shared memory of batch + 1 ints, `red` of
+// Computed by every CTA for itself; all NT threads take part. `room` is shared memory of kPlanBytes, `red` of
 // NT / 32 + 4 long longs. A worker takes min_units units at least: shorter pieces cost more to join than they save.
+constexpr int kPlanBytes = kMaxSeqs * (int)sizeof(Seq) + (kMaxSeqs + 1) * 4;
 template <int NT, class Split>
-KK3_DEV Share plan_share(const CallSeqs& a, const Split& split, int worker, int min_units, int* prefix, long long* red) {
+KK3_DEV Share plan_share(const CallSeqs& a, const Split& split, int worker, int min_units, void* room, long long* red) {
   const int tid = threadIdx.x, B = a.c.batch;
+  Seq* seqs = reinterpret_cast<Seq*>(room);
+  int* prefix = reinterpret_cast<int*>(seqs + B);
   const int per = (B + NT - 1) / NT, lo_b = min(B, tid * per), hi_b = min(B, lo_b + per);
   long long mine = 0, all;
-  for (int b = lo_b; b < hi_b; ++b) mine += split.tiles(a.seq(b));
+  for (int b = lo_b; b < hi_b; ++b) {
+    seqs[b] = a.seq(b);
+    mine += split.tiles(seqs[b]);
+  }
   int at = (int)block_scan<NT>(mine, red, &all);
   const int tiles = (int)all;
   for (int b = lo_b; b < hi_b; ++b) {
     prefix[b] = at;
-    at += split.tiles(a.seq(b));
+    at += split.tiles(seqs[b]);
   }
   if (tid == 0) prefix[B] = tiles;
   __syncthreads();
@@ -204,10 +210,9 @@ KK3_DEV Share plan_share(const CallSeqs& a, const Split& split, int worker, int 
   mine = 0;
   if (g0 < g1) {
     int b = b0;
-    Seq s = a.seq(b);
     for (int g = g0; g < g1; ++g) {
-      while (g >= prefix[b + 1]) s = a.seq(++b);
-      mine += split.size(s, g - prefix[b]);
+      while (g >= prefix[b + 1]) ++b;
+      mine += split.size(seqs[b], g - prefix[b]);
     }
   }
   Share sh;
@@ -223,10 +228,9 @@ KK3_DEV Share plan_share(const CallSeqs& a, const Split& split, int worker, int 
   if (before <= sh.begin && sh.begin < before + mine) {   // exactly one thread
     int b = b0;
     long long u = before;
-    Seq s = a.seq(b);
     for (int g = g0; g < g1; ++g) {
-      while (g >= prefix[b + 1]) s = a.seq(++b);
-      const int k = split.size(s, g - prefix[b]);
+      while (g >= prefix[b + 1]) ++b;
+      const int k = split.size(seqs[b], g - prefix[b]);
       if (u + k > sh.begin) {
         found[0] = b;
         found[1] = g - prefix[b];

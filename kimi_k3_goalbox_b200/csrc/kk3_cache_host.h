@@ -21,8 +21,9 @@ inline bool cache_queries(const void* ql, int64_t ql_token, int64_t ql_head, con
 }
 // checks a kk3_cache and turns it into the kernels' form
 int cache_pages(const kk3_cache* c, CachePages* out, int* error_word);
-// attention by CTA pairs (kk3_cache_tc.cu): a.workers pairs
+// attention (kk3_cache_tc.cu): tiles of kPairRows rows by CTA pairs, of kFewRows by single CTAs; a.workers of them
 int attend_pair(const kk3_cache* c, const AttendArgs& a, cudaStream_t st);
+int attend_few(const kk3_cache* c, const AttendArgs& a, cudaStream_t st);
 // SMs of the current device, looked up once per device
 int cache_sms(int* sms);
 

@@ -302,7 +302,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMassThreads, 1)
   const unsigned kbase = smem_u32(base), qbase = kbase + kBlocks * kMassKBlock;
   const int half = rows / 2, slot_bytes = half * 128, slots = min(kMassSlots, kMassRing / slot_bytes);
   const MassSplit split{kMassPos, rows, a.heads};
-  const Share sh = plan_share<kMassThreads>(a, split, worker, 1, reinterpret_cast<int*>(base), ctl.red);
+  const Share sh = plan_share<kMassThreads>(a, split, worker, 1, base, ctl.red);
   if (tid == 0 && rank == 0) a.meta[worker * 4 + 2] = 0;
   if (worker >= sh.workers) {   // both CTAs of the pair
     mass_rest(a, tid, kMassThreads);
@@ -628,7 +628,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPaThreads, 1)
   __syncwarp();
   cluster_arrive();   // the peer's barriers are needed after the plan
   const AttendSplit split{kPairRows, a.heads, kPaUnit, kPaTileCost};
-  const Share sh = plan_share<kPaThreads>(a, split, worker, kPaMinUnits, reinterpret_cast<int*>(smem_raw), ctl.red);
+  const Share sh = plan_share<kPaThreads>(a, split, worker, kPaMinUnits, smem_raw, ctl.red);
   if (tid == 0 && rank == 0) a.meta[worker * 4 + 2] = 0;
   tc_fence_before();
   __syncthreads();
@@ -1008,6 +1008,313 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPaThreads, 1)
 }
 
 // ---------------------------------------------------------------------------------------------
+// Attention of few rows (single tokens on one rank): a tile is 16 (token, head) rows, a unit 64 cached positions.
+//
+// The call is bound by the cache's bytes, so each entry comes into shared memory once, by TMA, and serves both products
+// from there at warp level (m16n8k16): 64 positions are 73.7 KB, 3200 clocks at one SM's share of HBM. 16 warps, four to
+// a scheduler, since what the work on a unit takes is latency. In the first product a warp holds the query's fragments of
+// half of the 576 dims in registers and takes 8 positions, in the second it owns 32 of the output dims. Six stages of 32
+// positions, of which a unit holds two; the warps issue the copies between them, two units ahead, and what frees a unit's
+// stages is the barrier that the next unit's scores need anyway. (Copies by cp.async with padded rows, 5 stages, took 165
+// us where these take the time noted with the launch.)
+// Probabilities are rounded to BF16 for the second product, the type that the instruction takes with BF16 latents; the
+// running sum adds them unrounded, since lse is an FP32 result.
+
+constexpr int kFewUnit = 64, kFewStage = 32, kFewStages = 6;
+constexpr int kFewThreads = 512;
+constexpr int kFewBlock = kFewStage * 128;              // 32 positions x 64 dims
+constexpr int kFewStageBytes = kBlocks * kFewBlock;
+constexpr int kFewMinUnits = 2;
+struct FewCtl {
+  float s[2][kFewRows][kFewUnit + 2];   // scores, one part from each half of the dims
+  alignas(16) bf16 p[kFewRows][kFewUnit + 8];
+  float alpha[kFewRows], m[kFewRows], l[kFewRows];
+  unsigned long long full[kFewStages];
+  int dead;
+};
+constexpr int kFewSmem = kFewStages * kFewStageBytes + (int)sizeof(FewCtl);
+static_assert(kFewSmem <= 232448, "shared memory of a CTA");
+static_assert(kFewStages * kFewStageBytes >= kPlanBytes + (kFewThreads / 32 + 4) * 8, "the plan lies in the ring");
+
+KK3_DEV void ldsm4(unsigned (&r)[4], unsigned a) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a) : "memory");
+}
+KK3_DEV void ldsm4t(unsigned (&r)[4], unsigned a) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a) : "memory");
+}
+KK3_DEV float redux_max(float v) {
+  float r;
+  asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+  return r;
+}
+// single-CTA copies
+KK3_DEV void load_box1(bool me, unsigned dst, const CUtensorMap* map, int x, int row, unsigned bar) {
+  asm volatile(
+      "{\n .reg .pred p;\n setp.ne.b32 p, %5, 0;\n"
+      " @p cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];\n}"
+      ::"r"(dst), "l"(map), "r"(x), "r"(row), "r"(bar), "r"((unsigned)me) : "memory");
+}
+KK3_DEV void gather4_1(bool me, unsigned dst, const CUtensorMap* map, int x, int r0, int r1, int r2, int r3, unsigned bar) {
+  asm volatile(
+      "{\n .reg .pred p;\n setp.ne.b32 p, %8, 0;\n"
+      " @p cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes [%0], "
+      "[%1, {%2, %3, %4, %5, %6}], [%7];\n}"
+      ::"r"(dst), "l"(map), "r"(x), "r"(r0), "r"(r1), "r"(r2), "r"(r3), "r"(bar), "r"((unsigned)me) : "memory");
+}
+
+// The two positions 2 lane, 2 lane + 1 of a unit: their pages, looked up ahead.
+struct FewIds {
+  int id[2];
+  KK3_DEV void fetch(const CachePages& c, int b, int unit, int end) {
+    const int pos = unit * kFewUnit + 2 * (threadIdx.x & 31);
+    const int* table = c.table + (long long)b * c.table_stride;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) id[i] = pos + i < end ? table[page_of(c, pos + i)] : -1;
+  }
+};
+
+// Copies of a unit's two stages, dealt out to the warps: a box of a 64-dim block each, or four rows where pages have odd
+// sizes or the tile's last position lies in the stage (what lies behind must be zeros).
+KK3_DEV void few_load(const AttendArgs& a, const PairRows& pr, const PairMaps& maps, const FewIds& ids, int unit, int end,
+                      const unsigned (&stage)[2], const unsigned (&bar)[2]) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const bool me = elect_one();
+  int kv[2], pe[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int pos = unit * kFewUnit + 2 * lane + i;
+    kv[i] = pr.kv_end;
+    pe[i] = pr.pe_end;
+    if (pos < end) {
+      if ((unsigned)ids.id[i] < (unsigned)a.c.num_pages) {
+        const int slot = pos - page_of(a.c, pos) * a.c.page_size;
+        kv[i] = ids.id[i] * pr.kv_ratio + slot;
+        pe[i] = ids.id[i] * pr.pe_ratio + slot;
+      } else {
+        cache_error(a.c);
+      }
+    }
+  }
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const int left = end - (unit * kFewUnit + h * kFewStage);
+    const bool single = pr.box == 0 || (left > 0 && left < kFewStage);
+    const int box = single ? 4 : min(pr.box, kFewStage), per = kFewStage / box;
+    if (warp == 8 * h && me) mbar_arrive_tx(bar[h], kFewStageBytes);
+    // the second stage's copies begin with the warps that the first left out
+    for (int it = (warp + 16 - 9 * h) & 15; it < kBlocks * per; it += 16) {
+      const int d = it % kBlocks, k = it / kBlocks, from = (h * kFewStage + k * box) >> 1;
+      const int r0 = __shfl_sync(0xffffffffu, d < kBlocks - 1 ? kv[0] : pe[0], from);
+      const unsigned dst = stage[h] + d * kFewBlock + k * box * 128;
+      const int x = d < kBlocks - 1 ? d * 64 : 0;
+      if (single) {
+        const int r1 = __shfl_sync(0xffffffffu, d < kBlocks - 1 ? kv[1] : pe[1], from);
+        const int r2 = __shfl_sync(0xffffffffu, d < kBlocks - 1 ? kv[0] : pe[0], from + 1);
+        const int r3 = __shfl_sync(0xffffffffu, d < kBlocks - 1 ? kv[1] : pe[1], from + 1);
+        gather4_1(me, dst, d < kBlocks - 1 ? &maps.kv_row : &maps.pe_row, x, r0, r1, r2, r3, bar[h]);
+      } else {
+        load_box1(me, dst, d < kBlocks - 1 ? &maps.kv_box : &maps.pe_box, x, r0, bar[h]);
+      }
+    }
+  }
+}
+
+__global__ void __launch_bounds__(kFewThreads, 1)
+    kk3_cache_attend_few_kernel(const AttendArgs a, const PairRows pr, const __grid_constant__ PairMaps maps) {
+  extern __shared__ __align__(1024) unsigned char smem_raw[];
+  FewCtl& ctl = *reinterpret_cast<FewCtl*>(smem_raw + kFewStages * kFewStageBytes);
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, worker = blockIdx.x;
+  const unsigned base = smem_u32(smem_raw), full = smem_u32(ctl.full);
+  volatile int* dead = &ctl.dead;
+  const AttendSplit split{kFewRows, a.heads, kFewUnit, 0};
+  if (tid == 0) {
+    for (int i = 0; i < kFewStages; ++i) mbar_init(full + 8 * i, 1);
+    ctl.dead = 0;
+    fence_mbar_init();
+  }
+  const Share sh = plan_share<kFewThreads>(a, split, worker, kFewMinUnits, smem_raw,
+                                           reinterpret_cast<long long*>(smem_raw + (kPlanBytes + 15) / 16 * 16));
+  if (tid == 0) a.meta[worker * 4 + 2] = 0;
+  if (base & 1023u) {   // dynamic shared memory begins on the swizzled blocks' boundary
+    if (tid == 0) cache_error(a.c);
+    return;
+  }
+  if (worker >= sh.workers) return;
+  int b = sh.b, t = sh.t;
+  long long at = sh.at;
+  int n = 0;   // units so far: unit n is in stages (2 n) % 6 and the next
+  bool ok = true;
+  const auto stages = [&](int unit, unsigned (&addr)[2], unsigned (&bar)[2]) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int st = (2 * unit + h) % kFewStages;
+      addr[h] = base + st * kFewStageBytes;
+      bar[h] = full + 8 * st;
+    }
+  };
+  for (; at < sh.end; ++t) {
+    Seq s = a.seq(b);
+    for (; t >= split.tiles(s); t = 0) s = a.seq(++b);
+    const int units = split.units(s, t), end = split.sees(s, t);
+    const int u0 = split.from(sh, at, units), u1 = split.to(sh, at, units);
+    const bool whole = u0 == 0 && u1 == units;
+    const int row0 = t * kFewRows, rows = min(kFewRows, s.n * a.heads - row0);
+    FewIds ids, ids1;
+    ids.fetch(a.c, b, u0, end);
+    ids1.fetch(a.c, b, u0 + 1, end);
+    __syncthreads();   // the plan, or the previous tile's readers, are done with the ring
+    fence_async_smem();
+    unsigned addr[2], bar[2];
+    stages(n, addr, bar);
+    few_load(a, pr, maps, ids, u0, end, addr, bar);
+    if (u0 + 1 < u1) {
+      stages(n + 1, addr, bar);
+      few_load(a, pr, maps, ids1, u0 + 1, end, addr, bar);
+    }
+    ids.fetch(a.c, b, u0 + 2, end);
+    // query rows into the stages of unit n + 2, which are filled later, for the warps to take their fragments; zeros
+    // below the last row
+    stages(n + 2, addr, bar);
+    for (int i = tid; i < kFewRows * (kEntry / 8); i += kFewThreads) {
+      const int r = i / (kEntry / 8), ch = i % (kEntry / 8);
+      uint4 v = {};
+      if (r < rows) {
+        const int g = row0 + r, tok = s.q0 + g / a.heads, head = g % a.heads;
+        v = *reinterpret_cast<const uint4*>(ch < kLat / 8 ? a.q_lat + tok * a.ql_tok + head * a.ql_head + ch * 8
+                                                          : a.q_pe + tok * a.qp_tok + head * a.qp_head + (ch - kLat / 8) * 8);
+      }
+      *reinterpret_cast<uint4*>(smem_raw + (addr[0] - base) + (ch >> 3) * (kFewRows * 128) + r * 128 + (((ch & 7) ^ (r & 7)) << 4)) = v;
+    }
+    __syncthreads();
+    const int ntile = warp & 7, half = warp >> 3;   // 8 positions of the unit; pairs 9 half .. + 8 of the 18 pairs of k-steps
+    unsigned qf[18][4];
+#pragma unroll
+    for (int k = 0; k < 18; ++k) {
+      const int step = half * 18 + k, r = lane & 15, ch = (step & 3) * 2 + (lane >> 4);
+      ldsm4(qf[k], addr[0] + (step >> 2) * (kFewRows * 128) + r * 128 + ((ch ^ (r & 7)) << 4));
+    }
+    fence_async_smem();   // this thread's accesses to stages that copies fill next
+    float acc[4][4] = {};
+    // softmax: row `warp`, two positions a lane
+    float m = -INFINITY, l = 0.0f;
+    const int sees = warp < rows ? s.len - s.n + (row0 + warp) / a.heads + 1 : 0;
+    for (int u = u0; u < u1; ++u, ++n) {
+      unsigned mine[2], in[2];
+      stages(n, mine, in);
+      const int use = (2 * n) / kFewStages;   // (both stages of a unit are in the same turn of the ring)
+      ok = pair_wait(a.c, in[ntile >> 2], use & 1, dead) && ok;
+      {
+        float c0[4] = {}, c1[4] = {};
+        const unsigned kb = mine[ntile >> 2] + ((ntile & 3) * 8 + (lane & 7)) * 128;
+#pragma unroll
+        for (int k = 0; k < 9; ++k) {
+          const int pair = half * 9 + k;
+          unsigned bf[4];
+          ldsm4(bf, kb + (pair >> 1) * kFewBlock + ((((pair & 1) * 4 + (lane >> 3)) ^ (lane & 7)) << 4));
+          mma_bf16(c0, qf[2 * k][0], qf[2 * k][1], qf[2 * k][2], qf[2 * k][3], bf[0], bf[1]);
+          mma_bf16(c1, qf[2 * k + 1][0], qf[2 * k + 1][1], qf[2 * k + 1][2], qf[2 * k + 1][3], bf[2], bf[3]);
+        }
+        const int r = lane >> 2, col = ntile * 8 + (lane & 3) * 2;
+        *reinterpret_cast<float2*>(&ctl.s[half][r][col]) = make_float2(c0[0] + c1[0], c0[1] + c1[1]);
+        *reinterpret_cast<float2*>(&ctl.s[half][r + 8][col]) = make_float2(c0[2] + c1[2], c0[3] + c1[3]);
+      }
+      __syncthreads();   // scores are there; every warp is done with the unit before, whose stages are filled again
+      if (u + 2 < u1) {
+        unsigned to[2], tobar[2];
+        stages(n + 2, to, tobar);
+        few_load(a, pr, maps, ids, u + 2, end, to, tobar);
+        ids.fetch(a.c, b, u + 3, end);
+      }
+      {
+        float v[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int col = i * 32 + lane;
+          v[i] = (ctl.s[0][warp][col] + ctl.s[1][warp][col]) * a.scale_log2;
+          if (u * kFewUnit + col >= sees) v[i] = -INFINITY;
+        }
+        const float top = fmaxf(m, redux_max(fmaxf(v[0], v[1]))), ref = top == -INFINITY ? 0.0f : top;
+        const float al = ex2(m - ref), p0 = ex2(v[0] - ref), p1 = ex2(v[1] - ref);
+        l = l * al + (p0 + p1);
+        m = top;
+        ctl.p[warp][lane] = f2bf(p0);
+        ctl.p[warp][32 + lane] = f2bf(p1);
+        if (lane == 0) ctl.alpha[warp] = al;
+      }
+      ok = pair_wait(a.c, in[(ntile >> 2) ^ 1], use & 1, dead) && ok;
+      __syncthreads();
+      const float a0 = ctl.alpha[lane >> 2], a1 = ctl.alpha[(lane >> 2) + 8];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        acc[i][0] *= a0;
+        acc[i][1] *= a0;
+        acc[i][2] *= a1;
+        acc[i][3] *= a1;
+      }
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        unsigned pf[4];
+        ldsm4(pf, smem_u32(&ctl.p[lane & 15][k * 16 + (lane >> 4) * 8]));
+        const int r = (k & 1) * 16 + (lane & 15);
+        const unsigned vb = mine[k >> 1] + (warp >> 1) * kFewBlock + r * 128;
+#pragma unroll
+        for (int i = 0; i < 4; i += 2) {
+          unsigned bf[4];
+          ldsm4t(bf, vb + ((((warp & 1) * 4 + i + (lane >> 4)) ^ (r & 7)) << 4));
+          mma_bf16(acc[i], pf[0], pf[1], pf[2], pf[3], bf[0], bf[1]);
+          mma_bf16(acc[i + 1], pf[0], pf[1], pf[2], pf[3], bf[2], bf[3]);
+        }
+      }
+    }
+    l = warp_sum(l);
+    if (lane == 0) {
+      ctl.m[warp] = m;
+      ctl.l[warp] = l;
+    }
+    __syncthreads();
+    const long long g = (long long)s.q0 * a.heads + row0;
+    // running sums for the join: slot 1 for the tile this worker begins and leaves, slot 0 for one it comes into
+    float* part = a.part + ((long long)worker * 2 + (u0 == 0 ? 1 : 0)) * kFewRows * kPartRow;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int r = (lane >> 2) + 8 * h;
+      if (ok && r < rows) {
+        const int dim = warp * 32 + (lane & 3) * 2;
+        const float lr = ctl.l[r], inv = lr > 0.0f || lr != lr ? 1.0f / lr : 0.0f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float x = acc[i][h * 2], y = acc[i][h * 2 + 1];
+          if (whole) *reinterpret_cast<__nv_bfloat162*>(a.out + (g + r) * kLat + dim + i * 8) = __floats2bfloat162_rn(x * inv, y * inv);
+          else *reinterpret_cast<float2*>(part + r * kPartRow + dim + i * 8) = make_float2(x, y);
+        }
+      }
+    }
+    if (ok && tid < rows) {
+      if (whole) {
+        a.lse[g + tid] = (ctl.m[tid] + log2f(ctl.l[tid])) * 0.69314718055994531f;
+      } else {
+        part[tid * kPartRow + kLat] = ctl.m[tid];
+        part[tid * kPartRow + kLat + 1] = ctl.l[tid];
+      }
+    }
+    if (ok && !whole && u0 == 0 && tid == 0) {   // the workers of this tile: up to the one that holds its last unit
+      int last = worker;
+      while (sh.total * (last + 1) / sh.workers < at + units) ++last;
+      a.meta[worker * 4] = b;
+      a.meta[worker * 4 + 1] = t;
+      a.meta[worker * 4 + 2] = last - worker + 1;
+    }
+    at += units;
+  }
+  // after a failed wait: a bounded time for the copies in flight
+  if (!ok && tid == 0)
+    for (int i = 0; i < 2 * kFewStages; ++i) mbar_wait_for(full + 8 * (i / 2), i & 1, kWaitNs / 16);
+  __syncthreads();
+}
+
+// ---------------------------------------------------------------------------------------------
 // host side
 
 static int encode_rows(CUtensorMap* map, const void* base, int cols, int64_t rows, int64_t pitch, int box) {
@@ -1050,14 +1357,19 @@ static int map_queries(CUtensorMap* map, const void* base, int cols, int64_t tok
   return encode_rows(map, base, cols, tokens * heads, head_stride, box);
 }
 
-static int pair_maps(const kk3_cache* c, const void* q_latent, int64_t ql_token, int64_t ql_head, const void* q_pe,
-                     int64_t qp_token, int64_t qp_head, int tokens, int heads, int q_box, PairMaps* m, PairRows* r) {
+// the cache's maps, in boxes of at most `most` rows
+static int cache_maps(const kk3_cache* c, int most, PairMaps* m, PairRows* r) {
   memset(m, 0, sizeof(*m));
-  r->box = 64;
+  r->box = most;
   while (c->page_size % r->box) r->box /= 2;
   if (r->box < 8) r->box = 0;
-  int rc = map_pages(&m->kv_box, &m->kv_row, &r->kv_ratio, &r->kv_end, c->kv, kLat, c, c->kv_page_stride, c->kv_row_stride, r->box);
-  if (!rc) rc = map_pages(&m->pe_box, &m->pe_row, &r->pe_ratio, &r->pe_end, c->pe, kRope, c, c->pe_page_stride, c->pe_row_stride, r->box);
+  const int rc = map_pages(&m->kv_box, &m->kv_row, &r->kv_ratio, &r->kv_end, c->kv, kLat, c, c->kv_page_stride, c->kv_row_stride, r->box);
+  return rc ? rc : map_pages(&m->pe_box, &m->pe_row, &r->pe_ratio, &r->pe_end, c->pe, kRope, c, c->pe_page_stride, c->pe_row_stride, r->box);
+}
+
+static int pair_maps(const kk3_cache* c, const void* q_latent, int64_t ql_token, int64_t ql_head, const void* q_pe,
+                     int64_t qp_token, int64_t qp_head, int tokens, int heads, int q_box, PairMaps* m, PairRows* r) {
+  int rc = cache_maps(c, 64, m, r);
   if (!rc) rc = map_queries(&m->ql, q_latent, kLat, tokens, heads, ql_token, ql_head, q_box);
   if (!rc) rc = map_queries(&m->qp, q_pe, kRope, tokens, heads, qp_token, qp_head, q_box);
   return rc;
@@ -1073,6 +1385,18 @@ int attend_pair(const kk3_cache* c, const AttendArgs& a, cudaStream_t st) {
   if (r) return r;
   kk3_cache_attend_pair_kernel<<<a.workers * 2, kPaThreads, kPaSmem, st>>>(a, pr, maps);
   return cache_cuda(cudaGetLastError(), "kk3_cache_attend_pair_kernel");
+}
+
+int attend_few(const kk3_cache* c, const AttendArgs& a, cudaStream_t st) {
+  PairMaps maps;
+  PairRows pr;
+  int r = cache_maps(c, kFewStage, &maps, &pr);
+  if (r) return r;
+  static std::atomic<bool> ready[kCacheMaxDevices];
+  r = cache_allow_smem(kk3_cache_attend_few_kernel, kFewSmem, ready, "cudaFuncSetAttribute(kk3_cache_attend_few_kernel)");
+  if (r) return r;
+  kk3_cache_attend_few_kernel<<<a.workers, kFewThreads, kFewSmem, st>>>(a, pr, maps);
+  return cache_cuda(cudaGetLastError(), "kk3_cache_attend_few_kernel");
 }
 
 // rows of a matrix instruction for the average rows of a sequence: the smallest of 32, 64, 128 and 256 that holds
