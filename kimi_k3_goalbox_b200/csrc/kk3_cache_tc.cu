@@ -1064,59 +1064,63 @@ KK3_DEV void gather4_1(bool me, unsigned dst, const CUtensorMap* map, int x, int
       ::"r"(dst), "l"(map), "r"(x), "r"(r0), "r"(r1), "r"(r2), "r"(r3), "r"(bar), "r"((unsigned)me) : "memory");
 }
 
-// The two positions 2 lane, 2 lane + 1 of a unit: their pages, looked up ahead.
-struct FewIds {
-  int id[2];
-  KK3_DEV void fetch(const CachePages& c, int b, int unit, int end) {
-    const int pos = unit * kFewUnit + 2 * (threadIdx.x & 31);
-    const int* table = c.table + (long long)b * c.table_stride;
-#pragma unroll
-    for (int i = 0; i < 2; ++i) id[i] = pos + i < end ? table[page_of(c, pos + i)] : -1;
-  }
-};
-
-// Copies of a unit's two stages, dealt out to the warps: a box of a 64-dim block each, or four rows where pages have odd
-// sizes or the tile's last position lies in the stage (what lies behind must be zeros).
-KK3_DEV void few_load(const AttendArgs& a, const PairRows& pr, const PairMaps& maps, const FewIds& ids, int unit, int end,
-                      const unsigned (&stage)[2], const unsigned (&bar)[2]) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const bool me = elect_one();
-  int kv[2], pe[2];
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int pos = unit * kFewUnit + 2 * lane + i;
-    kv[i] = pr.kv_end;
-    pe[i] = pr.pe_end;
-    if (pos < end) {
-      if ((unsigned)ids.id[i] < (unsigned)a.c.num_pages) {
-        const int slot = pos - page_of(a.c, pos) * a.c.page_size;
-        kv[i] = ids.id[i] * pr.kv_ratio + slot;
-        pe[i] = ids.id[i] * pr.pe_ratio + slot;
-      } else {
-        cache_error(a.c);
-      }
+// row numbers of the cached position `pos` of sequence `b`; at or behind `end`, or without a page: past the pool
+KK3_DEV void entry_row(const CachePages& c, const PairRows& pr, int b, int pos, int end, int* kv, int* pe) {
+  *kv = pr.kv_end;
+  *pe = pr.pe_end;
+  if (pos < end) {
+    int slot;
+    const int page = page_at(c, b, pos, &slot);
+    if (page >= 0) {
+      *kv = page * pr.kv_ratio + slot;
+      *pe = page * pr.pe_ratio + slot;
     }
   }
-#pragma unroll
+}
+// Page of position 8 lane of a unit (lanes 0 .. 7), looked up ahead; boxes begin at multiples of 8.
+KK3_DEV int few_page(const CachePages& c, int b, int unit, int end) {
+  const int lane = threadIdx.x & 31, pos = unit * kFewUnit + 8 * lane;
+  return lane < 8 && pos < end ? c.table[(long long)b * c.table_stride + page_of(c, pos)] : -1;
+}
+
+// A stage row by row: where pages have odd sizes, or the tile's last position lies in it (what lies behind must be zeros).
+KK3_DEV void few_gather(const AttendArgs& a, const PairRows& pr, const PairMaps& maps, int b, int pos0, int end, int d, unsigned dst,
+                        unsigned bar) {
+  const int lane = threadIdx.x & 31;
+  const bool me = elect_one();
+  const bool rope = d == kBlocks - 1;
+  int kv, pe;
+  entry_row(a.c, pr, b, pos0 + lane, end, &kv, &pe);
+  const int row = rope ? pe : kv;
+#pragma unroll 1
+  for (int k = 0; k < kFewStage; k += 4)
+    gather4_1(me, dst + k * 128, rope ? &maps.pe_row : &maps.kv_row, rope ? 0 : d * 64, __shfl_sync(0xffffffffu, row, k),
+              __shfl_sync(0xffffffffu, row, k + 1), __shfl_sync(0xffffffffu, row, k + 2), __shfl_sync(0xffffffffu, row, k + 3), bar);
+}
+
+// Copies of a unit's two stages (from `stage` and `bar` on): warp d < 9 brings 64-dim block d of both.
+KK3_DEV void few_load(const AttendArgs& a, const PairRows& pr, const PairMaps& maps, int b, int page, int unit, int end,
+                      unsigned stage, unsigned bar) {
+  const int lane = threadIdx.x & 31, d = threadIdx.x >> 5;
+  if (d >= kBlocks) return;
+  const bool me = elect_one(), rope = d == kBlocks - 1;
+  const int pos = unit * kFewUnit + 8 * lane;
+  int row = rope ? pr.pe_end : pr.kv_end;
+  if (lane < 8 && pos < end) {
+    if ((unsigned)page < (unsigned)a.c.num_pages) row = page * (rope ? pr.pe_ratio : pr.kv_ratio) + pos - page_of(a.c, pos) * a.c.page_size;
+    else cache_error(a.c);
+  }
+#pragma unroll 1
   for (int h = 0; h < 2; ++h) {
     const int left = end - (unit * kFewUnit + h * kFewStage);
-    const bool single = pr.box == 0 || (left > 0 && left < kFewStage);
-    const int box = single ? 4 : min(pr.box, kFewStage), per = kFewStage / box;
-    if (warp == 8 * h && me) mbar_arrive_tx(bar[h], kFewStageBytes);
-    // the second stage's copies begin with the warps that the first left out
-    for (int it = (warp + 16 - 9 * h) & 15; it < kBlocks * per; it += 16) {
-      const int d = it % kBlocks, k = it / kBlocks, from = (h * kFewStage + k * box) >> 1;
-      const int r0 = __shfl_sync(0xffffffffu, d < kBlocks - 1 ? kv[0] : pe[0], from);
-      const unsigned dst = stage[h] + d * kFewBlock + k * box * 128;
-      const int x = d < kBlocks - 1 ? d * 64 : 0;
-      if (single) {
-        const int r1 = __shfl_sync(0xffffffffu, d < kBlocks - 1 ? kv[1] : pe[1], from);
-        const int r2 = __shfl_sync(0xffffffffu, d < kBlocks - 1 ? kv[0] : pe[0], from + 1);
-        const int r3 = __shfl_sync(0xffffffffu, d < kBlocks - 1 ? kv[1] : pe[1], from + 1);
-        gather4_1(me, dst, d < kBlocks - 1 ? &maps.kv_row : &maps.pe_row, x, r0, r1, r2, r3, bar[h]);
-      } else {
-        load_box1(me, dst, d < kBlocks - 1 ? &maps.kv_box : &maps.pe_box, x, r0, bar[h]);
-      }
+    const unsigned dst = stage + h * kFewStageBytes + d * kFewBlock;
+    if (d == 0 && me) mbar_arrive_tx(bar + 8 * h, kFewStageBytes);
+    if (pr.box == 0 || (left > 0 && left < kFewStage)) {
+      few_gather(a, pr, maps, b, unit * kFewUnit + h * kFewStage, end, d, dst, bar + 8 * h);
+    } else {
+#pragma unroll 1
+      for (int k = 0; k < kFewStage; k += pr.box)
+        load_box1(me, dst + k * 128, rope ? &maps.pe_box : &maps.kv_box, rope ? 0 : d * 64, __shfl_sync(0xffffffffu, row, h * 4 + (k >> 3)), bar + 8 * h);
     }
   }
 }
@@ -1144,16 +1148,11 @@ __global__ void __launch_bounds__(kFewThreads, 1)
   if (worker >= sh.workers) return;
   int b = sh.b, t = sh.t;
   long long at = sh.at;
-  int n = 0;   // units so far: unit n is in stages (2 n) % 6 and the next
+  // the current unit's stages are `slot` and the next (a multiple of two), in turn `phase` of the ring
+  int slot = 0;
+  unsigned phase = 0;
   bool ok = true;
-  const auto stages = [&](int unit, unsigned (&addr)[2], unsigned (&bar)[2]) {
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int st = (2 * unit + h) % kFewStages;
-      addr[h] = base + st * kFewStageBytes;
-      bar[h] = full + 8 * st;
-    }
-  };
+  const auto ahead = [&](int units) { return (slot + 2 * units) % kFewStages; };   // the slot of a unit to come
   for (; at < sh.end; ++t) {
     Seq s = a.seq(b);
     for (; t >= split.tiles(s); t = 0) s = a.seq(++b);
@@ -1161,22 +1160,17 @@ __global__ void __launch_bounds__(kFewThreads, 1)
     const int u0 = split.from(sh, at, units), u1 = split.to(sh, at, units);
     const bool whole = u0 == 0 && u1 == units;
     const int row0 = t * kFewRows, rows = min(kFewRows, s.n * a.heads - row0);
-    FewIds ids, ids1;
-    ids.fetch(a.c, b, u0, end);
-    ids1.fetch(a.c, b, u0 + 1, end);
+    int page = few_page(a.c, b, u0, end);
+    const int page1 = few_page(a.c, b, u0 + 1, end);
     __syncthreads();   // the plan, or the previous tile's readers, are done with the ring
     fence_async_smem();
-    unsigned addr[2], bar[2];
-    stages(n, addr, bar);
-    few_load(a, pr, maps, ids, u0, end, addr, bar);
-    if (u0 + 1 < u1) {
-      stages(n + 1, addr, bar);
-      few_load(a, pr, maps, ids1, u0 + 1, end, addr, bar);
-    }
-    ids.fetch(a.c, b, u0 + 2, end);
-    // query rows into the stages of unit n + 2, which are filled later, for the warps to take their fragments; zeros
-    // below the last row
-    stages(n + 2, addr, bar);
+#pragma unroll 1
+    for (int i = 0; i < 2 && u0 + i < u1; ++i)
+      few_load(a, pr, maps, b, i ? page1 : page, u0 + i, end, base + ahead(i) * kFewStageBytes, full + 8 * ahead(i));
+    page = few_page(a.c, b, u0 + 2, end);
+    // query rows into the stages of the unit after the next, which are filled later, for the warps to take their
+    // fragments; zeros below the last row
+    const unsigned q_at = ahead(2) * kFewStageBytes;
     for (int i = tid; i < kFewRows * (kEntry / 8); i += kFewThreads) {
       const int r = i / (kEntry / 8), ch = i % (kEntry / 8);
       uint4 v = {};
@@ -1185,7 +1179,7 @@ __global__ void __launch_bounds__(kFewThreads, 1)
         v = *reinterpret_cast<const uint4*>(ch < kLat / 8 ? a.q_lat + tok * a.ql_tok + head * a.ql_head + ch * 8
                                                           : a.q_pe + tok * a.qp_tok + head * a.qp_head + (ch - kLat / 8) * 8);
       }
-      *reinterpret_cast<uint4*>(smem_raw + (addr[0] - base) + (ch >> 3) * (kFewRows * 128) + r * 128 + (((ch & 7) ^ (r & 7)) << 4)) = v;
+      *reinterpret_cast<uint4*>(smem_raw + q_at + (ch >> 3) * (kFewRows * 128) + r * 128 + (((ch & 7) ^ (r & 7)) << 4)) = v;
     }
     __syncthreads();
     const int ntile = warp & 7, half = warp >> 3;   // 8 positions of the unit; pairs 9 half .. + 8 of the 18 pairs of k-steps
@@ -1193,39 +1187,37 @@ __global__ void __launch_bounds__(kFewThreads, 1)
 #pragma unroll
     for (int k = 0; k < 18; ++k) {
       const int step = half * 18 + k, r = lane & 15, ch = (step & 3) * 2 + (lane >> 4);
-      ldsm4(qf[k], addr[0] + (step >> 2) * (kFewRows * 128) + r * 128 + ((ch ^ (r & 7)) << 4));
+      ldsm4(qf[k], base + q_at + (step >> 2) * (kFewRows * 128) + r * 128 + ((ch ^ (r & 7)) << 4));
     }
     fence_async_smem();   // this thread's accesses to stages that copies fill next
     float acc[4][4] = {};
     // softmax: row `warp`, two positions a lane
     float m = -INFINITY, l = 0.0f;
     const int sees = warp < rows ? s.len - s.n + (row0 + warp) / a.heads + 1 : 0;
-    for (int u = u0; u < u1; ++u, ++n) {
-      unsigned mine[2], in[2];
-      stages(n, mine, in);
-      const int use = (2 * n) / kFewStages;   // (both stages of a unit are in the same turn of the ring)
-      ok = pair_wait(a.c, in[ntile >> 2], use & 1, dead) && ok;
+    for (int u = u0; u < u1; ++u) {
+      const unsigned mine = base + slot * kFewStageBytes, in = full + 8 * slot;
+      ok = pair_wait(a.c, in + 8 * (ntile >> 2), phase, dead) && ok;
       {
-        float c0[4] = {}, c1[4] = {};
-        const unsigned kb = mine[ntile >> 2] + ((ntile & 3) * 8 + (lane & 7)) * 128;
+        float c[4][4] = {};   // four chains: a product waits for the one before it on its sums
+        const unsigned kb = mine + (ntile >> 2) * kFewStageBytes + ((ntile & 3) * 8 + (lane & 7)) * 128;
 #pragma unroll
         for (int k = 0; k < 9; ++k) {
           const int pair = half * 9 + k;
           unsigned bf[4];
           ldsm4(bf, kb + (pair >> 1) * kFewBlock + ((((pair & 1) * 4 + (lane >> 3)) ^ (lane & 7)) << 4));
-          mma_bf16(c0, qf[2 * k][0], qf[2 * k][1], qf[2 * k][2], qf[2 * k][3], bf[0], bf[1]);
-          mma_bf16(c1, qf[2 * k + 1][0], qf[2 * k + 1][1], qf[2 * k + 1][2], qf[2 * k + 1][3], bf[2], bf[3]);
+          mma_bf16(c[(k & 1) * 2], qf[2 * k][0], qf[2 * k][1], qf[2 * k][2], qf[2 * k][3], bf[0], bf[1]);
+          mma_bf16(c[(k & 1) * 2 + 1], qf[2 * k + 1][0], qf[2 * k + 1][1], qf[2 * k + 1][2], qf[2 * k + 1][3], bf[2], bf[3]);
         }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) c[0][i] = (c[0][i] + c[1][i]) + (c[2][i] + c[3][i]);
         const int r = lane >> 2, col = ntile * 8 + (lane & 3) * 2;
-        *reinterpret_cast<float2*>(&ctl.s[half][r][col]) = make_float2(c0[0] + c1[0], c0[1] + c1[1]);
-        *reinterpret_cast<float2*>(&ctl.s[half][r + 8][col]) = make_float2(c0[2] + c1[2], c0[3] + c1[3]);
+        *reinterpret_cast<float2*>(&ctl.s[half][r][col]) = make_float2(c[0][0], c[0][1]);
+        *reinterpret_cast<float2*>(&ctl.s[half][r + 8][col]) = make_float2(c[0][2], c[0][3]);
       }
       __syncthreads();   // scores are there; every warp is done with the unit before, whose stages are filled again
       if (u + 2 < u1) {
-        unsigned to[2], tobar[2];
-        stages(n + 2, to, tobar);
-        few_load(a, pr, maps, ids, u + 2, end, to, tobar);
-        ids.fetch(a.c, b, u + 3, end);
+        few_load(a, pr, maps, b, page, u + 2, end, base + ahead(2) * kFewStageBytes, full + 8 * ahead(2));
+        page = few_page(a.c, b, u + 3, end);
       }
       {
         float v[2];
@@ -1243,7 +1235,7 @@ __global__ void __launch_bounds__(kFewThreads, 1)
         ctl.p[warp][32 + lane] = f2bf(p1);
         if (lane == 0) ctl.alpha[warp] = al;
       }
-      ok = pair_wait(a.c, in[(ntile >> 2) ^ 1], use & 1, dead) && ok;
+      ok = pair_wait(a.c, in + 8 * ((ntile >> 2) ^ 1), phase, dead) && ok;
       __syncthreads();
       const float a0 = ctl.alpha[lane >> 2], a1 = ctl.alpha[(lane >> 2) + 8];
 #pragma unroll
@@ -1258,7 +1250,7 @@ __global__ void __launch_bounds__(kFewThreads, 1)
         unsigned pf[4];
         ldsm4(pf, smem_u32(&ctl.p[lane & 15][k * 16 + (lane >> 4) * 8]));
         const int r = (k & 1) * 16 + (lane & 15);
-        const unsigned vb = mine[k >> 1] + (warp >> 1) * kFewBlock + r * 128;
+        const unsigned vb = mine + (k >> 1) * kFewStageBytes + (warp >> 1) * kFewBlock + r * 128;
 #pragma unroll
         for (int i = 0; i < 4; i += 2) {
           unsigned bf[4];
@@ -1267,6 +1259,8 @@ __global__ void __launch_bounds__(kFewThreads, 1)
           mma_bf16(acc[i + 1], pf[0], pf[1], pf[2], pf[3], bf[2], bf[3]);
         }
       }
+      slot = ahead(1);
+      phase ^= slot == 0;
     }
     l = warp_sum(l);
     if (lane == 0) {
