@@ -1008,33 +1008,34 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPaThreads, 1)
 }
 
 // ---------------------------------------------------------------------------------------------
-// Attention of few rows (single tokens on one rank): a tile is 16 (token, head) rows, a unit 64 cached positions.
+// Attention of few rows (single tokens on one rank): a tile is 16 (token, head) rows, a unit 32 cached positions.
 //
 // The call is bound by the cache's bytes, so each entry comes into shared memory once, by TMA, and serves both products
-// from there at warp level (m16n8k16): 64 positions are 73.7 KB, 3200 clocks at one SM's share of HBM. 16 warps, four to
-// a scheduler, since what the work on a unit takes is latency. In the first product a warp holds the query's fragments of
-// half of the 576 dims in registers and takes 8 positions, in the second it owns 32 of the output dims. Six stages of 32
-// positions, of which a unit holds two; the warps issue the copies between them, two units ahead, and what frees a unit's
-// stages is the barrier that the next unit's scores need anyway. (Copies by cp.async with padded rows, 5 stages, took 165
-// us where these take the time noted with the launch.)
+// from there at warp level (m16n8k16): 32 positions are 36.9 KB, 1600 clocks at one SM's share of HBM. What the work on a
+// unit takes is latency, so 16 warps, four to a scheduler, run three units at a time: between two barriers they add the
+// values of one unit, take the softmax of the next and the scores of the one after it. In the first product a warp holds
+// the query's fragments of a quarter of the 576 dims in registers and takes 8 positions, in the second it owns 32 of the
+// output dims, in the softmax a row. Four more warps copy, one unit to a stage of five, and run ahead over the tiles.
+// (Copies by the 16 warps themselves, between the products, took 142 us where this takes the time noted with the launch.)
 // Probabilities are rounded to BF16 for the second product, the type that the instruction takes with BF16 latents; the
 // running sum adds them unrounded, since lse is an FP32 result.
 
-constexpr int kFewUnit = 64, kFewStage = 32, kFewStages = 6;
-constexpr int kFewThreads = 512;
-constexpr int kFewBlock = kFewStage * 128;              // 32 positions x 64 dims
+constexpr int kFewUnit = 32, kFewStages = 5;
+constexpr int kFewWork = 512, kFewCopies = 4, kFewThreads = kFewWork + 32 * kFewCopies;
+constexpr int kFewBlock = kFewUnit * 128;               // 32 positions x 64 dims
 constexpr int kFewStageBytes = kBlocks * kFewBlock;
-constexpr int kFewMinUnits = 2;
+constexpr int kFewMinUnits = 4;
+constexpr int kFewQuarter = 5;   // pairs of k-steps of a quarter of the 18: 5, 5, 4, 4
 struct FewCtl {
-  float s[2][kFewRows][kFewUnit + 2];   // scores, one part from each half of the dims
-  alignas(16) bf16 p[kFewRows][kFewUnit + 8];
-  float alpha[kFewRows], m[kFewRows], l[kFewRows];
-  unsigned long long full[kFewStages];
+  float s[2][4][kFewRows][kFewUnit + 8];   // scores of two units, a part from each quarter of the dims
+  alignas(16) bf16 p[2][kFewRows][kFewUnit + 8];
+  float alpha[2][kFewRows], m[kFewRows], l[kFewRows];
+  unsigned long long full[kFewStages], empty[kFewStages];
   int dead;
 };
 constexpr int kFewSmem = kFewStages * kFewStageBytes + (int)sizeof(FewCtl);
 static_assert(kFewSmem <= 232448, "shared memory of a CTA");
-static_assert(kFewStages * kFewStageBytes >= kPlanBytes + (kFewThreads / 32 + 4) * 8, "the plan lies in the ring");
+static_assert(kFewStages * kFewStageBytes >= kPlanBytes + 16 + (kFewThreads / 32 + 4) * 8, "the plan lies in the ring");
 
 KK3_DEV void ldsm4(unsigned (&r)[4], unsigned a) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
@@ -1044,11 +1045,18 @@ KK3_DEV void ldsm4t(unsigned (&r)[4], unsigned a) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a) : "memory");
 }
+// m16n8k16 without the order that a volatile one keeps: loads of operands may go ahead of it
+KK3_DEV void mma_free(float (&d)[4], const unsigned (&a)[4], unsigned b0, unsigned b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
 KK3_DEV float redux_max(float v) {
   float r;
   asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
   return r;
 }
+KK3_DEV void few_sync() { asm volatile("bar.sync 1, %0;" ::"n"(kFewWork) : "memory"); }
 // single-CTA copies
 KK3_DEV void load_box1(bool me, unsigned dst, const CUtensorMap* map, int x, int row, unsigned bar) {
   asm volatile(
@@ -1064,77 +1072,74 @@ KK3_DEV void gather4_1(bool me, unsigned dst, const CUtensorMap* map, int x, int
       ::"r"(dst), "l"(map), "r"(x), "r"(r0), "r"(r1), "r"(r2), "r"(r3), "r"(bar), "r"((unsigned)me) : "memory");
 }
 
-// row numbers of the cached position `pos` of sequence `b`; at or behind `end`, or without a page: past the pool
-KK3_DEV void entry_row(const CachePages& c, const PairRows& pr, int b, int pos, int end, int* kv, int* pe) {
-  *kv = pr.kv_end;
-  *pe = pr.pe_end;
-  if (pos < end) {
-    int slot;
-    const int page = page_at(c, b, pos, &slot);
-    if (page >= 0) {
-      *kv = page * pr.kv_ratio + slot;
-      *pe = page * pr.pe_ratio + slot;
-    }
+// Pages of 256 positions from `first` on, looked up ahead: position first + 8 lane and its slot in its page (boxes
+// begin at multiples of 8).
+struct FewPages {
+  int id, slot;
+  KK3_DEV void fetch(const CachePages& c, int b, int first, int end) {
+    const int pos = first + 8 * (threadIdx.x & 31), col = page_of(c, pos);
+    slot = pos - col * c.page_size;
+    id = -1;
+    if (pos < end) id = c.table[(long long)b * c.table_stride + col];
   }
-}
-// Page of position 8 lane of a unit (lanes 0 .. 7), looked up ahead; boxes begin at multiples of 8.
-KK3_DEV int few_page(const CachePages& c, int b, int unit, int end) {
-  const int lane = threadIdx.x & 31, pos = unit * kFewUnit + 8 * lane;
-  return lane < 8 && pos < end ? c.table[(long long)b * c.table_stride + page_of(c, pos)] : -1;
-}
+};
 
-// A stage row by row: where pages have odd sizes, or the tile's last position lies in it (what lies behind must be zeros).
-KK3_DEV void few_gather(const AttendArgs& a, const PairRows& pr, const PairMaps& maps, int b, int pos0, int end, int d, unsigned dst,
-                        unsigned bar) {
-  const int lane = threadIdx.x & 31;
+// A copy warp's part of a unit: every kFewCopies-th 64-dim block. Box by box where the unit lies within the tile's
+// positions, else row by row, with zeros for what lies behind (so that nothing there can reach the products).
+KK3_DEV void few_load(const AttendArgs& a, const PairRows& pr, const PairMaps& maps, int b, const FewPages& pages, int unit, int end,
+                      int part, unsigned stage, unsigned bar) {
+  const int lane = threadIdx.x & 31, pos0 = unit * kFewUnit, lane0 = (unit & 7) * 4;
   const bool me = elect_one();
-  const bool rope = d == kBlocks - 1;
-  int kv, pe;
-  entry_row(a.c, pr, b, pos0 + lane, end, &kv, &pe);
-  const int row = rope ? pe : kv;
+  if (me) mbar_arrive_tx(bar, ((kBlocks - 1 - part) / kFewCopies + 1) * kFewBlock);
+  if (pr.box && pos0 + kFewUnit <= end) {
+    const bool fine = (unsigned)pages.id < (unsigned)a.c.num_pages;
+    if (!fine && lane >= lane0 && lane < lane0 + 4) cache_error(a.c);
+    const int kv = fine ? pages.id * pr.kv_ratio + pages.slot : pr.kv_end, pe = fine ? pages.id * pr.pe_ratio + pages.slot : pr.pe_end;
 #pragma unroll 1
-  for (int k = 0; k < kFewStage; k += 4)
-    gather4_1(me, dst + k * 128, rope ? &maps.pe_row : &maps.kv_row, rope ? 0 : d * 64, __shfl_sync(0xffffffffu, row, k),
-              __shfl_sync(0xffffffffu, row, k + 1), __shfl_sync(0xffffffffu, row, k + 2), __shfl_sync(0xffffffffu, row, k + 3), bar);
-}
-
-// Copies of a unit's two stages (from `stage` and `bar` on): warp d < 9 brings 64-dim block d of both.
-KK3_DEV void few_load(const AttendArgs& a, const PairRows& pr, const PairMaps& maps, int b, int page, int unit, int end,
-                      unsigned stage, unsigned bar) {
-  const int lane = threadIdx.x & 31, d = threadIdx.x >> 5;
-  if (d >= kBlocks) return;
-  const bool me = elect_one(), rope = d == kBlocks - 1;
-  const int pos = unit * kFewUnit + 8 * lane;
-  int row = rope ? pr.pe_end : pr.kv_end;
-  if (lane < 8 && pos < end) {
-    if ((unsigned)page < (unsigned)a.c.num_pages) row = page * (rope ? pr.pe_ratio : pr.kv_ratio) + pos - page_of(a.c, pos) * a.c.page_size;
-    else cache_error(a.c);
-  }
+    for (int k = 0; k < kFewUnit; k += pr.box) {
+      const int row = __shfl_sync(0xffffffffu, kv, lane0 + (k >> 3)), rope = __shfl_sync(0xffffffffu, pe, lane0 + (k >> 3));
 #pragma unroll 1
-  for (int h = 0; h < 2; ++h) {
-    const int left = end - (unit * kFewUnit + h * kFewStage);
-    const unsigned dst = stage + h * kFewStageBytes + d * kFewBlock;
-    if (d == 0 && me) mbar_arrive_tx(bar + 8 * h, kFewStageBytes);
-    if (pr.box == 0 || (left > 0 && left < kFewStage)) {
-      few_gather(a, pr, maps, b, unit * kFewUnit + h * kFewStage, end, d, dst, bar + 8 * h);
-    } else {
+      for (int d = part; d < kBlocks - 1; d += kFewCopies) load_box1(me, stage + d * kFewBlock + k * 128, &maps.kv_box, d * 64, row, bar);
+      if (part == 0) load_box1(me, stage + (kBlocks - 1) * kFewBlock + k * 128, &maps.pe_box, 0, rope, bar);
+    }
+  } else {
+    const int pos = pos0 + lane;
+    int kv = pr.kv_end, pe = pr.pe_end;
+    if (pos < end) {
+      int slot;
+      const int page = page_at(a.c, b, pos, &slot);
+      if (page >= 0) {
+        kv = page * pr.kv_ratio + slot;
+        pe = page * pr.pe_ratio + slot;
+      }
+    }
 #pragma unroll 1
-      for (int k = 0; k < kFewStage; k += pr.box)
-        load_box1(me, dst + k * 128, rope ? &maps.pe_box : &maps.kv_box, rope ? 0 : d * 64, __shfl_sync(0xffffffffu, row, h * 4 + (k >> 3)), bar + 8 * h);
+    for (int d = part; d < kBlocks; d += kFewCopies) {
+      const bool rope = d == kBlocks - 1;
+      const int row = rope ? pe : kv;
+#pragma unroll 1
+      for (int k = 0; k < kFewUnit; k += 4)
+        gather4_1(me, stage + d * kFewBlock + k * 128, rope ? &maps.pe_row : &maps.kv_row, rope ? 0 : d * 64,
+                  __shfl_sync(0xffffffffu, row, k), __shfl_sync(0xffffffffu, row, k + 1), __shfl_sync(0xffffffffu, row, k + 2),
+                  __shfl_sync(0xffffffffu, row, k + 3), bar);
     }
   }
 }
 
 __global__ void __launch_bounds__(kFewThreads, 1)
     kk3_cache_attend_few_kernel(const AttendArgs a, const PairRows pr, const __grid_constant__ PairMaps maps) {
+  static_assert(kBlocks % kFewCopies == 1, "the rope block falls to the first copy warp");
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   FewCtl& ctl = *reinterpret_cast<FewCtl*>(smem_raw + kFewStages * kFewStageBytes);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, worker = blockIdx.x;
-  const unsigned base = smem_u32(smem_raw), full = smem_u32(ctl.full);
+  const unsigned base = smem_u32(smem_raw), full = smem_u32(ctl.full), empty = smem_u32(ctl.empty);
   volatile int* dead = &ctl.dead;
   const AttendSplit split{kFewRows, a.heads, kFewUnit, 0};
   if (tid == 0) {
-    for (int i = 0; i < kFewStages; ++i) mbar_init(full + 8 * i, 1);
+    for (int i = 0; i < kFewStages; ++i) {
+      mbar_init(full + 8 * i, kFewCopies);
+      mbar_init(empty + 8 * i, kFewWork / 32);
+    }
     ctl.dead = 0;
     fence_mbar_init();
   }
@@ -1148,163 +1153,184 @@ __global__ void __launch_bounds__(kFewThreads, 1)
   if (worker >= sh.workers) return;
   int b = sh.b, t = sh.t;
   long long at = sh.at;
-  // the current unit's stages are `slot` and the next (a multiple of two), in turn `phase` of the ring
-  int slot = 0;
+  int slot = 0;   // the ring's stage, in turn `phase`
   unsigned phase = 0;
   bool ok = true;
-  const auto ahead = [&](int units) { return (slot + 2 * units) % kFewStages; };   // the slot of a unit to come
-  for (; at < sh.end; ++t) {
-    Seq s = a.seq(b);
-    for (; t >= split.tiles(s); t = 0) s = a.seq(++b);
-    const int units = split.units(s, t), end = split.sees(s, t);
-    const int u0 = split.from(sh, at, units), u1 = split.to(sh, at, units);
-    const bool whole = u0 == 0 && u1 == units;
-    const int row0 = t * kFewRows, rows = min(kFewRows, s.n * a.heads - row0);
-    int page = few_page(a.c, b, u0, end);
-    const int page1 = few_page(a.c, b, u0 + 1, end);
-    __syncthreads();   // the plan, or the previous tile's readers, are done with the ring
+  __syncthreads();   // the plan's readers are done with the ring
+
+  if (warp >= kFewWork / 32) {
     fence_async_smem();
-#pragma unroll 1
-    for (int i = 0; i < 2 && u0 + i < u1; ++i)
-      few_load(a, pr, maps, b, i ? page1 : page, u0 + i, end, base + ahead(i) * kFewStageBytes, full + 8 * ahead(i));
-    page = few_page(a.c, b, u0 + 2, end);
-    // query rows into the stages of the unit after the next, which are filled later, for the warps to take their
-    // fragments; zeros below the last row
-    const unsigned q_at = ahead(2) * kFewStageBytes;
-    for (int i = tid; i < kFewRows * (kEntry / 8); i += kFewThreads) {
-      const int r = i / (kEntry / 8), ch = i % (kEntry / 8);
-      uint4 v = {};
-      if (r < rows) {
-        const int g = row0 + r, tok = s.q0 + g / a.heads, head = g % a.heads;
-        v = *reinterpret_cast<const uint4*>(ch < kLat / 8 ? a.q_lat + tok * a.ql_tok + head * a.ql_head + ch * 8
-                                                          : a.q_pe + tok * a.qp_tok + head * a.qp_head + (ch - kLat / 8) * 8);
+    const int part = warp - kFewWork / 32;
+    for (; at < sh.end && ok; ++t) {
+      Seq s = a.seq(b);
+      for (; t >= split.tiles(s); t = 0) s = a.seq(++b);
+      const int units = split.units(s, t), end = split.sees(s, t);
+      const int u0 = split.from(sh, at, units), u1 = split.to(sh, at, units);
+      FewPages pages, next;
+      next.fetch(a.c, b, (u0 & ~7) * kFewUnit, end);
+      for (int u = u0; u < u1 && ok; ++u) {
+        if (u == u0 || (u & 7) == 0) {
+          pages = next;
+          next.fetch(a.c, b, ((u & ~7) + 8) * kFewUnit, end);
+        }
+        ok = pair_wait(a.c, empty + 8 * slot, phase ^ 1, dead);
+        __syncwarp();
+        if (ok) few_load(a, pr, maps, b, pages, u, end, part, base + slot * kFewStageBytes, full + 8 * slot);
+        if (++slot == kFewStages) {
+          slot = 0;
+          phase ^= 1;
+        }
       }
-      *reinterpret_cast<uint4*>(smem_raw + q_at + (ch >> 3) * (kFewRows * 128) + r * 128 + (((ch & 7) ^ (r & 7)) << 4)) = v;
+      at += units;
     }
-    __syncthreads();
-    const int ntile = warp & 7, half = warp >> 3;   // 8 positions of the unit; pairs 9 half .. + 8 of the 18 pairs of k-steps
-    unsigned qf[18][4];
+    // after a failed wait: a bounded time for the copies in flight
+    if (*dead)
+      for (int i = 0; i < 2 * kFewStages; ++i) mbar_wait_for(full + 8 * (i / 2), i & 1, kWaitNs / 16);
+  } else {
+    const int ntile = warp & 3, quarter = warp >> 2;   // 8 positions of the unit; pairs quarter, quarter + 4 .. of the 18 pairs of k-steps
+    const bool fifth = quarter < 2;
+    // this lane's addresses in a stage: score operands (block quarter / 2 + 2 i for pair quarter + 4 i), values
+    const unsigned kat = (quarter >> 1) * kFewBlock + (ntile * 8 + (lane & 7)) * 128 + ((((quarter & 1) * 4 + (lane >> 3)) ^ (lane & 7)) << 4);
+    const unsigned vat = (warp >> 1) * kFewBlock + (lane & 15) * 128 + ((((warp & 1) * 4 + (lane >> 4)) ^ (lane & 7)) << 4);
+    const unsigned pat = smem_u32(&ctl.p[0][lane & 15][(lane >> 4) * 8]);
+    for (; at < sh.end; ++t) {
+      Seq s = a.seq(b);
+      for (; t >= split.tiles(s); t = 0) s = a.seq(++b);
+      const int units = split.units(s, t);
+      const int u0 = split.from(sh, at, units), u1 = split.to(sh, at, units);
+      const bool whole = u0 == 0 && u1 == units;
+      const int row0 = t * kFewRows, rows = min(kFewRows, s.n * a.heads - row0);
+      // query fragments, straight from memory; zeros below the last row
+      unsigned qf[2 * kFewQuarter][4];
 #pragma unroll
-    for (int k = 0; k < 18; ++k) {
-      const int step = half * 18 + k, r = lane & 15, ch = (step & 3) * 2 + (lane >> 4);
-      ldsm4(qf[k], base + q_at + (step >> 2) * (kFewRows * 128) + r * 128 + ((ch ^ (r & 7)) << 4));
-    }
-    fence_async_smem();   // this thread's accesses to stages that copies fill next
-    float acc[4][4] = {};
-    // softmax: row `warp`, two positions a lane
-    float m = -INFINITY, l = 0.0f;
-    const int sees = warp < rows ? s.len - s.n + (row0 + warp) / a.heads + 1 : 0;
-    for (int u = u0; u < u1; ++u) {
-      const unsigned mine = base + slot * kFewStageBytes, in = full + 8 * slot;
-      ok = pair_wait(a.c, in + 8 * (ntile >> 2), phase, dead) && ok;
-      {
+      for (int h = 0; h < 2; ++h) {
+        const int r = (lane >> 2) + 8 * h, g = row0 + r, tok = s.q0 + g / a.heads, head = g % a.heads;
+        const bf16* lat = a.q_lat + tok * a.ql_tok + head * a.ql_head + quarter * 32 + (lane & 3) * 2;
+        const bf16* rope = a.q_pe + tok * a.qp_tok + head * a.qp_head + (quarter & 1) * 32 + (lane & 3) * 2;
+#pragma unroll
+        for (int k = 0; k < 2 * kFewQuarter; ++k) {
+          const bool there = r < rows && (k < 8 || fifth);
+          const bf16* at8 = k < 8 ? lat + (k >> 1) * 128 + (k & 1) * 16 : rope + (k & 1) * 16;
+          qf[k][h] = there ? *reinterpret_cast<const unsigned*>(at8) : 0u;
+          qf[k][2 + h] = there ? *reinterpret_cast<const unsigned*>(at8 + 8) : 0u;
+        }
+      }
+      float acc[4][4] = {};
+      float m = -INFINITY, l = 0.0f;   // softmax: row `warp`, a position a lane
+      const int sees = warp < rows ? s.len - s.n + (row0 + warp) / a.heads + 1 : 0;
+      // unit u0 + i: scores, softmax, values; `in` is the stage of the unit whose scores come next, `out` of the one whose values do
+      int in = slot, out = slot;
+      const auto scores = [&](int i) {
+        ok = pair_wait(a.c, full + 8 * in, phase, dead) && ok;
+        const unsigned kb = base + in * kFewStageBytes + kat;
         float c[4][4] = {};   // four chains: a product waits for the one before it on its sums
-        const unsigned kb = mine + (ntile >> 2) * kFewStageBytes + ((ntile & 3) * 8 + (lane & 7)) * 128;
 #pragma unroll
-        for (int k = 0; k < 9; ++k) {
-          const int pair = half * 9 + k;
-          unsigned bf[4];
-          ldsm4(bf, kb + (pair >> 1) * kFewBlock + ((((pair & 1) * 4 + (lane >> 3)) ^ (lane & 7)) << 4));
-          mma_bf16(c[(k & 1) * 2], qf[2 * k][0], qf[2 * k][1], qf[2 * k][2], qf[2 * k][3], bf[0], bf[1]);
-          mma_bf16(c[(k & 1) * 2 + 1], qf[2 * k + 1][0], qf[2 * k + 1][1], qf[2 * k + 1][2], qf[2 * k + 1][3], bf[2], bf[3]);
+        for (int k = 0; k < kFewQuarter; ++k) {
+          if (k < 4 || fifth) {
+            unsigned bf[4];
+            ldsm4(bf, kb + k * 2 * kFewBlock);
+            mma_free(c[(k & 1) * 2], qf[2 * k], bf[0], bf[1]);
+            mma_free(c[(k & 1) * 2 + 1], qf[2 * k + 1], bf[2], bf[3]);
+          }
         }
 #pragma unroll
-        for (int i = 0; i < 4; ++i) c[0][i] = (c[0][i] + c[1][i]) + (c[2][i] + c[3][i]);
-        const int r = lane >> 2, col = ntile * 8 + (lane & 3) * 2;
-        *reinterpret_cast<float2*>(&ctl.s[half][r][col]) = make_float2(c[0][0], c[0][1]);
-        *reinterpret_cast<float2*>(&ctl.s[half][r + 8][col]) = make_float2(c[0][2], c[0][3]);
-      }
-      __syncthreads();   // scores are there; every warp is done with the unit before, whose stages are filled again
-      if (u + 2 < u1) {
-        few_load(a, pr, maps, b, page, u + 2, end, base + ahead(2) * kFewStageBytes, full + 8 * ahead(2));
-        page = few_page(a.c, b, u + 3, end);
-      }
-      {
-        float v[2];
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const int col = i * 32 + lane;
-          v[i] = (ctl.s[0][warp][col] + ctl.s[1][warp][col]) * a.scale_log2;
-          if (u * kFewUnit + col >= sees) v[i] = -INFINITY;
+        for (int j = 0; j < 4; ++j) c[0][j] = (c[0][j] + c[1][j]) + (c[2][j] + c[3][j]);
+        float* to = &ctl.s[i & 1][quarter][lane >> 2][ntile * 8 + (lane & 3) * 2];
+        *reinterpret_cast<float2*>(to) = make_float2(c[0][0], c[0][1]);
+        *reinterpret_cast<float2*>(to + 8 * (kFewUnit + 8)) = make_float2(c[0][2], c[0][3]);
+        if (++in == kFewStages) {
+          in = 0;
+          phase ^= 1;
         }
-        const float top = fmaxf(m, redux_max(fmaxf(v[0], v[1]))), ref = top == -INFINITY ? 0.0f : top;
-        const float al = ex2(m - ref), p0 = ex2(v[0] - ref), p1 = ex2(v[1] - ref);
-        l = l * al + (p0 + p1);
+      };
+      const auto softmax = [&](int i) {
+        float v = ((ctl.s[i & 1][0][warp][lane] + ctl.s[i & 1][1][warp][lane]) +
+                   (ctl.s[i & 1][2][warp][lane] + ctl.s[i & 1][3][warp][lane])) * a.scale_log2;
+        if ((u0 + i) * kFewUnit + lane >= sees) v = -INFINITY;
+        const float top = fmaxf(m, redux_max(v)), ref = top == -INFINITY ? 0.0f : top;
+        const float al = ex2(m - ref), p = ex2(v - ref);
+        l = l * al + p;
         m = top;
-        ctl.p[warp][lane] = f2bf(p0);
-        ctl.p[warp][32 + lane] = f2bf(p1);
-        if (lane == 0) ctl.alpha[warp] = al;
+        ctl.p[i & 1][warp][lane] = f2bf(p);
+        if (lane == 0) ctl.alpha[i & 1][warp] = al;
+      };
+      const auto values = [&](int i) {
+        const float a0 = ctl.alpha[i & 1][lane >> 2], a1 = ctl.alpha[i & 1][(lane >> 2) + 8];
+        const unsigned vb = base + out * kFewStageBytes + vat, pb = pat + (i & 1) * (kFewRows * (kFewUnit + 8) * 2);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          acc[j][0] *= a0;
+          acc[j][1] *= a0;
+          acc[j][2] *= a1;
+          acc[j][3] *= a1;
+        }
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          unsigned pf[4], b0[4], b1[4];
+          ldsm4(pf, pb + k * 32);
+          ldsm4t(b0, vb + k * 16 * 128);
+          ldsm4t(b1, (vb ^ 32u) + k * 16 * 128);
+          mma_free(acc[0], pf, b0[0], b0[1]);
+          mma_free(acc[1], pf, b0[2], b0[3]);
+          mma_free(acc[2], pf, b1[0], b1[1]);
+          mma_free(acc[3], pf, b1[2], b1[3]);
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(empty + 8 * out);
+        if (++out == kFewStages) out = 0;
+      };
+      const int n = u1 - u0;
+      scores(0);
+      few_sync();
+      for (int i = 0; i < n; ++i) {
+        softmax(i);
+        if (i > 0) values(i - 1);
+        if (i + 1 < n) scores(i + 1);
+        few_sync();
       }
-      ok = pair_wait(a.c, in + 8 * ((ntile >> 2) ^ 1), phase, dead) && ok;
-      __syncthreads();
-      const float a0 = ctl.alpha[lane >> 2], a1 = ctl.alpha[(lane >> 2) + 8];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        acc[i][0] *= a0;
-        acc[i][1] *= a0;
-        acc[i][2] *= a1;
-        acc[i][3] *= a1;
+      values(n - 1);
+      slot = in;
+      l = warp_sum(l);
+      if (lane == 0) {
+        ctl.m[warp] = m;
+        ctl.l[warp] = l;
       }
+      few_sync();
+      const long long g = (long long)s.q0 * a.heads + row0;
+      // running sums for the join: slot 1 for the tile this worker begins and leaves, slot 0 for one it comes into
+      float* part = a.part + ((long long)worker * 2 + (u0 == 0 ? 1 : 0)) * kFewRows * kPartRow;
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        unsigned pf[4];
-        ldsm4(pf, smem_u32(&ctl.p[lane & 15][k * 16 + (lane >> 4) * 8]));
-        const int r = (k & 1) * 16 + (lane & 15);
-        const unsigned vb = mine + (k >> 1) * kFewStageBytes + (warp >> 1) * kFewBlock + r * 128;
+      for (int h = 0; h < 2; ++h) {
+        const int r = (lane >> 2) + 8 * h;
+        if (ok && r < rows) {
+          const int dim = warp * 32 + (lane & 3) * 2;
+          const float lr = ctl.l[r], inv = lr > 0.0f || lr != lr ? 1.0f / lr : 0.0f;
 #pragma unroll
-        for (int i = 0; i < 4; i += 2) {
-          unsigned bf[4];
-          ldsm4t(bf, vb + ((((warp & 1) * 4 + i + (lane >> 4)) ^ (r & 7)) << 4));
-          mma_bf16(acc[i], pf[0], pf[1], pf[2], pf[3], bf[0], bf[1]);
-          mma_bf16(acc[i + 1], pf[0], pf[1], pf[2], pf[3], bf[2], bf[3]);
+          for (int i = 0; i < 4; ++i) {
+            const float x = acc[i][h * 2], y = acc[i][h * 2 + 1];
+            if (whole) *reinterpret_cast<__nv_bfloat162*>(a.out + (g + r) * kLat + dim + i * 8) = __floats2bfloat162_rn(x * inv, y * inv);
+            else *reinterpret_cast<float2*>(part + r * kPartRow + dim + i * 8) = make_float2(x, y);
+          }
         }
       }
-      slot = ahead(1);
-      phase ^= slot == 0;
-    }
-    l = warp_sum(l);
-    if (lane == 0) {
-      ctl.m[warp] = m;
-      ctl.l[warp] = l;
-    }
-    __syncthreads();
-    const long long g = (long long)s.q0 * a.heads + row0;
-    // running sums for the join: slot 1 for the tile this worker begins and leaves, slot 0 for one it comes into
-    float* part = a.part + ((long long)worker * 2 + (u0 == 0 ? 1 : 0)) * kFewRows * kPartRow;
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int r = (lane >> 2) + 8 * h;
-      if (ok && r < rows) {
-        const int dim = warp * 32 + (lane & 3) * 2;
-        const float lr = ctl.l[r], inv = lr > 0.0f || lr != lr ? 1.0f / lr : 0.0f;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float x = acc[i][h * 2], y = acc[i][h * 2 + 1];
-          if (whole) *reinterpret_cast<__nv_bfloat162*>(a.out + (g + r) * kLat + dim + i * 8) = __floats2bfloat162_rn(x * inv, y * inv);
-          else *reinterpret_cast<float2*>(part + r * kPartRow + dim + i * 8) = make_float2(x, y);
+      if (ok && tid < rows) {
+        if (whole) {
+          a.lse[g + tid] = (ctl.m[tid] + log2f(ctl.l[tid])) * 0.69314718055994531f;
+        } else {
+          part[tid * kPartRow + kLat] = ctl.m[tid];
+          part[tid * kPartRow + kLat + 1] = ctl.l[tid];
         }
       }
-    }
-    if (ok && tid < rows) {
-      if (whole) {
-        a.lse[g + tid] = (ctl.m[tid] + log2f(ctl.l[tid])) * 0.69314718055994531f;
-      } else {
-        part[tid * kPartRow + kLat] = ctl.m[tid];
-        part[tid * kPartRow + kLat + 1] = ctl.l[tid];
+      if (ok && !whole && u0 == 0 && tid == 0) {   // the workers of this tile: up to the one that holds its last unit
+        int last = worker;
+        while (sh.total * (last + 1) / sh.workers < at + units) ++last;
+        a.meta[worker * 4] = b;
+        a.meta[worker * 4 + 1] = t;
+        a.meta[worker * 4 + 2] = last - worker + 1;
       }
+      at += units;
     }
-    if (ok && !whole && u0 == 0 && tid == 0) {   // the workers of this tile: up to the one that holds its last unit
-      int last = worker;
-      while (sh.total * (last + 1) / sh.workers < at + units) ++last;
-      a.meta[worker * 4] = b;
-      a.meta[worker * 4 + 1] = t;
-      a.meta[worker * 4 + 2] = last - worker + 1;
-    }
-    at += units;
   }
-  // after a failed wait: a bounded time for the copies in flight
-  if (!ok && tid == 0)
-    for (int i = 0; i < 2 * kFewStages; ++i) mbar_wait_for(full + 8 * (i / 2), i & 1, kWaitNs / 16);
   __syncthreads();
 }
 
@@ -1384,7 +1410,7 @@ int attend_pair(const kk3_cache* c, const AttendArgs& a, cudaStream_t st) {
 int attend_few(const kk3_cache* c, const AttendArgs& a, cudaStream_t st) {
   PairMaps maps;
   PairRows pr;
-  int r = cache_maps(c, kFewStage, &maps, &pr);
+  int r = cache_maps(c, kFewUnit, &maps, &pr);
   if (r) return r;
   static std::atomic<bool> ready[kCacheMaxDevices];
   r = cache_allow_smem(kk3_cache_attend_few_kernel, kFewSmem, ready, "cudaFuncSetAttribute(kk3_cache_attend_few_kernel)");
