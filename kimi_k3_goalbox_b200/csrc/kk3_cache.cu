@@ -89,10 +89,12 @@ __global__ void __launch_bounds__(kAppendWarps * 32) kk3_cache_append_kernel(con
 }
 
 // ---------------------------------------------------------------------------------------------
-// Join of a split tile: out = sum_w 2^(m_w - m) O_w / sum_w 2^(m_w - m) l_w over the tile's workers in order. grid.x is
-// the worker that begins the tile, grid.y deals out its rows. Bound by the pieces' bytes in flight: a warp takes a row
-// of few pieces (16 dims a lane, four pieces at a time), the eight warps of a CTA share a row of many.
-constexpr int kJoinThreads = 256, kJoinFew = 8;
+// Join of split tiles: out = sum_w 2^(m_w - m) O_w / sum_w 2^(m_w - m) l_w over a tile's workers in order. Bound by the
+// pieces' bytes in flight: a warp takes a row of few pieces (16 dims a lane, four pieces at a time), the eight warps of
+// a CTA share a row of many. Every CTA finds the cut tiles among the workers' notes and takes its share of their rows,
+// so that the grid fits the GPU at once (16 CTAs for each worker, most with nothing to do, began 2.7 us later).
+constexpr int kJoinThreads = 256, kJoinFew = 8, kJoinPerSm = 3;
+static_assert(kMaxWorkers <= kJoinThreads, "a thread looks at a worker");
 
 // sums of pieces w0 .. w1 - 1 of a row, weighted; dims 4 lane + 128 j .. + 3 in sum[j]
 KK3_DEV void join_pieces(const float* first, const float* rest, long long pitch, int w0, int w1, float ref, float4 (&sum)[4]) {
@@ -114,29 +116,59 @@ KK3_DEV void join_pieces(const float* first, const float* rest, long long pitch,
   }
 }
 
-__global__ void __launch_bounds__(kJoinThreads) kk3_cache_join_kernel(const AttendArgs a, int tile_rows) {
+__global__ void __launch_bounds__(kJoinThreads, kJoinPerSm) kk3_cache_join_kernel(const AttendArgs a, int tile_rows) {
   __shared__ float4 shared_sum[kJoinThreads / 32][4][32];
-  const int worker = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  __shared__ int4 cut[kMaxWorkers];    // a worker's tile: first row among all, rows, pieces, items before it
+  __shared__ int sums[kJoinThreads / 32];
   constexpr int kWarps = kJoinThreads / 32;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   cache_follow();
-  const int n = a.meta[worker * 4 + 2];
-  if (n == 0) return;
-  const int b = a.meta[worker * 4], t = a.meta[worker * 4 + 1];
-  const Seq s = a.seq(b);
-  const int rows = (int)min((long long)tile_rows, (long long)s.n * a.heads - (long long)t * tile_rows);
-  const bool few = n <= kJoinFew;
-  const long long pitch = 2ll * tile_rows * kPartRow;   // from one worker's piece to the next one's
-  for (int row = few ? blockIdx.y * kWarps + warp : blockIdx.y; row < rows; row += gridDim.y * (few ? kWarps : 1)) {
+  // an item: a row of many pieces, or eight rows of few
+  int4 mine = tid < a.workers ? reinterpret_cast<const int4*>(a.meta)[tid] : make_int4(0, 0, 0, 0);
+  const int items = mine.z == 0 ? 0 : mine.z <= kJoinFew ? (mine.y + kWarps - 1) / kWarps : mine.y;
+  int before = items;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int u = __shfl_up_sync(0xffffffffu, before, o);
+    if (lane >= o) before += u;
+  }
+  if (lane == 31) sums[warp] = before;
+  __syncthreads();
+  int total = 0;
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) {
+    if (w < warp) before += sums[w];
+    total += sums[w];
+  }
+  mine.w = before - items;
+  if (tid < a.workers) cut[tid] = mine;
+  __syncthreads();
+  for (int item = blockIdx.x; item < total; item += gridDim.x) {
+    int worker = 0;   // the last one whose items begin at or before this one: those without any lie before it
+    for (int hi = a.workers; hi - worker > 1;) {
+      const int mid = (worker + hi) >> 1;
+      if (cut[mid].w <= item) worker = mid; else hi = mid;
+    }
+    const int g0 = cut[worker].x, rows = cut[worker].y, n = cut[worker].z;
+    const bool few = n <= kJoinFew;
+    const int row = few ? (item - cut[worker].w) * kWarps + warp : item - cut[worker].w;
+    const long long pitch = 2ll * tile_rows * kPartRow;   // from one worker's piece to the next one's
+    if (row >= rows) continue;   // some warps' rows of few pieces
     // the piece of the worker that begins the tile, and those of the workers that it continues into
     const float* first = a.part + (worker * 2ll + 1) * tile_rows * kPartRow + (long long)row * kPartRow;
     const float* rest = a.part + (worker + 1) * pitch + (long long)row * kPartRow;
-    const auto piece = [&](int w) { return w == 0 ? first : rest + (w - 1) * pitch; };
-    float top = -INFINITY;
-    for (int w = lane; w < n; w += 32) top = fmaxf(top, piece(w)[kLat]);
+    float2 ml[kMaxWorkers / 32];   // maximum and sum of pieces lane, lane + 32, ..
+    float top = -INFINITY, l = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kMaxWorkers / 32; ++i) {
+      const int w = lane + 32 * i;
+      ml[i] = w < n ? *reinterpret_cast<const float2*>((w == 0 ? first : rest + (w - 1) * pitch) + kLat) : make_float2(-INFINITY, 0.0f);
+      top = fmaxf(top, ml[i].x);
+    }
     top = warp_max(top);
     const float ref = top == -INFINITY ? 0.0f : top;
-    float l = 0.0f;
-    for (int w = lane; w < n; w += 32) l += exp2f(piece(w)[kLat] - ref) * piece(w)[kLat + 1];
+#pragma unroll
+    for (int i = 0; i < kMaxWorkers / 32; ++i) l += exp2f(ml[i].x - ref) * ml[i].y;
     l = warp_sum(l);
     float4 sum[4];
     if (few) {
@@ -161,7 +193,7 @@ __global__ void __launch_bounds__(kJoinThreads) kk3_cache_join_kernel(const Atte
       __syncthreads();
     }
     const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
-    const long long g = (long long)s.q0 * a.heads + (long long)t * tile_rows + row;
+    const long long g = g0 + row;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       if (!few && (j > 0 || warp >= 4)) break;
@@ -461,7 +493,8 @@ struct Plan {
   int workers, rows;
 };
 static Plan attend_plan(int64_t batch, int64_t tokens, int64_t heads, int sms) {
-  return tokens * heads <= kFewRows * batch ? Plan{sms, kFewRows} : Plan{sms / 2, kPairRows};
+  const int workers = sms < kMaxWorkers ? sms : kMaxWorkers;
+  return tokens * heads <= kFewRows * batch ? Plan{workers, kFewRows} : Plan{workers / 2, kPairRows};
 }
 
 extern "C" int64_t kk3_cache_attend_workspace(void) {
@@ -507,7 +540,7 @@ extern "C" int kk3_cache_attend(const kk3_cache_attend_args* x, void* stream) {
   const cudaStream_t st = (cudaStream_t)stream;
   const int r = p.rows == kFewRows ? attend_few(&x->cache, a, st) : attend_pair(&x->cache, a, st);
   if (r) return r;
-  return cache_launch_after(kk3_cache_join_kernel, dim3(p.workers, 16), kJoinThreads, st, "kk3_cache_join_kernel", a, p.rows);
+  return cache_launch_after(kk3_cache_join_kernel, dim3(kJoinPerSm * sms), kJoinThreads, st, "kk3_cache_join_kernel", a, p.rows);
 }
 
 extern "C" int kk3_cache_evict(const kk3_cache_evict_args* x, void* stream) {

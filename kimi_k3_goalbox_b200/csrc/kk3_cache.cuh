@@ -56,6 +56,9 @@ KK3_DEV int page_at(const CachePages& c, int b, int pos, int* slot) {
 
 // Wait for the kernel before this one on the stream (cache_launch_after) and see what it wrote.
 KK3_DEV void cache_follow() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+// The next kernel's CTAs may come in where there is room (they wait in cache_follow until all of this one is written).
+// Said at the start: from there to the next kernel's first instruction it takes 3.7 us.
+KK3_DEV void cache_go_on() { asm volatile("griddepcontrol.launch_dependents;"); }
 
 // A sequence of one call: its rows in the packed token arrays and its cached positions (new ones included).
 struct Seq {
@@ -68,7 +71,9 @@ struct CallSeqs {
   const int* cu_new;
   int tokens;
   int workers;   // CTAs (or CTA pairs) that share the call
-  int* meta;     // [workers][4]: sequence, tile, workers of the tile that this worker begins and leaves (0: none)
+  // [workers][4], of the tile that this worker begins and leaves: attention: its first row among all, its rows; weight:
+  // its sequence, its first position, and last the sequence's length; both: how many workers share it (0: no such tile)
+  int* meta;
   KK3_DEV Seq seq(int b) const {
     Seq s;
     const int a = min(max(cu_new[b], 0), tokens), e = min(max(cu_new[b + 1], a), tokens);
@@ -94,6 +99,7 @@ struct AttendArgs : CallSeqs {
   float* part;           // [workers][2][tile rows][kPartRow]: running sums of tiles that several workers share
 };
 constexpr int kFewRows = 16, kPairRows = 128;   // tiles of the two attention kernels
+constexpr int kMaxWorkers = 160;                // that the join keeps the statistics of in registers
 constexpr int kPartRow = kLat + 4;   // 512 sums, running maximum, running sum, padding to 16 bytes
 
 struct MassArgs : CallSeqs {
@@ -119,6 +125,8 @@ struct Share {
   long long at;      // units before the first tile
   int b, t;          // first tile: its sequence and its number within it
   int workers;       // workers that take part (this one does not when its number is not below)
+  Seq seq;           // the first tile's sequence
+  KK3_DEV int holder(long long end) const { return (int)((end * workers + total - 1) / total) - 1; }   // of the unit before `end`
 };
 
 // Attention: a tile is `rows` (token, head) rows of one sequence over the positions that its last row sees, a unit
@@ -221,6 +229,7 @@ KK3_DEV Share plan_share(const CallSeqs& a, const Split& split, int worker, int 
   sh.workers = (int)(most > a.workers ? a.workers : most);
   sh.begin = sh.end = sh.at = 0;
   sh.b = sh.t = 0;
+  sh.seq = Seq{0, 0, 0};
   if (worker >= sh.workers) return sh;
   sh.begin = sh.total * worker / sh.workers;
   sh.end = sh.total * (worker + 1) / sh.workers;
@@ -244,6 +253,7 @@ KK3_DEV Share plan_share(const CallSeqs& a, const Split& split, int worker, int 
   sh.b = (int)found[0];
   sh.t = (int)found[1];
   sh.at = found[2];
+  sh.seq = seqs[sh.b];
   __syncthreads();
   return sh;
 }

@@ -303,6 +303,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMassThreads, 1)
   const int half = rows / 2, slot_bytes = half * 128, slots = min(kMassSlots, kMassRing / slot_bytes);
   const MassSplit split{kMassPos, rows, a.heads};
   const Share sh = plan_share<kMassThreads>(a, split, worker, 1, base, ctl.red);
+  cache_go_on();
   if (tid == 0 && rank == 0) a.meta[worker * 4 + 2] = 0;
   if (worker >= sh.workers) {   // both CTAs of the pair
     mass_rest(a, tid, kMassThreads);
@@ -341,8 +342,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMassThreads, 1)
     int slot = 0, phase = 0, tile = 0, ahead_b = -1, ahead_t = -1;   // the tile whose page ids are there
     PageIds ids;
     bool ok = true;
+    Seq s = sh.seq;
     while (ok && at < sh.end) {
-      Seq s = a.seq(b);
       for (; t >= split.tiles(s); t = 0) s = a.seq(++b);
       const int units = split.units(s, t), first = split.first_unit(s, t);
       const int u0 = (int)max(0ll, sh.begin - at), u1 = (int)min((long long)units, sh.end - at);
@@ -390,8 +391,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMassThreads, 1)
       const unsigned idesc = pair_idesc(256, rows);
       int job = 0, unit = 0;
       bool ok = true;
+      Seq s = sh.seq;
       while (ok && at < sh.end) {
-        Seq s = a.seq(b);
         for (; t >= split.tiles(s); t = 0) s = a.seq(++b);
         const int units = split.units(s, t);
         const int u0 = (int)max(0ll, sh.begin - at), u1 = (int)min((long long)units, sh.end - at);
@@ -426,8 +427,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMassThreads, 1)
     const int group = warp >> 2, row = tid & 127;
     int unit = 0;
     bool ok = true;
+    Seq s = sh.seq;
     while (at < sh.end) {   // after a failed wait the rounds go on without work: the warps meet at barriers
-      Seq s = a.seq(b);
       for (; t >= split.tiles(s); t = 0) s = a.seq(++b);
       const int units = split.units(s, t), first = split.first_unit(s, t);
       const int u0 = (int)max(0ll, sh.begin - at), u1 = (int)min((long long)units, sh.end - at);
@@ -493,12 +494,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMassThreads, 1)
           }
         } else {
           a.part[(worker * 2 + (u0 == 0 ? 1 : 0)) * kMassPos + rank * 128 + row] = sum;
-          if (u0 == 0 && tid == 0 && rank == 0) {   // the workers of this tile: up to the one that holds its last unit
-            int last = worker;
-            while (sh.total * (last + 1) / sh.workers < at + units) ++last;
+          if (u0 == 0 && tid == 0 && rank == 0) {
             a.meta[worker * 4] = b;
-            a.meta[worker * 4 + 1] = t;
-            a.meta[worker * 4 + 2] = last - worker + 1;
+            a.meta[worker * 4 + 1] = t * kMassPos;
+            a.meta[worker * 4 + 2] = sh.holder(at + units) - worker + 1;
+            a.meta[worker * 4 + 3] = s.len;
           }
         }
       }
@@ -516,8 +516,8 @@ __global__ void __launch_bounds__(kMassPos) kk3_cache_mass_join_kernel(const Mas
   cache_follow();
   const int worker = blockIdx.x, n = a.meta[worker * 4 + 2];
   if (n == 0) return;
-  const int b = a.meta[worker * 4], pos = a.meta[worker * 4 + 1] * kMassPos + threadIdx.x;
-  if (pos >= a.seq(b).len) return;
+  const int b = a.meta[worker * 4], pos = a.meta[worker * 4 + 1] + threadIdx.x;
+  if (pos >= a.meta[worker * 4 + 3]) return;
   float sum = 0.0f;
 #pragma unroll 4
   for (int w = 0; w < n; ++w) sum += a.part[((worker + w) * 2 + (w == 0 ? 1 : 0)) * kMassPos + threadIdx.x];
@@ -629,6 +629,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPaThreads, 1)
   cluster_arrive();   // the peer's barriers are needed after the plan
   const AttendSplit split{kPairRows, a.heads, kPaUnit, kPaTileCost};
   const Share sh = plan_share<kPaThreads>(a, split, worker, kPaMinUnits, smem_raw, ctl.red);
+  cache_go_on();
   if (tid == 0 && rank == 0) a.meta[worker * 4 + 2] = 0;
   tc_fence_before();
   __syncthreads();
@@ -650,8 +651,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPaThreads, 1)
     const bool me = elect_one();
     with_box(pr.box, [&](auto box) {
       int slot = 0, phase = 0;
+      Seq s = sh.seq;
       for (; ok && at < sh.end; ++t, ++tile) {
-        Seq s = a.seq(b);
         for (; t >= split.tiles(s); t = 0) s = a.seq(++b);
         const int units = split.units(s, t), end = split.sees(s, t);
         const int u0 = split.from(sh, at, units), u1 = split.to(sh, at, units);
@@ -704,16 +705,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPaThreads, 1)
     __syncwarp();
   } else if (warp == 10) {
     // ---- the entries' pieces for the sums: piece (g, h) is dims 256 h + 128 rank .. + 127 of positions 64 g .. + 63 of
-    // the unit. Positions that no row sees must be zeros, whatever the page holds there: a group that `end` cuts comes
-    // row by row.
+    // the unit. Positions behind the sequence's end must be zeros, whatever the page holds there: a group that the end cuts
+    // comes row by row (3.4 us; the entries of tokens that come after the tile's have values and weights of zero).
     const unsigned lead_v = in_cta(vfull, 0);
     const bool me = elect_one();
     with_box(pr.box, [&](auto box) {
       int slot = 0, phase = 0;
+      Seq s = sh.seq;
       for (; ok && at < sh.end; ++t) {
-        Seq s = a.seq(b);
         for (; t >= split.tiles(s); t = 0) s = a.seq(++b);
-        const int units = split.units(s, t), end = split.sees(s, t);
+        const int units = split.units(s, t), end = s.len;
         const int u0 = split.from(sh, at, units), u1 = split.to(sh, at, units);
         if (u0 == u1) break;
         PageIds ids;
@@ -765,8 +766,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPaThreads, 1)
     // unrolled over the slots and the descriptors are sums of 16-byte offsets.
     if (lane == 0 && rank == 0) {
       constexpr unsigned id_s = pair_idesc(128, 256), id_o = id_s | (1u << 16);   // values are MN-major
+      Seq s = sh.seq;
       for (; ok && at < sh.end; ++t, ++tile) {
-        Seq s = a.seq(b);
         for (; t >= split.tiles(s); t = 0) s = a.seq(++b);
         const int units = split.units(s, t);
         const int u0 = split.from(sh, at, units), u1 = split.to(sh, at, units);
@@ -835,8 +836,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPaThreads, 1)
       return __all_sync(0xffffffffu, m == 0 || pair_wait(a.c, pvdone + 8 * ((m - 1) & 1), ((m - 1) >> 1) & 1, dead)) != 0;
     };
     const float sign = a.scale_log2 < 0.0f ? -1.0f : 1.0f, size = fabsf(a.scale_log2);
+    Seq s = sh.seq;
     for (; at < sh.end; ++t) {
-      Seq s = a.seq(b);
       for (; t >= split.tiles(s); t = 0) s = a.seq(++b);
       const int units = split.units(s, t);
       const int u0 = split.from(sh, at, units), u1 = split.to(sh, at, units);
@@ -989,12 +990,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPaThreads, 1)
           part[kLat + 1] = l;
         }
       }
-      if (ok && u0 == 0 && u1 < units && tid == 0 && rank == 0) {   // the workers of this tile: up to its last unit's
-        int last = worker;
-        while (sh.total * (last + 1) / sh.workers < at + kPaTileCost + units) ++last;
-        a.meta[worker * 4] = b;
-        a.meta[worker * 4 + 1] = t;
-        a.meta[worker * 4 + 2] = last - worker + 1;
+      if (ok && u0 == 0 && u1 < units && tid == 0 && rank == 0) {
+        a.meta[worker * 4] = s.q0 * a.heads + t * kPairRows;
+        a.meta[worker * 4 + 1] = min(kPairRows, s.n * a.heads - t * kPairRows);
+        a.meta[worker * 4 + 2] = sh.holder(at + kPaTileCost + units) - worker + 1;
       }
       at += units + kPaTileCost;
       tc_fence_before();   // TMEM is read before the next tile's first sums, which wait for its probabilities
@@ -1015,19 +1014,20 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPaThreads, 1)
 // unit takes is latency, so 16 warps, four to a scheduler, run three units at a time: between two barriers they add the
 // values of one unit, take the softmax of the next and the scores of the one after it. In the first product a warp holds
 // the query's fragments of a quarter of the 576 dims in registers and takes 8 positions, in the second it owns 32 of the
-// output dims, in the softmax a row. Four more warps copy, one unit to a stage of five, and run ahead over the tiles.
+// output dims, in the softmax a row. Four more warps copy, one unit to a stage of six, and run ahead over the tiles.
 // (Copies by the 16 warps themselves, between the products, took 142 us where this takes the time noted with the launch.)
 // Probabilities are rounded to BF16 for the second product, the type that the instruction takes with BF16 latents; the
 // running sum adds them unrounded, since lse is an FP32 result.
 
-constexpr int kFewUnit = 32, kFewStages = 5;
+constexpr int kFewUnit = 32, kFewStages = 6;
 constexpr int kFewWork = 512, kFewCopies = 4, kFewThreads = kFewWork + 32 * kFewCopies;
 constexpr int kFewBlock = kFewUnit * 128;               // 32 positions x 64 dims
 constexpr int kFewStageBytes = kBlocks * kFewBlock;
 constexpr int kFewMinUnits = 4;
 constexpr int kFewQuarter = 5;   // pairs of k-steps of a quarter of the 18: 5, 5, 4, 4
 struct FewCtl {
-  float s[2][4][kFewRows][kFewUnit + 8];   // scores of two units, a part from each quarter of the dims
+  // scores of a unit, a part from each quarter of the dims; column c of row r at c ^ 8 (r % 4)
+  float s[4][kFewRows][kFewUnit];
   alignas(16) bf16 p[2][kFewRows][kFewUnit + 8];
   float alpha[2][kFewRows], m[kFewRows], l[kFewRows];
   unsigned long long full[kFewStages], empty[kFewStages];
@@ -1145,6 +1145,7 @@ __global__ void __launch_bounds__(kFewThreads, 1)
   }
   const Share sh = plan_share<kFewThreads>(a, split, worker, kFewMinUnits, smem_raw,
                                            reinterpret_cast<long long*>(smem_raw + (kPlanBytes + 15) / 16 * 16));
+  cache_go_on();
   if (tid == 0) a.meta[worker * 4 + 2] = 0;
   if (base & 1023u) {   // dynamic shared memory begins on the swizzled blocks' boundary
     if (tid == 0) cache_error(a.c);
@@ -1161,8 +1162,8 @@ __global__ void __launch_bounds__(kFewThreads, 1)
   if (warp >= kFewWork / 32) {
     fence_async_smem();
     const int part = warp - kFewWork / 32;
+    Seq s = sh.seq;
     for (; at < sh.end && ok; ++t) {
-      Seq s = a.seq(b);
       for (; t >= split.tiles(s); t = 0) s = a.seq(++b);
       const int units = split.units(s, t), end = split.sees(s, t);
       const int u0 = split.from(sh, at, units), u1 = split.to(sh, at, units);
@@ -1193,8 +1194,8 @@ __global__ void __launch_bounds__(kFewThreads, 1)
     const unsigned kat = (quarter >> 1) * kFewBlock + (ntile * 8 + (lane & 7)) * 128 + ((((quarter & 1) * 4 + (lane >> 3)) ^ (lane & 7)) << 4);
     const unsigned vat = (warp >> 1) * kFewBlock + (lane & 15) * 128 + ((((warp & 1) * 4 + (lane >> 4)) ^ (lane & 7)) << 4);
     const unsigned pat = smem_u32(&ctl.p[0][lane & 15][(lane >> 4) * 8]);
+    Seq s = sh.seq;
     for (; at < sh.end; ++t) {
-      Seq s = a.seq(b);
       for (; t >= split.tiles(s); t = 0) s = a.seq(++b);
       const int units = split.units(s, t);
       const int u0 = split.from(sh, at, units), u1 = split.to(sh, at, units);
@@ -1220,10 +1221,12 @@ __global__ void __launch_bounds__(kFewThreads, 1)
       const int sees = warp < rows ? s.len - s.n + (row0 + warp) / a.heads + 1 : 0;
       // unit u0 + i: scores, softmax, values; `in` is the stage of the unit whose scores come next, `out` of the one whose values do
       int in = slot, out = slot;
-      const auto scores = [&](int i) {
+      float c[4][4];
+      const auto scores = [&]() {
         ok = pair_wait(a.c, full + 8 * in, phase, dead) && ok;
         const unsigned kb = base + in * kFewStageBytes + kat;
-        float c[4][4] = {};   // four chains: a product waits for the one before it on its sums
+#pragma unroll
+        for (int j = 0; j < 16; ++j) c[j >> 2][j & 3] = 0.0f;   // four chains: a product waits for the one before it on its sums
 #pragma unroll
         for (int k = 0; k < kFewQuarter; ++k) {
           if (k < 4 || fifth) {
@@ -1235,17 +1238,20 @@ __global__ void __launch_bounds__(kFewThreads, 1)
         }
 #pragma unroll
         for (int j = 0; j < 4; ++j) c[0][j] = (c[0][j] + c[1][j]) + (c[2][j] + c[3][j]);
-        float* to = &ctl.s[i & 1][quarter][lane >> 2][ntile * 8 + (lane & 3) * 2];
-        *reinterpret_cast<float2*>(to) = make_float2(c[0][0], c[0][1]);
-        *reinterpret_cast<float2*>(to + 8 * (kFewUnit + 8)) = make_float2(c[0][2], c[0][3]);
         if (++in == kFewStages) {
           in = 0;
           phase ^= 1;
         }
       };
+      const auto put_scores = [&]() {
+        float* to = &ctl.s[quarter][lane >> 2][(ntile * 8 + (lane & 3) * 2) ^ ((lane >> 2 & 3) << 3)];
+        *reinterpret_cast<float2*>(to) = make_float2(c[0][0], c[0][1]);
+        *reinterpret_cast<float2*>(to + 8 * kFewUnit) = make_float2(c[0][2], c[0][3]);
+      };
       const auto softmax = [&](int i) {
-        float v = ((ctl.s[i & 1][0][warp][lane] + ctl.s[i & 1][1][warp][lane]) +
-                   (ctl.s[i & 1][2][warp][lane] + ctl.s[i & 1][3][warp][lane])) * a.scale_log2;
+        const float* from = &ctl.s[0][warp][lane ^ ((warp & 3) << 3)];
+        constexpr int kPart = kFewRows * kFewUnit;
+        float v = ((from[0] + from[kPart]) + (from[2 * kPart] + from[3 * kPart])) * a.scale_log2;
         if ((u0 + i) * kFewUnit + lane >= sees) v = -INFINITY;
         const float top = fmaxf(m, redux_max(v)), ref = top == -INFINITY ? 0.0f : top;
         const float al = ex2(m - ref), p = ex2(v - ref);
@@ -1280,13 +1286,18 @@ __global__ void __launch_bounds__(kFewThreads, 1)
         if (++out == kFewStages) out = 0;
       };
       const int n = u1 - u0;
-      scores(0);
+      scores();
+      put_scores();
       few_sync();
       for (int i = 0; i < n; ++i) {
         softmax(i);
         if (i > 0) values(i - 1);
-        if (i + 1 < n) scores(i + 1);
-        few_sync();
+        if (i + 1 < n) scores();
+        few_sync();   // the unit's scores are read, its probabilities written
+        if (i + 1 < n) {
+          put_scores();
+          few_sync();
+        }
       }
       values(n - 1);
       slot = in;
@@ -1321,12 +1332,10 @@ __global__ void __launch_bounds__(kFewThreads, 1)
           part[tid * kPartRow + kLat + 1] = ctl.l[tid];
         }
       }
-      if (ok && !whole && u0 == 0 && tid == 0) {   // the workers of this tile: up to the one that holds its last unit
-        int last = worker;
-        while (sh.total * (last + 1) / sh.workers < at + units) ++last;
-        a.meta[worker * 4] = b;
-        a.meta[worker * 4 + 1] = t;
-        a.meta[worker * 4 + 2] = last - worker + 1;
+      if (ok && !whole && u0 == 0 && tid == 0) {
+        a.meta[worker * 4] = (int)g;
+        a.meta[worker * 4 + 1] = rows;
+        a.meta[worker * 4 + 2] = sh.holder(at + units) - worker + 1;
       }
       at += units;
     }
