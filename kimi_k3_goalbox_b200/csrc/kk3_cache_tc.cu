@@ -714,7 +714,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPaThreads, 1)
       Seq s = sh.seq;
       for (; ok && at < sh.end; ++t) {
         for (; t >= split.tiles(s); t = 0) s = a.seq(++b);
-        const int units = split.units(s, t), end = s.len;
+        const int units = split.units(s, t), end = min(s.len, (split.sees(s, t) + 63) & ~63);
         const int u0 = split.from(sh, at, units), u1 = split.to(sh, at, units);
         if (u0 == u1) break;
         PageIds ids;
@@ -769,7 +769,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPaThreads, 1)
       Seq s = sh.seq;
       for (; ok && at < sh.end; ++t, ++tile) {
         for (; t >= split.tiles(s); t = 0) s = a.seq(++b);
-        const int units = split.units(s, t);
+        const int units = split.units(s, t), sees = split.sees(s, t);
         const int u0 = split.from(sh, at, units), u1 = split.to(sh, at, units);
         if (u0 == u1) break;
         if (warp == 9) {
@@ -805,9 +805,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPaThreads, 1)
               if (!ok) break;
               tc_fence_after();
               const unsigned long long va = vd + slot * (kPaBlock >> 4);
+              if (i < 2 || u * kPaUnit + (i >> 1) * 64 < sees) {   // a unit's first group always: it sets the sums
 #pragma unroll
-              for (int k = 0; k < 4; ++k)
-                pair_mma(tmem + (i & 1) * 128, pd + (i >> 1) * (kPaQBlock >> 4) + k * 2, va + k * 128, id_o, (unsigned)(u > u0 || i > 1 || k));
+                for (int k = 0; k < 4; ++k)
+                  pair_mma(tmem + (i & 1) * 128, pd + (i >> 1) * (kPaQBlock >> 4) + k * 2, va + k * 128, id_o, (unsigned)(u > u0 || i > 1 || k));
+              }
               pair_commit(vempty + 8 * slot);
               if (i & 1) pair_commit(pfree + 4 * (i - 1));
             }
