@@ -81,6 +81,7 @@ def _explain(device, *expected) -> None:
         if t.dtype != dtype or (shape is not None and t.shape != shape):
             raise ValueError(f"{name} must be {dtype}{'' if shape is None else ' ' + str(list(shape))}, not {t.dtype} "
                              f"{list(t.shape)}")
+    for t, name, _, _, contiguous in expected:
         if not t.is_cuda:
             raise ValueError(f"{name} must be on a CUDA device (sm_100a kernels, no CPU path)")
         if t.get_device() != device:
@@ -120,7 +121,7 @@ def _cache(kv, pe, table):
     p0, p1, p2 = pe.stride()
     # the stride of a dim of one element means nothing
     if page == 1:
-        k1, p1 = LATENT, ROPE
+        k1, p1 = (k0, p0) if pages > 1 else (LATENT, ROPE)
     if pages == 1:
         k0, p0 = page * k1, page * p1
     if (k2 != 1 or p2 != 1 or (kv_at | pe_at) & 15 or (k0 | k1 | p0 | p1) & 7 or k1 < LATENT or p1 < ROPE or k0 < 0 or p0 < 0
@@ -309,6 +310,9 @@ def attention_mass(q_latent, q_pe, lse, kv, pe, table, lengths, cu_new, *, scale
         out = torch.empty((B, capacity), dtype=_F32, device=device)
     elif out.dtype != _F32 or out.shape != (B, capacity) or out.get_device() != dev or not out.is_contiguous():
         raise ValueError(f"out must be contiguous float32 {[B, capacity]} on the cache's device")
+    elif mass is not None and (before != (to := out.data_ptr()) or row != capacity) and to < before + 4 * ((B - 1) * row + capacity) \
+            and before < to + 4 * B * capacity:
+        raise ValueError("out may be mass itself, but must not overlap it in another way")
     work, nbytes = _workspace("kk3_cache_mass_workspace", device)
     _run("kk3_cache_mass", dev, _MASS.pack(*cache, *q, lse.data_ptr(), lengths.data_ptr(), cu_new.data_ptr(), before, row,
                                            out.data_ptr(), work.data_ptr(), nbytes, _error(error_word, dev), T, H, scale, 0))
