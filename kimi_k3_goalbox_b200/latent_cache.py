@@ -40,6 +40,7 @@ _EVICT = struct.Struct("=" + _CACHE + "QQqQqQQQQiiii")
 _LIB = None
 _WORKSPACE: dict = {}       # (operator, device index) -> bytes, the same for every call on a device
 _raw_stream = torch._C._cuda_getCurrentRawStream    # current_stream(device).cuda_stream without the Stream object
+_current_device = torch.cuda.current_device
 
 
 def _lib() -> ctypes.CDLL:
@@ -148,8 +149,10 @@ def _error(error_word, device: int) -> int:
 def _query_rows(t):
     """(tensor, token stride, head stride) of queries [T, heads, n] whose (token, head) rows lie at one pitch, 16-byte
     aligned, as the kernels' copies need; others are copied into that form."""
-    s0, s1, s2 = t.stride()
     n0, n1, n2 = t.shape
+    if t.is_contiguous() and not t.data_ptr() & 15:
+        return t, n1 * n2, n2
+    s0, s1, s2 = t.stride()
     if n1 == 1:
         s1 = n2 if n0 == 1 else s0
     if s2 != 1 or s1 < n2 or s1 % 8 or (n0 > 1 and s0 != n1 * s1) or t.data_ptr() % 16:
@@ -203,7 +206,7 @@ def _mass_stride(mass, name: str, dev: int, B: int, capacity: int) -> int:
 def _run(what: str, dev: int, args: bytes) -> None:
     """Call a C entry point on the cache's device and its current stream."""
     fn = getattr(_LIB or _lib(), what)
-    if torch.cuda.current_device() == dev:
+    if _current_device() == dev:
         rc = fn(args, _raw_stream(dev))
     else:
         with torch.cuda.device(dev):
@@ -276,11 +279,11 @@ def attend(q_latent, q_pe, kv, pe, table, lengths, cu_new, *, scale: float | Non
     T, H, scale, _keep, q = _queries(q_latent, q_pe, lengths, cu_new, dev, B, scale)
     device = kv.device
     if out is None:
-        out = torch.empty((T, H, LATENT), dtype=_BF16, device=device)
+        out = torch.empty_like(q_latent) if q_latent.is_contiguous() else torch.empty(T, H, LATENT, dtype=_BF16, device=device)
     elif out.dtype != _BF16 or out.shape != (T, H, LATENT) or out.get_device() != dev or not out.is_contiguous() or out.data_ptr() % 16:
         raise ValueError(f"out must be contiguous bfloat16 {[T, H, LATENT]} on the cache's device, 16-byte aligned")
     if lse is None:
-        lse = torch.empty((T, H), dtype=_F32, device=device)
+        lse = torch.empty(T, H, dtype=_F32, device=device)
     elif lse.dtype != _F32 or lse.shape != (T, H) or lse.get_device() != dev or not lse.is_contiguous():
         raise ValueError(f"lse must be contiguous float32 {[T, H]} on the cache's device")
     err = _error(error_word, dev)
@@ -307,7 +310,7 @@ def attention_mass(q_latent, q_pe, lse, kv, pe, table, lengths, cu_new, *, scale
         row, before = _mass_stride(mass, "mass", dev, B, capacity), mass.data_ptr()
     device = kv.device
     if out is None:
-        out = torch.empty((B, capacity), dtype=_F32, device=device)
+        out = torch.empty(B, capacity, dtype=_F32, device=device)
     elif out.dtype != _F32 or out.shape != (B, capacity) or out.get_device() != dev or not out.is_contiguous():
         raise ValueError(f"out must be contiguous float32 {[B, capacity]} on the cache's device")
     elif mass is not None and (before != (to := out.data_ptr()) or row != capacity) and to < before + 4 * ((B - 1) * row + capacity) \
@@ -353,8 +356,8 @@ def evict(kv, pe, table, lengths, mass, budget: int, *, sinks: int = 0, recent: 
         dst, dst_row = dst_table.data_ptr(), dst_row if B > 1 else dst_columns
     device = kv.device
     new_lengths = torch.empty_like(lengths)
-    new_mass = torch.empty((B, capacity), dtype=_F32, device=device)
-    kept = torch.empty((B, budget), dtype=_I32, device=device)
+    new_mass = torch.empty(B, capacity, dtype=_F32, device=device)
+    kept = torch.empty(B, budget, dtype=_I32, device=device)
     _run("kk3_cache_evict", dev, _EVICT.pack(*cache, lengths.data_ptr(), mass.data_ptr(), row, dst, dst_row,
                                              new_lengths.data_ptr(), new_mass.data_ptr(), kept.data_ptr(),
                                              _error(error_word, dev), budget, sinks, recent, dst_columns))
