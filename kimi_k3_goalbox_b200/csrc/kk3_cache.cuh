@@ -159,17 +159,23 @@ struct MassSplit {
   KK3_DEV int size(const Seq& s, int t) const { return units(s, t); }
 };
 
+// inclusive sums over the lanes of a warp
+template <class T>
+KK3_DEV T lane_sums(T v) {
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const T u = __shfl_up_sync(0xffffffffu, v, o);
+    if ((threadIdx.x & 31) >= o) v += u;
+  }
+  return v;
+}
+
 // Sum over the threads of a block of NT (a multiple of 32) threads before this one; *total over all of them. `red`
 // is shared memory of NT / 32 + 1 long longs.
 template <int NT>
 KK3_DEV long long block_scan(long long mine, long long* red, long long* total) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  long long v = mine;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const long long u = __shfl_up_sync(0xffffffffu, v, o);
-    if (lane >= o) v += u;
-  }
+  const long long v = lane_sums(mine);
   __syncthreads();
   if (lane == 31) red[warp] = v;
   __syncthreads();
@@ -183,11 +189,84 @@ KK3_DEV long long block_scan(long long mine, long long* red, long long* total) {
   return before;
 }
 
+// The worker's part of `total` units: false if it has none. A worker takes min_units units at least: shorter pieces cost
+// more to join than they save.
+KK3_DEV bool plan_part(Share& sh, long long total, int worker, int min_units, int workers) {
+  const long long most = (total + min_units - 1) / min_units;
+  sh.total = total;
+  sh.workers = (int)(most > workers ? workers : most);
+  sh.begin = sh.end = sh.at = 0;
+  sh.b = sh.t = 0;
+  sh.seq = Seq{0, 0, 0};
+  if (worker >= sh.workers) return false;
+  if (total < 1 << 22) {   // 32-bit divisions: the 64-bit ones take 600 clocks
+    sh.begin = (unsigned)total * (unsigned)worker / (unsigned)sh.workers;
+    sh.end = (unsigned)total * (unsigned)(worker + 1) / (unsigned)sh.workers;
+  } else {
+    sh.begin = total * worker / sh.workers;
+    sh.end = total * (worker + 1) / sh.workers;
+  }
+  return true;
+}
+
+// The plan of up to 128 sequences of up to 32 tiles each, by every warp for itself, four sequences a lane; false: there
+// are more. (A plan by the whole CTA has four barriers and takes 4700 clocks where this takes 1500, a third of the
+// time of a small call.)
+constexpr int kPlanDeep = 4;
+template <class Split>
+KK3_DEV bool plan_small(const CallSeqs& a, const Split& split, int worker, int min_units, Share& sh) {
+  const int lane = threadIdx.x & 31, B = a.c.batch;
+  if (B > 32 * kPlanDeep) return false;
+  const int per = (B + 31) / 32, lo = lane * per;
+  Seq s[kPlanDeep];
+  long long size[kPlanDeep], mine = 0;
+  bool small = true;
+#pragma unroll
+  for (int i = 0; i < kPlanDeep; ++i) {
+    s[i] = i < per && lo + i < B ? a.seq(lo + i) : Seq{0, 0, 0};
+    small = small && split.tiles(s[i]) <= 32;
+  }
+  if (!__all_sync(0xffffffffu, small)) return false;
+#pragma unroll
+  for (int i = 0; i < kPlanDeep; ++i) {
+    size[i] = 0;
+    const int tiles = split.tiles(s[i]);
+    for (int t = 0; t < tiles; ++t) size[i] += split.size(s[i], t);
+    mine += size[i];
+  }
+  const long long incl = lane_sums(mine);
+  if (!plan_part(sh, __shfl_sync(0xffffffffu, incl, 31), worker, min_units, a.workers)) return true;
+  // the sequence: of the first lane whose units end behind `begin`, and there the first one
+  long long u = incl - mine;
+  int i = 0;
+  Seq mine_seq = s[0];
+#pragma unroll
+  for (int k = 0; k + 1 < kPlanDeep; ++k)
+    if (i == k && u + size[k] <= sh.begin) {
+      u += size[k];
+      i = k + 1;
+      mine_seq = s[k + 1];
+    }
+  const int from = __ffs(__ballot_sync(0xffffffffu, incl > sh.begin)) - 1;
+  sh.b = from * per + __shfl_sync(0xffffffffu, i, from);
+  u = __shfl_sync(0xffffffffu, u, from);
+  sh.seq = Seq{__shfl_sync(0xffffffffu, mine_seq.q0, from), __shfl_sync(0xffffffffu, mine_seq.n, from),
+               __shfl_sync(0xffffffffu, mine_seq.len, from)};
+  // its tile: lane t looks at tile t
+  const int k = lane < split.tiles(sh.seq) ? split.size(sh.seq, lane) : 0;
+  u += lane_sums(k);
+  sh.t = __ffs(__ballot_sync(0xffffffffu, u > sh.begin)) - 1;
+  sh.at = __shfl_sync(0xffffffffu, u - k, sh.t);
+  return true;
+}
+
 // Computed by every CTA for itself; all NT threads take part. `room` is shared memory of kPlanBytes, `red` of
-// NT / 32 + 4 long longs. A worker takes min_units units at least: shorter pieces cost more to join than they save.
+// NT / 32 + 4 long longs.
 constexpr int kPlanBytes = kMaxSeqs * (int)sizeof(Seq) + (kMaxSeqs + 1) * 4;
 template <int NT, class Split>
 KK3_DEV Share plan_share(const CallSeqs& a, const Split& split, int worker, int min_units, void* room, long long* red) {
+  Share sh;
+  if (plan_small(a, split, worker, min_units, sh)) return sh;
   const int tid = threadIdx.x, B = a.c.batch;
   Seq* seqs = reinterpret_cast<Seq*>(room);
   int* prefix = reinterpret_cast<int*>(seqs + B);
@@ -223,16 +302,9 @@ KK3_DEV Share plan_share(const CallSeqs& a, const Split& split, int worker, int 
       mine += split.size(seqs[b], g - prefix[b]);
     }
   }
-  Share sh;
-  const long long before = block_scan<NT>(mine, red, &sh.total);
-  const long long most = (sh.total + min_units - 1) / min_units;
-  sh.workers = (int)(most > a.workers ? a.workers : most);
-  sh.begin = sh.end = sh.at = 0;
-  sh.b = sh.t = 0;
-  sh.seq = Seq{0, 0, 0};
-  if (worker >= sh.workers) return sh;
-  sh.begin = sh.total * worker / sh.workers;
-  sh.end = sh.total * (worker + 1) / sh.workers;
+  long long total;
+  const long long before = block_scan<NT>(mine, red, &total);
+  if (!plan_part(sh, total, worker, min_units, a.workers)) return sh;
   long long* found = red + NT / 32;
   if (before <= sh.begin && sh.begin < before + mine) {   // exactly one thread
     int b = b0;
