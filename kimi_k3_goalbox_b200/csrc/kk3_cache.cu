@@ -10,7 +10,8 @@ namespace kk3 {
 // ---------------------------------------------------------------------------------------------
 // append: latent = x[:512] / rms(x[:512]) * weight (FP32, rounded to BF16 once), rope = x[512:], into the page of the
 // token's position. One warp per token, bound by its 2304 bytes of traffic; 16-byte accesses throughout (lane l owns
-// the latent values 8 l .. 8 l + 7 and 256 + 8 l ..; eight lanes copy the rope part).
+// the latent values 8 l .. 8 l + 7 and 256 + 8 l ..; eight lanes copy the rope part). Five chunks of up to 4096 tokens take
+// 7.2 us, 5.2 TB/s; eight single tokens 2.7 us, a launch.
 
 struct AppendArgs {
   CachePages c;
@@ -354,7 +355,8 @@ __global__ void __launch_bounds__(kEvThreads) kk3_cache_select_kernel(const Evic
   if (tid == 0) a.new_lengths[b] = keep;
 }
 
-// Eviction, move into pages of their own: one warp per kept entry (1152 bytes), bound by the traffic.
+// Eviction, move into pages of their own: one warp per kept entry (1152 bytes), bound by the traffic: 65000 entries 23 us,
+// 6.5 TB/s.
 constexpr int kMoveWarps = 8;
 __global__ void __launch_bounds__(kMoveWarps * 32) kk3_cache_move_kernel(const EvictArgs a) {
   const int b = blockIdx.y, lane = threadIdx.x & 31;
@@ -383,7 +385,8 @@ __global__ void __launch_bounds__(kMoveWarps * 32) kk3_cache_move_kernel(const E
 
 // Eviction, move in place: entry kept[j] >= j goes to slot j, so batches in ascending j are safe when a batch is read
 // whole before it is written: later batches read slots at or above their own j, which earlier ones did not write.
-// The order holds per (sequence, 64-byte slice of the entry); the 18 slices of a sequence run side by side.
+// The order holds per (sequence, 64-byte slice of the entry); the 18 slices of a sequence run side by side, bound by the
+// batches' latencies: 16 sequences of up to 8192 positions cut down to 4096 take 47 us in place, 38 into other pages.
 constexpr int kSlideThreads = 512;
 constexpr int kSlideDeep = 8;    // rows in flight per thread: 1024 rows a batch
 __global__ void __launch_bounds__(kSlideThreads) kk3_cache_slide_kernel(const EvictArgs a) {
@@ -505,13 +508,18 @@ extern "C" int kk3_cache_append(const kk3_cache_append_args* x, void* stream) {
   return cache_cuda(cudaGetLastError(), "kk3_cache_append_kernel");
 }
 
-// The kernel for a call's average rows per sequence, and its workers: warp-level products up to 16 rows, CTA pairs above.
+// The kernel and its workers. Up to 16 rows a sequence on average fill the small tile: 64 sequences of 8192 positions
+// with 12 rows each take 134 us in it and 187 us in CTA pairs; with 24 rows, two small tiles that read the cache twice,
+// 243 and 195 us. A small call is faster in the small tile whatever its rows, since that begins and ends sooner: 48 rows
+// of one sequence take 20.5 against 24.0 us over 517 positions and 24.0 against 26.0 over 8192, 96 rows 27.4 against 26.7.
+// The host does not know the lengths, only what the table can hold.
 struct Plan {
   int workers, rows;
 };
-static Plan attend_plan(int64_t batch, int64_t tokens, int64_t heads, int sms) {
+static Plan attend_plan(int64_t batch, int64_t tokens, int64_t heads, int64_t capacity, int sms) {
   const int workers = sms < kMaxWorkers ? sms : kMaxWorkers;
-  return tokens * heads <= kFewRows * batch ? Plan{workers, kFewRows} : Plan{workers / 2, kPairRows};
+  const int64_t rows = tokens * heads;
+  return rows <= kFewRows * batch || (rows <= 4 * kFewRows && capacity <= 8192) ? Plan{workers, kFewRows} : Plan{workers / 2, kPairRows};
 }
 
 extern "C" int64_t kk3_cache_attend_workspace(void) {
@@ -550,7 +558,7 @@ extern "C" int kk3_cache_attend(const kk3_cache_attend_args* x, void* stream) {
   a.scale_log2 = x->scale * 1.4426950408889634f;
   a.out = (bf16*)x->out;
   a.lse = x->lse;
-  const Plan p = attend_plan(a.c.batch, tokens, heads, sms);
+  const Plan p = attend_plan(a.c.batch, tokens, heads, (int64_t)a.c.columns * a.c.page_size, sms);
   a.workers = p.workers;
   a.meta = (int*)x->workspace;
   a.part = (float*)((char*)x->workspace + (size_t)p.workers * 16);

@@ -256,8 +256,11 @@ KK3_DEV void with_box(int box, const F& f) {
 // the sums of one unit run under the products of the next. Where the rows fit one unit (single tokens) the tile's
 // blocks are freed one by one instead, and the kernel streams the cache with up to 147 KB in flight in each SM.
 //
-// Bounds of a unit of 256 rows: 2304 clocks of tensor time, as many of shared-memory reads (8 KB per 64-clock
-// instruction), and 2048 of exponentials (16 a clock).
+// Bounds of a unit of 256 rows: 4608 clocks of tensor time (256 x 256 x 576 products at 4096 a clock and SM), as many
+// of shared-memory reads (16 KB per 128-clock instruction), and 2048 of exponentials (16 a clock). Measured: 32 tokens
+// x 96 heads over four sequences of up to 8192 positions 74 us, 1070 TFLOP/s (47 us at the rate of a plain product);
+// 16 single tokens x 12 heads, bound by the cache's bytes, 32 us, 3.4 TB/s, of which 10 are the work split, the first
+// loads and the join.
 
 constexpr int kMassPos = 256;
 constexpr int kMassThreads = 320;   // warps 0-7 sums, 8 copies, 9 matrix instructions and TMEM
@@ -546,8 +549,15 @@ __global__ void __launch_bounds__(kMassPos) kk3_cache_mass_join_kernel(const Mas
 // the sums in TMEM are rarely rescaled. Probabilities are rounded to BF16 for the second product, the type that the
 // instruction takes with BF16 latents; the running sum adds them unrounded, since lse is an FP32 result.
 //
+// Both CTAs bring their part of every block and piece, if only zeros for positions behind the end (rows past the pool,
+// which cost no traffic): a CTA that sat a slot's turn out could be passed by two of its phases and wait for good.
+//
 // Bounds of a unit: 4352 clocks of tensor time (128 x 256 x 1088 products at 4096 a clock and SM), 4200 to issue its
-// scores, 278 KB of loads in each SM (mostly from L2); for few rows the 294 KB per pair from HBM.
+// scores, 278 KB of loads in each SM (mostly from L2). Measured: two chunks of 1024 tokens x 12 heads over up to 8192
+// positions 295 us, 1100 TFLOP/s, 6400 clocks a unit: the loads, 78 GB/s in each SM. Three prompts of 900 tokens x 24
+// heads 103 us: tiles of two or three units each, whose first scores, last sums and epilogue (6 us) nothing overlaps.
+// Eight single tokens x 96 heads over up to 8192 positions 38 us: 7 us to the first scores, three units of 3.6 us, 8 us for
+// the last sums and the running sums' way out, 8 us for their join.
 
 constexpr int kPaUnit = 256;
 constexpr int kPaThreads = 384;        // warps 0-7 softmax, 8 and 9 copies and instructions of scores, 10 and 11 of sums
@@ -1020,7 +1030,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPaThreads, 1)
 // values of one unit, take the softmax of the next and the scores of the one after it. In the first product a warp holds
 // the query's fragments of a quarter of the 576 dims in registers and takes 8 positions, in the second it owns 32 of the
 // output dims, in the softmax a row. Four more warps copy, one unit to a stage of six, and run ahead over the tiles.
-// (Copies by the 16 warps themselves, between the products, took 142 us where this takes the time noted with the launch.)
+// Measured: 64 single tokens x 12 heads over 8192 positions 135 us, 4.5 TB/s (5.5 TB/s for what the second 32 of them add;
+// the rest is the start, the workers' uneven ends and the join), one such token 17 us. With copies by the 16 warps
+// themselves, between the products, the 64 took 142 us.
 // Probabilities are rounded to BF16 for the second product, the type that the instruction takes with BF16 latents; the
 // running sum adds them unrounded, since lse is an FP32 result.
 
@@ -1451,8 +1463,9 @@ int attend_few(const kk3_cache* c, const AttendArgs& a, cudaStream_t st) {
 }
 
 // rows of a matrix instruction for the average rows of a sequence: the smallest of 32, 64, 128 and 256 that holds
-// them (a unit costs the same shared-memory reads of the cache blocks whatever its rows; fewer leave more room in
-// the ring), 256 for more
+// them, 256 for more. A unit's products take as long as its rows are many, and each unit reads the tile's blocks from
+// shared memory anew: 16 sequences of up to 8192 positions with 12 rows each take 31 us with 32 rows and 37 with 256,
+// four with 96 rows each 19 us with 128, 21 with 256 and 29 with 32.
 static int mass_rows(int64_t tokens, int64_t heads, int64_t batch) {
   int rows = 32;
   while (rows < 256 && (int64_t)rows * batch < tokens * heads) rows *= 2;
