@@ -193,7 +193,8 @@ typedef struct kk3_cache {
 /* Append: for each new token i of sequence b, position lengths[b] + i gets the entry of its projection row
  * raw[t] (bf16 [tokens, 576], the step's `ka` product): latent = x / sqrt(mean(x^2) + eps) * norm_weight over the
  * first 512 values (FP32, one rounding), rope part as it is. new_lengths[b] = lengths[b] + new tokens (another buffer
- * than lengths). A token that does not fit behind the last column is not written. */
+ * than lengths). A token that does not fit behind the last column is not written. Sequences may share pages, but no
+ * two may write to one slot. */
 typedef struct kk3_cache_append_args {
     kk3_cache cache;
     const void* raw;             /* bf16 [tokens, 576], row stride raw_stride */
@@ -268,7 +269,8 @@ int kk3_cache_mass(const kk3_cache_mass_args* args, void* stream);
 /* Eviction: each sequence keeps min(lengths[b], budget) positions: its first `sinks`, its last `recent`
  * (sinks + recent <= budget), and of the others those of the largest mass (equal ones: the lowest position; a NaN
  * counts as the largest). The kept entries move, in ascending order, to positions 0, 1, ... of dst_table's pages
- * (pages that no listed sequence uses: shared pages stay as they are), or in place (dst_table = NULL). new_lengths,
+ * (pages that no listed sequence uses: shared pages stay as they are), or in place (dst_table = NULL; then no two
+ * sequences may share a page). new_lengths,
  * new_mass (the kept positions' mass, zeros behind) and kept (their old positions, -1 behind) are other buffers than
  * the inputs. */
 typedef struct kk3_cache_evict_args {

@@ -274,7 +274,8 @@ def attend(q_latent, q_pe, kv, pe, table, lengths, cu_new, *, scale: float | Non
     all (token, head) rows lie at one 16-byte aligned pitch, they are copied first).
     lengths: cached positions, the new tokens included (append's result): token i of n sees the first
     lengths - n + i + 1. A token that sees nothing gets zeros and -inf. Rows behind cu_new[B] are not written (pass
-    `out` and `lse`, both contiguous, to keep theirs)."""
+    `out` and `lse`, both contiguous, to keep theirs). What pages hold behind a sequence's length is never used; what
+    they hold before it must be finite, also where a token does not see it."""
     cache, dev, B, _ = _cache(kv, pe, table)
     T, H, scale, _keep, q = _queries(q_latent, q_pe, lengths, cu_new, dev, B, scale)
     device = kv.device
@@ -328,7 +329,8 @@ def evict(kv, pe, table, lengths, mass, budget: int, *, sinks: int = 0, recent: 
     the largest mass (equal ones: the lowest position; NaN counts as the largest).
 
     The kept entries move, in ascending order, to positions 0, 1, ... of dst_table's pages (int32 [B, columns2]; pages
-    that none of the sequences uses, so that pages shared with others stay as they are), or in place (None). Returns
+    that none of the sequences uses, so that pages shared with others stay as they are), or in place (None; then no two
+    sequences may share a page). Returns
     (new lengths int64 [B], their mass f32 [B, columns * page_size] with zeros behind, their old positions int32
     [B, budget] with -1 behind)."""
     cache, dev, B, capacity = _cache(kv, pe, table)
