@@ -35,9 +35,9 @@ __global__ void __launch_bounds__(kAppendWarps * 32) kk3_cache_append_kernel(con
   if (blockIdx.x == 0) {
     for (int b = threadIdx.x; b < B; b += blockDim.x) {
       const int q0 = min(max(a.cu_new[b], 0), a.tokens), q1 = min(max(a.cu_new[b + 1], q0), a.tokens);
-      const long long l = a.lengths[b], sum = (l < 0 ? 0 : l) + (q1 - q0);
-      if (l < 0 || sum > cap) cache_error(a.c);
-      a.new_lengths[b] = sum > cap ? cap : sum;
+      const long long l = a.lengths[b], sum = min(max(l, 0ll), cap) + (q1 - q0);
+      if (l < 0 || l > cap || sum > cap) cache_error(a.c);
+      a.new_lengths[b] = min(sum, cap);
     }
   }
   if (tok >= a.tokens) return;
@@ -48,7 +48,7 @@ __global__ void __launch_bounds__(kAppendWarps * 32) kk3_cache_append_kernel(con
   }
   const int first = a.cu_new[lo];
   if (tok < first || tok >= a.cu_new[lo + 1] || first < 0) return;   // behind the last sequence: no one's token
-  const long long pos = max(a.lengths[lo], 0ll) + (tok - first);
+  const long long pos = min(max(a.lengths[lo], 0ll), cap) + (tok - first);
   if (pos >= cap) return;
   int slot;
   const int page = page_at(a.c, lo, (int)pos, &slot);
@@ -438,8 +438,6 @@ __global__ void __launch_bounds__(kSlideThreads) kk3_cache_slide_kernel(const Ev
 using namespace kk3;
 
 namespace kk3 {
-
-
 
 int cache_cuda(cudaError_t e, const char* what) {
   if (e == cudaSuccess) return KK3_OK;

@@ -142,7 +142,6 @@ KK3_DEV void tmem_ld32(unsigned taddr, float (&v)[32]) {
   for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
 }
 
-
 // instruction descriptor: kind::f16, D = F32, A = B = BF16, M rows and N columns over the pair, operands K-major
 KK3_DEV constexpr unsigned pair_idesc(int m, int n) {
   return (1u << 4) | (1u << 7) | (1u << 10) | ((unsigned)(n >> 3) << 17) | ((unsigned)(m >> 4) << 24);

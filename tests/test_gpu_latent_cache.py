@@ -285,7 +285,7 @@ def test_bad_pages_and_lengths_are_reported_and_not_followed(heads, new, page):
             else:
                 lc.attention_mass(x.q_latent, x.q_pe, ok_lse, x.kv, x.pe, table, x.lengths, x.cu_new, error_word=error)
             assert error.item() != 0
-    for length in (-5, x.columns * page + 1, 2 ** 40, -2 ** 40):
+    for length in (-5, x.columns * page + 1, 2 ** 40, -2 ** 40, 2 ** 63 - 1):
         lengths = x.lengths.clone()
         lengths[0] = length
         error.zero_()
@@ -389,6 +389,15 @@ def test_append_reports_what_does_not_fit():
     same[table[0, -1].long(), 15] = False
     same[table[2, 0].long(), 8:10] = False
     assert torch.equal(x.kv[same].view(torch.int16), kv0[same].view(torch.int16))
+    # lengths whose sum with the new tokens passes 64 bits
+    kv0 = x.kv.clone()
+    for length in (2 ** 63 - 1, 2 ** 62, cap + 1, cap, -2 ** 63):
+        error.zero_()
+        lengths = torch.tensor([length, length, length], device="cuda")
+        after = lc.append(raw, weight, x.kv, x.pe, table, lengths, x.cu_new, error_word=error)
+        assert after.tolist() == ([cap] * 3 if length > 0 else [4, 2, 2]) and error.item() != 0
+        if length > 0:
+            assert torch.equal(x.kv.view(torch.int16), kv0.view(torch.int16))
 
 
 # --- evict -----------------------------------------------------------------------------------------------------
