@@ -143,6 +143,11 @@ struct AttendSplit {
     return n > unit ? (n + unit - 1) / unit : 1;
   }
   KK3_DEV int size(const Seq& s, int t) const { return units(s, t) + cost; }
+  KK3_DEV long long all(const Seq& s) const {   // of its tiles
+    long long n = 0;
+    for (int t = 0; t < tiles(s); ++t) n += size(s, t);
+    return n;
+  }
   // the tile's units that a worker takes, of a tile that begins at `at`
   KK3_DEV int from(const Share& sh, long long at, int units) const { return (int)min((long long)units, max(0ll, sh.begin - at - cost)); }
   KK3_DEV int to(const Share& sh, long long at, int units) const { return (int)min((long long)units, max(0ll, sh.end - at - cost)); }
@@ -157,6 +162,12 @@ struct MassSplit {
   }
   KK3_DEV int units(const Seq& s, int t) const { return (s.n * heads + rows - 1) / rows - first_unit(s, t); }
   KK3_DEV int size(const Seq& s, int t) const { return units(s, t); }
+  KK3_DEV long long all(const Seq& s) const {   // of its tiles: every row sees the first ones whole
+    const int count = tiles(s), whole = min(count, max(0, s.len - s.n) / positions + 1);
+    long long n = count ? (long long)whole * units(s, 0) : 0;
+    for (int t = whole; t < count; ++t) n += size(s, t);
+    return n;
+  }
 };
 
 // inclusive sums over the lanes of a warp
@@ -229,9 +240,7 @@ KK3_DEV bool plan_small(const CallSeqs& a, const Split& split, int worker, int m
   if (!__all_sync(0xffffffffu, small)) return false;
 #pragma unroll
   for (int i = 0; i < kPlanDeep; ++i) {
-    size[i] = 0;
-    const int tiles = split.tiles(s[i]);
-    for (int t = 0; t < tiles; ++t) size[i] += split.size(s[i], t);
+    size[i] = split.all(s[i]);
     mine += size[i];
   }
   const long long incl = lane_sums(mine);

@@ -35,6 +35,11 @@ struct PairRows {
   int box;                  // rows of a box: divides a page and 64, 8 at least; 0: gathers only
 };
 
+// Thread i of the CTA has map i fetched, before the first copy needs it.
+KK3_DEV void fetch_maps(const PairMaps& maps) {
+  if (threadIdx.x < sizeof(PairMaps) / sizeof(CUtensorMap))
+    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<const CUtensorMap*>(&maps) + threadIdx.x) : "memory");
+}
 KK3_DEV unsigned smem_u32(const void* p) { return (unsigned)__cvta_generic_to_shared(p); }
 KK3_DEV unsigned cluster_rank() {
   unsigned r;
@@ -302,6 +307,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMassThreads, 1)
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, worker = blockIdx.x >> 1;
   const unsigned rank = cluster_rank();
   const unsigned kbase = smem_u32(base), qbase = kbase + kBlocks * kMassKBlock;
+  fetch_maps(maps);
   const int half = rows / 2, slot_bytes = half * 128, slots = min(kMassSlots, kMassRing / slot_bytes);
   const MassSplit split{kMassPos, rows, a.heads};
   const unsigned full = smem_u32(ctl.full), empty = smem_u32(ctl.empty), kempty = smem_u32(ctl.kempty),
@@ -609,6 +615,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPaThreads, 1)
                  pfull = smem_u32(ctl.pfull), pfree = smem_u32(ctl.pfree), pvdone = smem_u32(ctl.pvdone),
                  done = smem_u32(&ctl.done);
   volatile int* dead = &ctl.dead;
+  fetch_maps(maps);
   if (tid == 0) {
     mbar_init(qfull, 1);
     mbar_init(qempty, 1);
@@ -1150,6 +1157,7 @@ __global__ void __launch_bounds__(kFewThreads, 1)
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, worker = blockIdx.x;
   const unsigned base = smem_u32(smem_raw), full = smem_u32(ctl.full), empty = smem_u32(ctl.empty);
   volatile int* dead = &ctl.dead;
+  fetch_maps(maps);
   const AttendSplit split{kFewRows, a.heads, kFewUnit, 0};
   if (tid == 0) {
     for (int i = 0; i < kFewStages; ++i) {
