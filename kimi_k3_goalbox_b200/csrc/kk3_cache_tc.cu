@@ -963,9 +963,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPaThreads, 1)
       const long long out_row = (long long)s.q0 * a.heads + g;
       float* part = a.part + (((long long)worker * 2 + (u0 == 0 ? 1 : 0)) * kPairRows + rank * 64 + row) * kPartRow;
       const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
-      // through this warp's 2 KB of P, which the instructions have read, so that a row's dims leave in pieces of 64 bytes:
-      // 32 rows x 32 dims of results, 16 dims of running sums
-      unsigned char* stage = smem_raw + kPaP + warp * 2048;
+      // through 2 KB of the part of P that this warp fills (the instructions have read it, and no other warp's next
+      // probabilities come there), so that a row's dims leave in pieces of 64 bytes: 32 rows x 32 dims of results, 16
+      // dims of running sums
+      unsigned char* stage = smem_raw + kPaP + part64 * kPaQBlock + (quarter & 1) * 4096;
       const int dim0 = wg * 256 + (quarter >> 1) * 128, rows_here = s.n * a.heads - (g - lane);
       const int put = lane * 64, turn = (lane >> 1) & 3;
 #pragma unroll 1
