@@ -262,9 +262,9 @@ KK3_DEV void with_box(int box, const F& f) {
 //
 // Bounds of a unit of 256 rows: 4608 clocks of tensor time (256 x 256 x 576 products at 4096 a clock and SM), as many
 // of shared-memory reads (16 KB per 128-clock instruction), and 2048 of exponentials (16 a clock). Measured: 32 tokens
-// x 96 heads over four sequences of up to 8192 positions 74 us, 1070 TFLOP/s (47 us at the rate of a plain product);
-// 16 single tokens x 12 heads, bound by the cache's bytes, 32 us, 3.4 TB/s, of which 10 are the work split, the first
-// loads and the join.
+// x 96 heads over four sequences of up to 8192 positions 71 us, 1110 TFLOP/s (47 us at the rate of a plain product);
+// 16 single tokens x 12 heads, bound by the cache's bytes, 29 us, 3.7 TB/s: 3 us for the work split, 7 until the first
+// tile's sums, then 3.7 us a tile, the rate of HBM.
 
 constexpr int kMassPos = 256;
 constexpr int kMassThreads = 320;   // warps 0-7 sums, 8 copies, 9 matrix instructions and TMEM
@@ -559,8 +559,11 @@ __global__ void __launch_bounds__(kMassPos) kk3_cache_mass_join_kernel(const Mas
 //
 // Bounds of a unit: 4352 clocks of tensor time (128 x 256 x 1088 products at 4096 a clock and SM), 4200 to issue its
 // scores, 278 KB of loads in each SM (mostly from L2). Measured: two chunks of 1024 tokens x 12 heads over up to 8192
-// positions 295 us, 1100 TFLOP/s, 6400 clocks a unit: the loads, 78 GB/s in each SM. Three prompts of 900 tokens x 24
-// heads 103 us: tiles of two or three units each, whose first scores, last sums and epilogue (6 us) nothing overlaps.
+// positions 299 us, 1090 TFLOP/s (a plain product: 1679), 8600 clocks a unit: an instruction takes about 120 clocks
+// instead of 64 while the copies write to the shared memory that it reads, and both issuing threads are held up by it
+// three quarters of their time (a fourth slot for the sums' pieces, in place of half of P, took 311 us). Three prompts of
+// 900 tokens x 24 heads 101 us: tiles of two or three units each, whose first scores, last sums and epilogue (6 us)
+// nothing overlaps.
 // Eight single tokens x 96 heads over up to 8192 positions 38 us: 7 us to the first scores, three units of 3.6 us, 8 us for
 // the last sums and the running sums' way out, 8 us for their join.
 
@@ -1472,8 +1475,8 @@ int attend_few(const kk3_cache* c, const AttendArgs& a, cudaStream_t st) {
 
 // rows of a matrix instruction for the average rows of a sequence: the smallest of 32, 64, 128 and 256 that holds
 // them, 256 for more. A unit's products take as long as its rows are many, and each unit reads the tile's blocks from
-// shared memory anew: 16 sequences of up to 8192 positions with 12 rows each take 31 us with 32 rows and 37 with 256,
-// four with 96 rows each 19 us with 128, 21 with 256 and 29 with 32.
+// shared memory anew: 16 sequences of up to 8192 positions with 12 rows each took 31 us with 32 rows and 37 with
+// 256, four with 96 rows each 19 us with 128, 21 with 256 and 29 with 32.
 static int mass_rows(int64_t tokens, int64_t heads, int64_t batch) {
   int rows = 32;
   while (rows < 256 && (int64_t)rows * batch < tokens * heads) rows *= 2;
