@@ -43,7 +43,7 @@ class Problem:
         order = torch.randperm(pages, generator=gen, device="cuda").to(torch.int32)
         self.kv = torch.full((pages, page, 512), math.nan, dtype=BF, device="cuda")
         self.pe = torch.full((pages, page, 64), math.inf, dtype=BF, device="cuda")
-        self.table = torch.zeros((B, self.columns), dtype=torch.int32, device="cuda")
+        self.table = torch.full((B, self.columns), -1, dtype=torch.int32, device="cuda")   # no page behind the end
         self.entries = []
         at = 0
         for b, n in enumerate(lengths):
@@ -141,17 +141,22 @@ CASES = [
     ([2, 300], [9000, 2500], 64, 32),            # single tokens next to a chunk
     ([1], [64], 128, 64),
     ([1, 2, 1], [95, 96, 97], 5, 32),
+    ([1], [100003], 12, 64),
+    ([2], [70001], 40, 16),
+    ([3, 3], [65, 64], 21, 64),                  # few rows in all
 ]
 
 
 @pytest.mark.parametrize("new,lengths,heads,page", CASES)
 def test_attend_and_mass(new, lengths, heads, page):
     x = Problem(11, new, lengths, heads, page)
-    out, lse = lc.attend(x.q_latent, x.q_pe, *x.cache, x.lengths, x.cu_new)
+    error = torch.zeros(1, dtype=torch.int32, device="cuda")
+    out, lse = lc.attend(x.q_latent, x.q_pe, *x.cache, x.lengths, x.cu_new, error_word=error)
     x.check_attend(out, lse)
     before = torch.rand((len(new), x.columns * page), generator=x.gen, device="cuda")
-    got = lc.attention_mass(x.q_latent, x.q_pe, lse, *x.cache, x.lengths, x.cu_new, mass=before)
+    got = lc.attention_mass(x.q_latent, x.q_pe, lse, *x.cache, x.lengths, x.cu_new, mass=before, error_word=error)
     x.check_mass(got, before, lse)
+    assert error.item() == 0
     # the same results again, bit for bit, and in place
     out2, lse2 = lc.attend(x.q_latent, x.q_pe, *x.cache, x.lengths, x.cu_new)
     assert torch.equal(out, out2) and torch.equal(lse, lse2)
@@ -230,6 +235,23 @@ def test_strided_arguments_give_the_same(heads, new, page):
         got = lc.attention_mass(q[..., :512], q[..., 512:576], lse2, *cache, x.lengths, x.cu_new, mass=before)
         x.check_mass(got, before, lse2)
     assert torch.equal(mass, lc.attention_mass(both[..., :512], both[..., 512:], lse, *cache, x.lengths, x.cu_new))
+
+
+@pytest.mark.parametrize("heads,new", [(12, [1, 1, 1]), (24, [20, 9, 4])])
+def test_sequences_that_share_pages(heads, new):
+    """Three sequences of one prefix: the same pages in three rows of the table, and one of them twice in a row."""
+    x = Problem(8, new, [150, 160, 170], heads, 16)
+    x.table[1:, :9] = x.table[0, :9]
+    x.table[2, 3] = x.table[2, 5]
+    for b in (1, 2):
+        for e, first in zip(x.entries[b], x.entries[0]):
+            e[:144] = first[:144]
+    for e in x.entries[2]:
+        e[48:64] = e[80:96].clone()
+    out, lse = lc.attend(x.q_latent, x.q_pe, *x.cache, x.lengths, x.cu_new)
+    x.check_attend(out, lse)
+    before = torch.zeros((3, x.columns * 16), device="cuda")
+    x.check_mass(lc.attention_mass(x.q_latent, x.q_pe, lse, *x.cache, x.lengths, x.cu_new), before, lse)
 
 
 @pytest.mark.parametrize("heads,new", [(12, [1, 1]), (24, [30, 9])])
@@ -646,3 +668,31 @@ def test_prefill_evict_and_decode_with_the_step():
             q = actual["kv_write"][i][:, None] * 8
             out, lse = lc.attend(q, torch.zeros((B, 1, 64), dtype=BF, device="cuda"), *views[l], actual["cache_length"], one, scale=1.0)
             assert torch.equal(out[:, 0], actual["kv_write"][i])
+
+
+def test_attend_agrees_with_the_step_oracle():
+    """The absorbed queries and the attended latents of the oracle's MLA layers, with its new entries in the cache."""
+    from oracle import kimi_oracle as ko
+    from tests import gpu_helpers as gh
+
+    B, context = 3, 24
+    case = gh.small_case(B, context=context)
+    with torch.inference_mode():
+        values = ko.make_inputs(case, 53, "cuda")
+        values["reset"] = torch.zeros(B, dtype=torch.bool, device="cuda")
+        trace = {}
+        outputs = ko.reference(case, values, serial=True, trace=trace)
+        one = torch.arange(B + 1, dtype=torch.int32, device="cuda")
+        lengths = torch.full((B,), context + 1, dtype=torch.int64, device="cuda")
+        for i, l in enumerate(ko.mla_layer_ids(case)):
+            kv = torch.full((B, 32, 512), math.nan, dtype=BF, device="cuda")
+            pe = torch.full((B, 32, 64), math.nan, dtype=BF, device="cuda")
+            kv[:, :context], pe[:, :context] = values[f"l{l}_kv_cache"], values[f"l{l}_pe_cache"]
+            kv[:, context], pe[:, context] = outputs["kv_write"][i], outputs["pe_write"][i]
+            q, want = trace[f"l{l}_absorbed"], trace[f"l{l}_attn_latent"].to(F64)
+            out, lse = lc.attend(q, trace[f"l{l}_q"][..., 128:], *lc.paged_view(kv, pe, 8), lengths, one)
+            c = kv[:, :context + 1].to(F64)
+            s = (q.to(F64) @ c.mT + trace[f"l{l}_q"][..., 128:].to(F64) @ pe[:, :context + 1].to(F64).mT) * SCALE
+            mag = torch.softmax(s, -1) @ c.abs()
+            # both sides round the probabilities and the result once: 2^-8 of the summed magnitudes and of the value each
+            assert bool(((out.to(F64) - want).abs() <= 2 * 2 ** -8 * 1.05 * (mag + want.abs())).all())
