@@ -507,7 +507,7 @@ extern "C" int kk3_cache_append(const kk3_cache_append_args* x, void* stream) {
 }
 
 // The kernel and its workers. Up to 16 rows a sequence on average fill the small tile: 64 sequences of 8192 positions
-// with 12 rows each take 134 us in it and 187 us in CTA pairs; with 24 rows, two small tiles that read the cache twice,
+// with 12 rows each take 129 us in it and 187 us in CTA pairs; with 24 rows, two small tiles that read the cache twice,
 // 243 and 195 us. A small call is faster in the small tile whatever its rows, since that begins and ends sooner: 48 rows
 // of one sequence take 20.5 against 24.0 us over 517 positions and 24.0 against 26.0 over 8192, 96 rows 27.4 against 26.7.
 // The host does not know the lengths, only what the table can hold.

@@ -1039,22 +1039,24 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPaThreads, 1)
 // unit takes is latency, so 16 warps, four to a scheduler, run three units at a time: between two barriers they add the
 // values of one unit, take the softmax of the next and the scores of the one after it. In the first product a warp holds
 // the query's fragments of a quarter of the 576 dims in registers and takes 8 positions, in the second it owns 32 of the
-// output dims, in the softmax a row. Four more warps copy, one unit to a stage of six, and run ahead over the tiles.
-// Measured: 64 single tokens x 12 heads over 8192 positions 135 us, 4.5 TB/s (5.5 TB/s for what the second 32 of them add;
-// the rest is the start, the workers' uneven ends and the join), one such token 17 us. With copies by the 16 warps
-// themselves, between the products, the 64 took 142 us.
+// output dims, in the softmax a row; half of the warps begin with the scores, so that not all want the same at once. Four
+// more warps copy, one unit to a stage of five, and run ahead over the tiles.
+// Measured: 64 single tokens x 12 heads over 8192 positions 129 us, 4.7 TB/s, and 122 us where the cache stays in L2: the
+// 1800 clocks of a unit's instructions and shared-memory traffic, the start, the workers' uneven ends and the join (25 us
+// for the last three); one such token 17 us. With copies by the 16 warps themselves, between the products, the 64 took
+// 142 us; with six stages, scores of one unit in shared memory and two barriers a unit 134 us.
 // Probabilities are rounded to BF16 for the second product, the type that the instruction takes with BF16 latents; the
 // running sum adds them unrounded, since lse is an FP32 result.
 
-constexpr int kFewUnit = 32, kFewStages = 6;
+constexpr int kFewUnit = 32, kFewStages = 5;
 constexpr int kFewWork = 512, kFewCopies = 4, kFewThreads = kFewWork + 32 * kFewCopies;
 constexpr int kFewBlock = kFewUnit * 128;               // 32 positions x 64 dims
 constexpr int kFewStageBytes = kBlocks * kFewBlock;
 constexpr int kFewMinUnits = 4;
 constexpr int kFewQuarter = 5;   // pairs of k-steps of a quarter of the 18: 5, 5, 4, 4
 struct FewCtl {
-  // scores of a unit, a part from each quarter of the dims; column c of row r at c ^ 8 (r % 4)
-  float s[4][kFewRows][kFewUnit];
+  // scores of two units, a part from each quarter of the dims; column c of row r at c ^ 8 (r % 4)
+  float s[2][4][kFewRows][kFewUnit];
   alignas(16) bf16 p[2][kFewRows][kFewUnit + 8];
   float alpha[2][kFewRows], m[kFewRows], l[kFewRows];
   unsigned long long full[kFewStages], empty[kFewStages];
@@ -1217,7 +1219,7 @@ __global__ void __launch_bounds__(kFewThreads, 1)
       for (int i = 0; i < 2 * kFewStages; ++i) mbar_wait_for(full + 8 * (i / 2), i & 1, kWaitNs / 16);
   } else {
     const int ntile = warp & 3, quarter = warp >> 2;   // 8 positions of the unit; pairs quarter, quarter + 4 .. of the 18 pairs of k-steps
-    const bool fifth = quarter < 2;
+    const bool fifth = quarter < 2, scores_first = quarter >= 2;
     // this lane's addresses in a stage: score operands (block quarter / 2 + 2 i for pair quarter + 4 i), values
     const unsigned kat = (quarter >> 1) * kFewBlock + (ntile * 8 + (lane & 7)) * 128 + ((((quarter & 1) * 4 + (lane >> 3)) ^ (lane & 7)) << 4);
     const unsigned vat = (warp >> 1) * kFewBlock + (lane & 15) * 128 + ((((warp & 1) * 4 + (lane >> 4)) ^ (lane & 7)) << 4);
@@ -1266,35 +1268,33 @@ __global__ void __launch_bounds__(kFewThreads, 1)
       const int sees = warp < rows ? s.len - s.n + (row0 + warp) / a.heads + 1 : 0;
       // unit u0 + i: scores, softmax, values; `in` is the stage of the unit whose scores come next, `out` of the one whose values do
       int in = slot, out = slot;
-      float c[4][4];
-      const auto scores = [&]() {
+      const auto scores = [&](int i) {
+        float c[2][4];
         ok = pair_wait(a.c, full + 8 * in, phase, dead) && ok;
         const unsigned kb = base + in * kFewStageBytes + kat;
 #pragma unroll
-        for (int j = 0; j < 16; ++j) c[j >> 2][j & 3] = 0.0f;   // four chains: a product waits for the one before it on its sums
+        for (int j = 0; j < 8; ++j) c[j >> 2][j & 3] = 0.0f;   // two chains: a product waits for the one before it on its sums
 #pragma unroll
         for (int k = 0; k < kFewQuarter; ++k) {
           if (k < 4 || fifth) {
             unsigned bf[4];
             ldsm4(bf, kb + k * 2 * kFewBlock);
-            mma_free(c[(k & 1) * 2], qf[2 * k], bf[0], bf[1]);
-            mma_free(c[(k & 1) * 2 + 1], qf[2 * k + 1], bf[2], bf[3]);
+            mma_free(c[0], qf[2 * k], bf[0], bf[1]);
+            mma_free(c[1], qf[2 * k + 1], bf[2], bf[3]);
           }
         }
 #pragma unroll
-        for (int j = 0; j < 4; ++j) c[0][j] = (c[0][j] + c[1][j]) + (c[2][j] + c[3][j]);
+        for (int j = 0; j < 4; ++j) c[0][j] += c[1][j];
+        float* to = &ctl.s[i & 1][quarter][lane >> 2][(ntile * 8 + (lane & 3) * 2) ^ ((lane >> 2 & 3) << 3)];
+        *reinterpret_cast<float2*>(to) = make_float2(c[0][0], c[0][1]);
+        *reinterpret_cast<float2*>(to + 8 * kFewUnit) = make_float2(c[0][2], c[0][3]);
         if (++in == kFewStages) {
           in = 0;
           phase ^= 1;
         }
       };
-      const auto put_scores = [&]() {
-        float* to = &ctl.s[quarter][lane >> 2][(ntile * 8 + (lane & 3) * 2) ^ ((lane >> 2 & 3) << 3)];
-        *reinterpret_cast<float2*>(to) = make_float2(c[0][0], c[0][1]);
-        *reinterpret_cast<float2*>(to + 8 * kFewUnit) = make_float2(c[0][2], c[0][3]);
-      };
       const auto softmax = [&](int i) {
-        const float* from = &ctl.s[0][warp][lane ^ ((warp & 3) << 3)];
+        const float* from = &ctl.s[i & 1][0][warp][lane ^ ((warp & 3) << 3)];
         constexpr int kPart = kFewRows * kFewUnit;
         float v = ((from[0] + from[kPart]) + (from[2 * kPart] + from[3 * kPart])) * a.scale_log2;
         if ((u0 + i) * kFewUnit + lane >= sees) v = -INFINITY;
@@ -1331,18 +1331,14 @@ __global__ void __launch_bounds__(kFewThreads, 1)
         if (++out == kFewStages) out = 0;
       };
       const int n = u1 - u0;
-      scores();
-      put_scores();
+      scores(0);
       few_sync();
       for (int i = 0; i < n; ++i) {
+        if (scores_first && i + 1 < n) scores(i + 1);
         softmax(i);
         if (i > 0) values(i - 1);
-        if (i + 1 < n) scores();
-        few_sync();   // the unit's scores are read, its probabilities written
-        if (i + 1 < n) {
-          put_scores();
-          few_sync();
-        }
+        if (!scores_first && i + 1 < n) scores(i + 1);
+        few_sync();   // the unit's probabilities and the next one's scores are written, what they replace is read
       }
       values(n - 1);
       slot = in;
