@@ -266,9 +266,9 @@ typedef struct kk3_cache_mass_args {
 int64_t kk3_cache_mass_workspace(void);
 int kk3_cache_mass(const kk3_cache_mass_args* args, void* stream);
 
-/* Eviction: each sequence keeps min(lengths[b], budget) positions: its first `sinks`, its last `recent`
- * (sinks + recent <= budget), and of the others those of the largest mass (equal ones: the lowest position; a NaN
- * counts as the largest). The kept entries move, in ascending order, to positions 0, 1, ... of dst_table's pages
+/* Eviction: each sequence keeps min(lengths[b], budget) positions: its first `sinks` and its last `recent`
+ * (the lowest of them where they are more), and of the others those of the largest mass (equal ones: the lowest
+ * position; a NaN counts as the largest). The kept entries move, in ascending order, to positions 0, 1, ... of dst_table's pages
  * (pages that no listed sequence uses: shared pages stay as they are), or in place (dst_table = NULL; then no two
  * sequences may share a page). new_lengths,
  * new_mass (the kept positions' mass, zeros behind) and kept (their old positions, -1 behind) are other buffers than

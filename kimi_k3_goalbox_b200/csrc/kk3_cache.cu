@@ -254,9 +254,11 @@ __global__ void __launch_bounds__(kEvThreads) kk3_cache_select_kernel(const Evic
   const float* mass = a.mass + (long long)b * a.mass_row;
   float* out = a.new_mass + (long long)b * cap;
   int* kept = a.kept + (long long)b * a.budget;
-  const int sinks = min(a.sinks, len), tail = max(sinks, len - a.recent);   // free positions: [sinks, tail)
+  const int sinks = min(a.sinks, keep), tail = max(sinks, len - a.recent);   // free positions: [sinks, tail)
   unsigned border = 0xffffffffu;   // what stays lies above
   int want = keep - (sinks + len - tail);   // free positions to keep; at the end: those at the border
+  const int end = len + min(want, 0);   // of the protected positions that stay: the lowest ones where not all can
+  want = max(want, 0);
   const bool all = keep == len, held = len <= kEvHeld;
   const auto key = [&](int p) { return held ? held_keys[p] : mass_key(mass[p]); };
   if (!all && want > 0) {
@@ -316,7 +318,8 @@ __global__ void __launch_bounds__(kEvThreads) kk3_cache_select_kernel(const Evic
   const bool keyed = border != 0xffffffffu || want > 0;   // else no free position stays, or all do
   const auto state = [&](int p) -> int {   // 0 dropped, 1 kept, 2 kept if among the first `want` at the border
     if (p >= w1) return 0;
-    if (all || p < sinks || p >= tail) return 1;
+    if (all || p < sinks) return 1;
+    if (p >= tail) return p < end;
     if (!keyed) return 0;
     const unsigned k = key(p);
     return k > border ? 1 : k == border && want > 0 ? 2 : 0;
@@ -573,7 +576,7 @@ extern "C" int kk3_cache_evict(const kk3_cache_evict_args* x, void* stream) {
   if (rc) return rc;
   const int budget = x->budget;
   if (!cache_aligned(x->lengths, 8) || !cache_aligned(x->mass, 4) || x->mass_stride < 0 || budget < 1 || x->sinks < 0 ||
-      x->recent < 0 || (int64_t)x->sinks + x->recent > budget || !cache_aligned(x->new_lengths, 8) ||
+      x->recent < 0 || !cache_aligned(x->new_lengths, 8) ||
       !cache_aligned(x->new_mass, 4) || !cache_aligned(x->kept, 4) || x->lengths == x->new_lengths || x->mass == x->new_mass)
     return KK3_ERR_ARG;
   const int64_t cap = (int64_t)x->cache.columns * x->cache.page_size;

@@ -325,8 +325,9 @@ def attention_mass(q_latent, q_pe, lse, kv, pe, table, lengths, cu_new, *, scale
 
 def evict(kv, pe, table, lengths, mass, budget: int, *, sinks: int = 0, recent: int = 0, dst_table=None,
           error_word=None) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
-    """Cut every sequence down to `budget` positions: its first `sinks`, its last `recent`, and of the others those of
-    the largest mass (equal ones: the lowest position; NaN counts as the largest).
+    """Cut every sequence down to `budget` positions: its first `sinks` and its last `recent` (the lowest of them where
+    they are more than the budget), and of the others those of the largest mass (equal ones: the lowest position; NaN
+    counts as the largest).
 
     The kept entries move, in ascending order, to positions 0, 1, ... of dst_table's pages (int32 [B, columns2]; pages
     that none of the sequences uses, so that pages shared with others stay as they are), or in place (None; then no two
@@ -341,8 +342,8 @@ def evict(kv, pe, table, lengths, mass, budget: int, *, sinks: int = 0, recent: 
     budget, sinks, recent = int(budget), int(sinks), int(recent)
     if not 1 <= budget <= capacity:
         raise ValueError("budget must be 1 .. columns * page_size")
-    if sinks < 0 or recent < 0 or sinks + recent > budget:
-        raise ValueError("sinks + recent must not exceed the budget")
+    if not 0 <= sinks <= MAX_POSITIONS or not 0 <= recent <= MAX_POSITIONS:
+        raise ValueError(f"sinks and recent must be 0 .. {MAX_POSITIONS}")
     dst, dst_row, dst_columns = 0, 0, 0
     if dst_table is not None:
         if not isinstance(dst_table, torch.Tensor) or dst_table.dim() != 2:

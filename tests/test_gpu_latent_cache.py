@@ -343,7 +343,7 @@ def test_outputs_that_do_not_fit_are_refused():
     with pytest.raises(ValueError, match="heads"):
         lc.attend(torch.zeros((2, 129, 512), dtype=BF, device="cuda"), torch.zeros((2, 129, 64), dtype=BF, device="cuda"), *args[2:])
     mass = torch.zeros((2, 32), device="cuda")
-    for budget, sinks, recent in ((0, 0, 0), (33, 0, 0), (8, 5, 4), (8, -1, 0)):
+    for budget, sinks, recent in ((0, 0, 0), (33, 0, 0), (8, 0, -1), (8, -1, 0), (8, 1 << 40, 0)):
         with pytest.raises(ValueError):
             lc.evict(*x.cache, x.lengths, mass, budget, sinks=sinks, recent=recent)
     with pytest.raises(ValueError, match="hold the budget"):
@@ -433,7 +433,7 @@ def _kept(mass, length, budget, sinks, recent):
     guarded = [p for p in range(length) if p < sinks or p >= length - recent]
     rest = [p for p in range(length) if sinks <= p < length - recent]
     rest.sort(key=lambda p: (0 if math.isnan(m[p]) else 1, 0.0 if math.isnan(m[p]) else -m[p], p))
-    return sorted(guarded + rest[:keep - len(guarded)])
+    return sorted((guarded + rest)[:keep])
 
 
 def _mass(kind, B, n, gen):
@@ -459,6 +459,10 @@ EVICTIONS = [
     ([2100], 64, 1, 0, 0),
     ([700, 300], 48, 300, 150, 150),      # nothing but protected positions
     ([513, 40], 1, 512, 1, 0),
+    ([60, 9, 4, 5], 16, 4, 4, 1),         # more protected positions than the budget
+    ([100, 50, 3], 16, 10, 7, 20),
+    ([40, 10], 8, 5, 9, 1000),
+    ([64, 30], 16, 16, 0, 16),
     ([40000, 33000, 20], 64, 20000, 5, 9),
 ]
 

@@ -114,7 +114,7 @@ def test_entry_points_refuse_bad_caches(op, change):
         {"cu_new": 0}, {"tokens": -1}, {"heads": 0}, {"heads": 129}, {"scale": float("nan")}, {"tokens": 1 << 30})],
     ("attend", {"out": 0}), ("attend", {"out": P + 8}), ("mass", {"new_mass": 0}), ("mass", {"mass": P + 2}), ("mass", {"mass_stride": -1, "mass": P}),
     *[("evict", c) for c in ({"mass": 0}, {"mass_stride": -1}, {"budget": 0}, {"budget": 65}, {"sinks": -1}, {"recent": -1},
-                             {"sinks": 5, "recent": 4}, {"kept": 0}, {"new_mass": 0}, {"new_lengths": 0}, {"new_mass": P}, {"new_lengths": P},
+                             {"kept": 0}, {"new_mass": 0}, {"new_lengths": 0}, {"new_mass": P}, {"new_lengths": P},
                              {"dst_table": P + 2}, {"dst_table": P, "dst_columns": 0}, {"dst_table": P, "dst_columns": 4, "dst_stride": -4})]])
 def test_entry_points_refuse_bad_arguments(op, change):
     assert _refusal(op, **change) in (ERR_ARG, ERR_UNSUPPORTED)
