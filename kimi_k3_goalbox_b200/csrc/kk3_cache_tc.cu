@@ -267,7 +267,7 @@ KK3_DEV void with_box(int box, const F& f) {
 // tile's sums, then 3.7 us a tile, the rate of HBM.
 
 constexpr int kMassPos = 256;
-constexpr int kMassThreads = 320;   // warps 0-7 sums, 8 copies, 9 matrix instructions and TMEM
+constexpr int kMassSums = 256, kMassThreads = kMassSums + 64;   // warps 0-7 sums, 8 copies, 9 matrix instructions and TMEM
 constexpr int kMassKBlock = 128 * 128;
 constexpr int kMassRing = 65536;
 constexpr int kMassSlots = 16;
@@ -285,8 +285,10 @@ constexpr int kMassSmem = kBlocks * kMassKBlock + kMassRing + (int)sizeof(MassCt
 static_assert(kMassSmem <= 232448, "shared memory of a CTA");
 
 // What the call leaves as it is: positions behind the sequences' ends, and sequences without new tokens. The CTAs are
-// dealt out to the sequences; `threads` threads of each take part.
-KK3_DEV void mass_rest(const MassArgs& a, int tid, int threads) {
+// dealt out to the sequences; the first kMassSums threads of each take part, in CTAs with tiles and without alike: the
+// CTAs of a sequence take its positions in turn, so their steps have to be of one width.
+KK3_DEV void mass_rest(const MassArgs& a, int tid) {
+  if (tid >= kMassSums) return;
   const long long cap = (long long)a.c.columns * a.c.page_size;
   const int per = max(1, (int)gridDim.x / a.c.batch), groups = gridDim.x / per;
   if ((int)blockIdx.x >= groups * per) return;
@@ -294,7 +296,7 @@ KK3_DEV void mass_rest(const MassArgs& a, int tid, int threads) {
     const Seq s = a.seq(b);
     const float* from = a.mass ? a.mass + b * a.mass_row : nullptr;
 #pragma unroll 4
-    for (long long p = (s.n > 0 ? s.len : 0) + (int)(blockIdx.x % per) * threads + tid; p < cap; p += per * threads)
+    for (long long p = (s.n > 0 ? s.len : 0) + (int)(blockIdx.x % per) * kMassSums + tid; p < cap; p += per * kMassSums)
       a.out[b * cap + p] = from ? from[p] : 0.0f;
   }
 }
@@ -333,7 +335,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMassThreads, 1)
   cache_go_on();
   if (tid == 0 && rank == 0) a.meta[worker * 4 + 2] = 0;
   if (worker >= sh.workers) {   // both CTAs of the pair
-    mass_rest(a, tid, kMassThreads);
+    mass_rest(a, tid);
     cluster_wait();
     return;
   }
@@ -433,7 +435,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMassThreads, 1)
     __syncwarp();
   } else {
     // ---- sums: thread = position; warps 0-3 take the first half of the columns, warps 4-7 the second
-    mass_rest(a, tid, 256);
+    mass_rest(a, tid);
     const unsigned tlane = (unsigned)((warp & 3) * 32) << 16, lead_dempty = in_cta(dempty, 0);
     const int group = warp >> 2, row = tid & 127;
     int unit = 0;

@@ -700,3 +700,41 @@ def test_attend_agrees_with_the_step_oracle():
             mag = torch.softmax(s, -1) @ c.abs()
             # both sides round the probabilities and the result once: 2^-8 of the summed magnitudes and of the value each
             assert bool(((out.to(F64) - want).abs() <= 2 * 2 ** -8 * 1.05 * (mag + want.abs())).all())
+
+
+# --- caches with room to grow --------------------------------------------------------------------------------------
+
+ROOMY = [
+    # new tokens, cached positions, heads, page size, positions that the table has room for
+    ([1], [517], 12, 16, 8192),
+    ([1], [100], 12, 64, 1024),
+    ([1], [500], 12, 64, 131072),
+    ([1] * 16, [600] * 16, 12, 64, 8192),
+    ([1] * 8, [300] * 8, 12, 64, 8192),
+    ([1, 0], [300, 229], 12, 16, 4096),      # a sequence without new tokens beside a short one
+    ([1, 1], [300, 300], 12, 8, 4096),
+    ([40, 3], [333, 90], 96, 10, 8190),
+    ([1, 2, 0, 1], [1, 2, 0, 3000], 1, 1, 5000),
+    ([1] * 200, [1 + (53 * i) % 300 for i in range(200)], 3, 32, 1024),   # more sequences than CTAs
+    ([0, 0], [90, 0], 4, 16, 2048),          # nothing new at all
+]
+
+
+@pytest.mark.parametrize("new,lengths,heads,page,capacity", ROOMY)
+def test_mass_with_room_behind_the_lengths(new, lengths, heads, page, capacity):
+    """Every position behind a length keeps its mass (zero without one), however far the table goes on."""
+    x = Problem(61, new, lengths, heads, page)
+    table = torch.full((len(new), capacity // page), -1, dtype=torch.int32, device="cuda")
+    table[:, :x.columns] = x.table
+    cache = (x.kv, x.pe, table)
+    out, lse = lc.attend(x.q_latent, x.q_pe, *cache, x.lengths, x.cu_new)
+    x.check_attend(out, lse)
+    args = (x.q_latent, x.q_pe, lse, *cache, x.lengths, x.cu_new)
+    before = torch.rand((len(new), capacity), generator=x.gen, device="cuda")
+    for mass in (None, before):
+        got = torch.full((len(new), capacity), math.nan, device="cuda")
+        assert lc.attention_mass(*args, mass=mass, out=got) is got
+        x.check_mass(got, torch.zeros_like(before) if mass is None else mass, lse)
+    mine = before.clone()
+    lc.attention_mass(*args, mass=mine, out=mine)
+    assert torch.equal(mine, got)
