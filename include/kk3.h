@@ -193,8 +193,9 @@ typedef struct kk3_cache {
 /* Append: for each new token i of sequence b, position lengths[b] + i gets the entry of its projection row
  * raw[t] (bf16 [tokens, 576], the step's `ka` product): latent = x / sqrt(mean(x^2) + eps) * norm_weight over the
  * first 512 values (FP32, one rounding), rope part as it is. new_lengths[b] = lengths[b] + new tokens (another buffer
- * than lengths). A token that does not fit behind the last column is not written. Sequences may share pages, but no
- * two may write to one slot. */
+ * than lengths). A token that does not fit behind the last column is not written, nor are the tokens of a sequence whose
+ * length is negative (both set the error word; new_lengths[b] is then of the clamped length, at most columns *
+ * page_size). Sequences may share pages, but no two may write to one slot. */
 typedef struct kk3_cache_append_args {
     kk3_cache cache;
     const void* raw;             /* bf16 [tokens, 576], row stride raw_stride */

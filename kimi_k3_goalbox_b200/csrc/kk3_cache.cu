@@ -48,8 +48,8 @@ __global__ void __launch_bounds__(kAppendWarps * 32) kk3_cache_append_kernel(con
   }
   const int first = a.cu_new[lo];
   if (tok < first || tok >= a.cu_new[lo + 1] || first < 0) return;   // behind the last sequence: no one's token
-  const long long pos = min(max(a.lengths[lo], 0ll), cap) + (tok - first);
-  if (pos >= cap) return;
+  const long long held = a.lengths[lo], pos = min(held, cap) + (tok - first);
+  if (held < 0 || pos >= cap) return;   // no place that the sequence could mean
   int slot;
   const int page = page_at(a.c, lo, (int)pos, &slot);
   if (page < 0) return;

@@ -738,3 +738,22 @@ def test_mass_with_room_behind_the_lengths(new, lengths, heads, page, capacity):
     mine = before.clone()
     lc.attention_mass(*args, mass=mine, out=mine)
     assert torch.equal(mine, got)
+
+
+def test_append_writes_nothing_for_a_negative_length():
+    """A length below zero is reported and no token of its sequence is written, though the table has pages for them."""
+    x = Problem(63, [4, 2, 3], [30, 20, 10], 1, 16)
+    raw = torch.randn((9, 576), generator=x.gen, device="cuda").to(BF)
+    weight = torch.rand(512, generator=x.gen, device="cuda").to(BF)
+    error = torch.zeros(1, dtype=torch.int32, device="cuda")
+    for length in (-1, -3, -16, -2 ** 31, -2 ** 40, -2 ** 63):
+        kv0, pe0 = x.kv.clone(), x.pe.clone()
+        error.zero_()
+        lc.append(raw, weight, *x.cache, torch.tensor([5, length, 7], device="cuda"), x.cu_new, error_word=error)
+        assert error.item() != 0
+        written = torch.zeros(x.kv.shape[:2], dtype=torch.bool, device="cuda")
+        written[x.table[0, 0].long(), 5:9] = True
+        written[x.table[2, 0].long(), 7:10] = True
+        assert torch.equal(x.kv[~written].view(torch.int16), kv0[~written].view(torch.int16))
+        assert torch.equal(x.pe[~written].view(torch.int16), pe0[~written].view(torch.int16))
+        assert torch.equal(x.pe[x.table[2, 0].long(), 7:10], raw[6:, 512:])
