@@ -209,6 +209,11 @@ typedef struct kk3_cache_append_args {
     float eps;
 } kk3_cache_append_args;
 int kk3_cache_append(const kk3_cache_append_args* args, void* stream);
+/* The same with the decode step's rounding: x / sqrt(mean(x^2) + eps) is rounded to BF16 before the product with
+ * norm_weight, and the product again, as kk3_step and the model do (common.py:13-21). For caches that kk3_step_append
+ * continues: apart from the order of the FP32 sum of squares the entry is the step's kv_write of the same row (with one
+ * rounding a quarter of the values differ from it by a rounding, unless the weight is one). */
+int kk3_cache_append_step(const kk3_cache_append_args* args, void* stream);
 
 /* Attention of the new tokens over their sequence's cache in the latent space. `lengths` includes the new tokens
  * (already appended): token i of n sees the first lengths[b] - n + i + 1 positions. Per token and head

@@ -8,8 +8,9 @@
 namespace kk3 {
 
 // ---------------------------------------------------------------------------------------------
-// append: latent = x[:512] / rms(x[:512]) * weight (FP32, rounded to BF16 once), rope = x[512:], into the page of the
-// token's position. One warp per token, bound by its 2304 bytes of traffic; 16-byte accesses throughout (lane l owns
+// append: latent = x[:512] / rms(x[:512]) * weight, rope = x[512:], into the page of the token's position. In FP32, rounded
+// to BF16 once, or (STEP) as the decode step and the model round it: to BF16 before the product with the weight, and
+// after it (kimi.py:268, common.py:13-21), so that the entry is the one that the step would have cached. One warp per token, bound by its 2304 bytes of traffic; 16-byte accesses throughout (lane l owns
 // the latent values 8 l .. 8 l + 7 and 256 + 8 l ..; eight lanes copy the rope part). Five chunks of up to 4096 tokens take
 // 7.2 us, 5.2 TB/s; eight single tokens 2.7 us, a launch.
 
@@ -27,6 +28,7 @@ struct AppendArgs {
 
 constexpr int kAppendWarps = 4;
 
+template <bool STEP>
 __global__ void __launch_bounds__(kAppendWarps * 32) kk3_cache_append_kernel(const AppendArgs a) {
   const int lane = threadIdx.x & 31;
   const int tok = blockIdx.x * kAppendWarps + (threadIdx.x >> 5);
@@ -80,8 +82,11 @@ __global__ void __launch_bounds__(kAppendWarps * 32) kk3_cache_append_kernel(con
     const __nv_bfloat162* q = reinterpret_cast<const __nv_bfloat162*>(&w[h]);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const float2 f = __bfloat1622float2(p[i]), g = __bfloat1622float2(q[i]);
-      p[i] = __floats2bfloat162_rn(f.x * r * g.x, f.y * r * g.y);
+      float2 f = __bfloat1622float2(p[i]);
+      const float2 g = __bfloat1622float2(q[i]);
+      f = make_float2(f.x * r, f.y * r);
+      if (STEP) f = make_float2(round_bf(f.x), round_bf(f.y));
+      p[i] = __floats2bfloat162_rn(f.x * g.x, f.y * g.y);
     }
     *reinterpret_cast<uint4*>(kv + h * 256 + lane * 8) = v[h];
   }
@@ -487,7 +492,8 @@ int cache_sms(int* sms) {
 
 }  // namespace kk3
 
-extern "C" int kk3_cache_append(const kk3_cache_append_args* x, void* stream) {
+template <bool STEP>
+static int cache_append(const kk3_cache_append_args* x, void* stream) {
   if (!x) return KK3_ERR_ARG;
   AppendArgs a;
   const int rc = cache_pages(&x->cache, &a.c, x->error_word);
@@ -505,9 +511,12 @@ extern "C" int kk3_cache_append(const kk3_cache_append_args* x, void* stream) {
   a.tokens = x->tokens;
   a.eps = x->eps;
   const int grid = x->tokens > 0 ? (x->tokens + kAppendWarps - 1) / kAppendWarps : 1;
-  kk3_cache_append_kernel<<<grid, kAppendWarps * 32, 0, (cudaStream_t)stream>>>(a);
+  kk3_cache_append_kernel<STEP><<<grid, kAppendWarps * 32, 0, (cudaStream_t)stream>>>(a);
   return cache_cuda(cudaGetLastError(), "kk3_cache_append_kernel");
 }
+
+extern "C" int kk3_cache_append(const kk3_cache_append_args* x, void* stream) { return cache_append<false>(x, stream); }
+extern "C" int kk3_cache_append_step(const kk3_cache_append_args* x, void* stream) { return cache_append<true>(x, stream); }
 
 // The kernel and its workers. Up to 16 rows a sequence on average fill the small tile: 64 sequences of 8192 positions
 // with 12 rows each take 129 us in it and 187 us in CTA pairs; with 24 rows, two small tiles that read the cache twice,

@@ -47,7 +47,7 @@ def _lib() -> ctypes.CDLL:
     global _LIB
     if _LIB is None:
         lib = load_library()
-        for name in ("append", "attend", "mass", "evict"):
+        for name in ("append", "append_step", "attend", "mass", "evict"):
             getattr(lib, f"kk3_cache_{name}").argtypes = [ctypes.c_char_p, ctypes.c_void_p]
         for name in ("attend", "mass"):
             getattr(lib, f"kk3_cache_{name}_workspace").argtypes = []
@@ -229,12 +229,14 @@ def _workspace(what: str, device: torch.device) -> tuple[torch.Tensor, int]:
 
 # --- the operators ---------------------------------------------------------------------------------------------
 
-def append(raw, norm_weight, kv, pe, table, lengths, cu_new, *, eps: float = 1e-6, error_word=None) -> torch.Tensor:
+def append(raw, norm_weight, kv, pe, table, lengths, cu_new, *, eps: float = 1e-6, as_step: bool = False,
+           error_word=None) -> torch.Tensor:
     """Write the new tokens' entries behind their sequences and return the new lengths (int64 [B]).
 
     raw: bf16 [T, 576], the `ka` projection of the new tokens; its first 512 values are RMS-normalised with
-    norm_weight (bf16 [512]) in FP32 and rounded once, the other 64 are stored as they are. lengths: positions cached
-    before. A token behind the table's last column is not written, nor are those of a sequence whose length is negative
+    norm_weight (bf16 [512]) in FP32 and rounded once, the other 64 are stored as they are. as_step: rounded to bf16
+    before the product with norm_weight too, as the model and the decode step do; caches that `step_append` continues
+    want this, so that the entry is the one the step would have written. lengths: positions cached before. A token behind the table's last column is not written, nor are those of a sequence whose length is negative
     (its new length then counts from zero); both set error_word."""
     cache, dev, B, _ = _cache(kv, pe, table)
     try:
@@ -261,8 +263,8 @@ def append(raw, norm_weight, kv, pe, table, lengths, cu_new, *, eps: float = 1e-
     if not eps >= 0:
         raise ValueError("eps must not be negative")
     out = torch.empty_like(lengths)
-    _run("kk3_cache_append", dev, _APPEND.pack(*cache, at, row, weight, lengths.data_ptr(), cu_new.data_ptr(), out.data_ptr(),
-                                               _error(error_word, dev), T, eps))
+    _run("kk3_cache_append_step" if as_step else "kk3_cache_append", dev, _APPEND.pack(
+        *cache, at, row, weight, lengths.data_ptr(), cu_new.data_ptr(), out.data_ptr(), _error(error_word, dev), T, eps))
     return out
 
 

@@ -757,3 +757,79 @@ def test_append_writes_nothing_for_a_negative_length():
         assert torch.equal(x.kv[~written].view(torch.int16), kv0[~written].view(torch.int16))
         assert torch.equal(x.pe[~written].view(torch.int16), pe0[~written].view(torch.int16))
         assert torch.equal(x.pe[x.table[2, 0].long(), 7:10], raw[6:, 512:])
+
+
+# --- entries as the step writes them -------------------------------------------------------------------------------
+
+def _step_entries(raw, weight, eps):
+    """The two values that an entry rounded as the step's can take: bf16(bf16(x rs) w), where the FP32 rs and its product
+    are within 2^-20 of the exact ones (the sum of squares, its root and a product, as for append), so that the inner
+    rounding gives `low` or `high`, which agree but next to a tie. A product of two bf16 values is exact in FP32."""
+    x = raw[:, :512].to(F64)
+    y = x * torch.rsqrt((x * x).mean(-1, keepdim=True) + eps)
+    low, high = (((y * (1 + d)).to(F32).to(BF).to(F32) * weight.to(F32)).to(BF) for d in (-2 ** -20, 2 ** -20))
+    return low, high
+
+
+@pytest.mark.parametrize("kind", ["near one", "wide", "one"])
+@pytest.mark.parametrize("new,lengths,page", [([1], [0], 16), ([33, 0, 70], [5, 9, 100], 10), ([300], [1], 1)])
+def test_append_as_the_step_rounds(new, lengths, page, kind):
+    total = [n + m for n, m in zip(new, lengths)]
+    x = Problem(65, new, total, 1, page)
+    raw = torch.randn((x.T, 576), generator=x.gen, device="cuda").to(BF)
+    weight = {"near one": 1 + 0.1 * torch.randn(512, generator=x.gen, device="cuda"),
+              "wide": torch.randn(512, generator=x.gen, device="cuda") * 3, "one": torch.ones(512, device="cuda")}[kind].to(BF)
+    before = torch.tensor(lengths, device="cuda")
+    assert lc.append(raw, weight, *x.cache, before, x.cu_new, eps=1e-5, as_step=True).tolist() == total
+    low, high = _step_entries(raw, weight, 1e-5)
+    for b in range(len(new)):
+        pos = torch.arange(lengths[b], total[b], device="cuda")
+        pages, slots = x.table[b, pos // page].long(), pos % page
+        rows = slice(x.cu[b], x.cu[b + 1])
+        got = x.kv[pages, slots]
+        assert bool(((got == low[rows]) | (got == high[rows])).all())
+        assert torch.equal(x.pe[pages, slots], raw[rows, 512:])
+
+
+def test_append_writes_the_entry_that_the_step_writes():
+    """The step's own `ka` products of a layer, appended, against the entry that the step cached for them."""
+    from kimi_k3_goalbox_b200.runtime import StepContext
+    from oracle import kimi_oracle as ko
+    from tests import gpu_helpers as gh
+    from tests import test_gpu_append as ta
+
+    B, capacity = 3, 32
+    case = gh.small_case(B, context=capacity)
+    last = ko.mla_layer_ids(case)[-1]     # the layer whose products the scratch buffer holds after the step
+    q_rank = case["params"]["q_lora_rank"]
+    with torch.inference_mode():
+        values = ko.make_inputs(case, 67, "cuda")
+        weight = (1 + 0.1 * torch.randn(512, generator=torch.Generator(device="cuda").manual_seed(3), device="cuda")).to(BF)
+        values[f"l{last}_kn"] = weight
+        lengths = torch.tensor([9, 0, 30], dtype=torch.int64, device="cuda")
+        values["reset"] = torch.zeros(B, dtype=torch.bool, device="cuda")
+        conv, rec = ta._stacked_states(case, values)
+        ctx = StepContext(case)
+        try:
+            outputs = ctx.allocate_outputs()
+            outputs["conv_state"], outputs["recurrent_state"] = conv, rec
+            ctx.step_append(values, outputs, lengths)
+            torch.cuda.synchronize()
+            ctx.check()
+            raw = ctx.debug_buffer(gh.BUF["qkv"], BF, (B * (q_rank + 576),))[B * q_rank:].view(B, 576).clone()
+            step, step_pe = outputs["kv_write"][-1].clone(), outputs["pe_write"][-1].clone()
+        finally:
+            ctx.close()
+        assert torch.equal(raw[:, 512:], step_pe)     # these are that layer's products
+        kv, pe, table = lc.paged_view(torch.zeros((B, capacity, 512), dtype=BF, device="cuda"),
+                                      torch.zeros((B, capacity, 64), dtype=BF, device="cuda"), 8)
+        one = torch.arange(B + 1, dtype=torch.int32, device="cuda")
+        assert lc.append(raw, weight, kv, pe, table, lengths, one, as_step=True).tolist() == [10, 1, 31]
+        rows = torch.arange(B, device="cuda")
+        got = kv.view(B, capacity, 512)[rows, lengths]
+        low, high = _step_entries(raw, weight, 1e-6)
+        assert bool(((got == step) | (low != high)).all())
+        for entry in (got, step):
+            assert bool(((entry == low) | (entry == high)).all())
+        assert torch.equal(got, values[f"l{last}_kv_cache"][rows, lengths]) or bool((low != high).any())
+        assert torch.equal(pe.view(B, capacity, 64)[rows, lengths], values[f"l{last}_pe_cache"][rows, lengths])
