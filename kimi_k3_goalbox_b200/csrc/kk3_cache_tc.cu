@@ -332,6 +332,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMassThreads, 1)
   __syncwarp();
   cluster_arrive();   // the peer's barriers are needed after the plan
   const Share sh = plan_share<kMassThreads>(a, split, worker, 1, base, ctl.red);
+  fence_async_smem();   // the plan of a large call lay where the copies come
   cache_go_on();
   if (tid == 0 && rank == 0) a.meta[worker * 4 + 2] = 0;
   if (worker >= sh.workers) {   // both CTAs of the pair
@@ -653,6 +654,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPaThreads, 1)
   cluster_arrive();   // the peer's barriers are needed after the plan
   const AttendSplit split{kPairRows, a.heads, kPaUnit, kPaTileCost};
   const Share sh = plan_share<kPaThreads>(a, split, worker, kPaMinUnits, smem_raw, ctl.red);
+  fence_async_smem();   // the plan of a large call lay where the copies come
   cache_go_on();
   if (tid == 0 && rank == 0) a.meta[worker * 4 + 2] = 0;
   tc_fence_before();
@@ -1189,10 +1191,10 @@ __global__ void __launch_bounds__(kFewThreads, 1)
   int slot = 0;   // the ring's stage, in turn `phase`
   unsigned phase = 0;
   bool ok = true;
-  __syncthreads();   // the plan's readers are done with the ring
+  fence_async_smem();   // the plan of a large call lay where the copies come
+  __syncthreads();      // its readers are done with the ring
 
   if (warp >= kFewWork / 32) {
-    fence_async_smem();
     const int part = warp - kFewWork / 32;
     Seq s = sh.seq;
     for (; at < sh.end && ok; ++t) {

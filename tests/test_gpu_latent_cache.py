@@ -833,3 +833,25 @@ def test_append_writes_the_entry_that_the_step_writes():
             assert bool(((entry == low) | (entry == high)).all())
         assert torch.equal(got, values[f"l{last}_kv_cache"][rows, lengths]) or bool((low != high).any())
         assert torch.equal(pe.view(B, capacity, 64)[rows, lengths], values[f"l{last}_pe_cache"][rows, lengths])
+
+
+# --- plans that pass through shared memory -------------------------------------------------------------------------
+
+@pytest.mark.parametrize("new,lengths,heads,page", [
+    ([11 + i % 7 for i in range(140)], [30 + (41 * i) % 700 for i in range(140)], 24, 16),    # more than 128 sequences
+    ([700, 1], [1500, 900], 24, 64),                                                          # more than 32 tiles in one
+    ([1] * 200, [300 + (59 * i) % 800 for i in range(200)], 12, 10),
+    ([2, 1], [9001, 20000], 31, 10),                                                          # likewise, positions
+])
+def test_large_plans_before_the_copies(new, lengths, heads, page):
+    """Calls whose work split lies, while it is computed, in the shared memory that the first copies fill."""
+    x = Problem(71, new, lengths, heads, page)
+    before = torch.zeros((len(new), x.columns * page), device="cuda")
+    out, lse = lc.attend(x.q_latent, x.q_pe, *x.cache, x.lengths, x.cu_new)
+    x.check_attend(out, lse)
+    mass = lc.attention_mass(x.q_latent, x.q_pe, lse, *x.cache, x.lengths, x.cu_new)
+    x.check_mass(mass, before, lse)
+    for _ in range(10):
+        out2, lse2 = lc.attend(x.q_latent, x.q_pe, *x.cache, x.lengths, x.cu_new)
+        assert torch.equal(out, out2) and torch.equal(lse, lse2)
+        assert torch.equal(mass, lc.attention_mass(x.q_latent, x.q_pe, lse, *x.cache, x.lengths, x.cu_new))
