@@ -391,6 +391,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMassThreads, 1)
           }
         }
       });
+      __syncwarp();   // the table is read
       at += units;
       ++t;
       ++tile;

@@ -855,3 +855,17 @@ def test_large_plans_before_the_copies(new, lengths, heads, page):
         out2, lse2 = lc.attend(x.q_latent, x.q_pe, *x.cache, x.lengths, x.cu_new)
         assert torch.equal(out, out2) and torch.equal(lse, lse2)
         assert torch.equal(mass, lc.attention_mass(x.q_latent, x.q_pe, lse, *x.cache, x.lengths, x.cu_new))
+
+
+@pytest.mark.parametrize("new,heads", [(1, 12), (9, 40)])
+@pytest.mark.parametrize("page", [10, 1, 16])
+def test_mass_of_several_tiles_a_worker(new, heads, page):
+    """Tiles follow one another in a worker, each with its own table of rows, from which odd pages are gathered."""
+    B = 24
+    lengths = [2600 + 61 * i for i in range(B)]      # 264 or more tiles, over fewer workers
+    x = Problem(73, [new] * B, lengths, heads, page)
+    _, lse = lc.attend(x.q_latent, x.q_pe, *x.cache, x.lengths, x.cu_new)
+    mass = lc.attention_mass(x.q_latent, x.q_pe, lse, *x.cache, x.lengths, x.cu_new)
+    x.check_mass(mass, torch.zeros_like(mass), lse)
+    for _ in range(5):
+        assert torch.equal(mass, lc.attention_mass(x.q_latent, x.q_pe, lse, *x.cache, x.lengths, x.cu_new))
