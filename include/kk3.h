@@ -178,7 +178,8 @@ int kk3_step_noalloc(const kk3_config* cfg, const void* const* table, int table_
  * stride a multiple of its row's. Calls
  * enqueue kernels on `stream` and return; nothing is allocated or read back, so they can be captured. A table entry
  * outside the pool or a length outside [0, columns * page_size] is clamped (the position reads as zeros and is not
- * written) and sets *error_word (optional, zeroed by the caller) to a nonzero device code. What pages hold at or
+ * written) and sets *error_word (optional, zeroed by the caller) to a nonzero device code. So does a wait inside attention
+ * or weight that runs out (two seconds; no healthy call comes near it): what the call then lacks is NaN. What pages hold at or
  * behind a sequence's length is never used. Limits: batch <= 4096, heads <= 128, page_size <= 65536,
  * columns * page_size <= 2^27. */
 typedef struct kk3_cache {

@@ -80,6 +80,10 @@ static __device__ __noinline__ bool pair_wait_on(int* error_word, unsigned bar, 
     }
   }
 }
+// What a tile's sums become when a wait of the CTA has run out, so that no caller takes what was allocated or half done
+// for a result: NaN, which the division by a row's sum and the join of cut tiles carry to all that the tile gives. All
+// of the tile's waits lie before a barrier that its threads pass before they ask.
+KK3_DEV float or_lost(float v, volatile int* dead) { return *dead ? __int_as_float(0x7fffffff) : v; }
 KK3_DEV bool pair_wait(const CachePages& c, unsigned bar, unsigned parity, volatile int* dead) {
   return mbar_test(bar, parity) || pair_wait_on(c.error_word, bar, parity, dead);
 }
@@ -500,8 +504,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMassThreads, 1)
       }
       if (group == 1) ctl.sum[row] = sum;
       asm volatile("bar.sync 1, 256;" ::: "memory");
-      if (group == 0) sum += ctl.sum[row];
-      if (ok && group == 0) {
+      if (group == 0) {
+        sum = or_lost(sum + ctl.sum[row], dead);
         if (u0 == 0 && u1 == units) {
           if (pos < s.len) {
             const long long cap = (long long)a.c.columns * a.c.page_size;
@@ -862,7 +866,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPaThreads, 1)
     // two has every other unit, and where this is asked, the unit three before is known to be added (this thread's part
     // of P was free again from the one two before) and the next one waits for this thread.
     const auto all_added = [&](int m) {
-      return __all_sync(0xffffffffu, m == 0 || pair_wait(a.c, pvdone + 8 * ((m - 1) & 1), ((m - 1) >> 1) & 1, dead)) != 0;
+      __all_sync(0xffffffffu, m == 0 || pair_wait(a.c, pvdone + 8 * ((m - 1) & 1), ((m - 1) >> 1) & 1, dead));
     };
     const float sign = a.scale_log2 < 0.0f ? -1.0f : 1.0f, size = fabsf(a.scale_log2);
     Seq s = sh.seq;
@@ -878,7 +882,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPaThreads, 1)
       float m = -INFINITY, l = 0.0f;
       for (int u = u0; u < u1; ++u, ++n) {
         const int buf = n & 1;
-        ok = __all_sync(0xffffffffu, pair_wait(a.c, sfull + 8 * buf, (n >> 1) & 1, dead)) && ok;
+        __all_sync(0xffffffffu, pair_wait(a.c, sfull + 8 * buf, (n >> 1) & 1, dead));
         tc_fence_after();
         float v[2][32];
         tmem_ld32(tmem_s + buf * 128 + wg * 64 + tlane, v[0]);
@@ -914,7 +918,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPaThreads, 1)
         }
         const float ref = m == -INFINITY ? 0.0f : m;
         if (u > u0 && __any_sync(0xffffffffu, alpha != 1.0f)) {   // rescale, once the unit before has been added
-          ok = all_added(n) && ok;
+          all_added(n);
           tc_fence_after();
 #pragma unroll 1
           for (int c = 0; c < 128; c += 32) {
@@ -951,7 +955,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPaThreads, 1)
           w[i] = *reinterpret_cast<const unsigned*>(&h2);
         }
         // the sums of the unit before have read this part of P
-        if (n > 0) ok = __all_sync(0xffffffffu, pair_wait(a.c, pfree + 8 * part64, (n - 1) & 1, dead)) && ok;
+        if (n > 0) __all_sync(0xffffffffu, pair_wait(a.c, pfree + 8 * part64, (n - 1) & 1, dead));
 #pragma unroll
         for (int c = 0; c < 8; ++c)
           asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};"
@@ -961,12 +965,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPaThreads, 1)
         __syncwarp();
         if (lane == 0) arrive_cluster(lead_pfull);
       }
-      ok = all_added(n) && ok;
+      all_added(n);
       tc_fence_after();
       asm volatile("bar.sync %0, 128;" ::"r"(meet) : "memory");   // the last maxima are read
       ctl.top[0][part64][row] = l;
       asm volatile("bar.sync %0, 128;" ::"r"(meet) : "memory");
-      l = (ctl.top[0][0][row] + ctl.top[0][1][row]) + (ctl.top[0][2][row] + ctl.top[0][3][row]);
+      l = or_lost((ctl.top[0][0][row] + ctl.top[0][1][row]) + (ctl.top[0][2][row] + ctl.top[0][3][row]), dead);
       const bool whole = u0 == 0 && u1 == units;
       const long long out_row = (long long)s.q0 * a.heads + g;
       float* part = a.part + (((long long)worker * 2 + (u0 == 0 ? 1 : 0)) * kPairRows + rank * 64 + row) * kPartRow;
@@ -1004,7 +1008,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPaThreads, 1)
           for (int i = 0; i < 4; ++i) {
             const int r = i * 8 + (lane >> 2), ch = lane & 3;   // row of this warp's 32, and 16 bytes of it
             const uint4 v = *reinterpret_cast<const uint4*>(stage + r * 64 + (ch ^ ((r >> 1) & 3)) * 16);
-            if (ok && r < rows_here) {
+            if (r < rows_here) {
               if (whole) *reinterpret_cast<uint4*>(a.out + (out_row - lane + r) * kLat + dim0 + c + ch * 8) = v;
               else *reinterpret_cast<uint4*>(part + (long long)(r - lane) * kPartRow + dim0 + c + h * 16 + ch * 4) = v;
             }
@@ -1012,7 +1016,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPaThreads, 1)
           __syncwarp();
         }
       }
-      if (ok && live && part64 == 0) {
+      if (live && part64 == 0) {
         if (whole) {
           a.lse[out_row] = (m + log2f(l)) * 0.69314718055994531f;
         } else {
@@ -1020,7 +1024,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPaThreads, 1)
           part[kLat + 1] = l;
         }
       }
-      if (ok && u0 == 0 && u1 < units && tid == 0 && rank == 0) {
+      if (u0 == 0 && u1 < units && tid == 0 && rank == 0) {
         a.meta[worker * 4] = s.q0 * a.heads + t * kPairRows;
         a.meta[worker * 4 + 1] = min(kPairRows, s.n * a.heads - t * kPairRows);
         a.meta[worker * 4 + 2] = sh.holder(at + kPaTileCost + units) - worker + 1;
@@ -1275,7 +1279,7 @@ __global__ void __launch_bounds__(kFewThreads, 1)
       int in = slot, out = slot;
       const auto scores = [&](int i) {
         float c[2][4];
-        ok = pair_wait(a.c, full + 8 * in, phase, dead) && ok;
+        pair_wait(a.c, full + 8 * in, phase, dead);
         const unsigned kb = base + in * kFewStageBytes + kat;
 #pragma unroll
         for (int j = 0; j < 8; ++j) c[j >> 2][j & 3] = 0.0f;   // two chains: a product waits for the one before it on its sums
@@ -1350,7 +1354,7 @@ __global__ void __launch_bounds__(kFewThreads, 1)
       l = warp_sum(l);
       if (lane == 0) {
         ctl.m[warp] = m;
-        ctl.l[warp] = l;
+        ctl.l[warp] = or_lost(l, dead);
       }
       few_sync();
       const long long g = (long long)s.q0 * a.heads + row0;
@@ -1359,7 +1363,7 @@ __global__ void __launch_bounds__(kFewThreads, 1)
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const int r = (lane >> 2) + 8 * h;
-        if (ok && r < rows) {
+        if (r < rows) {
           const int dim = warp * 32 + (lane & 3) * 2;
           const float lr = ctl.l[r], inv = lr > 0.0f || lr != lr ? 1.0f / lr : 0.0f;
 #pragma unroll
@@ -1370,7 +1374,7 @@ __global__ void __launch_bounds__(kFewThreads, 1)
           }
         }
       }
-      if (ok && tid < rows) {
+      if (tid < rows) {
         if (whole) {
           a.lse[g + tid] = (ctl.m[tid] + log2f(ctl.l[tid])) * 0.69314718055994531f;
         } else {
@@ -1378,7 +1382,7 @@ __global__ void __launch_bounds__(kFewThreads, 1)
           part[tid * kPartRow + kLat + 1] = ctl.l[tid];
         }
       }
-      if (ok && !whole && u0 == 0 && tid == 0) {
+      if (!whole && u0 == 0 && tid == 0) {
         a.meta[worker * 4] = (int)g;
         a.meta[worker * 4 + 1] = rows;
         a.meta[worker * 4 + 2] = sh.holder(at + units) - worker + 1;

@@ -11,7 +11,10 @@ gives the packed rows of each sequence's new tokens, `lengths` int64 [B] the cac
 `cache_length`). All on one CUDA device; calls are enqueued on that device's current stream, allocate only through
 torch's allocator, never synchronise and can be captured into a graph. Device-side values are not read by the host: a
 page number outside the pool or a length outside the table reads as zeros, is not written, and sets `error_word`
-(optional int32 tensor, zeroed by the caller) to a nonzero code. There is no CPU path: without the library or a GPU
+(optional int32 tensor, zeroed by the caller) to a nonzero code. Without an error_word such a call is silent, so a
+program that fills its tables on the device should pass one and look at it now and then. A wait inside `attend` or
+`attention_mass` that runs out (two seconds; a defect, no healthy call comes near it) sets it as well, and the results
+that it was for are NaN. There is no CPU path: without the library or a GPU
 these raise.
 """
 

@@ -869,3 +869,26 @@ def test_mass_of_several_tiles_a_worker(new, heads, page):
     x.check_mass(mass, torch.zeros_like(mass), lse)
     for _ in range(5):
         assert torch.equal(mass, lc.attention_mass(x.q_latent, x.q_pe, lse, *x.cache, x.lengths, x.cu_new))
+
+
+# --- lost rows -----------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("new,lengths,heads", [
+    ([1, 1], [8000, 700], 12),         # single tokens, the first one's tile cut between many workers
+    ([1, 3], [90, 50], 12),            # whole tiles
+    ([60, 9], [9000, 333], 24),        # CTA pairs, cut tiles
+    ([300, 40], [300, 40], 24),        # CTA pairs, whole tiles among them
+])
+def test_rows_of_nan_stay_marked_and_alone(new, lengths, heads):
+    """A row whose sums are NaN (here by its query; by a wait that ran out, all rows of a tile) comes out as NaN in all of
+    `out` and `lse`, through a tile's own end and through the join of a cut one, and spoils no other row."""
+    x = Problem(75, new, lengths, heads, 16)
+    q = x.q_latent.clone()
+    bad = [0, x.T - 1, x.T // 2]
+    for i, t in enumerate(bad):
+        q[t, (5 * i) % heads] = math.nan
+    out, lse = lc.attend(q, x.q_pe, *x.cache, x.lengths, x.cu_new)
+    lost = torch.isnan(q[..., 0])
+    assert bool(torch.isnan(out[lost]).all()) and bool(torch.isnan(lse[lost]).all())
+    clean, clean_lse = lc.attend(x.q_latent, x.q_pe, *x.cache, x.lengths, x.cu_new)
+    assert torch.equal(out[~lost], clean[~lost]) and torch.equal(lse[~lost], clean_lse[~lost])
