@@ -248,7 +248,8 @@ int kk3_cache_attend(const kk3_cache_attend_args* args, void* stream);
 
 /* Accumulated attention weight: new_mass[b][p] = mass[b][p] + sum over the sequence's new tokens that see p and over
  * heads of exp(s_p - lse), with kk3_cache_attend's lse (rows with lse = -infinity add nothing). mass (optional, NULL:
- * zeros) and new_mass are f32 [batch, columns * page_size], mass with its own row stride; they may be the same buffer.
+ * zeros) and new_mass are f32 [batch, columns * page_size], mass with its own row stride; they may be the same buffer
+ * where that stride is columns * page_size (KK3_ERR_ARG otherwise), and must not overlap in another way.
  * Positions at or behind the length keep their mass. FP32 sums in a fixed order. Workspace as above, of
  * kk3_cache_mass_workspace() bytes. */
 typedef struct kk3_cache_mass_args {

@@ -1507,6 +1507,8 @@ extern "C" int kk3_cache_mass(const kk3_cache_mass_args* x, void* stream) {
   if (tokens < 0 || heads < 1 || !cache_aligned(x->lengths, 8) || !cache_aligned(x->cu_new, 4) || !(x->scale == x->scale) ||
       !cache_aligned(x->new_mass, 4) || (x->mass && ((uintptr_t)x->mass % 4 || x->mass_stride < 0)))
     return KK3_ERR_ARG;
+  // in place only row by row: with another stride a row is written while a CTA reads the one that lies there
+  if (x->mass == x->new_mass && a.c.batch > 1 && x->mass_stride != (int64_t)a.c.columns * a.c.page_size) return KK3_ERR_ARG;
   if (heads > kMaxHeads || (int64_t)tokens * heads > INT32_MAX / 2) return KK3_ERR_UNSUPPORTED;
   if (tokens > 0 && (!cache_queries(x->q_latent, x->ql_token, x->ql_head, x->q_pe, x->qp_token, x->qp_head) ||
                      !cache_aligned(x->lse, 4)))

@@ -135,3 +135,8 @@ def test_argument_blocks_match_the_header(tmp_path):
     sizes = [int(v) for v in subprocess.run([str(tmp_path / "s")], check=True, capture_output=True, text=True).stdout.split()]
     assert sizes == [layout.size for layout, _ in BLOCKS.values()]
     assert struct.calcsize("=" + lc._CACHE) == sizes[0] - struct.calcsize("=QqQQQQQif")
+
+
+@pytest.mark.parametrize("stride", [0, 32, 63, 65, 128])
+def test_mass_in_place_needs_the_stride_of_the_result(stride):
+    assert _refusal("mass", mass=P, new_mass=P, mass_stride=stride) == ERR_ARG
