@@ -545,7 +545,7 @@ extern "C" int kk3_cache_attend(const kk3_cache_attend_args* x, void* stream) {
   const int rc = cache_pages(&x->cache, &a.c, x->error_word);
   if (rc) return rc;
   const int tokens = x->tokens, heads = x->heads;
-  if (tokens < 0 || heads < 1 || !cache_aligned(x->lengths, 8) || !cache_aligned(x->cu_new, 4) || !(x->scale == x->scale))
+  if (tokens < 0 || heads < 1 || !cache_aligned(x->lengths, 8) || !cache_aligned(x->cu_new, 4) || !cache_scale(x->scale))
     return KK3_ERR_ARG;
   if (heads > kMaxHeads || (int64_t)tokens * heads > INT32_MAX / 2) return KK3_ERR_UNSUPPORTED;
   if (tokens == 0) return KK3_OK;

@@ -19,6 +19,8 @@ inline bool cache_queries(const void* ql, int64_t ql_token, int64_t ql_head, con
   return cache_aligned(ql, 16) && cache_aligned(qp, 16) && ((ql_token | ql_head | qp_token | qp_head) & 7) == 0 && ql_token >= 0 &&
          ql_head >= 0 && qp_token >= 0 && qp_head >= 0;
 }
+// a scale whose product with log2(e), on which the softmax runs, is finite in FP32 (3.40e38 / 1.4427)
+inline bool cache_scale(float scale) { return scale >= -2.35e38f && scale <= 2.35e38f; }
 // checks a kk3_cache and turns it into the kernels' form
 int cache_pages(const kk3_cache* c, CachePages* out, int* error_word);
 // attention (kk3_cache_tc.cu): tiles of kPairRows rows by CTA pairs, of kFewRows by single CTAs; a.workers of them

@@ -1504,7 +1504,7 @@ extern "C" int kk3_cache_mass(const kk3_cache_mass_args* x, void* stream) {
   const int rc = cache_pages(&x->cache, &a.c, x->error_word);
   if (rc) return rc;
   const int tokens = x->tokens, heads = x->heads;
-  if (tokens < 0 || heads < 1 || !cache_aligned(x->lengths, 8) || !cache_aligned(x->cu_new, 4) || !(x->scale == x->scale) ||
+  if (tokens < 0 || heads < 1 || !cache_aligned(x->lengths, 8) || !cache_aligned(x->cu_new, 4) || !cache_scale(x->scale) ||
       !cache_aligned(x->new_mass, 4) || (x->mass && ((uintptr_t)x->mass % 4 || x->mass_stride < 0)))
     return KK3_ERR_ARG;
   // in place only row by row: with another stride a row is written while a CTA reads the one that lies there

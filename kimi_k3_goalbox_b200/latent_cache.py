@@ -29,6 +29,7 @@ from .runtime import KK3Error, load_library
 
 LATENT, ROPE = 512, 64
 DEFAULT_SCALE = (128 + 64) ** -0.5      # (qk_nope_dim + qk_rope_dim) ** -0.5 (megabench/tasks/kimi.py:278)
+MAX_SCALE = 2.35e38                     # its product with log2(e) stays finite in FP32
 MAX_SEQUENCES, MAX_HEADS, MAX_PAGE, MAX_POSITIONS = 4096, 128, 65536, 1 << 27
 
 
@@ -187,8 +188,8 @@ def _queries(q_latent, q_pe, lengths, cu_new, dev: int, B: int, scale):
         scale = DEFAULT_SCALE
     else:
         scale = float(scale)
-        if scale != scale or abs(scale) == float("inf"):
-            raise ValueError("scale must be finite")
+        if not abs(scale) <= MAX_SCALE:
+            raise ValueError(f"scale must be finite, within {MAX_SCALE}")
     if T:
         q_latent, l0, l1 = _query_rows(q_latent)
         q_pe, p0, p1 = _query_rows(q_pe)

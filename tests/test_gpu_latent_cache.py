@@ -892,3 +892,24 @@ def test_rows_of_nan_stay_marked_and_alone(new, lengths, heads):
     assert bool(torch.isnan(out[lost]).all()) and bool(torch.isnan(lse[lost]).all())
     clean, clean_lse = lc.attend(x.q_latent, x.q_pe, *x.cache, x.lengths, x.cu_new)
     assert torch.equal(out[~lost], clean[~lost]) and torch.equal(lse[~lost], clean_lse[~lost])
+
+
+# --- scales --------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("heads,new", [(12, [1, 1]), (24, [9, 30])])
+def test_scales_that_leave_fp32_are_refused(heads, new):
+    x = Problem(77, new, [40, 50], heads, 16)
+    args = (*x.cache, x.lengths, x.cu_new)
+    _, lse = lc.attend(x.q_latent, x.q_pe, *args)
+    for scale in (2.4e38, -3e38, 1e39, -1e300, math.inf, -math.inf, math.nan):
+        with pytest.raises(ValueError, match="scale"):
+            lc.attend(x.q_latent, x.q_pe, *args, scale=scale)
+        with pytest.raises(ValueError, match="scale"):
+            lc.attention_mass(x.q_latent, x.q_pe, lse, *args, scale=scale)
+    # the largest ones, over products of zero: every position counts alike
+    none = torch.zeros_like(x.q_latent), torch.zeros_like(x.q_pe)
+    flat = lc.attend(*none, *args)
+    for scale in (lc.MAX_SCALE, -lc.MAX_SCALE):
+        got = lc.attend(*none, *args, scale=scale)
+        assert torch.equal(got[0], flat[0]) and torch.equal(got[1], flat[1])
+        assert torch.equal(lc.attention_mass(*none, flat[1], *args, scale=scale), lc.attention_mass(*none, flat[1], *args))

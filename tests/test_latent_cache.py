@@ -140,3 +140,9 @@ def test_argument_blocks_match_the_header(tmp_path):
 @pytest.mark.parametrize("stride", [0, 32, 63, 65, 128])
 def test_mass_in_place_needs_the_stride_of_the_result(stride):
     assert _refusal("mass", mass=P, new_mass=P, mass_stride=stride) == ERR_ARG
+
+
+@pytest.mark.parametrize("op", ["attend", "mass"])
+@pytest.mark.parametrize("scale", [2.4e38, -3e38, float("inf"), -float("inf"), float("nan")])
+def test_entry_points_refuse_scales_that_leave_fp32(op, scale):
+    assert _refusal(op, scale=scale) == ERR_ARG
