@@ -277,8 +277,9 @@ int kk3_cache_mass(const kk3_cache_mass_args* args, void* stream);
 /* Eviction: each sequence keeps min(lengths[b], budget) positions: its first `sinks` and its last `recent`
  * (the lowest of them where they are more), and of the others those of the largest mass (equal ones: the lowest
  * position; a NaN counts as the largest). The kept entries move, in ascending order, to positions 0, 1, ... of dst_table's pages
- * (pages that no listed sequence uses: shared pages stay as they are), or in place (dst_table = NULL; then no two
- * sequences may share a page). new_lengths,
+ * (pages that no listed sequence uses: shared pages stay as they are), or in place (dst_table = NULL; then no page may
+ * stand twice in the used part of the table). An entry whose page or new page is outside the pool is counted as kept but
+ * does not move: its new slot stays as it was, and the error word is set. new_lengths,
  * new_mass (the kept positions' mass, zeros behind) and kept (their old positions, -1 behind) are other buffers than
  * the inputs. */
 typedef struct kk3_cache_evict_args {

@@ -12,7 +12,7 @@ namespace kk3 {
 // to BF16 once, or (STEP) as the decode step and the model round it: to BF16 before the product with the weight, and
 // after it (kimi.py:268, common.py:13-21), so that the entry is the one that the step would have cached. One warp per token, bound by its 2304 bytes of traffic; 16-byte accesses throughout (lane l owns
 // the latent values 8 l .. 8 l + 7 and 256 + 8 l ..; eight lanes copy the rope part). Five chunks of up to 4096 tokens take
-// 7.2 us, 5.2 TB/s; eight single tokens 2.7 us, a launch.
+// 6.8 us, 5.5 TB/s (STEP 7.2); eight single tokens 2.4 us, a launch.
 
 struct AppendArgs {
   CachePages c;
@@ -394,7 +394,7 @@ __global__ void __launch_bounds__(kMoveWarps * 32) kk3_cache_move_kernel(const E
 // Eviction, move in place: entry kept[j] >= j goes to slot j, so batches in ascending j are safe when a batch is read
 // whole before it is written: later batches read slots at or above their own j, which earlier ones did not write.
 // The order holds per (sequence, 64-byte slice of the entry); the 18 slices of a sequence run side by side, bound by the
-// batches' latencies: 16 sequences of up to 8192 positions cut down to 4096 take 47 us in place, 38 into other pages.
+// batches' latencies: 16 sequences of up to 8192 positions cut down to 4096 take 46 us in place, 38 into other pages.
 constexpr int kSlideThreads = 512;
 constexpr int kSlideDeep = 8;    // rows in flight per thread: 1024 rows a batch
 __global__ void __launch_bounds__(kSlideThreads) kk3_cache_slide_kernel(const EvictArgs a) {
@@ -519,7 +519,7 @@ extern "C" int kk3_cache_append(const kk3_cache_append_args* x, void* stream) { 
 extern "C" int kk3_cache_append_step(const kk3_cache_append_args* x, void* stream) { return cache_append<true>(x, stream); }
 
 // The kernel and its workers. Up to 16 rows a sequence on average fill the small tile: 64 sequences of 8192 positions
-// with 12 rows each take 129 us in it and 187 us in CTA pairs; with 24 rows, two small tiles that read the cache twice,
+// with 12 rows each take 123 us in it and 187 us in CTA pairs; with 24 rows, two small tiles that read the cache twice,
 // 243 and 195 us. A small call is faster in the small tile whatever its rows, since that begins and ends sooner: 48 rows
 // of one sequence take 20.5 against 24.0 us over 517 positions and 24.0 against 26.0 over 8192, 96 rows 27.4 against 26.7.
 // The host does not know the lengths, only what the table can hold.

@@ -266,7 +266,8 @@ KK3_DEV void with_box(int box, const F& f) {
 //
 // Bounds of a unit of 256 rows: 4608 clocks of tensor time (256 x 256 x 576 products at 4096 a clock and SM), as many
 // of shared-memory reads (16 KB per 128-clock instruction), and 2048 of exponentials (16 a clock). Measured: 32 tokens
-// x 96 heads over four sequences of up to 8192 positions 71 us, 1110 TFLOP/s (47 us at the rate of a plain product);
+// x 96 heads over four sequences of up to 8192 positions 70 us, 1130 TFLOP/s (47 us at the rate of a plain product): the
+// ring's four slots of 16 KB cover 2048 clocks of products, and a slot's turn takes about that;
 // 16 single tokens x 12 heads, bound by the cache's bytes, 29 us, 3.7 TB/s: 3 us for the work split, 7 until the first
 // tile's sums, then 3.7 us a tile, the rate of HBM.
 
@@ -567,12 +568,12 @@ __global__ void __launch_bounds__(kMassPos) kk3_cache_mass_join_kernel(const Mas
 //
 // Bounds of a unit: 4352 clocks of tensor time (128 x 256 x 1088 products at 4096 a clock and SM), 4200 to issue its
 // scores, 278 KB of loads in each SM (mostly from L2). Measured: two chunks of 1024 tokens x 12 heads over up to 8192
-// positions 299 us, 1090 TFLOP/s (a plain product: 1679), 8600 clocks a unit, the tensor pipe active for half of them: a
+// positions 299 us, 1090 TFLOP/s (a plain product: 1679; back to back, at lower clocks, 312 us), 8600 clocks a unit, the tensor pipe active for half of them: a
 // slot's turn (copy issued, L2, instructions, commit) takes more than 2000 clocks, which seven slots do not cover, and
 // there is no shared memory for more (an eighth in place of half of P took 311 us, since the halves then wait for one
 // another). Three prompts of 900 tokens x 24 heads 100 to 107 us: tiles of two or three units each, whose first scores, last
 // sums and epilogue (6 us) nothing overlaps.
-// Eight single tokens x 96 heads over up to 8192 positions 38 us: 7 us to the first scores, three units of 3.6 us, 8 us for
+// Eight single tokens x 96 heads over up to 8192 positions 36 us: 7 us to the first scores, three units of 3.6 us, 8 us for
 // the last sums and the running sums' way out, 8 us for their join.
 
 constexpr int kPaUnit = 256;
@@ -1050,10 +1051,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPaThreads, 1)
 // the query's fragments of a quarter of the 576 dims in registers and takes 8 positions, in the second it owns 32 of the
 // output dims, in the softmax a row; half of the warps begin with the scores, so that not all want the same at once. Four
 // more warps copy, one unit to a stage of five, and run ahead over the tiles.
-// Measured: 64 single tokens x 12 heads over 8192 positions 129 us, 4.7 TB/s, and 122 us where the cache stays in L2: the
+// Measured: 64 single tokens x 12 heads over 8192 positions 123 us, 4.9 TB/s, and 119 us where the cache stays in L2: the
 // 1800 clocks of a unit's instructions and shared-memory traffic, the start, the workers' uneven ends and the join (25 us
-// for the last three); one such token 17 us. With copies by the 16 warps themselves, between the products, the 64 took
-// 142 us; with six stages, scores of one unit in shared memory and two barriers a unit 134 us.
+// for the last three); one token over 517 positions 15 us. Before the last two steps: with copies by the 16 warps themselves,
+// between the products, the 64 took 142 us; with six stages, scores of one unit in shared memory and two barriers a unit 134.
 // Probabilities are rounded to BF16 for the second product, the type that the instruction takes with BF16 latents; the
 // running sum adds them unrounded, since lse is an FP32 result.
 

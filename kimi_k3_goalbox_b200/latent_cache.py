@@ -14,7 +14,8 @@ page number outside the pool or a length outside the table reads as zeros, is no
 (optional int32 tensor, zeroed by the caller) to a nonzero code. Without an error_word such a call is silent, so a
 program that fills its tables on the device should pass one and look at it now and then. A wait inside `attend` or
 `attention_mass` that runs out (two seconds; a defect, no healthy call comes near it) sets it as well, and the results
-that it was for are NaN. There is no CPU path: without the library or a GPU
+that it was for are NaN. Nothing here is differentiable: results carry no gradient, whatever the inputs ask for.
+There is no CPU path: without the library or a GPU
 these raise.
 """
 
@@ -337,8 +338,9 @@ def evict(kv, pe, table, lengths, mass, budget: int, *, sinks: int = 0, recent: 
     counts as the largest).
 
     The kept entries move, in ascending order, to positions 0, 1, ... of dst_table's pages (int32 [B, columns2]; pages
-    that none of the sequences uses, so that pages shared with others stay as they are), or in place (None; then no two
-    sequences may share a page). Returns
+    that none of the sequences uses, so that pages shared with others stay as they are), or in place (None; then no page
+    may stand twice in the used part of the table). An entry whose page or new page is outside the pool is counted as
+    kept but does not move: its new slot stays as it was, and error_word is set. Returns
     (new lengths int64 [B], their mass f32 [B, columns * page_size] with zeros behind, their old positions int32
     [B, budget] with -1 behind)."""
     cache, dev, B, capacity = _cache(kv, pe, table)
