@@ -220,8 +220,8 @@ int kk3_cache_append_step(const kk3_cache_append_args* args, void* stream);
  * (already appended): token i of n sees the first lengths[b] - n + i + 1 positions. Per token and head
  *   s_p = scale * (q_latent . c_p + q_pe . r_p),  out = sum_p softmax(s)_p c_p  (bf16 [tokens, heads, 512]),
  *   lse = log sum_p exp(s_p)  (f32 [tokens, heads]).
- * |scale| is 2.35e38 at most. A token that sees nothing gets out = 0 and lse = -infinity. Queries: bf16, last dim contiguous, all (token,
- * head) rows at one pitch: the token stride is heads times the head stride (KK3_ERR_UNSUPPORTED otherwise).
+ * |scale| is 2.35e38 at most. A token that sees nothing gets out = 0 and lse = -infinity. Queries: bf16, last dim
+ * contiguous, all (token, head) rows at one pitch: the token stride is heads times the head stride (KK3_ERR_UNSUPPORTED otherwise).
  * Sums and softmax statistics are FP32, probabilities are rounded to bf16 for the second product. The
  * positions that a sequence holds must be finite for its tokens' results to be. workspace: 16-byte aligned,
  * kk3_cache_attend_workspace() bytes (the same for every call on a device; 0: no device), used until the call's kernels

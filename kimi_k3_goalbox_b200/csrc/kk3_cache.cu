@@ -10,9 +10,10 @@ namespace kk3 {
 // ---------------------------------------------------------------------------------------------
 // append: latent = x[:512] / rms(x[:512]) * weight, rope = x[512:], into the page of the token's position. In FP32, rounded
 // to BF16 once, or (STEP) as the decode step and the model round it: to BF16 before the product with the weight, and
-// after it (kimi.py:268, common.py:13-21), so that the entry is the one that the step would have cached. One warp per token, bound by its 2304 bytes of traffic; 16-byte accesses throughout (lane l owns
-// the latent values 8 l .. 8 l + 7 and 256 + 8 l ..; eight lanes copy the rope part). Five chunks of up to 4096 tokens take
-// 6.8 us, 5.5 TB/s (STEP 7.2); eight single tokens 2.4 us, a launch.
+// after it (kimi.py:265-270, common.py:13-21), so that the entry is the one that the step would have cached. One warp per
+// token, bound by its 2304 bytes of traffic; 16-byte accesses throughout (lane l owns the latent values 8 l .. 8 l + 7 and
+// 256 + 8 l ..; eight lanes copy the rope part). Five chunks of up to 4096 tokens take 6.8 us, 5.5 TB/s (STEP 7.2); eight
+// single tokens 2.4 us, a launch.
 
 struct AppendArgs {
   CachePages c;

@@ -241,7 +241,8 @@ def append(raw, norm_weight, kv, pe, table, lengths, cu_new, *, eps: float = 1e-
     raw: bf16 [T, 576], the `ka` projection of the new tokens; its first 512 values are RMS-normalised with
     norm_weight (bf16 [512]) in FP32 and rounded once, the other 64 are stored as they are. as_step: rounded to bf16
     before the product with norm_weight too, as the model and the decode step do; caches that `step_append` continues
-    want this, so that the entry is the one the step would have written. lengths: positions cached before. A token behind the table's last column is not written, nor are those of a sequence whose length is negative
+    want this, so that the entry is the one the step would have written. lengths: positions cached before. A token
+    behind the table's last column is not written, nor are those of a sequence whose length is negative
     (its new length then counts from zero); both set error_word."""
     cache, dev, B, _ = _cache(kv, pe, table)
     try:
