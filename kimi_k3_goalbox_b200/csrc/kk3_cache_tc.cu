@@ -569,10 +569,10 @@ __global__ void __launch_bounds__(kMassPos) kk3_cache_mass_join_kernel(const Mas
 // Bounds of a unit: 4352 clocks of tensor time (128 x 256 x 1088 products at 4096 a clock and SM), 4200 to issue its
 // scores, 278 KB of loads in each SM (mostly from L2). Measured: two chunks of 1024 tokens x 12 heads over up to 8192
 // positions 299 us, 1090 TFLOP/s (a plain product: 1679; back to back, at lower clocks, 312 us), 8600 clocks a unit, the
-// tensor pipe active for half of them: a slot's turn (copy issued, L2, instructions, commit) takes more than 2000 clocks, which seven slots do not cover, and
-// there is no shared memory for more (an eighth in place of half of P took 311 us, since the halves then wait for one
-// another). Three prompts of 900 tokens x 24 heads 100 to 107 us: tiles of two or three units each, whose first scores, last
-// sums and epilogue (6 us) nothing overlaps.
+// tensor pipe active for half of them: a slot's turn (copy issued, L2, instructions, commit) takes more than 2000 clocks,
+// which seven slots do not cover, and there is no shared memory for more (an eighth in place of half of P took 311 us,
+// since the halves then wait for one another). Three prompts of 900 tokens x 24 heads 99 to 107 us: tiles of two or three
+// units each, whose first scores, last sums and epilogue (6 us) nothing overlaps.
 // Eight single tokens x 96 heads over up to 8192 positions 36 us: 7 us to the first scores, three units of 3.6 us, 8 us for
 // the last sums and the running sums' way out, 8 us for their join.
 
